@@ -25,6 +25,9 @@ _lib = None
 _sz = C.c_size_t
 _vp = C.c_void_p
 _u32p = C.POINTER(C.c_uint32)
+_i32p = C.POINTER(C.c_int32)
+_u8p = C.POINTER(C.c_uint8)
+_f = C.c_float
 _i = C.c_int
 
 # (name, restype, argtypes) for every declaration of include/ckv.h
@@ -78,6 +81,14 @@ _SIGNATURES = [
     ("ckv_sigmoid_mul", _i, [_vp, _i, _vp, _vp, _vp, _sz]),
     ("ckv_checkpoint_export", _i, [_vp, _u32p, _sz, _sz, _vp, _vp]),
     ("ckv_checkpoint_import", _i, [_vp, _u32p, _sz, _sz, _vp, _vp]),
+    ("ckv_attention_window", _i, [_vp, _sz, _vp, _sz, _f, _sz, _sz, _vp, _vp, _sz]),
+    ("ckv_append_decode_window", _i, [_vp, _sz, _vp, _vp, _vp, _sz, _f, _sz, _sz, _vp, _vp, _sz]),
+    ("ckv_rope_append_decode_window", _i, [_vp, _sz, _vp, _vp, _vp, _sz, _f, _f, _sz, _sz, _sz,
+                                           _vp, _vp, _sz]),
+    ("ckv_rope_axes_upload", _i, [_vp, _u32p, _sz, _sz]),
+    ("ckv_rope_axes", _i, [_vp, _vp, _vp, _sz, _f, _sz, _u8p, _sz]),
+    ("ckv_rope_axes_append", _i, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _f, _sz, _u8p, _sz]),
+    ("ckv_compact", _i, [_vp, _u32p, _u32p, _i32p, _u32p, _sz, _f, _sz]),
 ]
 SYMBOLS = [name for name, _, _ in _SIGNATURES]
 
@@ -147,6 +158,19 @@ def _u32(a) -> Optional[np.ndarray]:
 
 def _p(a: Optional[np.ndarray]):
     return None if a is None else a.ctypes.data_as(_u32p)
+
+
+def rope_pair_axes(sections, interleaved: bool = False) -> np.ndarray:
+    """pair_axis of the rope_axes calls from the rotary pairs each axis turns
+    (sections[a]; their sum is rotary_dim / 2): one section after another, or
+    interleaved, the axes taken in turn while they have pairs left and the rest
+    by the first."""
+    if not interleaved:
+        return np.repeat(np.arange(len(sections)), sections).astype(np.uint8)
+    axes = np.zeros(sum(sections), np.uint8)
+    for a in range(1, len(sections)):
+        axes[a:sections[a] * len(sections):len(sections)] = a
+    return axes
 
 
 class Context:
@@ -378,6 +402,79 @@ class Pool:
         self.ctx.check(load().ckv_rope_append_decode(
             self.handle, layer, _ptr(keys), _ptr(values), _ptr(queries), q_heads, scale, theta,
             rotary_dim, None if gate is None else _ptr(gate), _ptr(output), rows))
+
+    def attention_window(self, layer, queries, q_heads, scale, window: int, output, sinks: int = 0,
+                         gate=None, rows=None) -> None:
+        """Attention to the last `window` tokens and the first `sinks`
+        (* sigmoid(gate)) (ckv_attention_window)."""
+        rows = queries.shape[0] if rows is None else rows
+        self.ctx.check(load().ckv_attention_window(self.handle, layer, _ptr(queries), q_heads,
+                                                   scale, window, sinks, _ptr(gate), _ptr(output),
+                                                   rows))
+
+    def append_decode_window(self, layer, keys, values, queries, q_heads, scale, window: int,
+                             output, sinks: int = 0, gate=None, rows=None) -> None:
+        """append, then attention_window of decode rows (ckv_append_decode_window)."""
+        rows = queries.shape[0] if rows is None else rows
+        self.ctx.check(load().ckv_append_decode_window(
+            self.handle, layer, _ptr(keys), _ptr(values), _ptr(queries), q_heads, scale, window,
+            sinks, _ptr(gate), _ptr(output), rows))
+
+    def rope_append_decode_window(self, layer, keys, values, queries, q_heads, scale, theta,
+                                  window: int, output, sinks: int = 0, rotary_dim: int = 0,
+                                  gate=None, rows=None) -> None:
+        """append_decode_window from unrotated queries and keys
+        (ckv_rope_append_decode_window)."""
+        rows = queries.shape[0] if rows is None else rows
+        self.ctx.check(load().ckv_rope_append_decode_window(
+            self.handle, layer, _ptr(keys), _ptr(values), _ptr(queries), q_heads, scale, theta,
+            rotary_dim, window, sinks, _ptr(gate), _ptr(output), rows))
+
+    def upload_axes(self, positions) -> None:
+        """The batch's positions on several axes, [axes, rows] (ckv_rope_axes_upload)."""
+        p = _u32(positions)
+        if p.ndim != 2:
+            raise ValueError("positions are [axes, rows]")
+        self.ctx.check(load().ckv_rope_axes_upload(self.handle, _p(p), p.shape[0], p.shape[1]))
+
+    def _pair_axis(self, pair_axis, rotary_dim: int) -> np.ndarray:
+        axes = np.ascontiguousarray(pair_axis, dtype=np.uint8)
+        if axes.size != (rotary_dim or self.geometry[4]) // 2:
+            raise ValueError("pair_axis has an axis for each of rotary_dim / 2 pairs")
+        return axes
+
+    def rope_axes(self, inputs, outputs, heads: int, theta: float, pair_axis, rotary_dim: int = 0,
+                  rows: Optional[int] = None) -> None:
+        """Rows rotated by their positions on several axes (ckv_rope_axes); see
+        rope_pair_axes for pair_axis."""
+        rows = inputs.shape[0] if rows is None else rows
+        a = self._pair_axis(pair_axis, rotary_dim)
+        self.ctx.check(load().ckv_rope_axes(self.handle, _ptr(inputs), _ptr(outputs), heads, theta,
+                                            rotary_dim, a.ctypes.data_as(_u8p), rows))
+
+    def rope_axes_append(self, layer: int, queries, rotated, q_heads: int, keys, values,
+                         theta: float, pair_axis, rotary_dim: int = 0,
+                         rows: Optional[int] = None) -> None:
+        """Queries rotated into `rotated`, keys rotated and values appended, in one
+        launch (ckv_rope_axes_append)."""
+        rows = keys.shape[0] if rows is None else rows
+        a = self._pair_axis(pair_axis, rotary_dim)
+        self.ctx.check(load().ckv_rope_axes_append(
+            self.handle, layer, _ptr(queries), _ptr(rotated), q_heads, _ptr(keys), _ptr(values),
+            theta, rotary_dim, a.ctypes.data_as(_u8p), rows))
+
+    def compact(self, from_slots, to_slots, counts, shift=None, theta: float = 0.0,
+                rotary_dim: int = 0) -> None:
+        """Kept tokens' K and V of every layer to other slots, keys turned by `shift`
+        positions (ckv_compact); counts are the moves of each sequence."""
+        f, t, c = _u32(from_slots), _u32(to_slots), _u32(counts)
+        s = None if shift is None else np.ascontiguousarray(shift, dtype=np.int32)
+        if f.size != t.size or int(c.sum(dtype=np.uint64)) != f.size \
+                or (s is not None and s.size != f.size):
+            raise ValueError("from_slots, to_slots and shift have an entry for each counted move")
+        self.ctx.check(load().ckv_compact(
+            self.handle, _p(f), _p(t), None if s is None else s.ctypes.data_as(_i32p), _p(c),
+            c.size, theta, rotary_dim))
 
     def copy_blocks(self, src, dst) -> None:
         s, d = _u32(src), _u32(dst)

@@ -416,10 +416,9 @@ int ensure_plan(ckv_pool* pool)
 // (record, kv head). The counters have a buffer of their own (the generic
 // decode writes its partials over d_partials) and are zeroed by a fill
 // kernel whenever it is allocated; launches leave them zero.
-int ensure_split(ckv_pool* pool, size_t q_heads, split_scratch& split)
+int ensure_split(ckv_pool* pool, const meta_view& m, size_t q_heads, split_scratch& split)
 {
     split = {};
-    const meta_view& m = pool->meta;
     if (!m.n_cut)
         return CKV_OK;
     ckv_context* ctx = pool->ctx;
@@ -454,15 +453,14 @@ int ensure_split(ckv_pool* pool, size_t q_heads, split_scratch& split)
     return CKV_OK;
 }
 
-// The split-KV work list, at the batch's first split decode launch: each
-// row's range 0..position cut into chunks of `chunk` tokens, (row, chunk)
-// pairs, plus each row's first item and item count.
-int ensure_work(ckv_pool* pool)
+// A split-KV work list: each row's range 0..position cut into chunks of `chunk`
+// tokens, (row, chunk) pairs, plus each row's first item and item count. It is
+// uploaded to `device`; `m` points at it and `multi` says whether some row has
+// several chunks.
+int put_work(ckv_pool* pool, const std::vector<uint32_t>& positions, meta_view& m,
+             uint32_t** device, size_t* device_words, bool& some_multi)
 {
-    if (pool->work_ready)
-        return CKV_OK;
     ckv_context* ctx = pool->ctx;
-    const std::vector<uint32_t>& positions = pool->positions;
     const size_t rows = positions.size();
     uint64_t token_heads = 0, n_items = 0;
     for (const uint32_t p : positions)
@@ -491,41 +489,117 @@ int ensure_work(ckv_pool* pool)
             w[2 * item + 1] = c;
         }
     }
-    status = ensure_device(ctx, &pool->d_work, &pool->d_work_words, words, "decode work list");
+    status = ensure_device(ctx, device, device_words, words, "decode work list");
     if (status)
         return status;
-    status = upload_staged(ctx, pool->d_work, words * sizeof(uint32_t));
+    status = upload_staged(ctx, *device, words * sizeof(uint32_t));
     if (status)
         return status;
-    meta_view& m = pool->meta;
-    m.items = pool->d_work;
-    m.row_first = pool->d_work + s_first;
-    m.row_count = pool->d_work + s_count;
+    m.items = *device;
+    m.row_first = *device + s_first;
+    m.row_count = *device + s_count;
     m.n_items = (uint32_t)n_items;
     m.chunk = chunk;
-    pool->work_multi = multi;
-    pool->work_ready = true;
+    some_multi = multi;
     return CKV_OK;
 }
 
+// The batch's work list, at its first split decode launch.
+int ensure_work(ckv_pool* pool)
+{
+    if (pool->work_ready)
+        return CKV_OK;
+    const int status = put_work(pool, pool->positions, pool->meta, &pool->d_work,
+                                &pool->d_work_words, pool->work_multi);
+    pool->work_ready = status == CKV_OK;
+    return status;
+}
+
+// ---- the batch through a window ---------------------------------------------------
+
+// Whether the context's stream is being captured into a graph (or cannot be asked
+// while another is): a launch there takes no upload and no allocation, whose replays
+// would read staging memory of other uploads or free what a graph uses.
+bool capturing(const ckv_context* ctx)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing(ctx->stream, &status);
+    if (e != hipSuccess)
+        (void)hipGetLastError();
+    return e != hipSuccess || status != hipStreamCaptureStatusNone;
+}
+
+int refuse_captured(ckv_context* ctx)
+{
+    return set_error(ctx, CKV_E_INVALID_ARGUMENT,
+                     "the stream is being captured and the call has something to upload or "
+                     "allocate: make it once on this batch before the capture");
+}
+
+// A window past every row's position leaves the batch as it is (all_keys).
+key_window window_of(const ckv_pool* pool, size_t window, size_t sinks)
+{
+    const key_window w { (uint32_t)std::min<size_t>(window, UINT32_MAX),
+                         (uint32_t)std::min<size_t>(sinks, UINT32_MAX) };
+    return window_low(pool->last_position, w) > w.sinks ? w : all_keys;
+}
+
+// Selects the batch's window: its positions less the tokens of the units it skips.
+void select_window(ckv_pool* pool, key_window w)
+{
+    if (pool->window.window == w.window && pool->window.sinks == w.sinks
+        && pool->window_positions.size() == pool->positions.size())
+        return;
+    pool->window_positions.clear(); // stays so if what follows throws
+    pool->window_plan_ready = pool->window_work_ready = false;
+    pool->window = w;
+    pool->window_meta = pool->meta;
+    pool->window_positions.resize(pool->positions.size());
+}
+
+// The window's work list of the generic decode, in tokens.
+int ensure_window_work(ckv_pool* pool)
+{
+    if (pool->window_work_ready)
+        return CKV_OK;
+    if (capturing(pool->ctx))
+        return refuse_captured(pool->ctx);
+    const key_window w = pool->window;
+    std::vector<uint32_t>& left = pool->window_positions;
+    for (size_t r = 0; r < left.size(); ++r) {
+        const uint32_t p = pool->positions[r];
+        left[r] = p - window_gap_of(window_low(p, w), w.sinks, 1).skip;
+    }
+    const int status = put_work(pool, left, pool->window_meta, &pool->d_window_work,
+                                &pool->d_window_work_words, pool->window_work_multi);
+    pool->window_work_ready = status == CKV_OK;
+    return status;
+}
+
 int run_decode(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale,
-               void* output, const void* gate = nullptr)
+               void* output, const void* gate = nullptr, key_window window = all_keys)
 {
     ckv_context* ctx = pool->ctx;
     const pool_view view = view_of(pool);
     float* partials = nullptr;
     split_scratch split {};
-    const bool fast = decode_fast_applies(view, (uint32_t)q_heads, queries, output);
-    int status = fast ? ensure_plan(pool) : ensure_work(pool);
+    const bool windowed = window.window != all_keys.window;
+    const bool fast = !windowed && decode_fast_applies(view, (uint32_t)q_heads, queries, output);
+    if (windowed)
+        select_window(pool, window);
+    int status = windowed ? ensure_window_work(pool) : fast ? ensure_plan(pool) : ensure_work(pool);
+    const meta_view& m = windowed ? pool->window_meta : pool->meta;
     if (!status && fast)
-        status = ensure_split(pool, q_heads, split);
+        status = ensure_split(pool, m, q_heads, split);
     if (status)
         return status;
-    const bool needs_merge = !fast && pool->work_multi;
+    const bool needs_merge = !fast && (windowed ? pool->window_work_multi : pool->work_multi);
     if (needs_merge) {
         size_t capacity_floats = pool->d_partials_bytes / sizeof(float);
-        const size_t needed = (size_t)pool->meta.n_items * q_heads
+        const size_t needed = (size_t)m.n_items * q_heads
             * partial_record_floats((uint32_t)pool->head_dim);
+        if (windowed && needed > capacity_floats && capturing(ctx))
+            return refuse_captured(ctx);
         status = ensure_device(ctx, &pool->d_partials, &capacity_floats, needed,
                                "decode partials");
         // stored whatever the outcome: a failed regrow leaves no buffer and
@@ -535,16 +609,14 @@ int run_decode(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads
             return status;
         partials = pool->d_partials;
     }
-    status = run_kernel(ctx, "paged_attention_decode", [&] {
-        return launch_decode(ctx->stream, view, pool->meta, (uint32_t)layer, queries,
-                             (uint32_t)q_heads, scale, output, partials, ctx->cu_count, gate,
-                             split);
+    status = run_kernel(ctx, windowed ? "window_attention_decode" : "paged_attention_decode", [&] {
+        return launch_decode(ctx->stream, view, m, (uint32_t)layer, queries, (uint32_t)q_heads,
+                             scale, output, partials, ctx->cu_count, gate, split, window);
     });
     if (status || !needs_merge)
         return status;
     return run_kernel(ctx, "paged_attention_merge", [&] {
-        return launch_merge(ctx->stream, view, pool->meta, (uint32_t)q_heads, output, partials,
-                            gate);
+        return launch_merge(ctx->stream, view, m, (uint32_t)q_heads, output, partials, gate);
     });
 }
 
@@ -748,6 +820,38 @@ int create_pool(ckv_context* ctx, size_t layers, size_t blocks, size_t block_siz
     }
     *out = pool;
     return CKV_OK;
+}
+
+// Entry points through this make their context's device current while they run, and
+// give a status for what the host code throws.
+struct device_scope {
+    int before = -1;
+    explicit device_scope(int device)
+    {
+        if (hipGetDevice(&before) != hipSuccess || before == device)
+            before = -1;
+        else
+            (void)hipSetDevice(device);
+    }
+    ~device_scope()
+    {
+        if (before >= 0)
+            (void)hipSetDevice(before);
+    }
+};
+
+template <class Call>
+int guarded(ckv_pool* pool, Call&& call) noexcept
+{
+    if (!pool)
+        return CKV_E_INVALID_ARGUMENT;
+    try {
+        const device_scope scope(pool->ctx->device);
+        return call();
+    } catch (const std::exception&) {
+        pool->ctx->last_error.assign("host memory"); // within the string's reserve
+        return CKV_E_TENSOR_ALLOCATION_FAILED;
+    }
 }
 
 } // namespace
@@ -1106,6 +1210,12 @@ int ckv_pool_destroy(ckv_pool* pool)
         (void)dev_free(ctx, pool->d_spill);
     if (pool->d_rope_q)
         (void)dev_free(ctx, pool->d_rope_q);
+    if (pool->d_window_plan)
+        (void)dev_free(ctx, pool->d_window_plan);
+    if (pool->d_window_work)
+        (void)dev_free(ctx, pool->d_window_work);
+    if (pool->d_axes)
+        (void)dev_free(ctx, pool->d_axes);
     delete pool;
     return CKV_OK;
 }
@@ -1156,8 +1266,11 @@ void adopt_batch(ckv_pool* pool, size_t rows, size_t n_entries, bool with_slots,
     m.n_entries = (uint32_t)n_entries;
     m.rows = (uint32_t)rows;
     uint64_t pages = 0;
-    for (const uint32_t position : pool->positions)
+    pool->last_position = 0;
+    for (const uint32_t position : pool->positions) {
         pages += position / pool->block_size + 1;
+        pool->last_position = std::max(pool->last_position, position);
+    }
     m.mean_pages = rows ? (uint32_t)(pages / rows) : 0;
     m.items = m.row_first = m.row_count = nullptr;
     m.n_items = 0;
@@ -1174,6 +1287,9 @@ void adopt_batch(ckv_pool* pool, size_t rows, size_t n_entries, bool with_slots,
     pool->fusable = fusable;
     pool->plan_ready = plan_uploaded;
     pool->work_ready = false;
+    pool->window_positions.clear();
+    pool->window_plan_ready = pool->window_work_ready = false;
+    pool->axes = 0;
     pool->uploaded = true;
 }
 
@@ -1793,7 +1909,7 @@ int append_decode_impl(ckv_pool* pool, size_t layer, const void* keys, const voi
         split_scratch split {};
         status = ensure_plan(pool);
         if (!status)
-            status = ensure_split(pool, q_heads, split);
+            status = ensure_split(pool, pool->meta, q_heads, split);
         if (status)
             return status;
         return run_kernel(ctx, "append_decode", [&] {
@@ -1952,7 +2068,7 @@ int ckv_rope_append_decode(ckv_pool* pool, size_t layer, const void* keys, const
         split_scratch split {};
         status = ensure_plan(pool);
         if (!status)
-            status = ensure_split(pool, q_heads, split);
+            status = ensure_split(pool, pool->meta, q_heads, split);
         if (status)
             return status;
         return run_kernel(ctx, "rope_append_decode", [&] {
@@ -2056,6 +2172,317 @@ int ckv_append_decode_noalloc(ckv_pool* pool, size_t layer, const void* keys, co
     if (e != hipSuccess)
         return fail_fixed(ctx, CKV_E_HIP_FAILURE, hipGetErrorString(e));
     return CKV_OK;
+}
+
+namespace {
+
+// An optional gate, as check_gate's where there is one.
+int check_optional_gate(const ckv_pool* pool, const void* gate, const void* queries,
+                        const void* output)
+{
+    if (gate && (gate == queries || gate == output))
+        return set_error(pool->ctx, CKV_E_UNSUPPORTED_ALIASING, "gate overlaps queries or output");
+    return CKV_OK;
+}
+
+int check_window(const ckv_pool* pool, size_t window)
+{
+    return window ? CKV_OK
+                  : set_error(pool->ctx, CKV_E_INVALID_ARGUMENT,
+                              "window == 0: a row attends itself at least");
+}
+
+int check_slots(const ckv_pool* pool, size_t layer, const void* keys, const void* values,
+                size_t rows)
+{
+    ckv_context* ctx = pool->ctx;
+    if (rows && (!keys || !values))
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "keys and values are required");
+    if (!pool->uploaded || !pool->has_slots)
+        return set_error(ctx, CKV_E_NO_TABLES, "append before slots were uploaded");
+    if (rows != pool->slot_rows)
+        return set_error(ctx, CKV_E_CACHE_SLOT_COUNT_MISMATCH, "rows != uploaded slots");
+    if (layer >= pool->layers)
+        return set_error(ctx, CKV_E_CACHE_LAYER_OUT_OF_RANGE, "layer >= layers");
+    return CKV_OK;
+}
+
+} // namespace
+
+int ckv_attention_window(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads,
+                         float scale, size_t window, size_t sinks, const void* gate, void* output,
+                         size_t rows)
+{
+    return guarded(pool, [&]() -> int {
+        int status = check_attention(pool, layer, queries, q_heads, output, rows);
+        if (!status)
+            status = check_window(pool, window);
+        if (!status)
+            status = check_optional_gate(pool, gate, queries, output);
+        if (status || !rows)
+            return status;
+        return run_decode(pool, layer, queries, q_heads, scale, output, gate,
+                          window_of(pool, window, sinks));
+    });
+}
+
+int ckv_append_decode_window(ckv_pool* pool, size_t layer, const void* keys, const void* values,
+                             const void* queries, size_t q_heads, float scale, size_t window,
+                             size_t sinks, const void* gate, void* output, size_t rows)
+{
+    return guarded(pool, [&]() -> int {
+        int status = check_slots(pool, layer, keys, values, rows);
+        if (!status)
+            status = check_attention(pool, layer, queries, q_heads, output, rows);
+        if (!status)
+            status = check_window(pool, window);
+        if (!status)
+            status = check_optional_gate(pool, gate, queries, output);
+        if (status || !rows)
+            return status;
+        const key_window w = window_of(pool, window, sinks);
+        if (w.window == all_keys.window)
+            return append_decode_impl(pool, layer, keys, values, queries, q_heads, scale, output,
+                                      rows, gate);
+        status = ckv_append(pool, layer, keys, values, rows);
+        if (status)
+            return status;
+        return run_decode(pool, layer, queries, q_heads, scale, output, gate, w);
+    });
+}
+
+int ckv_rope_append_decode_window(ckv_pool* pool, size_t layer, const void* keys,
+                                  const void* values, const void* queries, size_t q_heads,
+                                  float scale, float theta, size_t rotary_dim, size_t window,
+                                  size_t sinks, const void* gate, void* output, size_t rows)
+{
+    return guarded(pool, [&]() -> int {
+        int status = check_slots(pool, layer, keys, values, rows);
+        if (!status)
+            status = check_attention(pool, layer, queries, q_heads, output, rows);
+        if (!status)
+            status = check_window(pool, window);
+        if (!status)
+            status = check_optional_gate(pool, gate, queries, output);
+        ckv::rope_table freq;
+        uint32_t rotary = 0;
+        if (!status)
+            status = check_rope(pool, q_heads, theta, rotary_dim, freq, rotary);
+        if (status || !rows)
+            return status;
+        const key_window w = window_of(pool, window, sinks);
+        if (w.window == all_keys.window)
+            return ckv_rope_append_decode(pool, layer, keys, values, queries, q_heads, scale,
+                                          theta, rotary_dim, gate, output, rows);
+        ckv_context* ctx = pool->ctx;
+        const size_t q_bytes = rows * q_heads * pool->head_dim * pool->elem_size;
+        if (q_bytes > pool->d_rope_q_bytes && capturing(ctx))
+            return refuse_captured(ctx);
+        status = ensure_device(ctx, &pool->d_rope_q, &pool->d_rope_q_bytes, q_bytes,
+                               "rotated queries");
+        if (!status)
+            status = ckv_rope(pool, queries, pool->d_rope_q, q_heads, theta, rotary_dim, rows);
+        if (!status)
+            status = ckv_rope_append(pool, layer, keys, values, theta, rotary_dim, rows);
+        if (status)
+            return status;
+        return run_decode(pool, layer, pool->d_rope_q, q_heads, scale, output, gate, w);
+    });
+}
+
+int ckv_rope_axes_upload(ckv_pool* pool, const uint32_t* positions, size_t axes, size_t rows)
+{
+    return guarded(pool, [&]() -> int {
+        ckv_context* ctx = pool->ctx;
+        if (!axes || axes > ckv::max_axes || (rows && !positions))
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT,
+                             "positions on 1 to " + std::to_string(ckv::max_axes) + " axes");
+        if (!pool->uploaded)
+            return set_error(ctx, CKV_E_NO_TABLES, "axes before ckv_tables_upload");
+        if (rows != pool->positions.size())
+            return set_error(ctx, CKV_E_POSITION_COUNT_MISMATCH, "rows != uploaded positions");
+        if (capturing(ctx))
+            return refuse_captured(ctx);
+        const size_t words = std::max<size_t>(axes * rows, 4);
+        void* host = nullptr;
+        int status = stage(ctx, words * sizeof(uint32_t), &host);
+        if (status)
+            return status;
+        if (rows)
+            std::memcpy(host, positions, axes * rows * sizeof(uint32_t));
+        pool->axes = 0; // until the copy is on its way
+        status = ensure_device(ctx, &pool->d_axes, &pool->d_axes_words, words, "axis positions");
+        if (!status)
+            status = upload_staged(ctx, pool->d_axes, words * sizeof(uint32_t));
+        if (!status)
+            pool->axes = (uint32_t)axes;
+        return status;
+    });
+}
+
+namespace {
+
+// The checks of rope on several axes after the row count; fills the tables.
+int check_rope_axes(ckv_pool* pool, size_t heads, float theta, size_t rotary_dim,
+                    const uint8_t* pair_axis, ckv::turn_table& turns, ckv::axis_table& axes,
+                    uint32_t& rotary)
+{
+    ckv_context* ctx = pool->ctx;
+    if (heads == 0)
+        return set_error(ctx, CKV_E_INVALID_HEAD_COUNT, "heads == 0");
+    const size_t head_dim = pool->head_dim;
+    if (rotary_dim == 0)
+        rotary_dim = head_dim;
+    if (head_dim % 2 != 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim
+        || rotary_dim / 2 > ckv::max_turn_pairs)
+        return set_error(ctx, CKV_E_INVALID_HEAD_DIMENSION,
+                         "head_dim and rotary_dim must be even, rotary_dim <= head_dim and at most "
+                             + std::to_string(2 * ckv::max_turn_pairs));
+    if (!std::isfinite(theta) || theta <= 0.0f)
+        return set_error(ctx, CKV_E_INVALID_ROPE_THETA, "theta must be positive and finite");
+    if ((uint64_t)heads * head_dim > UINT32_MAX)
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "row too wide");
+    if (!pair_axis)
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "pair_axis is required");
+    if (!pool->axes)
+        return set_error(ctx, CKV_E_NO_TABLES, "rope axes before ckv_rope_axes_upload");
+    rotary = (uint32_t)rotary_dim;
+    for (uint32_t j = 0; j < rotary / 2; ++j) {
+        if (pair_axis[j] >= pool->axes)
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT,
+                             "axis of pair " + std::to_string(j) + " was not uploaded");
+        axes.axis[j] = pair_axis[j];
+    }
+    ckv::turn_steps(theta, rotary, turns);
+    return CKV_OK;
+}
+
+} // namespace
+
+int ckv_rope_axes(ckv_pool* pool, const void* input, void* output, size_t heads, float theta,
+                  size_t rotary_dim, const uint8_t* pair_axis, size_t rows)
+{
+    return guarded(pool, [&]() -> int {
+        ckv_context* ctx = pool->ctx;
+        if (rows && (!input || !output))
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT, "input and output are required");
+        if (!pool->uploaded)
+            return set_error(ctx, CKV_E_NO_TABLES, "rope before ckv_tables_upload");
+        if (rows != pool->positions.size())
+            return set_error(ctx, CKV_E_POSITION_COUNT_MISMATCH, "rows != uploaded positions");
+        ckv::turn_table turns;
+        ckv::axis_table axes;
+        uint32_t rotary = 0;
+        if (const int status = check_rope_axes(pool, heads, theta, rotary_dim, pair_axis, turns,
+                                               axes, rotary))
+            return status;
+        const pool_view view = view_of(pool);
+        return run_kernel(ctx, "rope_axes", [&] {
+            return launch_rope_axes(ctx->stream, view, pool->meta, 0,
+                                    { input, output, nullptr, nullptr }, (uint32_t)rows,
+                                    (uint32_t)heads, rotary, turns, axes, pool->d_axes);
+        });
+    });
+}
+
+int ckv_rope_axes_append(ckv_pool* pool, size_t layer, const void* queries, void* rotated,
+                         size_t q_heads, const void* keys, const void* values, float theta,
+                         size_t rotary_dim, const uint8_t* pair_axis, size_t rows)
+{
+    return guarded(pool, [&]() -> int {
+        ckv_context* ctx = pool->ctx;
+        int status = check_slots(pool, layer, keys, values, rows);
+        if (status)
+            return status;
+        if (rows && q_heads && (!queries || !rotated))
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT, "queries and rotated are required");
+        if (rows && (rotated == keys || rotated == values))
+            return set_error(ctx, CKV_E_UNSUPPORTED_ALIASING, "rotated overlaps keys or values");
+        ckv::turn_table turns;
+        ckv::axis_table axes;
+        uint32_t rotary = 0;
+        status = check_rope_axes(pool, q_heads + pool->kv_heads, theta, rotary_dim, pair_axis,
+                                 turns, axes, rotary);
+        if (status)
+            return status;
+        const pool_view view = view_of(pool);
+        return run_kernel(ctx, "rope_axes_append", [&] {
+            return launch_rope_axes(ctx->stream, view, pool->meta, (uint32_t)layer,
+                                    { queries, rotated, keys, values }, (uint32_t)rows,
+                                    (uint32_t)q_heads, rotary, turns, axes, pool->d_axes);
+        });
+    });
+}
+
+int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const int32_t* shift,
+                const uint32_t* counts, size_t n_sequences, float theta, size_t rotary_dim)
+{
+    return guarded(pool, [&]() -> int {
+        ckv_context* ctx = pool->ctx;
+        if (!n_sequences)
+            return CKV_OK;
+        if (!counts)
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT, "counts are required");
+        uint64_t n = 0;
+        for (size_t q = 0; q < n_sequences; ++q)
+            n += counts[q];
+        if (!n)
+            return CKV_OK;
+        if (!from || !to)
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT, "slots are required");
+        if (n > pool->blocks * pool->block_size)
+            return set_error(ctx, CKV_E_UNSUPPORTED_ALIASING, "two moves share a target");
+        ckv::turn_table turns;
+        uint32_t rotary = 0;
+        if (shift) {
+            const size_t width = rotary_dim ? rotary_dim : pool->head_dim;
+            if (width % 2 != 0 || width > pool->head_dim || width / 2 > ckv::max_turn_pairs)
+                return set_error(ctx, CKV_E_INVALID_HEAD_DIMENSION,
+                                 "rotary_dim must be even, <= head_dim and at most "
+                                     + std::to_string(2 * ckv::max_turn_pairs));
+            if (!std::isfinite(theta) || theta <= 0.0f)
+                return set_error(ctx, CKV_E_INVALID_ROPE_THETA,
+                                 "theta must be positive and finite");
+            rotary = (uint32_t)width;
+            ckv::turn_steps(theta, rotary, turns);
+        }
+        std::vector<uint32_t> kept, runs;
+        int status = CKV_OK;
+        if (const char* why = plan_compaction(pool->marks, pool->blocks * pool->block_size, from, to,
+                                              shift, counts, n_sequences, kept, runs, status))
+            return set_error(ctx, status, why);
+        if (kept.empty())
+            return CKV_OK;
+        if (capturing(ctx))
+            return refuse_captured(ctx);
+        // up: runs | from | to | shift
+        const size_t s_from = round4(runs.size()), s_to = s_from + round4(kept.size());
+        const size_t s_shift = s_to + round4(kept.size()), words = s_shift + kept.size();
+        void* host = nullptr;
+        status = stage(ctx, words * sizeof(uint32_t), &host);
+        if (status)
+            return status;
+        auto* w = static_cast<uint32_t*>(host);
+        std::copy(runs.begin(), runs.end(), w);
+        for (size_t k = 0; k < kept.size(); ++k) {
+            w[s_from + k] = from[kept[k]];
+            w[s_to + k] = to[kept[k]];
+            w[s_shift + k] = shift ? (uint32_t)shift[kept[k]] : 0;
+        }
+        status = ensure_device(ctx, &pool->d_pairs, &pool->d_pairs_words, words, "move lists");
+        if (!status)
+            status = upload_staged(ctx, pool->d_pairs, words * sizeof(uint32_t));
+        if (status)
+            return status;
+        const uint32_t* d = pool->d_pairs;
+        const compact_moves moves { d, d + s_from, d + s_to,
+                                    reinterpret_cast<const int32_t*>(d + s_shift),
+                                    (uint32_t)(runs.size() / 2) };
+        const pool_view view = view_of(pool);
+        return run_kernel(ctx, "compact", [&] {
+            return launch_compact(ctx->stream, view, (uint32_t)pool->layers, moves, rotary, turns);
+        });
+    });
 }
 
 int ckv_sigmoid_mul(ckv_context* ctx, int dtype, const void* gate, const void* input,

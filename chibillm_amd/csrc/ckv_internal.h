@@ -76,6 +76,34 @@ struct split_scratch {
     uint32_t* arrivals;
 };
 
+// The keys a row at position p attends: those at t <= p with t > p - window or
+// t < sinks. all_keys: every t <= p.
+struct key_window {
+    uint32_t window; // at least 1: a row attends itself
+    uint32_t sinks;
+};
+constexpr key_window all_keys { UINT32_MAX, 0 };
+
+// The window's first key.
+__host__ __device__ inline uint32_t window_low(uint32_t position, key_window w)
+{
+    return position >= w.window ? position - w.window + 1 : 0;
+}
+
+// Of a row's units of `unit` tokens (tokens, pages or key blocks) in order, those
+// that hold no key it attends: `skip` of them from unit `kept` on. What a kernel
+// walks is the row's other units: unit u < kept as it is, a later one skip on.
+struct window_gap {
+    uint32_t kept, skip;
+};
+__host__ __device__ inline window_gap window_gap_of(uint32_t low, uint32_t sinks, uint32_t unit)
+{
+    const uint32_t first = low / unit; // the window's first unit
+    const uint32_t held = sinks < low ? sinks / unit + (sinks % unit != 0) : first;
+    const uint32_t kept = held < first ? held : first;
+    return { kept, first - kept };
+}
+
 constexpr size_t tile_entry_words = 4;
 
 // Device scratch of a prefill launch whose tiles' key blocks are split
@@ -134,6 +162,20 @@ struct rope_pairs {
     float inv_freq[N];
 };
 
+// Turns of a position's angle on each rotary pair: the fraction of a whole turn
+// by which a step of one position turns the pair, times 2^64, so that a position's
+// angle modulo a turn is one 64-bit product (rope_turns.h). By value as a kernel
+// argument, like rope_table.
+constexpr uint32_t max_turn_pairs = 256;
+struct turn_table {
+    uint64_t step[max_turn_pairs];
+};
+// The axis whose position turns each pair.
+constexpr uint32_t max_axes = 4;
+struct axis_table {
+    uint8_t axis[max_turn_pairs];
+};
+
 // One rotary pair (a, b) -> (a cos - b sin, b cos + a sin), written once with
 // explicit fused multiply-adds for every kernel that rotates (ckv_rope,
 // ckv_rope_append, the fused decode).
@@ -142,6 +184,13 @@ __device__ __forceinline__ void rope_pair(float a, float b, float c, float s, fl
     ra = __builtin_fmaf(a, c, -(b * s));
     rb = __builtin_fmaf(b, c, a * s);
 }
+
+// The moves of a compaction that read each slot (the first and the last), and
+// whether one writes it, by the generation of the call that marked them.
+struct move_marks {
+    std::vector<uint32_t> read, first, last, written;
+    uint32_t generation = 0;
+};
 
 struct pending_timing {
     const char* name;
@@ -224,6 +273,7 @@ struct ckv_pool {
     size_t n_entries = 0; // entries of the table the rows index
     size_t slot_rows = 0; // rows with an uploaded slot (0 without slots)
     std::vector<uint32_t> positions;
+    uint32_t last_position = 0; // the largest of them
     std::vector<uint32_t> row_offsets; // each row's table offset (the decode plan's entries)
     bool shared_tile = false;
     bool fusable = false; // slots are the rows' own positions, one row per table range
@@ -265,6 +315,27 @@ struct ckv_pool {
     size_t seq_max = 0, seq_cap = 0;
     std::vector<uint32_t> seq_len, seq_host, dirty;
     std::vector<uint8_t> seq_dirty;
+
+    // The current batch through a window: the same rows with the plan and work
+    // list of what the window leaves of them, derived at the first launch with it
+    // and kept until another window or batch comes.
+    ckv::key_window window = ckv::all_keys;
+    bool window_plan_ready = false;
+    bool window_work_ready = false;
+    bool window_work_multi = false;
+    std::vector<uint32_t> window_positions; // positions less the tokens of the skipped pages
+    ckv::meta_view window_meta {};
+    uint32_t* d_window_plan = nullptr;
+    size_t d_window_plan_words = 0;
+    uint32_t* d_window_work = nullptr;
+    size_t d_window_work_words = 0;
+
+    // the batch rows' positions on several axes ([axes][rows], ckv_rope_axes_upload)
+    uint32_t axes = 0;
+    uint32_t* d_axes = nullptr;
+    size_t d_axes_words = 0;
+
+    ckv::move_marks marks; // of ckv_compact's slots
 
     // device scratch
     float* d_partials = nullptr;
@@ -366,7 +437,7 @@ void write_decode_plan(const std::vector<uint32_t>& positions,
 hipError_t launch_decode(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
                          const void* q, uint32_t q_heads, float scale, void* out,
                          float* partials, int cu_count, const void* gate = nullptr,
-                         split_scratch split = {});
+                         split_scratch split = {}, key_window window = all_keys);
 bool decode_fast_applies(const pool_view& p, uint32_t q_heads, const void* q, const void* out);
 // store_kv + fast decode in one launch; the caller has checked
 // decode_fast_applies, 16-byte aligned inputs, and that every row's slot is
@@ -381,6 +452,9 @@ hipError_t launch_append_decode(hipStream_t s, const pool_view& p, const meta_vi
 hipError_t launch_merge(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t q_heads,
                         void* out, const float* partials, const void* gate = nullptr);
 bool decode_uses_fast_path(const pool_view& p, uint32_t q_heads);
+// Sets every entry of a plan written from the window's positions to its row's position.
+void place_window_plan(const std::vector<uint32_t>& positions, const decode_plan_shape& shape,
+                       uint32_t* plan);
 // Floats per (work item, q head) partial record: [max, denominator, 0, 0, acc[head_dim]].
 uint32_t partial_record_floats(uint32_t head_dim);
 
@@ -426,5 +500,46 @@ hipError_t launch_rope(hipStream_t s, const pool_view& p, const meta_view& m, co
 hipError_t launch_rope_append(hipStream_t s, const pool_view& p, const meta_view& m,
                               uint32_t layer, const void* keys, const void* values, uint32_t rows,
                               uint32_t rotary, const rope_table& freq);
+
+// ---- launchers (kernels_rope_axes.hip) ----------------------------------------------
+// theta^(-2j/rotary) of a radian per position, as turn_table's steps
+void turn_steps(float theta, uint32_t rotary, turn_table& out);
+// Query rows [rows, q_heads, head_dim] rotated into `rotated` and, with keys, key
+// rows rotated and value rows copied into the uploaded slots of `layer`; pair j
+// turns by positions[axis[j]][row]. q_heads 0: keys and values alone.
+struct axes_rows {
+    const void* queries;
+    void* rotated;
+    const void* keys;
+    const void* values;
+};
+hipError_t launch_rope_axes(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
+                            const axes_rows& x, uint32_t rows, uint32_t q_heads, uint32_t rotary,
+                            const turn_table& turns, const axis_table& axes,
+                            const uint32_t* positions);
+
+// ---- launchers (kernels_compact.hip) --------------------------------------------------
+// Moves of a compaction on the device: `runs` holds n_runs (first move, moves), each
+// run's moves in order, and the moves' source slots, target slots and position
+// shifts. A run's moves may overwrite what the same run reads at or before them;
+// nothing a run reads or writes is written by another.
+struct compact_moves {
+    const uint32_t* runs;
+    const uint32_t* from;
+    const uint32_t* to;
+    const int32_t* shift;
+    uint32_t n_runs;
+};
+// Checks the moves of ckv_compact and cuts them into runs. `kept` are the moves that
+// change something, `runs` pairs (first of kept, how many): a sequence whose targets
+// no other move reads is cut into runs of at most compact_run moves, another stays
+// one run. Returns null, or why the moves are refused, with the status.
+constexpr uint32_t compact_run = 64;
+const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* from,
+                            const uint32_t* to, const int32_t* shift, const uint32_t* counts,
+                            size_t n_sequences, std::vector<uint32_t>& kept,
+                            std::vector<uint32_t>& runs, int& status);
+hipError_t launch_compact(hipStream_t s, const pool_view& p, uint32_t layers,
+                          const compact_moves& moves, uint32_t rotary, const turn_table& turns);
 
 } // namespace ckv

@@ -1039,7 +1039,8 @@ __global__ __launch_bounds__(64) void decode_generic_kernel(pool_view p, meta_vi
                                                             uint32_t q_heads, float scale_log2,
                                                             void* __restrict__ out,
                                                             float* __restrict__ partials,
-                                                            const void* __restrict__ gate)
+                                                            const void* __restrict__ gate,
+                                                            key_window window)
 {
     constexpr int NF = generic_max_features_per_lane;
     const uint32_t H = p.kv_heads;
@@ -1050,8 +1051,10 @@ __global__ __launch_bounds__(64) void decode_generic_kernel(pool_view p, meta_vi
     const uint32_t chunk_index = m.items[2 * item + 1];
     const uint32_t position = m.positions[row];
     const uint32_t table_base = m.offsets[row];
+    // the row's keys in order, without those its window skips
+    const window_gap gap = window_gap_of(window_low(position, window), window.sinks, 1);
     const uint32_t begin = chunk_index * m.chunk;
-    const uint32_t end = min(position + 1, begin + m.chunk);
+    const uint32_t end = min(position + 1 - gap.skip, begin + m.chunk);
     const uint32_t lane = threadIdx.x;
     const uint32_t G = q_heads / H;
     const uint32_t bs = p.block_size;
@@ -1068,8 +1071,10 @@ __global__ __launch_bounds__(64) void decode_generic_kernel(pool_view p, meta_vi
             qf[k] = f < D ? load_elem<DT>(q, q_base + f) : 0.0f;
             acc[k] = 0.0f;
         }
-        float mx = -INFINITY, den = 0.0f;
-        for (uint32_t t = begin; t < end; ++t) {
+        // (the lowest finite maximum: a score of -inf weighs 0 also where it comes first)
+        float mx = -FLT_MAX, den = 0.0f;
+        for (uint32_t i = begin; i < end; ++i) {
+            const uint32_t t = i < gap.kept ? i : i + gap.skip;
             const uint64_t slot = (uint64_t)m.table[table_base + t / bs] * bs + t % bs;
             const uint64_t base = ((uint64_t)layer * slot_count + slot) * p.features + kv_head * D;
             float d = 0.0f;
@@ -1734,12 +1739,13 @@ bool decode_fast_applies(const pool_view& p, uint32_t q_heads, const void* q, co
 
 hipError_t launch_decode(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
                          const void* q, uint32_t q_heads, float scale, void* out,
-                         float* partials, int cu_count, const void* gate, split_scratch split)
+                         float* partials, int cu_count, const void* gate, split_scratch split,
+                         key_window window)
 {
     if (!m.rows)
         return hipSuccess;
     const float scale_log2 = scale * log2e;
-    if (decode_fast_applies(p, q_heads, q, out)) {
+    if (window.window == all_keys.window && decode_fast_applies(p, q_heads, q, out)) {
         const void* no_row = nullptr;
         return launch_width(p.head_dim, q_heads / p.kv_heads, s, p, m, layer, q, q_heads,
                             scale_log2, out, p.dtype, no_row, no_row, gate, cu_count, split);
@@ -1750,15 +1756,15 @@ hipError_t launch_decode(hipStream_t s, const pool_view& p, const meta_view& m, 
     switch (p.dtype) {
     case CKV_F32:
         decode_generic_kernel<CKV_F32><<<grid, block, 0, s>>>(p, m, layer, q, q_heads, scale_log2,
-                                                              out, partials, gate);
+                                                              out, partials, gate, window);
         break;
     case CKV_BF16:
         decode_generic_kernel<CKV_BF16><<<grid, block, 0, s>>>(p, m, layer, q, q_heads,
-                                                               scale_log2, out, partials, gate);
+                                                               scale_log2, out, partials, gate, window);
         break;
     default:
         decode_generic_kernel<CKV_F16><<<grid, block, 0, s>>>(p, m, layer, q, q_heads, scale_log2,
-                                                              out, partials, gate);
+                                                              out, partials, gate, window);
         break;
     }
     return hipGetLastError();
@@ -1795,6 +1801,13 @@ hipError_t launch_merge(hipStream_t s, const pool_view& p, const meta_view& m, u
         break;
     }
     return hipGetLastError();
+}
+
+void place_window_plan(const std::vector<uint32_t>& positions, const decode_plan_shape& shape,
+                       uint32_t* plan)
+{
+    for (size_t i = 0; i < shape.n_items; ++i)
+        plan[plan_entry_words * i + 2] = positions[plan[plan_entry_words * i]];
 }
 
 uint32_t partial_record_floats(uint32_t head_dim)

@@ -138,7 +138,9 @@ int ckv_copy_to_host(ckv_context* ctx, void* host_dst, const void* device_src, s
  * "paged_attention_prefill", "copy_blocks", "checkpoint_pack",
  * "checkpoint_unpack", "tables_patch", "tables_fill", "batch_expand", "rope",
  * "rope_append", "rope_append_decode", "sigmoid_mul", "checkpoint_export",
- * "checkpoint_import". */
+ * "checkpoint_import", "window_attention_decode", "window_attention_prefill",
+ * "append_decode_window", "rope_append_decode_window", "rope_axes",
+ * "rope_axes_append", "compact". */
 int ckv_profile_enable(ckv_context* ctx, int enabled);
 int ckv_profile_query(ckv_context* ctx, const char* kernel, double* total_ms,
                       uint64_t* launches);
@@ -365,6 +367,45 @@ int ckv_append_decode_gated(ckv_pool* pool, size_t layer, const void* keys, cons
 int ckv_sigmoid_mul(ckv_context* ctx, int dtype, const void* gate, const void* input,
                     void* output, size_t count);
 
+/* ---- Attention through a window, with sinks ------------------------------------------
+ * No counterpart in the reference: attention for contexts longer than what a
+ * layer reads of them. A row at position p attends key t when t <= p and
+ * (t > p - window or t < sinks): the last `window` tokens, itself among them,
+ * and the sequence's first `sinks`. output = softmax(q . k * scale) . v over
+ * those, with fp32 accumulation. window must be at least 1 (invalid_argument);
+ * any larger value, and any sinks from 0 on, are taken.
+ * Pages that hold no key a row attends are not read, whatever is in them: a
+ * sequence may give them back, as long as its table keeps some page id of the
+ * pool in their place. Keys outside the window in pages that are read weigh
+ * nothing, whatever their values.
+ * Each batch keeps the work lists of one window at a time; a layer's calls with
+ * the same window reuse them, a call with another replaces them (one small
+ * upload). A call on a stream under capture is refused (invalid_argument) when
+ * it would upload or allocate: make it once on the batch before the capture.
+ * gate may be NULL; otherwise as ckv_attention_gated's, and it must not be the
+ * queries' or the output's memory (unsupported_aliasing). */
+
+/* The rows of the current batch, prefill tiles or decode rows, as ckv_attention
+ * selects. Checks: those of ckv_attention, then the window and the gate.
+ * Profile names "window_attention_decode", "window_attention_prefill". */
+int ckv_attention_window(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads,
+                         float scale, size_t window, size_t sinks, const void* gate, void* output,
+                         size_t rows);
+/* ckv_append then ckv_attention_window of decode rows, in one launch where
+ * ckv_append_decode's applies. Checks: those of ckv_append, then those of
+ * ckv_attention_window. Profile name "append_decode_window". */
+int ckv_append_decode_window(ckv_pool* pool, size_t layer, const void* keys, const void* values,
+                             const void* queries, size_t q_heads, float scale, size_t window,
+                             size_t sinks, const void* gate, void* output, size_t rows);
+/* The same from unrotated queries and keys, as ckv_rope_append_decode: keys are
+ * rotated by their batch positions, whatever the window. Checks: those of
+ * ckv_append_decode_window, then those of ckv_rope (with q_heads). Profile name
+ * "rope_append_decode_window". */
+int ckv_rope_append_decode_window(ckv_pool* pool, size_t layer, const void* keys,
+                                  const void* values, const void* queries, size_t q_heads,
+                                  float scale, float theta, size_t rotary_dim, size_t window,
+                                  size_t sinks, const void* gate, void* output, size_t rows);
+
 /* ---- Rotary position embedding ------------------------------------------------------ */
 /* rope (src/tensor/tensor_ops.cc:356-410; kernel rope_f32,
  * src/metal/kernels/tensor_ops.metal:158-195) on device rows
@@ -404,6 +445,53 @@ int ckv_rope_append(ckv_pool* pool, size_t layer, const void* keys, const void* 
 int ckv_rope_append_decode(ckv_pool* pool, size_t layer, const void* keys, const void* values,
                            const void* queries, size_t q_heads, float scale, float theta,
                            size_t rotary_dim, const void* gate, void* output, size_t rows);
+
+/* ---- Rotary positions on several axes ------------------------------------------------
+ * No counterpart in the reference: tokens of images and video have a position in
+ * time, height and width, apart from their place in the cache. Within every head,
+ * pair j < rotary_dim/2 rotates elements j and j + rotary_dim/2 by
+ * position[pair_axis[j]] * theta^(-2j/rotary_dim); the rest is copied. pair_axis is a
+ * host array of rotary_dim/2 axes (sections one after another, or taken in turn).
+ * Angles are reduced exactly (64-bit fractions of a turn), at any 32-bit position. */
+
+/* The current batch's positions on 1 to 4 axes, host [axes][rows]: axis a of row r at
+ * positions[a * rows + r]. They hold until the next batch is uploaded. Checks:
+ * invalid_argument (axes, a null array, a stream under capture), no_tables,
+ * position_count_mismatch (rows != uploaded rows). */
+int ckv_rope_axes_upload(ckv_pool* pool, const uint32_t* positions, size_t axes, size_t rows);
+/* Device rows [rows, heads*head_dim] of the pool dtype; input may equal output (in
+ * place) but not overlap it otherwise. rotary_dim 0 means head_dim; at most 512.
+ * Checks: those of ckv_rope, then invalid_argument (no pair_axis, or an axis not
+ * uploaded) and no_tables (before ckv_rope_axes_upload). */
+int ckv_rope_axes(ckv_pool* pool, const void* input, void* output, size_t heads, float theta,
+                  size_t rotary_dim, const uint8_t* pair_axis, size_t rows);
+/* One launch for a layer's rows before its attention: query rows rotated into
+ * `rotated` (which may be queries, but no other argument), key rows rotated and value
+ * rows copied into the uploaded slots of `layer`. q_heads 0: keys and values alone.
+ * Checks: those of ckv_append, the queries' (invalid_argument), unsupported_aliasing
+ * (rotated is keys or values), then those of ckv_rope_axes. */
+int ckv_rope_axes_append(ckv_pool* pool, size_t layer, const void* queries, void* rotated,
+                         size_t q_heads, const void* keys, const void* values, float theta,
+                         size_t rotary_dim, const uint8_t* pair_axis, size_t rows);
+
+/* ---- Compaction ------------------------------------------------------------------------
+ * No counterpart in the reference: a cache that has to drop tokens moves those it keeps
+ * together, so that the pages behind them can be given back. For every layer, move i
+ * copies the K and V rows of slot from[i] to slot to[i]; with shift, the key's pairs
+ * (as ckv_rope's, over rotary_dim; 0: head_dim, at most 512) turn by shift[i] *
+ * theta^(-2j/rotary_dim): a key cached at position p becomes the key at p + shift[i],
+ * rounded once more. Values, and keys with shift 0 or without shift, are copied bit for
+ * bit. Slots are those of ckv_tables_upload (block * block_size + offset).
+ * The moves of sequence q are counts[q] consecutive ones. All targets are distinct. A
+ * slot may be both read and written (in place) if its write comes at or after every
+ * move that reads it, within one sequence: kept tokens moving towards the front, in
+ * order, are such moves. Nothing else is changed; the tables are the caller's.
+ * Checks, before anything changes: invalid_argument (a null array, a stream under
+ * capture), invalid_head_dimension and invalid_rope_theta (with shift),
+ * cache_slot_out_of_range, unsupported_aliasing (a repeated target, or one that a later
+ * move or another sequence reads). Profile name "compact". */
+int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const int32_t* shift,
+                const uint32_t* counts, size_t n_sequences, float theta, size_t rotary_dim);
 
 /* ---- Pages: copy-on-write and checkpoints ------------------------------------------ */
 /* For every layer, keys and values: page dst[i] := page src[i]. The copy-on-write

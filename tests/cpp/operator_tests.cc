@@ -1,0 +1,273 @@
+// Windowed attention, rotation on several axes and compaction on the CPU: the window's
+// arithmetic against its definition, the fixed-point turns against long doubles, the
+// runs that moves are cut into, and what the entry points refuse (over a pool without
+// a GPU: every call here ends in its checks).
+#include <algorithm>
+#include <cmath>
+#include <random>
+
+#include "check.h"
+#include "ckv_internal.h"
+
+namespace {
+
+using namespace ckv;
+
+bool attends(uint32_t p, uint32_t t, key_window w)
+{
+    return t <= p && ((uint64_t)t + w.window > p || t < w.sinks);
+}
+
+// The units that a kernel walks are those with a key the row attends, in order.
+TEST("window: the units walked are those with a key the row attends")
+{
+    for (const uint32_t unit : { 1u, 8u, 16u, 32u })
+        for (const uint32_t window : { 1u, 2u, 7u, 15u, 16u, 17u, 40u, 64u, 300u, UINT32_MAX })
+            for (const uint32_t sinks : { 0u, 1u, 4u, 15u, 16u, 17u, 33u, 250u, UINT32_MAX })
+                for (uint32_t p = 0; p < 280; p = p < 70 ? p + 1 : p + 13) {
+                    const key_window w { window, sinks };
+                    const window_gap gap = window_gap_of(window_low(p, w), sinks, unit);
+                    const uint32_t units = p / unit + 1;
+                    REQUIRE(gap.kept + gap.skip < units);
+                    for (uint32_t u = 0; u < units; ++u) {
+                        bool some = false;
+                        for (uint32_t t = u * unit; t < (u + 1) * unit; ++t)
+                            some = some || attends(p, t, w);
+                        const bool walked = u < gap.kept || u >= gap.kept + gap.skip;
+                        CHECK(walked == some);
+                    }
+                }
+    // positions near the type's end
+    const key_window w { 100, 4 };
+    CHECK(window_low(0xFFFFFFF0u, w) == 0xFFFFFFF0u - 99u);
+    CHECK(window_low(99, w) == 0);
+    CHECK(window_low(100, w) == 1);
+    CHECK(window_low(0xFFFFFFF0u, all_keys) == 0);
+}
+
+// A position's turn, as the device takes it from the steps, within 2^-32 of a turn of
+// the angle in long double, for positions as far as 32 bits go.
+TEST("rope axes: fixed-point turns match long doubles at every position")
+{
+    const long double two_pi = 2.0L * 3.14159265358979323846264338327950288L;
+    for (const float theta : { 1e4f, 1e6f, 1e7f, 2.5f, 0.5f })
+        for (const uint32_t rotary : { 2u, 16u, 64u, 128u, 512u }) {
+            turn_table t {};
+            turn_steps(theta, rotary, t);
+            for (uint32_t j = 0; j < rotary / 2; j += rotary > 64 ? 7 : 1) {
+                const long double step = std::pow((long double)theta, -2.0L * j / rotary) / two_pi;
+                for (const int64_t p : { 0LL, 1LL, 2LL, 1000LL, 131071LL, 5000011LL, -1LL, -4096LL, 4294967295LL }) {
+                    const uint64_t turn = t.step[j] * (uint64_t)p;
+                    const long double got = (long double)turn / 0x1p64L;
+                    // step * p in long double is good to |p| 2^-62 of a turn
+                    long double off = got - (step * p - std::floor(step * p));
+                    off -= std::round(off);
+                    CHECK(std::fabs(off) < 0x1p-32L + std::fabs((long double)p) * 0x1p-55L * (step > 1 ? step : 1));
+                }
+            }
+        }
+}
+
+struct plan {
+    std::vector<uint32_t> kept, runs;
+    int status = -1;
+    bool refused = false;
+};
+
+plan compaction(move_marks& marks, size_t slots, const std::vector<uint32_t>& from,
+                const std::vector<uint32_t>& to, const std::vector<uint32_t>& counts,
+                const int32_t* shift = nullptr)
+{
+    plan p;
+    p.refused = plan_compaction(marks, slots, from.data(), to.data(), shift, counts.data(),
+                                counts.size(), p.kept, p.runs, p.status) != nullptr;
+    return p;
+}
+
+// Runs done concurrently, each in its order, leave what all reads before all writes do.
+TEST("compaction: concurrent runs leave what reads before writes do")
+{
+    std::mt19937_64 rng(7);
+    move_marks marks;
+    for (int trial = 0; trial < 300; ++trial) {
+        const uint32_t slots = 600;
+        std::vector<uint32_t> order(slots), from, to, counts;
+        for (uint32_t i = 0; i < slots; ++i)
+            order[i] = i;
+        std::shuffle(order.begin(), order.end(), rng);
+        for (uint32_t q = 0; q < 3; ++q) { // a sequence: 200 slots of its own
+            const uint32_t* at = order.data() + 200 * q;
+            uint32_t n = 0;
+            const bool fresh = rng() % 3 == 0;
+            const uint32_t of = fresh ? 100 : 200;
+            for (uint32_t t = 0; t < of; ++t)
+                if (rng() % 5) {
+                    from.push_back(at[t]);
+                    to.push_back(at[fresh ? 100 + n : n]);
+                    ++n;
+                }
+            counts.push_back(n);
+        }
+        const plan p = compaction(marks, slots, from, to, counts);
+        REQUIRE(!p.refused && p.status == CKV_OK);
+        std::vector<uint32_t> want(slots), got(slots);
+        for (uint32_t i = 0; i < slots; ++i)
+            want[i] = got[i] = 1000 + i;
+        for (size_t i = 0; i < from.size(); ++i)
+            want[to[i]] = 1000 + from[i];
+        // the runs in a random interleaving of their moves
+        std::vector<size_t> next(p.runs.size() / 2, 0);
+        size_t left = p.kept.size();
+        std::vector<int> done(from.size(), 0);
+        while (left) {
+            const size_t r = rng() % next.size();
+            if (next[r] == p.runs[2 * r + 1])
+                continue;
+            const uint32_t i = p.kept[p.runs[2 * r] + next[r]++];
+            REQUIRE(!done[i]);
+            done[i] = 1;
+            got[to[i]] = got[from[i]];
+            --left;
+        }
+        CHECK(got == want);
+    }
+}
+
+TEST("compaction: unsafe moves are refused")
+{
+    move_marks marks;
+    const size_t n = 64;
+    CHECK(compaction(marks, n, { 3, 64 }, { 1, 2 }, { 2 }).status == CKV_E_CACHE_SLOT_OUT_OF_RANGE);
+    CHECK(compaction(marks, n, { 3, 4 }, { 1, 99 }, { 2 }).status == CKV_E_CACHE_SLOT_OUT_OF_RANGE);
+    CHECK(compaction(marks, n, { 3, 4 }, { 1, 1 }, { 2 }).status == CKV_E_UNSUPPORTED_ALIASING);
+    // a target read by a later move, and by another sequence before or after it
+    CHECK(compaction(marks, n, { 3, 4 }, { 4, 5 }, { 2 }).status == CKV_E_UNSUPPORTED_ALIASING);
+    CHECK(compaction(marks, n, { 3, 4 }, { 4, 5 }, { 1, 1 }).status == CKV_E_UNSUPPORTED_ALIASING);
+    CHECK(compaction(marks, n, { 3, 4 }, { 5, 3 }, { 1, 1 }).status == CKV_E_UNSUPPORTED_ALIASING);
+    // towards the front, and one slot read twice
+    CHECK(compaction(marks, n, { 3, 4 }, { 2, 3 }, { 2 }).status == CKV_OK);
+    CHECK(compaction(marks, n, { 3, 3 }, { 1, 2 }, { 2 }).status == CKV_OK);
+    // an exchange is none: its second move reads what the first wrote
+    CHECK(compaction(marks, n, { 3, 4 }, { 4, 3 }, { 2 }).status == CKV_E_UNSUPPORTED_ALIASING);
+    // moves that change nothing are left out; with a shift they are not
+    CHECK(compaction(marks, n, { 3, 4 }, { 3, 4 }, { 2 }).kept.empty());
+    const int32_t shift[] = { 0, -2 };
+    CHECK(compaction(marks, n, { 3, 4 }, { 3, 4 }, { 2 }, shift).kept == std::vector<uint32_t> { 1 });
+    // the generation's wrap forgets old marks
+    marks.generation = UINT32_MAX;
+    CHECK(compaction(marks, n, { 3, 4 }, { 2, 3 }, { 2 }).status == CKV_OK);
+    CHECK(marks.generation == 1);
+}
+
+// Every argument that the entry points refuse, over a batch of two rows.
+TEST("entry points: what is refused")
+{
+    ckv_context ctx;
+    ckv_pool pool;
+    pool.ctx = &ctx;
+    pool.layers = 2;
+    pool.blocks = 8;
+    pool.block_size = 16;
+    pool.kv_heads = 2;
+    pool.head_dim = 128;
+    int x[4]; // never read: no call gets that far
+    void *k = x, *v = x + 1, *q = x + 2, *o = x + 3;
+    const size_t rows = 2;
+    auto attend = [&](size_t layer, const void* q, size_t heads, size_t window, const void* gate,
+                      void* out, size_t n) {
+        return ckv_attention_window(&pool, layer, q, heads, 1.0f, window, 4, gate, out, n);
+    };
+    CHECK(ckv_attention_window(nullptr, 0, q, 4, 1.0f, 8, 0, nullptr, o, 1) == CKV_E_INVALID_ARGUMENT);
+    CHECK(attend(0, q, 4, 8, nullptr, o, rows) == CKV_E_NO_TABLES);
+    CHECK(ckv_rope_axes_upload(&pool, nullptr, 3, rows) == CKV_E_INVALID_ARGUMENT);
+    const uint32_t positions[8] = {};
+    CHECK(ckv_rope_axes_upload(&pool, positions, 3, rows) == CKV_E_NO_TABLES);
+    pool.uploaded = true;
+    pool.positions = { 40, 50 };
+    pool.last_position = 50;
+    CHECK(attend(0, nullptr, 4, 8, nullptr, o, rows) == CKV_E_INVALID_ARGUMENT);
+    CHECK(attend(0, q, 4, 8, nullptr, nullptr, rows) == CKV_E_INVALID_ARGUMENT);
+    CHECK(attend(0, q, 4, 8, nullptr, o, 3) == CKV_E_POSITION_COUNT_MISMATCH);
+    CHECK(attend(0, q, 0, 8, nullptr, o, rows) == CKV_E_INVALID_HEAD_COUNT);
+    CHECK(attend(0, q, 3, 8, nullptr, o, rows) == CKV_E_INVALID_KV_HEAD_MAPPING);
+    CHECK(attend(2, q, 4, 8, nullptr, o, rows) == CKV_E_CACHE_LAYER_OUT_OF_RANGE);
+    CHECK(attend(0, q, 4, 0, nullptr, o, rows) == CKV_E_INVALID_ARGUMENT);
+    CHECK(attend(0, q, 4, 8, q, o, rows) == CKV_E_UNSUPPORTED_ALIASING);
+    CHECK(attend(0, q, 4, 8, o, o, rows) == CKV_E_UNSUPPORTED_ALIASING);
+    auto append = [&](size_t layer, const void* k, const void* v, size_t window, size_t n) {
+        const int a = ckv_append_decode_window(&pool, layer, k, v, q, 4, 1.0f, window, 4, nullptr, o, n);
+        const int b = ckv_rope_append_decode_window(&pool, layer, k, v, q, 4, 1.0f, 1e4f, 0, window, 4,
+                                                    nullptr, o, n);
+        CHECK(a == b);
+        return a;
+    };
+    CHECK(append(0, k, v, 8, rows) == CKV_E_NO_TABLES); // no slots
+    pool.has_slots = true;
+    pool.slot_rows = rows;
+    CHECK(append(0, nullptr, v, 8, rows) == CKV_E_INVALID_ARGUMENT);
+    CHECK(append(0, k, nullptr, 8, rows) == CKV_E_INVALID_ARGUMENT);
+    CHECK(append(0, k, v, 8, 3) == CKV_E_CACHE_SLOT_COUNT_MISMATCH);
+    CHECK(append(2, k, v, 8, rows) == CKV_E_CACHE_LAYER_OUT_OF_RANGE);
+    CHECK(append(0, k, v, 0, rows) == CKV_E_INVALID_ARGUMENT);
+    auto rope_window = [&](float theta, size_t rotary) {
+        return ckv_rope_append_decode_window(&pool, 0, k, v, q, 4, 1.0f, theta, rotary, 8, 4, nullptr,
+                                             o, rows);
+    };
+    CHECK(rope_window(0.0f, 0) == CKV_E_INVALID_ROPE_THETA);
+    CHECK(rope_window(1e4f, 3) == CKV_E_INVALID_HEAD_DIMENSION);
+
+    CHECK(ckv_rope_axes_upload(&pool, positions, 0, rows) == CKV_E_INVALID_ARGUMENT);
+    CHECK(ckv_rope_axes_upload(&pool, positions, 5, rows) == CKV_E_INVALID_ARGUMENT);
+    CHECK(ckv_rope_axes_upload(&pool, positions, 3, 1) == CKV_E_POSITION_COUNT_MISMATCH);
+    uint8_t axis[64] = {};
+    auto axes = [&](size_t heads, float theta, size_t rotary, const uint8_t* a, size_t n = rows) {
+        const int one = ckv_rope_axes(&pool, q, o, heads, theta, rotary, a, n);
+        return one;
+    };
+    CHECK(axes(4, 1e4f, 0, axis) == CKV_E_NO_TABLES); // before the upload
+    pool.axes = 3;
+    CHECK(axes(4, 1e4f, 0, axis, 3) == CKV_E_POSITION_COUNT_MISMATCH);
+    CHECK(axes(0, 1e4f, 0, axis) == CKV_E_INVALID_HEAD_COUNT);
+    CHECK(axes(4, 1e4f, 130, axis) == CKV_E_INVALID_HEAD_DIMENSION);
+    CHECK(axes(4, 1e4f, 7, axis) == CKV_E_INVALID_HEAD_DIMENSION);
+    CHECK(axes(4, -1.0f, 0, axis) == CKV_E_INVALID_ROPE_THETA);
+    CHECK(axes(4, INFINITY, 0, axis) == CKV_E_INVALID_ROPE_THETA);
+    CHECK(axes(4, 1e4f, 0, nullptr) == CKV_E_INVALID_ARGUMENT);
+    axis[63] = 3;
+    CHECK(axes(4, 1e4f, 0, axis) == CKV_E_INVALID_ARGUMENT);
+    auto axes_append = [&](const void* queries, void* rotated, size_t heads, const void* keys) {
+        return ckv_rope_axes_append(&pool, 0, queries, rotated, heads, keys, v, 1e4f, 0, axis, rows);
+    };
+    CHECK(axes_append(q, o, 4, k) == CKV_E_INVALID_ARGUMENT); // axis 3 again
+    axis[63] = 0;
+    CHECK(axes_append(nullptr, o, 4, k) == CKV_E_INVALID_ARGUMENT);
+    CHECK(axes_append(q, nullptr, 4, k) == CKV_E_INVALID_ARGUMENT);
+    CHECK(axes_append(q, k, 4, k) == CKV_E_UNSUPPORTED_ALIASING);
+    CHECK(axes_append(q, v, 4, k) == CKV_E_UNSUPPORTED_ALIASING);
+    pool.head_dim = 1024;
+    CHECK(axes(4, 1e4f, 0, axis) == CKV_E_INVALID_HEAD_DIMENSION);
+    pool.head_dim = 128;
+
+    const uint32_t from[] = { 5, 6 }, to[] = { 1, 2 }, counts[] = { 2 };
+    const int32_t shift[] = { -4, -4 };
+    CHECK(ckv_compact(nullptr, from, to, shift, counts, 1, 1e4f, 0) == CKV_E_INVALID_ARGUMENT);
+    CHECK(ckv_compact(&pool, from, to, shift, nullptr, 1, 1e4f, 0) == CKV_E_INVALID_ARGUMENT);
+    CHECK(ckv_compact(&pool, nullptr, to, shift, counts, 1, 1e4f, 0) == CKV_E_INVALID_ARGUMENT);
+    CHECK(ckv_compact(&pool, from, nullptr, shift, counts, 1, 1e4f, 0) == CKV_E_INVALID_ARGUMENT);
+    CHECK(ckv_compact(&pool, from, to, shift, counts, 1, 0.0f, 0) == CKV_E_INVALID_ROPE_THETA);
+    CHECK(ckv_compact(&pool, from, to, shift, counts, 1, 1e4f, 129) == CKV_E_INVALID_HEAD_DIMENSION);
+    CHECK(ckv_compact(&pool, from, to, shift, counts, 1, 1e4f, 256) == CKV_E_INVALID_HEAD_DIMENSION);
+    const uint32_t far[] = { 5, 128 }, same[] = { 1, 1 };
+    CHECK(ckv_compact(&pool, far, to, nullptr, counts, 1, 0.0f, 0) == CKV_E_CACHE_SLOT_OUT_OF_RANGE);
+    CHECK(ckv_compact(&pool, from, same, nullptr, counts, 1, 0.0f, 0) == CKV_E_UNSUPPORTED_ALIASING);
+    const uint32_t many[] = { UINT32_MAX, UINT32_MAX };
+    CHECK(ckv_compact(&pool, from, to, nullptr, many, 2, 0.0f, 0) == CKV_E_UNSUPPORTED_ALIASING);
+    // nothing to do
+    const uint32_t none[] = { 0 };
+    CHECK(ckv_compact(&pool, nullptr, nullptr, nullptr, none, 1, 0.0f, 0) == CKV_OK);
+    CHECK(ckv_compact(&pool, from, from, nullptr, counts, 1, 0.0f, 0) == CKV_OK);
+    pool.positions.clear();
+    CHECK(attend(0, nullptr, 4, 8, nullptr, nullptr, 0) == CKV_OK);
+}
+
+} // namespace
