@@ -365,16 +365,15 @@ size_t plan_words(const decode_plan_shape& shape, size_t rows)
     return round4(plan_entry_words * shape.n_items) + round4(rows) + shape.n_cut;
 }
 
-// Writes the plan at `words` (plan_words long) and points the batch's
-// meta_view at `device`, its device copy.
-void put_plan(ckv_pool* pool, const decode_plan_shape& shape, uint32_t* words,
-              const uint32_t* device)
+// Writes the plan of rows at `positions` at `words` (plan_words long) and points
+// `m` at `device`, its device copy.
+void put_plan(ckv_pool* pool, const std::vector<uint32_t>& positions, meta_view& m,
+              const decode_plan_shape& shape, uint32_t* words, const uint32_t* device)
 {
     const size_t s_first = round4(plan_entry_words * shape.n_items);
-    const size_t s_cut = s_first + round4(pool->positions.size());
-    write_decode_plan(pool->positions, pool->row_offsets, (uint32_t)pool->block_size, shape,
+    const size_t s_cut = s_first + round4(positions.size());
+    write_decode_plan(positions, pool->row_offsets, (uint32_t)pool->block_size, shape,
                       pool->sort_keys, words, words + s_first, words + s_cut);
-    meta_view& m = pool->meta;
     m.plan = device;
     m.split_first = device + s_first;
     m.cut = device + s_cut;
@@ -403,12 +402,31 @@ int ensure_plan(ckv_pool* pool)
     status = ensure_device(ctx, &pool->d_plan, &pool->d_plan_words, words, "decode plan");
     if (status)
         return status;
-    put_plan(pool, shape, static_cast<uint32_t*>(host), pool->d_plan);
+    put_plan(pool, pool->positions, pool->meta, shape, static_cast<uint32_t*>(host), pool->d_plan);
     status = upload_staged(ctx, pool->d_plan, words * sizeof(uint32_t));
     if (status)
         return status;
     pool->plan_ready = true;
     return CKV_OK;
+}
+
+// Whether the context's stream is being captured into a graph (or cannot be asked
+// while another is): a launch there takes no upload and no allocation, whose replays
+// would read staging memory of other uploads or free what a graph uses.
+bool capturing(const ckv_context* ctx)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing(ctx->stream, &status);
+    if (e != hipSuccess)
+        (void)hipGetLastError();
+    return e != hipSuccess || status != hipStreamCaptureStatusNone;
+}
+
+int refuse_captured(ckv_context* ctx)
+{
+    return set_error(ctx, CKV_E_INVALID_ARGUMENT,
+                     "the stream is being captured and the call has something to upload or "
+                     "allocate: make it once on this batch before the capture");
 }
 
 // Scratch of the fast decode when its plan cuts rows into chunks: a partial
@@ -425,6 +443,10 @@ int ensure_split(ckv_pool* pool, const meta_view& m, size_t q_heads, split_scrat
     size_t capacity_floats = pool->d_partials_bytes / sizeof(float);
     const size_t floats = (size_t)m.n_records * q_heads
         * partial_record_floats((uint32_t)pool->head_dim);
+    if (m.window.window != all_keys.window
+        && (floats > capacity_floats || m.n_records * pool->kv_heads > pool->d_arrivals_words)
+        && capturing(ctx))
+        return refuse_captured(ctx);
     int status = ensure_device(ctx, &pool->d_partials, &capacity_floats, floats,
                                "decode partials");
     pool->d_partials_bytes = capacity_floats * sizeof(float);
@@ -517,25 +539,6 @@ int ensure_work(ckv_pool* pool)
 
 // ---- the batch through a window ---------------------------------------------------
 
-// Whether the context's stream is being captured into a graph (or cannot be asked
-// while another is): a launch there takes no upload and no allocation, whose replays
-// would read staging memory of other uploads or free what a graph uses.
-bool capturing(const ckv_context* ctx)
-{
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    const hipError_t e = hipStreamIsCapturing(ctx->stream, &status);
-    if (e != hipSuccess)
-        (void)hipGetLastError();
-    return e != hipSuccess || status != hipStreamCaptureStatusNone;
-}
-
-int refuse_captured(ckv_context* ctx)
-{
-    return set_error(ctx, CKV_E_INVALID_ARGUMENT,
-                     "the stream is being captured and the call has something to upload or "
-                     "allocate: make it once on this batch before the capture");
-}
-
 // A window past every row's position leaves the batch as it is (all_keys).
 key_window window_of(const ckv_pool* pool, size_t window, size_t sinks)
 {
@@ -544,36 +547,95 @@ key_window window_of(const ckv_pool* pool, size_t window, size_t sinks)
     return window_low(pool->last_position, w) > w.sinks ? w : all_keys;
 }
 
-// Selects the batch's window: its positions less the tokens of the units it skips.
+// Selects the batch's window; its plan and work list are derived anew unless they
+// are this window's already.
 void select_window(ckv_pool* pool, key_window w)
 {
-    if (pool->window.window == w.window && pool->window.sinks == w.sinks
+    meta_view& m = pool->window_meta;
+    if (m.window.window == w.window && m.window.sinks == w.sinks
         && pool->window_positions.size() == pool->positions.size())
         return;
     pool->window_positions.clear(); // stays so if what follows throws
     pool->window_plan_ready = pool->window_work_ready = false;
-    pool->window = w;
-    pool->window_meta = pool->meta;
     pool->window_positions.resize(pool->positions.size());
+    m = pool->meta;
+    m.window = w;
 }
 
-// The window's work list of the generic decode, in tokens.
+// The rows' positions less the tokens of the units (of `unit` tokens) that the
+// window skips.
+const std::vector<uint32_t>& close_window_gaps(ckv_pool* pool, uint32_t unit)
+{
+    const key_window w = pool->window_meta.window;
+    std::vector<uint32_t>& left = pool->window_positions;
+    for (size_t r = 0; r < left.size(); ++r) {
+        const uint32_t p = pool->positions[r];
+        left[r] = p - window_gap_of(window_low(p, w), w.sinks, unit).skip * unit;
+    }
+    return left;
+}
+
+// The window's work list of the generic decode, in tokens, at its first launch.
 int ensure_window_work(ckv_pool* pool)
 {
     if (pool->window_work_ready)
         return CKV_OK;
     if (capturing(pool->ctx))
         return refuse_captured(pool->ctx);
-    const key_window w = pool->window;
-    std::vector<uint32_t>& left = pool->window_positions;
-    for (size_t r = 0; r < left.size(); ++r) {
-        const uint32_t p = pool->positions[r];
-        left[r] = p - window_gap_of(window_low(p, w), w.sinks, 1).skip;
-    }
-    const int status = put_work(pool, left, pool->window_meta, &pool->d_window_work,
-                                &pool->d_window_work_words, pool->window_work_multi);
+    const int status = put_work(pool, close_window_gaps(pool, 1), pool->window_meta,
+                                &pool->d_window_work, &pool->d_window_work_words,
+                                pool->window_work_multi);
     pool->window_work_ready = status == CKV_OK;
     return status;
+}
+
+// The window's plan of the fast decode, in pages, at its first launch.
+int ensure_window_plan(ckv_pool* pool)
+{
+    if (pool->window_plan_ready)
+        return CKV_OK;
+    ckv_context* ctx = pool->ctx;
+    if (capturing(ctx))
+        return refuse_captured(ctx);
+    const uint32_t bs = (uint32_t)pool->block_size;
+    const std::vector<uint32_t>& left = close_window_gaps(pool, bs);
+    const decode_plan_shape shape =
+        shape_decode_plan(left, bs, (uint32_t)pool->kv_heads, ctx->cu_count,
+                          decode_form_of(pool->dtype, (uint32_t)pool->head_dim));
+    const size_t words = std::max<size_t>(plan_words(shape, left.size()), 4);
+    void* host = nullptr;
+    int status = stage(ctx, words * sizeof(uint32_t), &host);
+    if (!status)
+        status = ensure_device(ctx, &pool->d_window_plan, &pool->d_window_plan_words, words,
+                               "decode plan");
+    if (status)
+        return status;
+    auto* w = static_cast<uint32_t*>(host);
+    put_plan(pool, left, pool->window_meta, shape, w, pool->d_window_plan);
+    place_window_plan(pool->positions, shape, w);
+    uint64_t pages = 0;
+    for (const uint32_t p : left)
+        pages += p / bs + 1;
+    pool->window_meta.mean_pages = left.empty() ? 0 : (uint32_t)(pages / left.size());
+    status = upload_staged(ctx, pool->d_window_plan, words * sizeof(uint32_t));
+    pool->window_plan_ready = status == CKV_OK;
+    return status;
+}
+
+// What a decode launch runs over: the batch, or the batch through a window.
+meta_view& decode_meta(ckv_pool* pool, key_window window)
+{
+    if (window.window == all_keys.window)
+        return pool->meta;
+    select_window(pool, window);
+    return pool->window_meta;
+}
+
+// The plan and scratch of a fast decode launch over `m` (decode_meta).
+int ensure_fast(ckv_pool* pool, const meta_view& m, size_t q_heads, split_scratch& split)
+{
+    const int status = &m == &pool->meta ? ensure_plan(pool) : ensure_window_plan(pool);
+    return status ? status : ensure_split(pool, m, q_heads, split);
 }
 
 int run_decode(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale,
@@ -583,14 +645,12 @@ int run_decode(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads
     const pool_view view = view_of(pool);
     float* partials = nullptr;
     split_scratch split {};
-    const bool windowed = window.window != all_keys.window;
-    const bool fast = !windowed && decode_fast_applies(view, (uint32_t)q_heads, queries, output);
-    if (windowed)
-        select_window(pool, window);
-    int status = windowed ? ensure_window_work(pool) : fast ? ensure_plan(pool) : ensure_work(pool);
-    const meta_view& m = windowed ? pool->window_meta : pool->meta;
-    if (!status && fast)
-        status = ensure_split(pool, m, q_heads, split);
+    const bool fast = decode_fast_applies(view, (uint32_t)q_heads, queries, output);
+    meta_view& m = decode_meta(pool, window);
+    const bool windowed = &m != &pool->meta;
+    int status = fast ? ensure_fast(pool, m, q_heads, split)
+        : windowed    ? ensure_window_work(pool)
+                      : ensure_work(pool);
     if (status)
         return status;
     const bool needs_merge = !fast && (windowed ? pool->window_work_multi : pool->work_multi);
@@ -611,7 +671,7 @@ int run_decode(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads
     }
     status = run_kernel(ctx, windowed ? "window_attention_decode" : "paged_attention_decode", [&] {
         return launch_decode(ctx->stream, view, m, (uint32_t)layer, queries, (uint32_t)q_heads,
-                             scale, output, partials, ctx->cu_count, gate, split, window);
+                             scale, output, partials, ctx->cu_count, gate, split);
     });
     if (status || !needs_merge)
         return status;
@@ -1409,7 +1469,7 @@ int ckv_tables_upload(ckv_pool* pool, const uint32_t* block_table, size_t n_entr
     if (status)
         return status;
     if (with_plan)
-        put_plan(pool, plan_shape, w + s_plan, pool->d_meta + s_plan);
+        put_plan(pool, pool->positions, pool->meta, plan_shape, w + s_plan, pool->d_meta + s_plan);
     status = upload_staged(ctx, pool->d_meta, words * sizeof(uint32_t));
     if (status)
         return status;
@@ -1679,7 +1739,7 @@ int ckv_batch_upload(ckv_pool* pool, const uint32_t* seq, const uint32_t* first_
         return status;
     uint32_t* d = pool->d_meta;
     if (with_plan)
-        put_plan(pool, plan_shape, section(s_plan), d + s_plan);
+        put_plan(pool, positions, pool->meta, plan_shape, section(s_plan), d + s_plan);
     status = upload_staged(ctx, d + s_pairs, up_words * sizeof(uint32_t));
     if (status)
         return status;
@@ -1886,12 +1946,9 @@ int decode_impl(ckv_pool* pool, size_t layer, const void* queries, size_t q_head
     return run_decode(pool, layer, queries, q_heads, scale, output, gate);
 }
 
-int append_decode_impl(ckv_pool* pool, size_t layer, const void* keys, const void* values,
-                       const void* queries, size_t q_heads, float scale, void* output,
-                       size_t rows, const void* gate)
+// The checks of an append before those of its attention.
+int check_append(ckv_pool* pool, const void* keys, const void* values, size_t rows)
 {
-    if (!pool)
-        return CKV_E_INVALID_ARGUMENT;
     ckv_context* ctx = pool->ctx;
     if (rows && (!keys || !values))
         return set_error(ctx, CKV_E_INVALID_ARGUMENT, "keys and values are required");
@@ -1899,29 +1956,47 @@ int append_decode_impl(ckv_pool* pool, size_t layer, const void* keys, const voi
         return set_error(ctx, CKV_E_NO_TABLES, "append before slots were uploaded");
     if (rows != pool->slot_rows)
         return set_error(ctx, CKV_E_CACHE_SLOT_COUNT_MISMATCH, "rows != uploaded slots");
-    int status = check_attention(pool, layer, queries, q_heads, output, rows);
-    if (status || !rows)
-        return status;
+    return CKV_OK;
+}
+
+// The append and attention of checked decode rows.
+int run_append_decode(ckv_pool* pool, size_t layer, const void* keys, const void* values,
+                      const void* queries, size_t q_heads, float scale, void* output, size_t rows,
+                      const void* gate, key_window window)
+{
+    ckv_context* ctx = pool->ctx;
     const pool_view view = view_of(pool);
     const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     if (pool->fusable && decode_fast_applies(view, (uint32_t)q_heads, queries, output)
         && aligned(keys) && aligned(values)) {
         split_scratch split {};
-        status = ensure_plan(pool);
-        if (!status)
-            status = ensure_split(pool, pool->meta, q_heads, split);
-        if (status)
+        const meta_view& m = decode_meta(pool, window);
+        if (const int status = ensure_fast(pool, m, q_heads, split))
             return status;
-        return run_kernel(ctx, "append_decode", [&] {
-            return launch_append_decode(ctx->stream, view, pool->meta, (uint32_t)layer, keys,
-                                        values, queries, (uint32_t)q_heads, scale, output, gate,
+        return run_kernel(ctx, &m == &pool->meta ? "append_decode" : "append_decode_window", [&] {
+            return launch_append_decode(ctx->stream, view, m, (uint32_t)layer, keys, values,
+                                        queries, (uint32_t)q_heads, scale, output, gate,
                                         ctx->cu_count, split);
         });
     }
-    status = ckv_append(pool, layer, keys, values, rows);
-    if (status)
+    if (const int status = ckv_append(pool, layer, keys, values, rows))
         return status;
-    return run_decode(pool, layer, queries, q_heads, scale, output, gate);
+    return run_decode(pool, layer, queries, q_heads, scale, output, gate, window);
+}
+
+int append_decode_impl(ckv_pool* pool, size_t layer, const void* keys, const void* values,
+                       const void* queries, size_t q_heads, float scale, void* output,
+                       size_t rows, const void* gate)
+{
+    if (!pool)
+        return CKV_E_INVALID_ARGUMENT;
+    int status = check_append(pool, keys, values, rows);
+    if (!status)
+        status = check_attention(pool, layer, queries, q_heads, output, rows);
+    if (status || !rows)
+        return status;
+    return run_append_decode(pool, layer, keys, values, queries, q_heads, scale, output, rows, gate,
+                             all_keys);
 }
 
 int prefill_impl(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale,
@@ -2036,6 +2111,52 @@ int ckv_append_decode_gated(ckv_pool* pool, size_t layer, const void* keys, cons
                               gate);
 }
 
+namespace {
+
+// The rotation, append and attention of checked decode rows.
+int run_rope_append_decode(ckv_pool* pool, size_t layer, const void* keys, const void* values,
+                           const void* queries, size_t q_heads, float scale, float theta,
+                           size_t rotary_dim, const ckv::rope_table& freq, uint32_t rotary,
+                           const void* gate, void* output, size_t rows, key_window window)
+{
+    ckv_context* ctx = pool->ctx;
+    const pool_view view = view_of(pool);
+    const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const bool windowed = window.window != all_keys.window;
+    // the fused kernel rotates 16-bit pages in lane pairs part ^ (rotary / 16)
+    const bool lane_pairs = view.dtype != CKV_F32 && rotary >= 16 && (rotary & (rotary - 1)) == 0;
+    if (pool->fusable && lane_pairs && decode_fast_applies(view, (uint32_t)q_heads, queries, output)
+        && aligned(keys) && aligned(values) && (!gate || aligned(gate))) {
+        split_scratch split {};
+        const meta_view& m = decode_meta(pool, window);
+        if (const int status = ensure_fast(pool, m, q_heads, split))
+            return status;
+        return run_kernel(ctx, windowed ? "rope_append_decode_window" : "rope_append_decode", [&] {
+            return launch_append_decode(ctx->stream, view, m, (uint32_t)layer, keys, values,
+                                        queries, (uint32_t)q_heads, scale, output, gate,
+                                        ctx->cu_count, split, &freq, rotary);
+        });
+    }
+    // unfused: queries rotated into a pool buffer, keys rotated into their
+    // slots, then the attention over the rotated queries
+    const size_t q_bytes = rows * q_heads * pool->head_dim * pool->elem_size;
+    if (windowed && q_bytes > pool->d_rope_q_bytes && capturing(ctx))
+        return refuse_captured(ctx);
+    int status = ensure_device(ctx, &pool->d_rope_q, &pool->d_rope_q_bytes, q_bytes,
+                               "rotated queries");
+    if (status)
+        return status;
+    status = ckv_rope(pool, queries, pool->d_rope_q, q_heads, theta, rotary_dim, rows);
+    if (status)
+        return status;
+    status = ckv_rope_append(pool, layer, keys, values, theta, rotary_dim, rows);
+    if (status)
+        return status;
+    return run_decode(pool, layer, pool->d_rope_q, q_heads, scale, output, gate, window);
+}
+
+} // namespace
+
 int ckv_rope_append_decode(ckv_pool* pool, size_t layer, const void* keys, const void* values,
                            const void* queries, size_t q_heads, float scale, float theta,
                            size_t rotary_dim, const void* gate, void* output, size_t rows)
@@ -2043,13 +2164,9 @@ int ckv_rope_append_decode(ckv_pool* pool, size_t layer, const void* keys, const
     if (!pool)
         return CKV_E_INVALID_ARGUMENT;
     ckv_context* ctx = pool->ctx;
-    if (rows && (!keys || !values))
-        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "keys and values are required");
-    if (!pool->uploaded || !pool->has_slots)
-        return set_error(ctx, CKV_E_NO_TABLES, "append before slots were uploaded");
-    if (rows != pool->slot_rows)
-        return set_error(ctx, CKV_E_CACHE_SLOT_COUNT_MISMATCH, "rows != uploaded slots");
-    int status = check_attention(pool, layer, queries, q_heads, output, rows);
+    int status = check_append(pool, keys, values, rows);
+    if (!status)
+        status = check_attention(pool, layer, queries, q_heads, output, rows);
     if (status)
         return status;
     if (gate && (gate == queries || gate == output))
@@ -2059,37 +2176,8 @@ int ckv_rope_append_decode(ckv_pool* pool, size_t layer, const void* keys, const
     status = check_rope(pool, q_heads, theta, rotary_dim, freq, rotary);
     if (status || !rows)
         return status;
-    const pool_view view = view_of(pool);
-    const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    // the fused kernel rotates 16-bit pages in lane pairs part ^ (rotary / 16)
-    const bool lane_pairs = view.dtype != CKV_F32 && rotary >= 16 && (rotary & (rotary - 1)) == 0;
-    if (pool->fusable && lane_pairs && decode_fast_applies(view, (uint32_t)q_heads, queries, output)
-        && aligned(keys) && aligned(values) && (!gate || aligned(gate))) {
-        split_scratch split {};
-        status = ensure_plan(pool);
-        if (!status)
-            status = ensure_split(pool, pool->meta, q_heads, split);
-        if (status)
-            return status;
-        return run_kernel(ctx, "rope_append_decode", [&] {
-            return launch_append_decode(ctx->stream, view, pool->meta, (uint32_t)layer, keys,
-                                        values, queries, (uint32_t)q_heads, scale, output, gate,
-                                        ctx->cu_count, split, &freq, rotary);
-        });
-    }
-    // unfused: queries rotated into a pool buffer, keys rotated into their
-    // slots, then the attention over the rotated queries
-    const size_t q_bytes = rows * q_heads * pool->head_dim * pool->elem_size;
-    status = ensure_device(ctx, &pool->d_rope_q, &pool->d_rope_q_bytes, q_bytes, "rotated queries");
-    if (status)
-        return status;
-    status = ckv_rope(pool, queries, pool->d_rope_q, q_heads, theta, rotary_dim, rows);
-    if (status)
-        return status;
-    status = ckv_rope_append(pool, layer, keys, values, theta, rotary_dim, rows);
-    if (status)
-        return status;
-    return run_decode(pool, layer, pool->d_rope_q, q_heads, scale, output, gate);
+    return run_rope_append_decode(pool, layer, keys, values, queries, q_heads, scale, theta,
+                                  rotary_dim, freq, rotary, gate, output, rows, all_keys);
 }
 
 namespace {
@@ -2192,21 +2280,6 @@ int check_window(const ckv_pool* pool, size_t window)
                               "window == 0: a row attends itself at least");
 }
 
-int check_slots(const ckv_pool* pool, size_t layer, const void* keys, const void* values,
-                size_t rows)
-{
-    ckv_context* ctx = pool->ctx;
-    if (rows && (!keys || !values))
-        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "keys and values are required");
-    if (!pool->uploaded || !pool->has_slots)
-        return set_error(ctx, CKV_E_NO_TABLES, "append before slots were uploaded");
-    if (rows != pool->slot_rows)
-        return set_error(ctx, CKV_E_CACHE_SLOT_COUNT_MISMATCH, "rows != uploaded slots");
-    if (layer >= pool->layers)
-        return set_error(ctx, CKV_E_CACHE_LAYER_OUT_OF_RANGE, "layer >= layers");
-    return CKV_OK;
-}
-
 } // namespace
 
 int ckv_attention_window(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads,
@@ -2231,7 +2304,7 @@ int ckv_append_decode_window(ckv_pool* pool, size_t layer, const void* keys, con
                              size_t sinks, const void* gate, void* output, size_t rows)
 {
     return guarded(pool, [&]() -> int {
-        int status = check_slots(pool, layer, keys, values, rows);
+        int status = check_append(pool, keys, values, rows);
         if (!status)
             status = check_attention(pool, layer, queries, q_heads, output, rows);
         if (!status)
@@ -2240,14 +2313,8 @@ int ckv_append_decode_window(ckv_pool* pool, size_t layer, const void* keys, con
             status = check_optional_gate(pool, gate, queries, output);
         if (status || !rows)
             return status;
-        const key_window w = window_of(pool, window, sinks);
-        if (w.window == all_keys.window)
-            return append_decode_impl(pool, layer, keys, values, queries, q_heads, scale, output,
-                                      rows, gate);
-        status = ckv_append(pool, layer, keys, values, rows);
-        if (status)
-            return status;
-        return run_decode(pool, layer, queries, q_heads, scale, output, gate, w);
+        return run_append_decode(pool, layer, keys, values, queries, q_heads, scale, output, rows,
+                                 gate, window_of(pool, window, sinks));
     });
 }
 
@@ -2257,7 +2324,7 @@ int ckv_rope_append_decode_window(ckv_pool* pool, size_t layer, const void* keys
                                   size_t sinks, const void* gate, void* output, size_t rows)
 {
     return guarded(pool, [&]() -> int {
-        int status = check_slots(pool, layer, keys, values, rows);
+        int status = check_append(pool, keys, values, rows);
         if (!status)
             status = check_attention(pool, layer, queries, q_heads, output, rows);
         if (!status)
@@ -2270,23 +2337,9 @@ int ckv_rope_append_decode_window(ckv_pool* pool, size_t layer, const void* keys
             status = check_rope(pool, q_heads, theta, rotary_dim, freq, rotary);
         if (status || !rows)
             return status;
-        const key_window w = window_of(pool, window, sinks);
-        if (w.window == all_keys.window)
-            return ckv_rope_append_decode(pool, layer, keys, values, queries, q_heads, scale,
-                                          theta, rotary_dim, gate, output, rows);
-        ckv_context* ctx = pool->ctx;
-        const size_t q_bytes = rows * q_heads * pool->head_dim * pool->elem_size;
-        if (q_bytes > pool->d_rope_q_bytes && capturing(ctx))
-            return refuse_captured(ctx);
-        status = ensure_device(ctx, &pool->d_rope_q, &pool->d_rope_q_bytes, q_bytes,
-                               "rotated queries");
-        if (!status)
-            status = ckv_rope(pool, queries, pool->d_rope_q, q_heads, theta, rotary_dim, rows);
-        if (!status)
-            status = ckv_rope_append(pool, layer, keys, values, theta, rotary_dim, rows);
-        if (status)
-            return status;
-        return run_decode(pool, layer, pool->d_rope_q, q_heads, scale, output, gate, w);
+        return run_rope_append_decode(pool, layer, keys, values, queries, q_heads, scale, theta,
+                                      rotary_dim, freq, rotary, gate, output, rows,
+                                      window_of(pool, window, sinks));
     });
 }
 
@@ -2391,9 +2444,11 @@ int ckv_rope_axes_append(ckv_pool* pool, size_t layer, const void* queries, void
 {
     return guarded(pool, [&]() -> int {
         ckv_context* ctx = pool->ctx;
-        int status = check_slots(pool, layer, keys, values, rows);
+        int status = check_append(pool, keys, values, rows);
         if (status)
             return status;
+        if (layer >= pool->layers)
+            return set_error(ctx, CKV_E_CACHE_LAYER_OUT_OF_RANGE, "layer >= layers");
         if (rows && q_heads && (!queries || !rotated))
             return set_error(ctx, CKV_E_INVALID_ARGUMENT, "queries and rotated are required");
         if (rows && (rotated == keys || rotated == values))

@@ -28,6 +28,34 @@ struct pool_view {
     int dtype; // ckv_dtype
 };
 
+// The keys a row at position p attends: those at t <= p with t > p - window or
+// t < sinks. all_keys: every t <= p.
+struct key_window {
+    uint32_t window; // at least 1: a row attends itself
+    uint32_t sinks;
+};
+constexpr key_window all_keys { UINT32_MAX, 0 };
+
+// The window's first key.
+__host__ __device__ inline uint32_t window_low(uint32_t position, key_window w)
+{
+    return position >= w.window ? position - w.window + 1 : 0;
+}
+
+// Of a row's units of `unit` tokens (tokens, pages or key blocks) in order, those
+// that hold no key it attends: `skip` of them from unit `kept` on. What a kernel
+// walks is the row's other units: unit u < kept as it is, a later one skip on.
+struct window_gap {
+    uint32_t kept, skip;
+};
+__host__ __device__ inline window_gap window_gap_of(uint32_t low, uint32_t sinks, uint32_t unit)
+{
+    const uint32_t first = low / unit; // the window's first unit
+    const uint32_t held = sinks < low ? sinks / unit + (sinks % unit != 0) : first;
+    const uint32_t kept = held < first ? held : first;
+    return { kept, first - kept };
+}
+
 // Device pointers into the uploaded metadata block (one H2D copy per upload).
 struct meta_view {
     const uint32_t* table;
@@ -63,6 +91,7 @@ struct meta_view {
     uint32_t split_pages; // the plan's pages per chunk or per workgroup; 0: one row per workgroup
     uint32_t n_records;   // partial records of the rows cut into chunks
     uint32_t n_cut;       // rows cut into chunks
+    key_window window = all_keys;
 };
 
 // Device scratch of the fast decode's cut rows: a partial record
@@ -75,34 +104,6 @@ struct split_scratch {
     float* records;
     uint32_t* arrivals;
 };
-
-// The keys a row at position p attends: those at t <= p with t > p - window or
-// t < sinks. all_keys: every t <= p.
-struct key_window {
-    uint32_t window; // at least 1: a row attends itself
-    uint32_t sinks;
-};
-constexpr key_window all_keys { UINT32_MAX, 0 };
-
-// The window's first key.
-__host__ __device__ inline uint32_t window_low(uint32_t position, key_window w)
-{
-    return position >= w.window ? position - w.window + 1 : 0;
-}
-
-// Of a row's units of `unit` tokens (tokens, pages or key blocks) in order, those
-// that hold no key it attends: `skip` of them from unit `kept` on. What a kernel
-// walks is the row's other units: unit u < kept as it is, a later one skip on.
-struct window_gap {
-    uint32_t kept, skip;
-};
-__host__ __device__ inline window_gap window_gap_of(uint32_t low, uint32_t sinks, uint32_t unit)
-{
-    const uint32_t first = low / unit; // the window's first unit
-    const uint32_t held = sinks < low ? sinks / unit + (sinks % unit != 0) : first;
-    const uint32_t kept = held < first ? held : first;
-    return { kept, first - kept };
-}
 
 constexpr size_t tile_entry_words = 4;
 
@@ -319,7 +320,6 @@ struct ckv_pool {
     // The current batch through a window: the same rows with the plan and work
     // list of what the window leaves of them, derived at the first launch with it
     // and kept until another window or batch comes.
-    ckv::key_window window = ckv::all_keys;
     bool window_plan_ready = false;
     bool window_work_ready = false;
     bool window_work_multi = false;
@@ -437,7 +437,7 @@ void write_decode_plan(const std::vector<uint32_t>& positions,
 hipError_t launch_decode(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
                          const void* q, uint32_t q_heads, float scale, void* out,
                          float* partials, int cu_count, const void* gate = nullptr,
-                         split_scratch split = {}, key_window window = all_keys);
+                         split_scratch split = {});
 bool decode_fast_applies(const pool_view& p, uint32_t q_heads, const void* q, const void* out);
 // store_kv + fast decode in one launch; the caller has checked
 // decode_fast_applies, 16-byte aligned inputs, and that every row's slot is
@@ -452,6 +452,13 @@ hipError_t launch_append_decode(hipStream_t s, const pool_view& p, const meta_vi
 hipError_t launch_merge(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t q_heads,
                         void* out, const float* partials, const void* gate = nullptr);
 bool decode_uses_fast_path(const pool_view& p, uint32_t q_heads);
+// The fast decode of a batch through a window (m.window), its arguments already
+// checked and scaled by launch_decode and launch_append_decode.
+hipError_t launch_window_fast(hipStream_t s, const pool_view& p, const meta_view& m,
+                              uint32_t layer, const void* q, uint32_t q_heads, float scale_log2,
+                              void* out, const void* k_in, const void* v_in, const void* gate,
+                              int cu_count, split_scratch split, const rope_table* rope,
+                              uint32_t rotary);
 // Sets every entry of a plan written from the window's positions to its row's position.
 void place_window_plan(const std::vector<uint32_t>& positions, const decode_plan_shape& shape,
                        uint32_t* plan);
