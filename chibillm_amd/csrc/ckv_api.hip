@@ -1999,25 +1999,21 @@ int append_decode_impl(ckv_pool* pool, size_t layer, const void* keys, const voi
                              all_keys);
 }
 
-int prefill_impl(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale,
-                 void* output, size_t rows, const void* gate)
+// The prefill form of checked rows, over the batch or the batch through a window.
+int run_prefill(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale,
+                void* output, const void* gate, const meta_view& m)
 {
-    if (!pool)
-        return CKV_E_INVALID_ARGUMENT;
-    const int status = check_attention(pool, layer, queries, q_heads, output, rows);
-    if (status || !rows)
-        return status;
     const pool_view view = view_of(pool);
-    const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    // the MFMA kernel tracks maxima of the unscaled scores, which needs scale > 0;
-    // the decode kernels scale first and take any scale, one row at a time
-    if (!prefill_supported(view, (uint32_t)q_heads, queries, output) || (gate && !aligned(gate))
-        || !(scale > 0.0f))
-        return run_decode(pool, layer, queries, q_heads, scale, output, gate);
     ckv_context* ctx = pool->ctx;
-    const prefill_shape_info plan = prefill_plan(view, pool->meta, (uint32_t)q_heads, ctx->cu_count);
+    const bool windowed = &m != &pool->meta;
+    const prefill_shape_info plan = prefill_plan(view, m, (uint32_t)q_heads, ctx->cu_count);
     prefill_split split { nullptr, nullptr, plan.n_split, plan.min_blocks };
     if (plan.n_split > 1) {
+        if (windowed
+            && (plan.records_floats > pool->d_pre_records_floats
+                || plan.counters > pool->d_pre_arrivals_words)
+            && capturing(ctx))
+            return refuse_captured(ctx);
         int status = ensure_device(ctx, &pool->d_pre_records, &pool->d_pre_records_floats,
                                    (size_t)plan.records_floats, "prefill split records");
         if (status)
@@ -2042,10 +2038,40 @@ int prefill_impl(ckv_pool* pool, size_t layer, const void* queries, size_t q_hea
         split.records = pool->d_pre_records;
         split.arrivals = pool->d_pre_arrivals;
     }
-    return run_kernel(ctx, "paged_attention_prefill", [&] {
-        return launch_prefill(ctx->stream, view, pool->meta, (uint32_t)layer, queries,
-                              (uint32_t)q_heads, scale, output, gate, plan, split);
+    return run_kernel(ctx, windowed ? "window_attention_prefill" : "paged_attention_prefill", [&] {
+        return launch_prefill(ctx->stream, view, m, (uint32_t)layer, queries, (uint32_t)q_heads,
+                              scale, output, gate, plan, split);
     });
+}
+
+// Whether the matrix-core prefill takes these rows. It tracks maxima of the unscaled
+// scores, which needs scale > 0; the decode kernels scale first and take any scale, one
+// row at a time.
+bool prefill_takes(const ckv_pool* pool, const void* queries, size_t q_heads, float scale,
+                   const void* output, const void* gate)
+{
+    return prefill_supported(view_of(pool), (uint32_t)q_heads, queries, output)
+        && (!gate || reinterpret_cast<uintptr_t>(gate) % 16 == 0) && scale > 0.0f;
+}
+
+int prefill_impl(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale,
+                 void* output, size_t rows, const void* gate)
+{
+    if (!pool)
+        return CKV_E_INVALID_ARGUMENT;
+    const int status = check_attention(pool, layer, queries, q_heads, output, rows);
+    if (status || !rows)
+        return status;
+    if (!prefill_takes(pool, queries, q_heads, scale, output, gate))
+        return run_decode(pool, layer, queries, q_heads, scale, output, gate);
+    return run_prefill(pool, layer, queries, q_heads, scale, output, gate, pool->meta);
+}
+
+// Tiles are used when some run of rows shares a query tile and head_dim <= 128
+// (src/tensor/attention.cc:290-309); here 256-wide heads have tiles too.
+bool batch_has_tiles(const ckv_pool* pool)
+{
+    return pool->shared_tile && (pool->head_dim <= 128 || pool->head_dim == 256);
 }
 
 int attention_impl(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale,
@@ -2053,9 +2079,7 @@ int attention_impl(ckv_pool* pool, size_t layer, const void* queries, size_t q_h
 {
     if (!pool)
         return CKV_E_INVALID_ARGUMENT;
-    // src/tensor/attention.cc:290-309: tiles are used when some run of rows
-    // shares a query tile and head_dim <= 128; here 256-wide heads have tiles too
-    if (pool->shared_tile && (pool->head_dim <= 128 || pool->head_dim == 256))
+    if (batch_has_tiles(pool))
         return prefill_impl(pool, layer, queries, q_heads, scale, output, rows, gate);
     return decode_impl(pool, layer, queries, q_heads, scale, output, rows, gate);
 }
@@ -2294,8 +2318,13 @@ int ckv_attention_window(ckv_pool* pool, size_t layer, const void* queries, size
             status = check_optional_gate(pool, gate, queries, output);
         if (status || !rows)
             return status;
-        return run_decode(pool, layer, queries, q_heads, scale, output, gate,
-                          window_of(pool, window, sinks));
+        const key_window w = window_of(pool, window, sinks);
+        if (!batch_has_tiles(pool)
+            || !prefill_takes(pool, queries, q_heads, scale, output, gate))
+            return run_decode(pool, layer, queries, q_heads, scale, output, gate, w);
+        // also a window that leaves nothing out: its kernels hold probabilities in more bits
+        select_window(pool, w.window != all_keys.window ? w : key_window { UINT32_MAX - 1, 0 });
+        return run_prefill(pool, layer, queries, q_heads, scale, output, gate, pool->window_meta);
     });
 }
 

@@ -41,6 +41,7 @@
 // Keys past the tile's last position are read from a zero row (never from
 // the pool), so no page outside a row's table is touched and masked keys
 // carry finite zeros into P.V.
+#include "attend_alone.h"
 #include "ckv_internal.h"
 #include "prefill_records.h"
 #include "prefill_tile.h"
@@ -96,13 +97,13 @@ __device__ __forceinline__ void dma16_pair(const void* kb, uint32_t koff, uint32
 
 // Probabilities of one q-block against the running maximum m (raw q.k
 // units; c = scale * log2(e) so every exponential is one exp2), added to
-// this lane's share of the denominator.
+// this lane's share of the denominator, all of them at 2^scale.
 template <bool GUARD>
-__device__ __forceinline__ void exponentiate(f32x16_t& s, float m, float& l, float c)
+__device__ __forceinline__ void exponentiate(f32x16_t& s, float m, float& l, float c, float scale)
 {
     // GUARD: a workgroup that attends only part of the keys may have seen no
     // unmasked key of a query yet (m = -inf); its probabilities are then 0
-    const float mc = GUARD && m == -__builtin_inff() ? 0.0f : m * c;
+    const float mc = GUARD && m == -__builtin_inff() ? 0.0f : m * c - scale;
 #pragma unroll
     for (int r = 0; r < 16; ++r)
         s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -mc));
@@ -124,13 +125,26 @@ struct prefill_shape {
     static constexpr uint32_t dmas = 2 * regions;        // DMA loads per block and wave
 };
 
-template <int G, bool F16, bool WIDE, int W>
+// WINDOW (4 waves): rows attend through md.window. Blocks that no row of the
+// workgroup attends are left out of the count (in_table gives a block's place in the
+// sequence); keys that none attends in the blocks at the gap's edges are staged from
+// the zero row. A probability enters P.V as two 16-bit terms, the second the rounding
+// of what the first left: a window's rows weigh few keys, and one term's rounding
+// (8 bits in bf16) was 1.7 times the output's own. fp16 terms are taken at 2^6 times
+// the probability, which the final division removes, so that the second stays out of
+// fp16's subnormals. Rows to which a tile gave a value that is not finite are attended
+// again alone (attend_alone.h), as 256-wide heads' are. A GQA group of 8 takes two
+// workgroups of 4 heads each.
+template <int G, bool F16, bool WIDE, int W, bool WINDOW>
 __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     pool_view p, meta_view md, uint32_t layer, const uint16_t* __restrict__ q,
     uint16_t* __restrict__ out, uint32_t q_heads, float c, const uint16_t* __restrict__ gate,
     prefill_split split_scratch)
 {
     static_assert(W == 8 || (W == 4 && G <= 4), "a workgroup covers every q head of its group");
+    static_assert(!WINDOW || W == 4);
+    constexpr int terms = WINDOW ? 2 : 1;
+    constexpr float p_scale = WINDOW && F16 ? 6.0f : 0.0f; // log2
     // 4-wave workgroups may split a tile's key blocks between workgroups
     constexpr bool SPLIT = W == 4;
     using shape = prefill_shape<W>;
@@ -142,13 +156,18 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
 
     const uint32_t kv_heads = p.kv_heads;
     const uint32_t kvh = blockIdx.x % kv_heads; // consecutive workgroups: different heads/XCDs
+    const uint32_t group = WINDOW ? q_heads / kv_heads : G;
+    const uint32_t passes = WINDOW ? group / G : 1; // workgroups a GQA group takes
+    const uint32_t unit = WINDOW ? blockIdx.x / kv_heads : 0;
+    const uint32_t pass = WINDOW ? unit % passes : 0;
+    const uint32_t of_pass = WINDOW ? unit / passes : blockIdx.x / kv_heads;
     // key ranges vary slowest: every tile's first range is dispatched before
     // any second one (ranges interleaved with the rows placed the ranges that
     // find no keys, and the long ones, unevenly: +5 to +29 % launch time)
     const uint32_t n_split = SPLIT ? split_scratch.n_split : 1;
     const uint32_t n_rest = md.n_tiles * subs;
-    const uint32_t rest = blockIdx.x / kv_heads % n_rest;
-    const uint32_t part = blockIdx.x / kv_heads / n_rest; // this workgroup's range of the keys
+    const uint32_t rest = of_pass % n_rest;
+    const uint32_t part = of_pass / n_rest; // this workgroup's range of the keys
     const uint32_t sub = rest % subs;
     const uint32_t tile = rest / subs;
     // one scalar load gives the tile: first row, rows, first position, table offset
@@ -162,7 +181,15 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     const uint32_t pos0 = te.z + r0; // positions are consecutive inside a tile
     const uint32_t pos_last = pos0 + nrows - 1;
     const uint32_t* table = md.table + te.w;
-    const uint32_t n_blocks = pos_last / block_keys + 1;
+    // the first row's window begins at `low`, no later row's before it
+    const key_window window = md.window;
+    const uint32_t low = WINDOW ? window_low(pos0, window) : 0;
+    const window_gap gap = WINDOW ? window_gap_of(low, window.sinks, block_keys) : window_gap {};
+    auto in_table = [&](uint32_t kb) { return WINDOW && kb >= gap.kept ? kb + gap.skip : kb; };
+    auto some_row_attends = [&](uint32_t key) {
+        return key <= pos_last && (!WINDOW || key >= low || key < window.sinks);
+    };
+    const uint32_t n_blocks = pos_last / block_keys + 1 - gap.skip;
     // Key blocks [kb_begin, kb_end) of this workgroup: the tile's blocks cut
     // into n_parts ranges of at least min_blocks (uniform over the tile's
     // workgroups), range `part`.
@@ -184,7 +211,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
 
     // this wave's q-block: head kvh * G + wave % G, tile rows 32 * (wave / G) + n
     const uint32_t rb = wave / G;
-    const uint32_t head = kvh * G + wave % G;
+    const uint32_t head = kvh * group + pass * G + wave % G;
     const uint32_t row = rb * 32 + n;
     const bool valid = row < nrows;
     const bool active = rb * 32 < nrows;
@@ -232,7 +259,8 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     // read one block before that block's loads are issued.
     uint32_t page_a = 0, page_b = 0;
     const uint32_t last_entry = pos_last / page_tokens; // the tile's last table entry
-    auto fetch_pages_unchecked = [&](uint32_t kb) {
+    auto fetch_pages_unchecked = [&](uint32_t at) {
+        const uint32_t kb = in_table(at);
         using c32 = const __attribute__((address_space(4))) uint32_t;
         const auto* cb = (const __attribute__((address_space(4))) uint8_t*)(uintptr_t)table;
         page_a = *(c32*)(cb + 8 * kb);
@@ -275,12 +303,14 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
         load_full(pg0, pg1, lds_base + (kb % n_stages) * stage_bytes);
     };
     auto load_block = [&](uint32_t kb) {
-        const uint32_t key0 = kb * block_keys;
+        const uint32_t key0 = in_table(kb) * block_keys;
         const uint32_t pg0 = __builtin_amdgcn_readfirstlane(page_a);
         const uint32_t pg1 = __builtin_amdgcn_readfirstlane(page_b);
         fetch_pages(kb + 1);
         const uint32_t st = lds_base + (kb % n_stages) * stage_bytes;
-        if (key0 + block_keys - 1 <= pos_last) { // every key of the block is in the tile
+        const uint32_t end = key0 + block_keys - 1;
+        // every key of the block is in the tile
+        if (end <= pos_last && (!WINDOW || key0 >= low || end < window.sinks)) {
             load_full(pg0, pg1, st);
         } else {
             const uint8_t* k0 = kbytes + pg0 * page_bytes;
@@ -289,11 +319,12 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
             for (uint32_t r = 0; r < R; ++r) {
                 const uint32_t region = wave_u + r * W;
                 const uint8_t* vp = vbytes + (region >= 4 ? pg1 : pg0) * page_bytes;
-                const uint8_t* ksrc = key0 + k_key <= pos_last ? (k_hi ? k1 : k0) + k_off[r]
-                                                               : zbytes + k_feat[r] * 2;
+                const uint8_t* ksrc = some_row_attends(key0 + k_key)
+                    ? (k_hi ? k1 : k0) + k_off[r]
+                    : zbytes + k_feat[r] * 2;
                 dma16(ksrc, st + region * 1024);
-                const uint8_t* vsrc = key0 + vd_key[r] <= pos_last ? vp + v_off[r]
-                                                                   : zbytes + (lane & 15) * 16;
+                const uint8_t* vsrc = some_row_attends(key0 + vd_key[r]) ? vp + v_off[r]
+                                                                         : zbytes + (lane & 15) * 16;
                 dma16(vsrc, st + k_stage_bytes + region * vg_bytes);
             }
         }
@@ -350,27 +381,51 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
                 va[mt][h] = make_uint4(l2.x, l2.y, h2.x, h2.y);
             }
     };
-    auto probabilities = [&](uint4 (&pt)[2]) {
-        exponentiate<SPLIT>(sp, m, l, c);
+    auto probabilities = [&](uint4 (&pt)[terms][2]) {
+        exponentiate<SPLIT>(sp, m, l, c, p_scale);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            pt[h] = make_uint4(pack2<F16>(sp[8 * h + 0], sp[8 * h + 1]),
-                               pack2<F16>(sp[8 * h + 2], sp[8 * h + 3]),
-                               pack2<F16>(sp[8 * h + 4], sp[8 * h + 5]),
-                               pack2<F16>(sp[8 * h + 6], sp[8 * h + 7]));
+        for (int h = 0; h < 2; ++h) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                w[i] = pack2<F16>(sp[8 * h + 2 * i], sp[8 * h + 2 * i + 1]);
+            pt[0][h] = make_uint4(w[0], w[1], w[2], w[3]);
+            if constexpr (terms == 2) { // what the first term's rounding left
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = pack2<F16>(sp[8 * h + 2 * i] - word_value<F16>(w[i], 0),
+                                      sp[8 * h + 2 * i + 1] - word_value<F16>(w[i], 1));
+                pt[1][h] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
     };
-    auto pv = [&](const uint4 (&va)[4][2], const uint4 (&pt)[2]) {
+    auto pv = [&](const uint4 (&va)[4][2], const uint4 (&pt)[terms][2]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int mt = 0; mt < 4; ++mt)
-                o[mt] = mfma<F16>(va[mt][h], pt[h], o[mt]);
+            for (int t = 0; t < terms; ++t)
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt)
+                    o[mt] = mfma<F16>(va[mt][h], pt[t][h], o[mt]);
     };
     // causal mask and maxima of S(kb); moves it to sp; true when some lane's
     // maximum grew past the rescale threshold (m = -inf before block 0).
     // `clear`: block kb is known to end before the q-block's first position.
+    const uint32_t q_low = WINDOW ? window_low(qpos, window) : 0;
+    const uint32_t low_hi = WINDOW
+        ? __builtin_amdgcn_readfirstlane(window_low(pos0 + min(rb * 32 + 31, nrows - 1), window))
+        : 0;
     auto stats = [&](uint32_t kb, bool clear) {
-        const uint32_t key0 = kb * block_keys;
+        const uint32_t key0 = in_table(kb) * block_keys;
+        // some row's window begins past the block's first key, and not all of it are sinks
+        if (WINDOW && key0 < low_hi && key0 + block_keys - 1 >= window.sinks) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const uint32_t kpos = key0 + 16 * (r >> 3) + 8 * g + (r & 7);
+                if (kpos < q_low && kpos >= window.sinks)
+                    sc[r] = -__builtin_inff();
+            }
+        }
         if (!clear && key0 + block_keys - 1 > pos_lo) { // the diagonal crosses this block
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -459,7 +514,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
         else
             __builtin_amdgcn_s_setprio(0);
         uint4 ka[8], va[4][2];
-        uint4 pt[2];
+        uint4 pt[terms][2];
         read_k(kb, ka);
         // the K operand reads go out before the exponentials
         __builtin_amdgcn_sched_barrier(0);
@@ -550,7 +605,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
             else if (kb + 2 < kb_end)
                 load_block(kb + 2);
             uint4 ka[8], va[4][2];
-            uint4 pt[2];
+            uint4 pt[terms][2];
             read_k(kb, ka);
             __builtin_amdgcn_sched_barrier(0);
             probabilities(pt); // vector: block kb - 1
@@ -564,15 +619,16 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
                 rescale();
         };
         uint32_t kb = kb_begin + 1;
-        for (; kb + 2 < kb_end && kb + 3 < n_blocks; ++kb)
-            iteration4(kb, std::true_type {});
+        if constexpr (!WINDOW) // blocks at the gap's edges need the checks
+            for (; kb + 2 < kb_end && kb + 3 < n_blocks; ++kb)
+                iteration4(kb, std::true_type {});
         for (; kb < kb_end; ++kb)
             iteration4(kb, std::false_type {});
     }
     // the last block's probabilities and product
     {
         uint4 va[4][2];
-        uint4 pt[2];
+        uint4 pt[terms][2];
         probabilities(pt);
         read_v(kb_end - 1, va);
         pv(va, pt);
@@ -587,7 +643,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
         // bytes per access. The share that arrives last folds every share's
         // record, its own included, in share order (the result does not
         // depend on the order of arrival), with weights 2^(m_s - M).
-        const uint32_t pair = (tile * subs + sub) * kv_heads + kvh;
+        const uint32_t pair = ((tile * subs + sub) * passes + pass) * kv_heads + kvh;
         const uint32_t qv = wave * 32 + n; // this lane's query vector in the workgroup
         constexpr uint32_t QV = 32 * W, chunks = prefill_record_floats / 4;
         const __amdgpu_buffer_rsrc_t rs = record_rsrc(
@@ -661,37 +717,64 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
         // lt > 0 for a valid row: the tile's first share attends key 0
     }
 
-    if (!active || !valid)
-        return;
     const float inv = 1.0f / lt;
     uint16_t* dst = out + qoff;
+    uint32_t alone = 0; // the q-block's rows that are attended again
+    if constexpr (WINDOW) {
+        // 0 unless some result of the query is infinite or NaN (either lane half)
+        float odd = inv * 0.0f;
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
+        for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-        for (int quad = 0; quad < 4; ++quad) {
-            const uint32_t f = 32 * mt + 8 * quad + 4 * g;
-            const f32x16_t& acc = o[mt];
-            float x[4] = { acc[4 * quad] * inv, acc[4 * quad + 1] * inv,
-                           acc[4 * quad + 2] * inv, acc[4 * quad + 3] * inv };
-            if (gate) { // sigmoid_mul (src/qwen/qwen_layer.cc:204) in the epilogue
-                const uint2 gv = *reinterpret_cast<const uint2*>(gate + qoff + f);
-                const uint32_t w[2] = { gv.x, gv.y };
+            for (int r = 0; r < 16; ++r)
+                odd = __builtin_fmaf(o[mt][r], 0.0f, odd);
+        const uint64_t odd_lanes = __ballot(valid && odd != 0.0f);
+        alone = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
+    }
+    if (active && valid && !(alone >> n & 1)) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    x[e] *= sigmoid(half_value<F16>((uint16_t)(w[e / 2] >> (16 * (e % 2)))));
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int quad = 0; quad < 4; ++quad) {
+                const uint32_t f = 32 * mt + 8 * quad + 4 * g;
+                const f32x16_t& acc = o[mt];
+                float x[4] = { acc[4 * quad] * inv, acc[4 * quad + 1] * inv,
+                               acc[4 * quad + 2] * inv, acc[4 * quad + 3] * inv };
+                if (gate) { // sigmoid_mul (src/qwen/qwen_layer.cc:204) in the epilogue
+                    const uint2 gv = *reinterpret_cast<const uint2*>(gate + qoff + f);
+                    const uint32_t w[2] = { gv.x, gv.y };
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        x[e] *= sigmoid(half_value<F16>((uint16_t)(w[e / 2] >> (16 * (e % 2)))));
+                }
+                *reinterpret_cast<uint2*>(dst + f) =
+                    make_uint2(pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]));
             }
-            *reinterpret_cast<uint2*>(dst + f) =
-                make_uint2(pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]));
+    }
+    if constexpr (WINDOW) {
+        if (__builtin_expect(alone == 0, 1))
+            return;
+        const size_t first = (size_t)(row0 + rb * 32) * q_stride + (size_t)head * dim;
+        for (uint32_t left = alone; left;) {
+            uint32_t some = left; // the lowest alone_queries of them
+#pragma unroll
+            for (uint32_t i = 0; i < alone_queries; ++i)
+                left &= left - 1;
+            some ^= left;
+            attend_alone<dim, F16 ? CKV_F16 : CKV_BF16, true>(
+                kbase, vbase, table, F, __builtin_amdgcn_readfirstlane(some), pos_lo, q + first,
+                q_stride, c, gate ? gate + first : nullptr, out + first, lane, window);
         }
+    }
 }
 
-template <int G, int W>
+template <int G, int W, bool WINDOW = false>
 hipError_t launch_gw(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
                      const void* q, uint32_t q_heads, float c, void* out, const void* gate,
                      prefill_split split)
 {
     const uint64_t grid = (uint64_t)m.n_tiles * (256 / (32 * W / G)) * p.kv_heads
-        * (W == 4 ? split.n_split : 1);
+        * (WINDOW ? q_heads / p.kv_heads / G : 1) * (W == 4 ? split.n_split : 1);
     if (!grid)
         return hipSuccess;
     if (grid > 0x7FFFFFFFull)
@@ -704,16 +787,16 @@ hipError_t launch_gw(hipStream_t s, const pool_view& p, const meta_view& m, uint
     const bool f16 = p.dtype == CKV_F16;
     const dim3 g((uint32_t)grid), b(64 * W);
     if (f16 && wide)
-        hipLaunchKernelGGL((prefill_kernel<G, true, true, W>), g, b, 0, s, p, m, layer, qq, oo,
+        hipLaunchKernelGGL((prefill_kernel<G, true, true, W, WINDOW>), g, b, 0, s, p, m, layer, qq, oo,
                            q_heads, c, gg, split);
     else if (f16)
-        hipLaunchKernelGGL((prefill_kernel<G, true, false, W>), g, b, 0, s, p, m, layer, qq, oo,
+        hipLaunchKernelGGL((prefill_kernel<G, true, false, W, WINDOW>), g, b, 0, s, p, m, layer, qq, oo,
                            q_heads, c, gg, split);
     else if (wide)
-        hipLaunchKernelGGL((prefill_kernel<G, false, true, W>), g, b, 0, s, p, m, layer, qq, oo,
+        hipLaunchKernelGGL((prefill_kernel<G, false, true, W, WINDOW>), g, b, 0, s, p, m, layer, qq, oo,
                            q_heads, c, gg, split);
     else
-        hipLaunchKernelGGL((prefill_kernel<G, false, false, W>), g, b, 0, s, p, m, layer, qq, oo,
+        hipLaunchKernelGGL((prefill_kernel<G, false, false, W, WINDOW>), g, b, 0, s, p, m, layer, qq, oo,
                            q_heads, c, gg, split);
     return hipGetLastError();
 }
@@ -724,6 +807,8 @@ hipError_t launch_g(hipStream_t s, const pool_view& p, const meta_view& m, uint3
                     const prefill_shape_info& plan, prefill_split split)
 {
     if constexpr (G <= 4) {
+        if (m.window.window != all_keys.window)
+            return launch_gw<G, 4, true>(s, p, m, layer, q, q_heads, c, out, gate, split);
         if (plan.waves == 4)
             return launch_gw<G, 4>(s, p, m, layer, q, q_heads, c, out, gate, split);
     }
@@ -788,6 +873,23 @@ prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t
         }
         return plan;
     }
+    if (m.window.window != all_keys.window) {
+        // 4-wave workgroups, two to a compute unit; a launch that leaves some idle splits
+        // each tile's keys between as many as fill them
+        const uint32_t G = std::min(group, 4u), passes = group / G;
+        const uint64_t busy = (uint64_t)m.row_blocks[G == 4 ? 0 : G == 2 ? 1 : 2] * passes * p.kv_heads;
+        const uint64_t pairs = (uint64_t)m.n_tiles * (2 * G) * passes * p.kv_heads;
+        uint64_t split = busy && cu_count > 0 ? 2 * (uint64_t)cu_count / busy : 1;
+        if (const char* forced = std::getenv("CKV_PREFILL_SPLIT"))
+            split = (uint64_t)std::max(1L, std::strtol(forced, nullptr, 10));
+        plan.waves = 4;
+        plan.n_split = (uint32_t)std::clamp<uint64_t>(split, 1, split_max);
+        if (plan.n_split > 1) {
+            plan.records_floats = pairs * plan.n_split * 128 * prefill_record_floats;
+            plan.counters = pairs;
+        }
+        return plan;
+    }
     if (group == 0 || group > 4)
         return plan;
     const uint64_t grid8 = (uint64_t)m.n_tiles * group * p.kv_heads;
@@ -849,6 +951,8 @@ hipError_t launch_prefill(hipStream_t s, const pool_view& p, const meta_view& m,
     case 4:
         return launch_g<4>(s, p, m, layer, q, q_heads, c, out, gate, plan, split);
     case 8:
+        if (m.window.window != all_keys.window) // two workgroups of 4 heads
+            return launch_g<4>(s, p, m, layer, q, q_heads, c, out, gate, plan, split);
         return launch_g<8>(s, p, m, layer, q, q_heads, c, out, gate, plan, split);
     default:
         return hipErrorInvalidValue;

@@ -37,15 +37,14 @@
 // between up to 8 workgroups, as the 16-bit kernel does (kernels_prefill.hip):
 // each stores its unnormalised state as 16-byte records, and the last to
 // arrive folds them in range order.
+#include <type_traits>
+
+#include "attend_alone.h"
 #include "ckv_internal.h"
 #include "prefill_records.h"
 
 namespace ckv {
 namespace {
-
-constexpr float log2e = 1.4426950408889634f;
-
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr uint32_t dim = 128;
 constexpr uint32_t page_tokens = 16;
@@ -61,13 +60,8 @@ __device__ __forceinline__ f32x16_t mfma(float a, float b, const f32x16_t& c)
     return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
 }
 
-// 1 / (1 + e^-g) in float (src/metal/kernels/tensor_ops.metal:108-124 with sigmoid_only)
-__device__ __forceinline__ float sigmoid(float g)
-{
-    return 1.0f / (1.0f + __builtin_amdgcn_exp2f(-g * log2e));
-}
-
-template <int G>
+// WINDOW: rows attend through md.window, as in kernels_prefill.hip.
+template <int G, bool WINDOW>
 __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
     pool_view p, meta_view md, uint32_t layer, const float* __restrict__ q,
     float* __restrict__ out, uint32_t q_heads, float c, const float* __restrict__ gate,
@@ -96,7 +90,15 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
     const uint32_t pos0 = te.z + r0; // positions are consecutive inside a tile
     const uint32_t pos_last = pos0 + nrows - 1;
     const uint32_t* table = md.table + te.w;
-    const uint32_t n_blocks = pos_last / block_keys + 1;
+    // the first row's window begins at `low`, no later row's before it
+    const key_window window = md.window;
+    const uint32_t low = WINDOW ? window_low(pos0, window) : 0;
+    const window_gap gap = WINDOW ? window_gap_of(low, window.sinks, block_keys) : window_gap {};
+    auto in_table = [&](uint32_t kb) { return WINDOW && kb >= gap.kept ? kb + gap.skip : kb; };
+    auto some_row_attends = [&](uint32_t key) {
+        return key <= pos_last && (!WINDOW || key >= low || key < window.sinks);
+    };
+    const uint32_t n_blocks = pos_last / block_keys + 1 - gap.skip;
     const uint32_t last_entry = pos_last / page_tokens;
     // key blocks [kb_begin, kb_end) of this workgroup
     const uint32_t n_parts = prefill_range_count(n_blocks, n_split, split_scratch.min_blocks);
@@ -143,15 +145,15 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
     const uint64_t srow = (uint64_t)sr * p.features * 4 + scol;
     uint4 k_a, k_b, v_a, v_b; // the staged 16 bytes of each page's K and V row
     auto fetch = [&](uint32_t kb) __attribute__((always_inline)) {
-        const uint32_t key0 = kb * block_keys;
-        const uint64_t pa = table[2 * kb];
-        const uint64_t pb = table[min(2 * kb + 1, last_entry)];
+        const uint32_t key0 = in_table(kb) * block_keys;
+        const uint64_t pa = table[2 * in_table(kb)];
+        const uint64_t pb = table[min(2 * in_table(kb) + 1, last_entry)];
         k_a = k_b = v_a = v_b = make_uint4(0, 0, 0, 0);
-        if (key0 + sr <= pos_last) {
+        if (some_row_attends(key0 + sr)) {
             k_a = *reinterpret_cast<const uint4*>(kbase + pa * page_bytes + srow);
             v_a = *reinterpret_cast<const uint4*>(vbase + pa * page_bytes + srow);
         }
-        if (key0 + 16 + sr <= pos_last) {
+        if (some_row_attends(key0 + 16 + sr)) {
             k_b = *reinterpret_cast<const uint4*>(kbase + pb * page_bytes + srow);
             v_b = *reinterpret_cast<const uint4*>(vbase + pb * page_bytes + srow);
         }
@@ -170,6 +172,11 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
         o[a] = f32x16_t {};
     float m = -__builtin_inff(), l = 0.0f; // running maximum (log2 units), denominator share
 
+    const uint32_t q_low = WINDOW ? window_low(qpos, window) : 0;
+    const uint32_t low_hi = WINDOW
+        ? __builtin_amdgcn_readfirstlane(
+              window_low(pos0 + min((wave / G) * 32 + 31, nrows - 1), window))
+        : 0;
     auto attend = [&](uint32_t kb) __attribute__((always_inline)) {
         const uint8_t* st = lds + (kb % n_stages) * stage_bytes;
         // S^T = K . Q^T
@@ -184,10 +191,19 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
             s1 = mfma(kv.w, qr[4 * t + 3], s1);
         }
         // causal mask, scores in log2 units, the block maximum of the query
-        const uint32_t key0 = kb * block_keys;
+        const uint32_t key0 = in_table(kb) * block_keys;
         float s[16];
         float mx = -__builtin_inff();
-        if (key0 + block_keys - 1 <= pos_lo) { // every key precedes every query
+        if (WINDOW && key0 < low_hi && key0 + block_keys - 1 >= window.sinks) {
+            // some row's window begins past the block's first key, and not all of it are sinks
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const uint32_t key = key0 + 8 * (r >> 2) + 4 * h + (r & 3);
+                s[r] = key <= qpos && (key >= q_low || key < window.sinks) ? (s0[r] + s1[r]) * c
+                                                                           : -__builtin_inff();
+                mx = fmaxf(mx, s[r]);
+            }
+        } else if (key0 + block_keys - 1 <= pos_lo) { // every key precedes every query
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 s[r] = (s0[r] + s1[r]) * c;
@@ -323,32 +339,60 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
         // lt > 0 for a valid row: the tile's first range attends key 0
     }
 
-    if (!valid)
-        return;
     const float inv = 1.0f / lt;
     float* dst = out + qoff;
+    uint32_t alone = 0; // the q-block's rows that are attended again
+    if constexpr (WINDOW) {
+        // 0 unless some result of the query is infinite or NaN (either lane half)
+        float odd = inv * 0.0f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        // features 4 * (8 * (r / 4) + 4h + r % 4) + 0..3: accumulators 0..3
-        const uint32_t f = 32 * (r >> 2) + 16 * h + 4 * (r & 3);
-        float x[4] = { o[0][r] * inv, o[1][r] * inv, o[2][r] * inv, o[3][r] * inv };
-        if (gate) { // sigmoid_mul (src/qwen/qwen_layer.cc:204) in the epilogue
-            const float4 gv = *reinterpret_cast<const float4*>(gate + qoff + f);
-            x[0] *= sigmoid(gv.x);
-            x[1] *= sigmoid(gv.y);
-            x[2] *= sigmoid(gv.z);
-            x[3] *= sigmoid(gv.w);
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                odd = __builtin_fmaf(o[a][r], 0.0f, odd);
+        const uint64_t odd_lanes = __ballot(valid && odd != 0.0f);
+        alone = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
+    }
+    if (valid && !(alone >> n & 1)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            // features 4 * (8 * (r / 4) + 4h + r % 4) + 0..3: accumulators 0..3
+            const uint32_t f = 32 * (r >> 2) + 16 * h + 4 * (r & 3);
+            float x[4] = { o[0][r] * inv, o[1][r] * inv, o[2][r] * inv, o[3][r] * inv };
+            if (gate) { // sigmoid_mul (src/qwen/qwen_layer.cc:204) in the epilogue
+                const float4 gv = *reinterpret_cast<const float4*>(gate + qoff + f);
+                x[0] *= sigmoid(gv.x);
+                x[1] *= sigmoid(gv.y);
+                x[2] *= sigmoid(gv.z);
+                x[3] *= sigmoid(gv.w);
+            }
+            *reinterpret_cast<float4*>(dst + f) = make_float4(x[0], x[1], x[2], x[3]);
         }
-        *reinterpret_cast<float4*>(dst + f) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+    if constexpr (WINDOW) {
+        if (__builtin_expect(alone == 0, 1))
+            return;
+        const size_t first = (size_t)(row0 + (wave / G) * 32) * q_stride + (size_t)head * dim;
+        for (uint32_t left = alone; left;) {
+            uint32_t some = left; // the lowest alone_queries of them
+#pragma unroll
+            for (uint32_t i = 0; i < alone_queries; ++i)
+                left &= left - 1;
+            some ^= left;
+            attend_alone<dim, CKV_F32, true>(
+                reinterpret_cast<const float*>(kbase), reinterpret_cast<const float*>(vbase), table,
+                p.features, __builtin_amdgcn_readfirstlane(some), pos_lo, q + first, q_stride, c,
+                gate ? gate + first : nullptr, out + first, lane, window);
+        }
     }
 }
 
-template <int G>
+template <int G, bool WINDOW>
 hipError_t launch_g(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
                     const void* q, uint32_t q_heads, float c, void* out, uint32_t grid,
                     const void* gate, prefill_split split)
 {
-    hipLaunchKernelGGL((prefill_f32_kernel<G>), dim3(grid), dim3(64 * waves), 0, s, p, m, layer,
+    hipLaunchKernelGGL((prefill_f32_kernel<G, WINDOW>), dim3(grid), dim3(64 * waves), 0, s, p, m, layer,
                        static_cast<const float*>(q), static_cast<float*>(out), q_heads, c,
                        static_cast<const float*>(gate), split);
     return hipGetLastError();
@@ -370,18 +414,24 @@ hipError_t launch_prefill_f32(hipStream_t s, const pool_view& p, const meta_view
     if (grid > 0x7FFFFFFFull)
         return hipErrorInvalidValue;
     const float c = scale * log2e;
-    switch (group) {
-    case 1:
-        return launch_g<1>(s, p, m, layer, q, q_heads, c, out, (uint32_t)grid, gate, split);
-    case 2:
-        return launch_g<2>(s, p, m, layer, q, q_heads, c, out, (uint32_t)grid, gate, split);
-    case 4:
-        return launch_g<4>(s, p, m, layer, q, q_heads, c, out, (uint32_t)grid, gate, split);
-    case 8:
-        return launch_g<8>(s, p, m, layer, q, q_heads, c, out, (uint32_t)grid, gate, split);
-    default:
-        return hipErrorInvalidValue;
-    }
+    const uint32_t n = (uint32_t)grid;
+    const auto launch = [&](auto windowed) {
+        constexpr bool WINDOW = decltype(windowed)::value;
+        switch (group) {
+        case 1:
+            return launch_g<1, WINDOW>(s, p, m, layer, q, q_heads, c, out, n, gate, split);
+        case 2:
+            return launch_g<2, WINDOW>(s, p, m, layer, q, q_heads, c, out, n, gate, split);
+        case 4:
+            return launch_g<4, WINDOW>(s, p, m, layer, q, q_heads, c, out, n, gate, split);
+        case 8:
+            return launch_g<8, WINDOW>(s, p, m, layer, q, q_heads, c, out, n, gate, split);
+        default:
+            return hipErrorInvalidValue;
+        }
+    };
+    return m.window.window != all_keys.window ? launch(std::true_type {})
+                                              : launch(std::false_type {});
 }
 
 } // namespace ckv

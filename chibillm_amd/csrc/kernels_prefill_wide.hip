@@ -41,12 +41,12 @@
 // rescales; the third term adds about 480. Issuing the loads in twos between those
 // phases took 64.1 to 64.7 us in all instead of 62.3; reading both halves of V
 // before the scores 64.7.
+#include "attend_alone.h"
 #include "ckv_internal.h"
 #include "prefill_records.h"
 #include "prefill_tile.h"
 
 #include <algorithm>
-#include <cfloat>
 #include <cstdlib>
 
 namespace ckv {
@@ -74,23 +74,16 @@ constexpr uint32_t v_half_bytes = 8 * vg_bytes;
 constexpr uint32_t v_stage_bytes = 2 * v_half_bytes;
 constexpr uint32_t regions = 4; // K regions, and V groups, a wave stages per block
 
-// 16-bit terms of a probability.
-constexpr int terms = 3;
+// 16-bit terms of a probability. Through a window two: 16 bits in bf16, 22 in fp16,
+// far below an output's rounding (8 and 11 bits) for rows that come and go with it.
+template <bool WINDOW>
+constexpr int p_terms = WINDOW ? 2 : 3;
 // Scale of fp16 probabilities (log2): with the running maximum up to 2^8 stale
 // they reach 2^14, within fp16's range.
 constexpr float p_scale_f16 = 6.0f;
 
 // The source of masked K and V rows.
 __device__ const uint4 zero_row[32] = {};
-
-template <bool F16>
-__device__ __forceinline__ float word_value(uint32_t w, int e)
-{
-    if constexpr (F16)
-        return half_value<true>(static_cast<uint16_t>(w >> (16 * e)));
-    else
-        return __builtin_bit_cast(float, e ? w & 0xFFFF0000u : w << 16);
-}
 
 __device__ __forceinline__ void wait_all_but(uint32_t loads)
 {
@@ -104,149 +97,18 @@ __device__ __forceinline__ void wait_all_but(uint32_t loads)
         __builtin_amdgcn_s_waitcnt(0x0F70);
 }
 
-// Sum over each row of 16 lanes, result in every lane of the row.
-__device__ __forceinline__ float row16_sum(float v)
-{
-    auto add = [&](int moved) { v += __builtin_bit_cast(float, moved); };
-    const auto bits = [&]() { return __builtin_bit_cast(int, v); };
-    add(__builtin_amdgcn_mov_dpp(bits(), 0xB1, 0xF, 0xF, true));  // quad_perm [1,0,3,2]
-    add(__builtin_amdgcn_mov_dpp(bits(), 0x4E, 0xF, 0xF, true));  // quad_perm [2,3,0,1]
-    add(__builtin_amdgcn_mov_dpp(bits(), 0x141, 0xF, 0xF, true)); // row_half_mirror
-    add(__builtin_amdgcn_mov_dpp(bits(), 0x140, 0xF, 0xF, true)); // row_mirror
-    return v;
-}
-
-// Up to alone_queries rows of one query head (bits of `rows`, from row r0 on) against
-// their keys by vector arithmetic: what a wave falls back to for the queries to
-// which the tile gave a value that is not finite. A product with P^T
-// multiplies every key of a block for all its queries, so an infinity or NaN
-// in a V row also meets the zeros of the queries that do not attend it (and of a
-// low term), and 0 * inf is NaN; the decode kernels give such a row only to the
-// queries that attend it, and so does this. Sixteen lanes hold a row, four rows
-// a step, the next step's in flight; finite results never come here. An infinity
-// early in a shared prefix sends every query of a launch here, so a K/V row read
-// and widened serves several queries: with one in the first page of each
-// sequence the launch below takes 1.81 ms (two at a time 2.29, eight 1.96, one
-// 5.84; the general path took 3.93 for these rows). The cost grows with the
-// rows' positions, as theirs did.
-constexpr uint32_t alone_queries = 4;
-
-template <bool F16>
-__device__ __forceinline__ void attend_alone(const uint16_t* __restrict__ keys,
-                                             const uint16_t* __restrict__ values,
-                                             const uint32_t* __restrict__ table, uint32_t F,
-                                             uint32_t rows, uint32_t pos0, const uint16_t* q,
-                                             size_t q_stride, float c, const uint16_t* gate,
-                                             uint16_t* out, uint32_t lane)
-{
-    constexpr uint32_t each = dim / 16, Q = alone_queries;
-    const uint32_t f = (lane & 15) * each, sub = lane >> 4;
-    struct words {
-        u32x4_t w[2];
-    };
-    auto load = [&](const uint16_t* at) {
-        return words { { reinterpret_cast<const u32x4_t*>(at + f)[0],
-                         reinterpret_cast<const u32x4_t*>(at + f)[1] } };
-    };
-    auto widen = [](const words& r, float (&x)[each]) {
-#pragma unroll
-        for (uint32_t i = 0; i < each; ++i)
-            x[i] = word_value<F16>(r.w[i / 8][i / 2 % 4], i % 2);
-    };
-    auto weight = [&](float ms, float to) { return __builtin_amdgcn_exp2f((ms - to) * c); };
-    // the rows (the first again in the places left over) and their states, which
-    // start at the lowest finite maximum: without keys a state weighs 0 or holds 0
-    uint32_t row[Q], count = 0;
-    float qf[Q][each], acc[Q][each], m[Q], l[Q];
-#pragma unroll
-    for (uint32_t i = 0; i < Q; ++i) {
-        row[i] = rows ? __builtin_ctz(rows) : row[0];
-        count += rows != 0;
-        rows &= rows - (rows != 0);
-        widen(load(q + row[i] * q_stride), qf[i]);
-        m[i] = -FLT_MAX;
-        l[i] = 0.0f;
-#pragma unroll
-        for (uint32_t j = 0; j < each; ++j)
-            acc[i][j] = 0.0f;
-    }
-    const uint32_t last = pos0 + row[count - 1]; // the rows ascend
-    uint32_t page = table[0];
-    auto at_key = [&](uint32_t key) { // in the page at hand; past the last key, that one
-        return ((uint64_t)page * page_tokens + min(key, last) % page_tokens) * F;
-    };
-    words k_next = load(keys + at_key(sub)), v_next = load(values + at_key(sub));
-#pragma unroll 1
-    for (uint32_t key0 = 0; key0 <= last; key0 += 4) {
-        const words k_now = k_next, v_now = v_next;
-        const uint32_t key = key0 + sub, next = key0 + 4;
-        if (next <= last) {
-            if (next % page_tokens == 0)
-                page = table[next / page_tokens];
-            k_next = load(keys + at_key(next + sub));
-            v_next = load(values + at_key(next + sub));
-        }
-        float x[each], s[Q];
-        widen(k_now, x);
-#pragma unroll
-        for (uint32_t i = 0; i < Q; ++i) {
-            s[i] = 0.0f;
-#pragma unroll
-            for (uint32_t j = 0; j < each; ++j)
-                s[i] = __builtin_fmaf(qf[i][j], x[j], s[i]);
-            s[i] = row16_sum(s[i]);
-        }
-        widen(v_now, x);
-#pragma unroll
-        for (uint32_t i = 0; i < Q; ++i)
-            if (key <= pos0 + row[i]) {
-                const float m_new = fmaxf(m[i], s[i]);
-                const float keep = weight(m[i], m_new), w = weight(s[i], m_new);
-                m[i] = m_new;
-                l[i] = l[i] * keep + w;
-#pragma unroll
-                for (uint32_t j = 0; j < each; ++j)
-                    acc[i][j] = acc[i][j] * keep + w * x[j];
-            }
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < Q; ++i) {
-#pragma unroll
-        for (uint32_t d = 16; d < 64; d *= 2) {
-            const float m_other = __shfl_xor(m[i], d), l_other = __shfl_xor(l[i], d);
-            const float m_new = fmaxf(m[i], m_other);
-            const float keep = weight(m[i], m_new), w = weight(m_other, m_new);
-            m[i] = m_new;
-            l[i] = l[i] * keep + l_other * w;
-#pragma unroll
-            for (uint32_t j = 0; j < each; ++j) {
-                const float other = __shfl_xor(acc[i][j], d);
-                acc[i][j] = acc[i][j] * keep + other * w;
-            }
-        }
-        if (i >= count || sub)
-            continue;
-        const float inv = 1.0f / l[i];
-        const size_t at = row[i] * q_stride + f;
-#pragma unroll
-        for (uint32_t j = 0; j < each; j += 2) {
-            float y[2] = { acc[i][j] * inv, acc[i][j + 1] * inv };
-            if (gate)
-                for (int e = 0; e < 2; ++e)
-                    y[e] *= sigmoid(half_value<F16>(gate[at + j + e]));
-            *reinterpret_cast<uint32_t*>(out + at + j) = pack2<F16>(y[0], y[1]);
-        }
-    }
-}
-
-// FAR: a layer spans more than 4 GiB, so page offsets take 64 bits.
-template <int G, bool F16, bool FAR>
+// FAR: a layer spans more than 4 GiB, so page offsets take 64 bits. WINDOW: blocks
+// that no row of the workgroup attends are left out of the count (in_table gives a
+// block's place); keys that none attends in the blocks at the gap's edges are staged
+// from the zero row, so what they hold never enters a product.
+template <int G, bool F16, bool FAR, bool WINDOW>
 __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
     pool_view p, meta_view md, uint32_t layer, const uint16_t* __restrict__ q,
     uint16_t* __restrict__ out, uint32_t q_heads, float c, const uint16_t* __restrict__ gate,
     prefill_split split_scratch)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[n_stages * (k_stage_bytes + v_stage_bytes)];
+    constexpr int terms = p_terms<WINDOW>;
     constexpr uint32_t tile_rows = 32 * waves / G;
     constexpr uint32_t subs = prefill_tile_rows / tile_rows; // workgroups per (tile, head pass, kv head)
 
@@ -272,7 +134,19 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
     const uint32_t pos0 = te.z + r0;
     const uint32_t pos_last = pos0 + nrows - 1;
     const uint32_t* table = md.table + te.w;
-    const uint32_t n_blocks = pos_last / block_keys + 1;
+    // the first row's window begins at `low`, no later row's before it
+    const key_window window = md.window;
+    const uint32_t low = WINDOW ? window_low(pos0, window) : 0;
+    const window_gap gap = WINDOW ? window_gap_of(low, window.sinks, block_keys) : window_gap {};
+    auto in_table = [&](uint32_t kb) { return WINDOW && kb >= gap.kept ? kb + gap.skip : kb; };
+    auto some_row_attends = [&](uint32_t key) {
+        return key <= pos_last && (!WINDOW || key >= low || key < window.sinks);
+    };
+    auto all_in_tile = [&](uint32_t key0) { // no key of the block needs the zero row
+        const uint32_t end = key0 + block_keys - 1;
+        return end <= pos_last && (!WINDOW || key0 >= low || end < window.sinks);
+    };
+    const uint32_t n_blocks = pos_last / block_keys + 1 - gap.skip;
     const uint32_t n_parts = prefill_range_count(n_blocks, n_split, split_scratch.min_blocks);
     if (part >= n_parts)
         return;
@@ -336,8 +210,8 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
         return FAR ? page * page_bytes : (uint64_t)(page * (uint32_t)page_bytes);
     };
     auto load_k = [&](uint32_t kb, uint32_t pg0, uint32_t pg1) {
-        const uint32_t key0 = kb * block_keys;
-        const bool whole = key0 + block_keys - 1 <= pos_last;
+        const uint32_t key0 = in_table(kb) * block_keys;
+        const bool whole = all_in_tile(key0);
 #pragma unroll
         for (uint32_t r = 0; r < regions; ++r) { // the block's page r / 2, rows 8 * (r % 2) ..
             const uint32_t st = lds_base + k_stage(kb) + (wave + 4 * r) * 1024;
@@ -345,14 +219,14 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
             if (whole) {
                 dma16_s(pk, k_off[r % 2], st);
             } else {
-                const bool live = key0 + page_tokens * (r / 2) + k_row[r % 2] <= pos_last;
+                const bool live = some_row_attends(key0 + page_tokens * (r / 2) + k_row[r % 2]);
                 dma16(live ? pk + k_off[r % 2] : zbytes + n * 16, st);
             }
         }
     };
     auto load_v = [&](uint32_t kb, uint32_t pg0, uint32_t pg1) {
-        const uint32_t key0 = kb * block_keys;
-        const bool whole = key0 + block_keys - 1 <= pos_last;
+        const uint32_t key0 = in_table(kb) * block_keys;
+        const bool whole = all_in_tile(key0);
 #pragma unroll
         for (uint32_t r = 0; r < regions; ++r) { // half r / 2, the block's page r % 2
             const uint32_t st = lds_base + v_stage(kb) + (r / 2) * v_half_bytes
@@ -361,7 +235,7 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
             if (whole) {
                 dma16_s(pv, v_off, st);
             } else {
-                const bool live = key0 + page_tokens * (r % 2) + v_key <= pos_last;
+                const bool live = some_row_attends(key0 + page_tokens * (r % 2) + v_key);
                 dma16(live ? pv + v_off : zbytes + (lane & 15) * 16, st);
             }
         }
@@ -457,9 +331,21 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
                     o[4 * half + mt] = mfma<F16>(va[mt][h], pt[t][h], o[4 * half + mt]);
     };
     // causal mask and maxima of block kb's scores, which become sp
+    const uint32_t q_low = WINDOW ? window_low(qpos, window) : 0;
+    const uint32_t low_hi = WINDOW ? window_low(pos0 + min(rb * 32 + 31, nrows - 1), window) : 0;
     auto stats = [&](uint32_t kb, const f32x16_t& s) {
         sp = s;
-        const uint32_t key0 = kb * block_keys;
+        const uint32_t key0 = in_table(kb) * block_keys;
+        // some row's window begins past the block's first key, and not all of it are sinks
+        if (WINDOW && key0 < low_hi && key0 + block_keys - 1 >= window.sinks) {
+            asm volatile("");
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const uint32_t kpos = key0 + 16 * (r >> 3) + 8 * g + (r & 7);
+                if (kpos < q_low && kpos >= window.sinks)
+                    sp[r] = -__builtin_inff();
+            }
+        }
         if (key0 + block_keys - 1 > pos_lo) {
             asm volatile(""); // a branch: most blocks end before the diagonal
 #pragma unroll
@@ -495,8 +381,8 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
         uint32_t pg[4][2];
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-            pg[i][0] = page_of(2 * (b + i));
-            pg[i][1] = page_of(2 * (b + i) + 1);
+            pg[i][0] = page_of(2 * in_table(b + i));
+            pg[i][1] = page_of(2 * in_table(b + i) + 1);
         }
         auto first_k = [&](uint32_t i) {
             if (b + i < kb_end)
@@ -523,8 +409,8 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
         read_k(min(b + 1, kb_end - 1));
         stats(b, s);
         rescale();
-        pk0 = page_of(2 * (b + 4));
-        pk1 = page_of(2 * (b + 4) + 1);
+        pk0 = page_of(2 * in_table(b + 4));
+        pk1 = page_of(2 * in_table(b + 4) + 1);
         pw0 = pg[3][0];
         pw1 = pg[3][1];
         wait_all_but(b + 3 < kb_end ? 3 * regions : 0); // K(b + 2) and V(b)
@@ -563,8 +449,8 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
         pv(1, vb, pt);
         pw0 = pk0;
         pw1 = pk1;
-        pk0 = page_of(2 * (kb + 4));
-        pk1 = page_of(2 * (kb + 4) + 1);
+        pk0 = page_of(2 * in_table(kb + 4));
+        pk1 = page_of(2 * in_table(kb + 4) + 1);
         const bool grew = stats(kb, s); // vector: block kb
         wait_all_but(newest);
         __syncthreads();
@@ -691,14 +577,14 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
         for (uint32_t i = 0; i < alone_queries; ++i)
             left &= left - 1;
         some ^= left;
-        attend_alone<F16>(static_cast<const uint16_t*>(p.keys) + base_elems,
-                          static_cast<const uint16_t*>(p.values) + base_elems, table, F, some,
-                          pos_lo, q + first, q_stride, c, gate ? gate + first : nullptr,
-                          out + first, lane);
+        attend_alone<dim, F16 ? CKV_F16 : CKV_BF16, WINDOW>(
+            static_cast<const uint16_t*>(p.keys) + base_elems,
+            static_cast<const uint16_t*>(p.values) + base_elems, table, F, some, pos_lo, q + first,
+            q_stride, c, gate ? gate + first : nullptr, out + first, lane, window);
     }
 }
 
-template <int G>
+template <int G, bool WINDOW>
 hipError_t launch_g(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
                     const void* q, uint32_t q_heads, float c, void* out, const void* gate,
                     uint32_t grid, prefill_split split)
@@ -710,13 +596,13 @@ hipError_t launch_g(hipStream_t s, const pool_view& p, const meta_view& m, uint3
     const auto* gg = static_cast<const uint16_t*>(gate);
     const dim3 blocks(grid), threads(64 * waves);
     if (f16 && far)
-        prefill_wide_kernel<G, true, true><<<blocks, threads, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
+        prefill_wide_kernel<G, true, true, WINDOW><<<blocks, threads, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
     else if (f16)
-        prefill_wide_kernel<G, true, false><<<blocks, threads, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
+        prefill_wide_kernel<G, true, false, WINDOW><<<blocks, threads, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
     else if (far)
-        prefill_wide_kernel<G, false, true><<<blocks, threads, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
+        prefill_wide_kernel<G, false, true, WINDOW><<<blocks, threads, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
     else
-        prefill_wide_kernel<G, false, false><<<blocks, threads, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
+        prefill_wide_kernel<G, false, false, WINDOW><<<blocks, threads, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
     return hipGetLastError();
 }
 
@@ -767,14 +653,20 @@ hipError_t launch_prefill_wide(hipStream_t s, const pool_view& p, const meta_vie
     if (grid > 0x7FFFFFFFull)
         return hipErrorInvalidValue;
     const float c = scale * log2e;
-    switch (G) {
-    case 1:
-        return launch_g<1>(s, p, m, layer, q, q_heads, c, out, gate, (uint32_t)grid, split);
-    case 2:
-        return launch_g<2>(s, p, m, layer, q, q_heads, c, out, gate, (uint32_t)grid, split);
-    default:
-        return launch_g<4>(s, p, m, layer, q, q_heads, c, out, gate, (uint32_t)grid, split);
-    }
+    const uint32_t n = (uint32_t)grid;
+    const auto launch = [&](auto windowed) {
+        constexpr bool WINDOW = decltype(windowed)::value;
+        switch (G) {
+        case 1:
+            return launch_g<1, WINDOW>(s, p, m, layer, q, q_heads, c, out, gate, n, split);
+        case 2:
+            return launch_g<2, WINDOW>(s, p, m, layer, q, q_heads, c, out, gate, n, split);
+        default:
+            return launch_g<4, WINDOW>(s, p, m, layer, q, q_heads, c, out, gate, n, split);
+        }
+    };
+    return m.window.window != all_keys.window ? launch(std::true_type {})
+                                              : launch(std::false_type {});
 }
 
 } // namespace ckv
