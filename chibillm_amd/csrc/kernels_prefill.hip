@@ -847,6 +847,8 @@ bool prefill_supported(const pool_view& p, uint32_t q_heads, const void* q, cons
 // a launch of more than half a round of 8-wave workgroups, and less than one,
 // takes 4-wave workgroups unless its shortest tile attends more 32-key blocks
 constexpr uint32_t sub_round_max_blocks = 40;
+// Shortest key range of a windowed f32 tile, in blocks.
+constexpr uint32_t window_min_blocks_f32 = 2;
 
 prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t q_heads,
                                 int cu_count)
@@ -857,6 +859,7 @@ prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t
         plan.min_blocks = (uint32_t)std::max(1L, std::strtol(forced, nullptr, 10));
     if (p.head_dim == 256)
         return prefill_wide_plan(p, m, q_heads, cu_count, plan.min_blocks);
+    const bool windowed = m.window.window != all_keys.window;
     if (p.dtype == CKV_F32) {
         // f32 pools: 8-wave workgroups, two to a compute unit; a launch that
         // gives at most one to each splits its long tiles' keys to fill them
@@ -867,13 +870,15 @@ prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t
         if (const char* forced = std::getenv("CKV_PREFILL_SPLIT"))
             split = (uint64_t)std::max(1L, std::strtol(forced, nullptr, 10));
         plan.n_split = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(split, 1), split_max);
+        if (windowed && !std::getenv("CKV_PREFILL_SPLIT_MIN"))
+            plan.min_blocks = window_min_blocks_f32;
         if (plan.n_split > 1) {
             plan.records_floats = grid * plan.n_split * 256 * prefill_record_floats;
             plan.counters = grid;
         }
         return plan;
     }
-    if (m.window.window != all_keys.window) {
+    if (windowed) {
         // 4-wave workgroups, two to a compute unit; a launch that leaves some idle splits
         // each tile's keys between as many as fill them
         const uint32_t G = std::min(group, 4u), passes = group / G;

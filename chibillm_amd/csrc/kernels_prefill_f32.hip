@@ -177,6 +177,16 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
         ? __builtin_amdgcn_readfirstlane(
               window_low(pos0 + min((wave / G) * 32 + 31, nrows - 1), window))
         : 0;
+    // Whether some row of the wave attends a key of the block (uniform over the wave). A
+    // block costs a wave 3.4 us, so those of the tile's other rows are left to them.
+    const uint32_t pos_hi = __builtin_amdgcn_readfirstlane(
+        pos0 + min((wave / G) * 32 + 31, nrows - 1));
+    const uint32_t low_lo = WINDOW ? window_low(pos_lo, window) : 0;
+    auto needed = [&](uint32_t kb) {
+        const uint32_t key0 = in_table(kb) * block_keys;
+        return pos_lo <= pos_hi && key0 <= pos_hi
+            && (key0 + block_keys - 1 >= low_lo || key0 < window.sinks);
+    };
     auto attend = [&](uint32_t kb) __attribute__((always_inline)) {
         const uint8_t* st = lds + (kb % n_stages) * stage_bytes;
         // S^T = K . Q^T
@@ -256,7 +266,8 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
         const bool more = kb + 1 < kb_end; // workgroup-uniform
         if (more)
             fetch(kb + 1);
-        attend(kb);
+        if (!WINDOW || needed(kb))
+            attend(kb);
         if (more)
             store(kb + 1); // stage (kb + 1) % 2 was last read in iteration kb - 1
         __syncthreads();
