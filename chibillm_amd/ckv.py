@@ -26,7 +26,6 @@ _sz = C.c_size_t
 _vp = C.c_void_p
 _u32p = C.POINTER(C.c_uint32)
 _i32p = C.POINTER(C.c_int32)
-_u8p = C.POINTER(C.c_uint8)
 _f = C.c_float
 _i = C.c_int
 
@@ -86,8 +85,8 @@ _SIGNATURES = [
     ("ckv_rope_append_decode_window", _i, [_vp, _sz, _vp, _vp, _vp, _sz, _f, _f, _sz, _sz, _sz,
                                            _vp, _vp, _sz]),
     ("ckv_rope_axes_upload", _i, [_vp, _u32p, _sz, _sz]),
-    ("ckv_rope_axes", _i, [_vp, _vp, _vp, _sz, _f, _sz, _u8p, _sz]),
-    ("ckv_rope_axes_append", _i, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _f, _sz, _u8p, _sz]),
+    ("ckv_rope_axes", _i, [_vp, _vp, _vp, _sz, _f, _sz, C.c_char_p, _sz]),
+    ("ckv_rope_axes_append", _i, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _f, _sz, C.c_char_p, _sz]),
     ("ckv_compact", _i, [_vp, _u32p, _u32p, _i32p, _u32p, _sz, _f, _sz]),
 ]
 SYMBOLS = [name for name, _, _ in _SIGNATURES]
@@ -437,9 +436,9 @@ class Pool:
             raise ValueError("positions are [axes, rows]")
         self.ctx.check(load().ckv_rope_axes_upload(self.handle, _p(p), p.shape[0], p.shape[1]))
 
-    def _pair_axis(self, pair_axis, rotary_dim: int) -> np.ndarray:
-        axes = np.ascontiguousarray(pair_axis, dtype=np.uint8)
-        if axes.size != (rotary_dim or self.geometry[4]) // 2:
+    def _pair_axis(self, pair_axis, rotary_dim: int) -> bytes:
+        axes = np.asarray(pair_axis, dtype=np.uint8).tobytes()
+        if len(axes) != (rotary_dim or self.geometry[4]) // 2:
             raise ValueError("pair_axis has an axis for each of rotary_dim / 2 pairs")
         return axes
 
@@ -450,7 +449,7 @@ class Pool:
         rows = inputs.shape[0] if rows is None else rows
         a = self._pair_axis(pair_axis, rotary_dim)
         self.ctx.check(load().ckv_rope_axes(self.handle, _ptr(inputs), _ptr(outputs), heads, theta,
-                                            rotary_dim, a.ctypes.data_as(_u8p), rows))
+                                            rotary_dim, a, rows))
 
     def rope_axes_append(self, layer: int, queries, rotated, q_heads: int, keys, values,
                          theta: float, pair_axis, rotary_dim: int = 0,
@@ -461,7 +460,7 @@ class Pool:
         a = self._pair_axis(pair_axis, rotary_dim)
         self.ctx.check(load().ckv_rope_axes_append(
             self.handle, layer, _ptr(queries), _ptr(rotated), q_heads, _ptr(keys), _ptr(values),
-            theta, rotary_dim, a.ctypes.data_as(_u8p), rows))
+            theta, rotary_dim, a, rows))
 
     def compact(self, from_slots, to_slots, counts, shift=None, theta: float = 0.0,
                 rotary_dim: int = 0) -> None:

@@ -2530,11 +2530,12 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
             rotary = (uint32_t)width;
             ckv::turn_steps(theta, rotary, turns);
         }
-        std::vector<uint32_t> kept, runs;
+        compact_plan plan;
         int status = CKV_OK;
         if (const char* why = plan_compaction(pool->marks, pool->blocks * pool->block_size, from, to,
-                                              shift, counts, n_sequences, kept, runs, status))
+                                              shift, counts, n_sequences, plan, status))
             return set_error(ctx, status, why);
+        const std::vector<uint32_t>&kept = plan.kept, &runs = plan.runs;
         if (kept.empty())
             return CKV_OK;
         if (capturing(ctx))
@@ -2559,12 +2560,19 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
         if (status)
             return status;
         const uint32_t* d = pool->d_pairs;
-        const compact_moves moves { d, d + s_from, d + s_to,
-                                    reinterpret_cast<const int32_t*>(d + s_shift),
-                                    (uint32_t)(runs.size() / 2) };
         const pool_view view = view_of(pool);
         return run_kernel(ctx, "compact", [&] {
-            return launch_compact(ctx->stream, view, (uint32_t)pool->layers, moves, rotary, turns);
+            hipError_t e = hipSuccess;
+            const uint32_t* first = d;
+            for (const uint32_t n_runs : plan.launches) {
+                const compact_moves moves { first, d + s_from, d + s_to,
+                                            reinterpret_cast<const int32_t*>(d + s_shift), n_runs };
+                if (e == hipSuccess)
+                    e = launch_compact(ctx->stream, view, (uint32_t)pool->layers, moves, rotary,
+                                       turns);
+                first += 2 * n_runs;
+            }
+            return e;
         });
     });
 }

@@ -538,14 +538,21 @@ struct compact_moves {
     uint32_t n_runs;
 };
 // Checks the moves of ckv_compact and cuts them into runs. `kept` are the moves that
-// change something, `runs` pairs (first of kept, how many): a sequence whose targets
-// no other move reads is cut into runs of at most compact_run moves, another stays
-// one run. Returns null, or why the moves are refused, with the status.
+// change something, `runs` pairs (first of kept, how many), in the order of their
+// launches, whose numbers of runs `launches` holds. The runs of one launch depend on
+// each other in no way. A sequence's moves fall into waves, in none of which a move
+// overwrites what another reads; a wave is cut into runs of at most compact_run moves
+// and has a launch of its own, but for a sequence's first ones, where going through them
+// in one run, in order, is estimated to take less than their launches. Returns null, or
+// why the moves are refused, with the status.
 constexpr uint32_t compact_run = 64;
+constexpr uint32_t compact_launches = 6;
+struct compact_plan {
+    std::vector<uint32_t> kept, runs, launches;
+};
 const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* from,
                             const uint32_t* to, const int32_t* shift, const uint32_t* counts,
-                            size_t n_sequences, std::vector<uint32_t>& kept,
-                            std::vector<uint32_t>& runs, int& status);
+                            size_t n_sequences, compact_plan& plan, int& status);
 hipError_t launch_compact(hipStream_t s, const pool_view& p, uint32_t layers,
                           const compact_moves& moves, uint32_t rotary, const turn_table& turns);
 

@@ -20,6 +20,125 @@ namespace ckv {
 namespace {
 
 constexpr uint32_t block_threads = 256;
+
+// Rows whose rotary and head widths are whole pairs of 16-byte words: a thread moves a
+// word of a head's first half and the one it is turned with (or two words past the
+// rotary width) for `ahead` tokens at a time. The workgroup goes through `heads` heads of
+// a chunk of tokens, whose angles it computes once, then to the next chunk; the next
+// head's rows are in flight while this one's are turned and written. Rows are read and
+// written once: past the caches, as checkpoints are.
+constexpr uint32_t ahead = 2;
+
+template <int DT>
+__global__ __launch_bounds__(block_threads) void compact_rows_kernel(pool_view p, compact_moves m,
+                                                                    uint32_t rotary, uint32_t heads,
+                                                                    turn_table turns)
+{
+    using E = turn_element<DT>;
+    using T = typename E::type;
+    constexpr uint32_t each = 16 / sizeof(T); // elements of a word
+    union word {
+        u32x4_t v;
+        T e[each];
+    };
+    struct slots {
+        uint32_t from[ahead], to[ahead];
+        int32_t shift[ahead];
+        bool live[ahead];
+    };
+    struct rows {
+        word a[ahead], b[ahead];
+    };
+    const uint32_t d = p.head_dim, half = rotary / 2;
+    const uint32_t groups = d / (2 * each), step = block_threads / groups; // tokens side by side
+    const uint32_t t = threadIdx.x / groups, p0 = threadIdx.x % groups * each;
+    const bool turned = p0 < half;
+    const uint32_t at = turned ? p0 : 2 * p0, apart = turned ? half : each;
+    const uint32_t parts = p.kv_heads / heads;
+    const uint32_t run = blockIdx.x / parts, head0 = blockIdx.x % parts * heads;
+    const bool keys = blockIdx.z == 0;
+    T* base = static_cast<T*>(keys ? p.keys : p.values) + blockIdx.y * p.layer_elems + head0 * d + at;
+    const uint32_t first = m.runs[2 * run], count = m.runs[2 * run + 1];
+    const uint32_t chunk = ahead * step;
+
+    auto slots_of = [&](uint32_t i0) {
+        slots s;
+#pragma unroll
+        for (uint32_t k = 0; k < ahead; ++k) {
+            const uint32_t i = i0 + k * step + t, move = first + min(i, count - 1);
+            s.live[k] = t < step && i < count;
+            s.from[k] = m.from[move];
+            s.to[k] = m.to[move];
+            s.shift[k] = m.shift[move];
+        }
+        return s;
+    };
+    auto read = [&](const slots& s, uint32_t h) {
+        rows x;
+#pragma unroll
+        for (uint32_t k = 0; k < ahead; ++k) {
+            const T* src = base + (uint64_t)s.from[k] * p.features + h * d;
+            x.a[k].v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(src));
+            x.b[k].v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(src + apart));
+        }
+        return x;
+    };
+    uint64_t turn[each]; // of the thread's pairs
+#pragma unroll
+    for (uint32_t e = 0; e < each; ++e) {
+        turn[e] = turned ? turns.step[p0 + e] : 0;
+        asm volatile("" : "+v"(turn[e])); // read once, not beside the rows in flight
+    }
+    slots now = slots_of(0), next = slots_of(chunk);
+    rows x = read(now, 0);
+    for (uint32_t i0 = 0; i0 < count; i0 += chunk) {
+        const slots later = slots_of(i0 + 2 * chunk);
+        float c[ahead][each], sn[ahead][each];
+        if (keys && turned) {
+#pragma unroll
+            for (uint32_t k = 0; k < ahead; ++k)
+#pragma unroll
+                for (uint32_t e = 0; e < each; ++e)
+                    sincos_turn(turn[e], (uint64_t)(int64_t)now.shift[k], sn[k][e], c[k][e]);
+        }
+        for (uint32_t h = 0; h < heads; ++h) {
+            // every wave's rows of this chunk and head have arrived: they may be overwritten
+#pragma unroll
+            for (uint32_t k = 0; k < ahead; ++k)
+                asm volatile("" : "+v"(x.a[k].v), "+v"(x.b[k].v)::"memory");
+            __syncthreads();
+            // (past the run's end its last row again, which is not written)
+            const bool same = h + 1 < heads;
+            slots ahead_of = next;
+#pragma unroll
+            for (uint32_t k = 0; k < ahead; ++k)
+                ahead_of.from[k] = same ? now.from[k] : next.from[k];
+            const rows y = read(ahead_of, same ? h + 1 : 0);
+#pragma unroll
+            for (uint32_t k = 0; k < ahead; ++k) {
+                if (keys && turned && now.shift[k]) {
+#pragma unroll
+                    for (uint32_t e = 0; e < each; ++e) {
+                        float r1, r2;
+                        rope_pair(E::load(x.a[k].e[e]), E::load(x.b[k].e[e]), c[k][e], sn[k][e], r1, r2);
+                        x.a[k].e[e] = E::store(r1);
+                        x.b[k].e[e] = E::store(r2);
+                    }
+                }
+                if (now.live[k]) {
+                    T* dst = base + (uint64_t)now.to[k] * p.features + h * d;
+                    __builtin_nontemporal_store(x.a[k].v, reinterpret_cast<u32x4_t*>(dst));
+                    __builtin_nontemporal_store(x.b[k].v, reinterpret_cast<u32x4_t*>(dst + apart));
+                }
+            }
+            x = y;
+        }
+        now = next;
+        next = later;
+    }
+}
+
+// Any other geometry, an element at a time.
 constexpr uint32_t items = 8; // pairs a thread holds
 
 template <int DT>
@@ -78,8 +197,7 @@ __global__ __launch_bounds__(block_threads) void compact_kernel(pool_view p, com
 
 const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* from,
                             const uint32_t* to, const int32_t* shift, const uint32_t* counts,
-                            size_t n_sequences, std::vector<uint32_t>& kept,
-                            std::vector<uint32_t>& runs, int& status)
+                            size_t n_sequences, compact_plan& plan, int& status)
 {
     size_t n = 0;
     for (size_t q = 0; q < n_sequences; ++q)
@@ -106,26 +224,60 @@ const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* fro
         marks.last[from[i]] = (uint32_t)i;
     }
     status = CKV_E_UNSUPPORTED_ALIASING;
+    plan.kept.reserve(n);
+    std::vector<uint32_t> runs[compact_launches];
+    std::vector<size_t> waves; // where a sequence's waves begin, in kept
     for (size_t q = 0, begin = 0; q < n_sequences; begin += counts[q], ++q) {
-        const size_t end = begin + counts[q], first = kept.size();
-        bool free = true; // no target is read by another move
+        const size_t end = begin + counts[q];
+        size_t wave = begin; // the wave's first move
+        waves.assign(1, plan.kept.size());
         for (size_t i = begin; i < end; ++i) {
             if (marks.written[to[i]] == g)
                 return "two moves share a target";
             marks.written[to[i]] = g;
             if (marks.read[to[i]] == g) {
-                if (marks.first[to[i]] < begin || marks.last[to[i]] > i)
+                const size_t first = marks.first[to[i]], last = marks.last[to[i]];
+                if (first < begin || last > i)
                     return "a move's target is read by a later move or another sequence";
-                free = free && marks.first[to[i]] == i;
+                if (last == i ? first < i : last >= wave) { // read in this wave (or perhaps)
+                    wave = i;
+                    if (plan.kept.size() > waves.back())
+                        waves.push_back(plan.kept.size());
+                }
             }
             if (from[i] != to[i] || (shift && shift[i]))
-                kept.push_back((uint32_t)i);
+                plan.kept.push_back((uint32_t)i);
         }
-        const size_t moves = kept.size() - first;
-        const size_t each = free ? compact_run : std::max<size_t>(moves, 1);
-        for (size_t at = 0; at < moves; at += each)
-            runs.insert(runs.end(), { (uint32_t)(first + at), (uint32_t)std::min(each, moves - at) });
+        const size_t moves = plan.kept.size();
+        if (waves.size() > 1 && waves.back() == moves)
+            waves.pop_back();
+        // The last `split` waves with launches of their own, 5 us each where the GPU is
+        // not busy with their bytes, those before in one run, 16 moves a microsecond.
+        const size_t all = waves.size();
+        size_t split = 0, best = SIZE_MAX;
+        for (size_t c = 0; c < std::min<size_t>(all, compact_launches); ++c) {
+            const size_t before = (all - c < all ? waves[all - c] : moves) - waves[0];
+            const size_t cost = (all - c > 1 ? before / 16 : 0) + 5 * c;
+            if (cost < best) {
+                best = cost;
+                split = c;
+            }
+        }
+        auto cut = [&](std::vector<uint32_t>& into, size_t first, size_t last, size_t each) {
+            for (size_t at = first; at < last; at += each)
+                into.insert(into.end(), { (uint32_t)at, (uint32_t)std::min(each, last - at) });
+        };
+        const size_t tail = split ? waves[all - split] : moves;
+        cut(runs[0], waves[0], tail, all - split > 1 ? std::max<size_t>(tail, 1) : compact_run);
+        for (size_t c = 0; c < split; ++c)
+            cut(runs[1 + c], waves[all - split + c], c + 1 < split ? waves[all - split + c + 1] : moves,
+                compact_run);
     }
+    for (const auto& r : runs)
+        if (!r.empty()) {
+            plan.launches.push_back((uint32_t)(r.size() / 2));
+            plan.runs.insert(plan.runs.end(), r.begin(), r.end());
+        }
     status = CKV_OK;
     return nullptr;
 }
@@ -135,10 +287,26 @@ hipError_t launch_compact(hipStream_t s, const pool_view& p, uint32_t layers,
 {
     if (!moves.n_runs)
         return hipSuccess;
-    const uint64_t blocks = (uint64_t)moves.n_runs * p.kv_heads;
+    const uint32_t each = 16 / p.elem_size;
+    const auto aligned = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
+    const bool words = p.head_dim % (2 * each) == 0 && rotary % (2 * each) == 0
+        && p.head_dim / (2 * each) <= block_threads && aligned(p.keys) && aligned(p.values);
+    // heads a workgroup goes through: all of them, unless that leaves fewer workgroups
+    // than keep the memory busy
+    uint32_t heads = words ? p.kv_heads : 1;
+    while (heads % 2 == 0 && (uint64_t)moves.n_runs * layers * 2 * (p.kv_heads / heads) < 2048)
+        heads /= 2;
+    const uint64_t blocks = (uint64_t)moves.n_runs * (p.kv_heads / heads);
     if (blocks > 0x7FFFFFFFull || layers > 65535)
         return hipErrorInvalidValue;
     const dim3 grid((uint32_t)blocks, layers, 2);
+    if (words) {
+        auto* kernel = p.dtype == CKV_F32 ? compact_rows_kernel<CKV_F32>
+            : p.dtype == CKV_BF16         ? compact_rows_kernel<CKV_BF16>
+                                          : compact_rows_kernel<CKV_F16>;
+        kernel<<<grid, block_threads, 0, s>>>(p, moves, rotary, heads, turns);
+        return hipGetLastError();
+    }
     auto* kernel = p.dtype == CKV_F32 ? compact_kernel<CKV_F32>
         : p.dtype == CKV_BF16         ? compact_kernel<CKV_BF16>
                                       : compact_kernel<CKV_F16>;

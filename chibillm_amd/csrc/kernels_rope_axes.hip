@@ -16,7 +16,87 @@ namespace {
 
 constexpr uint32_t block_threads = 256;
 
-// One thread per (head, pair) and grid row per row: heads 0 .. q_heads - 1 are the
+// Rows whose rotary and head widths are whole pairs of 16-byte words: a thread takes
+// one word of a head's first half and the one it is turned with (or two words past the
+// rotary width) in `per` heads of a row, whose angles it computes once, with the rows'
+// words in flight meanwhile.
+template <int DT, int PER>
+__global__ __launch_bounds__(block_threads) void rope_axes_words_kernel(
+    pool_view p, const uint32_t* __restrict__ slots, uint32_t layer, axes_rows x, uint32_t rows,
+    uint32_t q_heads, uint32_t heads, uint32_t rotary, turn_table turns, axis_table axes,
+    const uint32_t* __restrict__ positions)
+{
+    using E = turn_element<DT>;
+    using T = typename E::type;
+    constexpr uint32_t each = 16 / sizeof(T); // elements of a word
+    union word {
+        uint4 v;
+        T e[each];
+    };
+    const uint32_t d = p.head_dim, half = rotary / 2;
+    const uint32_t groups = d / (2 * each), parts = (heads + PER - 1) / PER;
+    const uint64_t item = (uint64_t)blockIdx.x * block_threads + threadIdx.x;
+    const uint32_t row = (uint32_t)(item / (groups * parts));
+    if (row >= rows)
+        return;
+    const uint32_t rest = (uint32_t)(item % (groups * parts));
+    const uint32_t p0 = rest % groups * each, head0 = rest / groups * PER;
+    const bool turned = p0 < half;
+    const uint32_t at = turned ? p0 : 2 * p0, apart = turned ? half : each;
+    const uint64_t q_row = (uint64_t)row * q_heads * d, k_row = (uint64_t)row * p.features;
+    word a[PER], b[PER];
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) {
+        const uint32_t h = min(head0 + i, heads - 1); // past the last head: it again
+        const T* src = (h < q_heads ? static_cast<const T*>(x.queries) + q_row + h * d
+                                    : static_cast<const T*>(x.keys) + k_row + (h - q_heads) * d)
+            + at;
+        a[i].v = *reinterpret_cast<const uint4*>(src);
+        b[i].v = *reinterpret_cast<const uint4*>(src + apart);
+    }
+    const uint64_t slot_row = head0 + PER > q_heads
+        ? layer * p.layer_elems + (uint64_t)slots[row] * p.features
+        : 0;
+    float c[each], s[each];
+    if (turned) {
+#pragma unroll
+        for (uint32_t e = 0; e < each; ++e)
+            sincos_turn(turns.step[p0 + e],
+                        positions[(uint64_t)axes.axis[p0 + e] * rows + row], s[e], c[e]);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) {
+        const uint32_t h = head0 + i;
+        if (h >= heads)
+            break;
+        if (turned) {
+#pragma unroll
+            for (uint32_t e = 0; e < each; ++e) {
+                float r1, r2;
+                rope_pair(E::load(a[i].e[e]), E::load(b[i].e[e]), c[e], s[e], r1, r2);
+                a[i].e[e] = E::store(r1);
+                b[i].e[e] = E::store(r2);
+            }
+        }
+        T* dst;
+        if (h < q_heads) {
+            dst = static_cast<T*>(x.rotated) + q_row + h * d + at;
+        } else {
+            const uint32_t in_row = (h - q_heads) * d + at;
+            const T* vs = static_cast<const T*>(x.values) + k_row + in_row;
+            T* vd = static_cast<T*>(p.values) + slot_row + in_row;
+            const uint4 va = *reinterpret_cast<const uint4*>(vs);
+            const uint4 vb = *reinterpret_cast<const uint4*>(vs + apart);
+            *reinterpret_cast<uint4*>(vd) = va;
+            *reinterpret_cast<uint4*>(vd + apart) = vb;
+            dst = static_cast<T*>(p.keys) + slot_row + in_row;
+        }
+        *reinterpret_cast<uint4*>(dst) = a[i].v;
+        *reinterpret_cast<uint4*>(dst + apart) = b[i].v;
+    }
+}
+
+// Any other geometry: one thread per (head, pair) and grid row per row: heads 0 .. q_heads - 1 are the
 // query row's, the next kv_heads the key's and value's.
 template <int DT>
 __global__ __launch_bounds__(block_threads) void rope_axes_kernel(
@@ -71,9 +151,9 @@ void turn_steps(float theta, uint32_t rotary, turn_table& out)
     const long double ratio = std::pow((long double)theta, -2.0L / rotary);
     long double turn = 1.0L / (2.0L * 3.14159265358979323846264338327950288L);
     for (uint32_t pair = 0; pair < rotary / 2; ++pair, turn *= ratio) {
-        // whole turns per position fall away; a fraction that rounds to one does too
-        const long double scaled = std::ldexp(turn - std::floor(turn), 64);
-        out.step[pair] = scaled >= 0x1p64L ? 0 : (uint64_t)scaled;
+        // whole turns per position fall away
+        const long double part = turn < 1.0L ? turn : turn - std::floor(turn);
+        out.step[pair] = (uint64_t)(part * 0x1p64L);
     }
 }
 
@@ -85,6 +165,27 @@ hipError_t launch_rope_axes(hipStream_t s, const pool_view& p, const meta_view& 
     const uint32_t heads = q_heads + (x.keys ? p.kv_heads : 0);
     if (!rows || !heads)
         return hipSuccess;
+    const uint32_t each = 16 / p.elem_size;
+    const auto aligned = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
+    if (p.head_dim % (2 * each) == 0 && rotary % (2 * each) == 0 && aligned(x.queries)
+        && aligned(x.rotated) && aligned(x.keys) && aligned(x.values)
+        && (!x.keys || (aligned(p.keys) && aligned(p.values)))) {
+        const uint64_t words = (uint64_t)rows * (p.head_dim / (2 * each)); // of a head's halves
+        // four heads a thread, unless that leaves fewer than two workgroups per compute unit
+        const bool four = words * heads / 4 >= 512 * block_threads;
+        const uint64_t parts = four ? (heads + 3) / 4 : heads;
+        const uint64_t blocks = (words * parts + block_threads - 1) / block_threads;
+        if (blocks > 0x7FFFFFFFull)
+            return hipErrorInvalidValue;
+        auto* kernel = p.dtype == CKV_F32
+            ? (four ? rope_axes_words_kernel<CKV_F32, 4> : rope_axes_words_kernel<CKV_F32, 1>)
+            : p.dtype == CKV_BF16
+            ? (four ? rope_axes_words_kernel<CKV_BF16, 4> : rope_axes_words_kernel<CKV_BF16, 1>)
+            : (four ? rope_axes_words_kernel<CKV_F16, 4> : rope_axes_words_kernel<CKV_F16, 1>);
+        kernel<<<(uint32_t)blocks, block_threads, 0, s>>>(p, m.slots, layer, x, rows, q_heads, heads,
+                                                          rotary, turns, axes, positions);
+        return hipGetLastError();
+    }
     const uint64_t threads = (uint64_t)heads * (p.head_dim / 2);
     const uint64_t blocks = (threads + block_threads - 1) / block_threads;
     if (blocks > 0x7FFFFFFFull)

@@ -68,8 +68,7 @@ TEST("rope axes: fixed-point turns match long doubles at every position")
         }
 }
 
-struct plan {
-    std::vector<uint32_t> kept, runs;
+struct plan : compact_plan {
     int status = -1;
     bool refused = false;
 };
@@ -80,57 +79,126 @@ plan compaction(move_marks& marks, size_t slots, const std::vector<uint32_t>& fr
 {
     plan p;
     p.refused = plan_compaction(marks, slots, from.data(), to.data(), shift, counts.data(),
-                                counts.size(), p.kept, p.runs, p.status) != nullptr;
+                                counts.size(), p, p.status) != nullptr;
     return p;
 }
 
-// Runs done concurrently, each in its order, leave what all reads before all writes do.
+// Launches one after another, their runs concurrently, each in its order, leave what all
+// reads before all writes do. A run's moves are interleaved with the other runs' as two
+// steps, a read of up to 32 of them and then their writes.
+void run_and_compare(const plan& p, uint32_t slots, const std::vector<uint32_t>& from,
+                     const std::vector<uint32_t>& to, std::mt19937_64& rng)
+{
+    REQUIRE(!p.refused && p.status == CKV_OK);
+    std::vector<uint32_t> want(slots), got(slots);
+    for (uint32_t i = 0; i < slots; ++i)
+        want[i] = got[i] = 1000 + i;
+    for (size_t i = 0; i < from.size(); ++i)
+        want[to[i]] = 1000 + from[i];
+    std::vector<int> done(from.size(), 0);
+    size_t first = 0;
+    REQUIRE(p.launches.size() <= compact_launches);
+    for (const uint32_t n : p.launches) {
+        struct walk {
+            uint32_t at, end;
+            std::vector<uint32_t> held;
+        };
+        std::vector<walk> runs;
+        for (size_t r = first; r < first + n; ++r)
+            runs.push_back({ p.runs[2 * r], p.runs[2 * r] + p.runs[2 * r + 1], {} });
+        first += n;
+        while (!runs.empty()) {
+            const size_t r = rng() % runs.size();
+            walk& w = runs[r];
+            const uint32_t k = std::min<uint32_t>(32, w.end - w.at);
+            if (w.held.empty()) {
+                for (uint32_t j = 0; j < k; ++j)
+                    w.held.push_back(got[from[p.kept[w.at + j]]]);
+            } else {
+                for (uint32_t j = 0; j < k; ++j) {
+                    const uint32_t i = p.kept[w.at + j];
+                    REQUIRE(!done[i]);
+                    done[i] = 1;
+                    got[to[i]] = w.held[j];
+                }
+                w.held.clear();
+                w.at += k;
+                if (w.at == w.end)
+                    runs.erase(runs.begin() + r);
+            }
+        }
+    }
+    REQUIRE(2 * first == p.runs.size());
+    for (const uint32_t i : p.kept)
+        CHECK(done[i]);
+    CHECK(got == want);
+}
+
 TEST("compaction: concurrent runs leave what reads before writes do")
 {
     std::mt19937_64 rng(7);
     move_marks marks;
-    for (int trial = 0; trial < 300; ++trial) {
-        const uint32_t slots = 600;
+    for (int trial = 0; trial < 400; ++trial) {
+        const uint32_t each = trial % 4 ? 200 : 1500, slots = 3 * each;
         std::vector<uint32_t> order(slots), from, to, counts;
         for (uint32_t i = 0; i < slots; ++i)
             order[i] = i;
         std::shuffle(order.begin(), order.end(), rng);
-        for (uint32_t q = 0; q < 3; ++q) { // a sequence: 200 slots of its own
-            const uint32_t* at = order.data() + 200 * q;
+        for (uint32_t q = 0; q < 3; ++q) { // a sequence: slots of its own
+            const uint32_t* at = order.data() + each * q;
             uint32_t n = 0;
             const bool fresh = rng() % 3 == 0;
-            const uint32_t of = fresh ? 100 : 200;
-            for (uint32_t t = 0; t < of; ++t)
-                if (rng() % 5) {
+            const uint32_t of = fresh ? each / 2 : each, kind = rng() % 4;
+            for (uint32_t t = 0; t < of; ++t) {
+                const bool keep = kind == 0 ? rng() % 5 != 0
+                    : kind == 1             ? t < 4 || t >= of / 2
+                    : kind == 2             ? t != 3
+                                            : t < 20 || t >= 90; // 70 leave
+                if (keep) {
                     from.push_back(at[t]);
-                    to.push_back(at[fresh ? 100 + n : n]);
+                    to.push_back(at[fresh ? of + n : n]);
                     ++n;
                 }
+            }
             counts.push_back(n);
         }
-        const plan p = compaction(marks, slots, from, to, counts);
-        REQUIRE(!p.refused && p.status == CKV_OK);
-        std::vector<uint32_t> want(slots), got(slots);
-        for (uint32_t i = 0; i < slots; ++i)
-            want[i] = got[i] = 1000 + i;
-        for (size_t i = 0; i < from.size(); ++i)
-            want[to[i]] = 1000 + from[i];
-        // the runs in a random interleaving of their moves
-        std::vector<size_t> next(p.runs.size() / 2, 0);
-        size_t left = p.kept.size();
-        std::vector<int> done(from.size(), 0);
-        while (left) {
-            const size_t r = rng() % next.size();
-            if (next[r] == p.runs[2 * r + 1])
-                continue;
-            const uint32_t i = p.kept[p.runs[2 * r] + next[r]++];
-            REQUIRE(!done[i]);
-            done[i] = 1;
-            got[to[i]] = got[from[i]];
-            --left;
-        }
-        CHECK(got == want);
+        run_and_compare(compaction(marks, slots, from, to, counts), slots, from, to, rng);
     }
+    // slots read several times, and moves that change a key where it stands
+    for (int trial = 0; trial < 200; ++trial) {
+        std::vector<uint32_t> from, to;
+        std::vector<int32_t> shift;
+        for (uint32_t i = 0; i < 150; ++i) {
+            to.push_back(i);
+            from.push_back(i + rng() % 3 * (rng() % 40));
+            shift.push_back(-(int32_t)(rng() % 3));
+        }
+        const plan p = compaction(marks, 250, from, to, { 150 }, shift.data());
+        run_and_compare(p, 250, from, to, rng);
+    }
+}
+
+TEST("compaction: a middle that leaves takes two launches, one token one run")
+{
+    move_marks marks;
+    std::vector<uint32_t> from, to;
+    for (uint32_t t = 0; t < 2000; ++t)
+        if (t < 4 || t >= 1000) {
+            to.push_back((uint32_t)to.size());
+            from.push_back(t);
+        }
+    plan p = compaction(marks, 2000, from, to, { (uint32_t)to.size() });
+    CHECK(p.launches.size() == 2);
+    CHECK(p.kept.size() == 1000 && p.launches[0] == (996 + 63) / 64 && p.launches[1] == 1);
+    from.clear();
+    to.clear();
+    for (uint32_t t = 0; t < 2000; ++t)
+        if (t != 4) {
+            to.push_back((uint32_t)to.size());
+            from.push_back(t);
+        }
+    p = compaction(marks, 2000, from, to, { (uint32_t)to.size() });
+    CHECK(p.launches.size() == 1 && p.launches[0] == 1 && p.kept.size() == 1995);
 }
 
 TEST("compaction: unsafe moves are refused")
