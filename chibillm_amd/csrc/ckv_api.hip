@@ -2532,8 +2532,10 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
         }
         compact_plan plan;
         int status = CKV_OK;
-        if (const char* why = plan_compaction(pool->marks, pool->blocks * pool->block_size, from, to,
-                                              shift, counts, n_sequences, plan, status))
+        const pool_view view = view_of(pool);
+        if (const char* why = plan_compaction(
+                pool->marks, pool->blocks * pool->block_size, from, to, shift, counts, n_sequences,
+                compact_cost_of(view, (uint32_t)pool->layers), plan, status))
             return set_error(ctx, status, why);
         const std::vector<uint32_t>&kept = plan.kept, &runs = plan.runs;
         if (kept.empty())
@@ -2560,7 +2562,6 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
         if (status)
             return status;
         const uint32_t* d = pool->d_pairs;
-        const pool_view view = view_of(pool);
         return run_kernel(ctx, "compact", [&] {
             hipError_t e = hipSuccess;
             const uint32_t* first = d;

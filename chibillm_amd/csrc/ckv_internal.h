@@ -550,9 +550,16 @@ constexpr uint32_t compact_launches = 6;
 struct compact_plan {
     std::vector<uint32_t> kept, runs, launches;
 };
+// What a move costs, in microseconds: its bytes, its share of a run done in order, and
+// a launch.
+struct compact_cost {
+    double move_bytes, move_in_run, launch;
+};
+compact_cost compact_cost_of(const pool_view& p, uint32_t layers);
 const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* from,
                             const uint32_t* to, const int32_t* shift, const uint32_t* counts,
-                            size_t n_sequences, compact_plan& plan, int& status);
+                            size_t n_sequences, const compact_cost& cost, compact_plan& plan,
+                            int& status);
 hipError_t launch_compact(hipStream_t s, const pool_view& p, uint32_t layers,
                           const compact_moves& moves, uint32_t rotary, const turn_table& turns);
 

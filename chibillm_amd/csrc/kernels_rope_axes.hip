@@ -18,7 +18,7 @@ constexpr uint32_t block_threads = 256;
 
 // Rows whose rotary and head widths are whole pairs of 16-byte words: a thread takes
 // one word of a head's first half and the one it is turned with (or two words past the
-// rotary width) in `per` heads of a row, whose angles it computes once, with the rows'
+// rotary width, of its halves likewise) in `per` heads of a row, whose angles it computes once, with the rows'
 // words in flight meanwhile.
 template <int DT, int PER>
 __global__ __launch_bounds__(block_threads) void rope_axes_words_kernel(
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(block_threads) void rope_axes_words_kernel(
     const uint32_t rest = (uint32_t)(item % (groups * parts));
     const uint32_t p0 = rest % groups * each, head0 = rest / groups * PER;
     const bool turned = p0 < half;
-    const uint32_t at = turned ? p0 : 2 * p0, apart = turned ? half : each;
+    const uint32_t at = turned ? p0 : half + p0, apart = turned ? half : (d - rotary) / 2;
     const uint64_t q_row = (uint64_t)row * q_heads * d, k_row = (uint64_t)row * p.features;
     word a[PER], b[PER];
 #pragma unroll

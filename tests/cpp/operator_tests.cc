@@ -75,11 +75,11 @@ struct plan : compact_plan {
 
 plan compaction(move_marks& marks, size_t slots, const std::vector<uint32_t>& from,
                 const std::vector<uint32_t>& to, const std::vector<uint32_t>& counts,
-                const int32_t* shift = nullptr)
+                const int32_t* shift = nullptr, const compact_cost& cost = { 0.007, 0.05, 8.0 })
 {
     plan p;
     p.refused = plan_compaction(marks, slots, from.data(), to.data(), shift, counts.data(),
-                                counts.size(), p, p.status) != nullptr;
+                                counts.size(), cost, p, p.status) != nullptr;
     return p;
 }
 
@@ -162,7 +162,10 @@ TEST("compaction: concurrent runs leave what reads before writes do")
             }
             counts.push_back(n);
         }
-        run_and_compare(compaction(marks, slots, from, to, counts), slots, from, to, rng);
+        // rates that favour launches, one run, and either
+        const compact_cost costs[] = { { 0.0, 1.0, 0.1 }, { 1.0, 0.0, 9.0 }, { 0.007, 0.05, 8.0 } };
+        run_and_compare(compaction(marks, slots, from, to, counts, nullptr, costs[trial % 3]), slots, from,
+                        to, rng);
     }
     // slots read several times, and moves that change a key where it stands
     for (int trial = 0; trial < 200; ++trial) {
