@@ -557,6 +557,7 @@ void select_window(ckv_pool* pool, key_window w)
         return;
     pool->window_positions.clear(); // stays so if what follows throws
     pool->window_plan_ready = pool->window_work_ready = false;
+    pool->window_tile_rows = 0;
     pool->window_positions.resize(pool->positions.size());
     m = pool->meta;
     m.window = w;
@@ -620,6 +621,49 @@ int ensure_window_plan(ckv_pool* pool)
     status = upload_staged(ctx, pool->d_window_plan, words * sizeof(uint32_t));
     pool->window_plan_ready = status == CKV_OK;
     return status;
+}
+
+// The window's tiles of at most `rows` rows, one for each workgroup (tiles of up to 256
+// rows whose empty places return at once left those that work on a quarter of the
+// compute units: 32 sequences of 64 rows behind a window of 512 took 59 us, twice
+// what 16 took), those with the most key blocks first, at their first launch.
+int ensure_window_tiles(ckv_pool* pool, uint32_t rows)
+{
+    if (pool->window_tile_rows == rows)
+        return CKV_OK;
+    ckv_context* ctx = pool->ctx;
+    if (capturing(ctx))
+        return refuse_captured(ctx);
+    const key_window w = pool->window_meta.window;
+    const std::vector<uint32_t>& all = pool->tiles;
+    std::vector<std::pair<uint32_t, std::array<uint32_t, tile_entry_words>>> parts;
+    for (size_t t = 0; t < all.size(); t += tile_entry_words)
+        for (uint32_t r = 0; r < all[t + 1]; r += rows) {
+            const uint32_t n = std::min(rows, all[t + 1] - r), first = all[t + 2] + r;
+            const uint32_t blocks = (first + n - 1) / 32 + 1
+                - window_gap_of(window_low(first, w), w.sinks, 32).skip;
+            parts.push_back({ blocks, { all[t] + r, n, first, all[t + 3] } });
+        }
+    std::stable_sort(parts.begin(), parts.end(),
+                     [](const auto& a, const auto& b) { return a.first > b.first; });
+    const size_t words = std::max<size_t>(parts.size() * tile_entry_words, 4);
+    void* host = nullptr;
+    int status = stage(ctx, words * sizeof(uint32_t), &host);
+    if (!status)
+        status = ensure_device(ctx, &pool->d_window_tiles, &pool->d_window_tiles_words, words,
+                               "window tiles");
+    if (status)
+        return status;
+    auto* to = static_cast<uint32_t*>(host);
+    for (const auto& part : parts)
+        to = std::copy(part.second.begin(), part.second.end(), to);
+    status = upload_staged(ctx, pool->d_window_tiles, words * sizeof(uint32_t));
+    if (status)
+        return status;
+    pool->window_meta.tiles = pool->d_window_tiles;
+    pool->window_meta.n_tiles = (uint32_t)parts.size();
+    pool->window_tile_rows = rows;
+    return CKV_OK;
 }
 
 // What a decode launch runs over: the batch, or the batch through a window.
@@ -1274,6 +1318,8 @@ int ckv_pool_destroy(ckv_pool* pool)
         (void)dev_free(ctx, pool->d_window_plan);
     if (pool->d_window_work)
         (void)dev_free(ctx, pool->d_window_work);
+    if (pool->d_window_tiles)
+        (void)dev_free(ctx, pool->d_window_tiles);
     if (pool->d_axes)
         (void)dev_free(ctx, pool->d_axes);
     delete pool;
@@ -1349,6 +1395,7 @@ void adopt_batch(ckv_pool* pool, size_t rows, size_t n_entries, bool with_slots,
     pool->work_ready = false;
     pool->window_positions.clear();
     pool->window_plan_ready = pool->window_work_ready = false;
+    pool->window_tile_rows = 0;
     pool->axes = 0;
     pool->uploaded = true;
 }
@@ -1482,6 +1529,7 @@ int ckv_tables_upload(ckv_pool* pool, const uint32_t* block_table, size_t n_entr
     m.slots = pool->d_meta + s_slots;
     m.tiles = pool->d_meta + s_tiles;
     m.n_tiles = (uint32_t)(tiles.size() / tile_entry_words);
+    pool->tiles = tiles;
     m.tile_blocks = shortest_tile_blocks(tiles);
     count_row_blocks(tiles, m.row_blocks);
     adopt_batch(pool, rows, n_entries, slots != nullptr, shared, fusable, with_plan, false);
@@ -1772,6 +1820,7 @@ int ckv_batch_upload(ckv_pool* pool, const uint32_t* seq, const uint32_t* first_
     m.slots = d + s_slots;
     m.tiles = d + s_tiles;
     m.n_tiles = (uint32_t)(tiles.size() / tile_entry_words);
+    pool->tiles = tiles;
     m.tile_blocks = shortest_tile_blocks(tiles);
     count_row_blocks(tiles, m.row_blocks);
     adopt_batch(pool, rows, pool->seq_max * pool->seq_cap, with_slots != 0, shared, fusable,
@@ -2324,6 +2373,9 @@ int ckv_attention_window(ckv_pool* pool, size_t layer, const void* queries, size
             return run_decode(pool, layer, queries, q_heads, scale, output, gate, w);
         // also a window that leaves nothing out: its kernels hold probabilities in more bits
         select_window(pool, w.window != all_keys.window ? w : key_window { UINT32_MAX - 1, 0 });
+        status = ensure_window_tiles(pool, prefill_window_rows(view_of(pool), (uint32_t)q_heads));
+        if (status)
+            return status;
         return run_prefill(pool, layer, queries, q_heads, scale, output, gate, pool->window_meta);
     });
 }

@@ -276,6 +276,7 @@ struct ckv_pool {
     std::vector<uint32_t> positions;
     uint32_t last_position = 0; // the largest of them
     std::vector<uint32_t> row_offsets; // each row's table offset (the decode plan's entries)
+    std::vector<uint32_t> tiles; // the batch's query tiles (meta_view::tiles)
     bool shared_tile = false;
     bool fusable = false; // slots are the rows' own positions, one row per table range
     // while fusable: each row's own table index (offset + position / block_size)
@@ -329,6 +330,9 @@ struct ckv_pool {
     size_t d_window_plan_words = 0;
     uint32_t* d_window_work = nullptr;
     size_t d_window_work_words = 0;
+    uint32_t window_tile_rows = 0; // rows of window_meta's tiles at most; 0: none yet
+    uint32_t* d_window_tiles = nullptr;
+    size_t d_window_tiles_words = 0;
 
     // the batch rows' positions on several axes ([axes][rows], ckv_rope_axes_upload)
     uint32_t axes = 0;
@@ -486,6 +490,8 @@ hipError_t launch_prefill(hipStream_t s, const pool_view& p, const meta_view& m,
                           const void* q, uint32_t q_heads, float scale, void* out,
                           const void* gate, const prefill_shape_info& plan,
                           prefill_split split);
+// Rows of a workgroup of the windowed prefill: its tiles have at most so many.
+uint32_t prefill_window_rows(const pool_view& p, uint32_t q_heads);
 // The same for 16-bit pools of 256-wide heads (kernels_prefill_wide.hip).
 prefill_shape_info prefill_wide_plan(const pool_view& p, const meta_view& m, uint32_t q_heads,
                                      int cu_count, uint32_t min_blocks);

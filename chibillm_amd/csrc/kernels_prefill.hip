@@ -152,7 +152,8 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     constexpr uint32_t R = shape::regions;
     __shared__ __attribute__((aligned(16))) uint8_t lds[n_stages * stage_bytes];
     constexpr uint32_t tile_rows = 32 * W / G;
-    constexpr uint32_t subs = 256 / tile_rows; // workgroups per (tile, kv head)
+    // workgroups per (tile, kv head); a window's tiles are of a workgroup's rows
+    constexpr uint32_t subs = WINDOW ? 1 : 256 / tile_rows;
 
     const uint32_t kv_heads = p.kv_heads;
     const uint32_t kvh = blockIdx.x % kv_heads; // consecutive workgroups: different heads/XCDs
@@ -773,8 +774,8 @@ hipError_t launch_gw(hipStream_t s, const pool_view& p, const meta_view& m, uint
                      const void* q, uint32_t q_heads, float c, void* out, const void* gate,
                      prefill_split split)
 {
-    const uint64_t grid = (uint64_t)m.n_tiles * (256 / (32 * W / G)) * p.kv_heads
-        * (WINDOW ? q_heads / p.kv_heads / G : 1) * (W == 4 ? split.n_split : 1);
+    const uint64_t per_tile = WINDOW ? q_heads / p.kv_heads / G : 256 / (32 * W / G);
+    const uint64_t grid = (uint64_t)m.n_tiles * per_tile * p.kv_heads * (W == 4 ? split.n_split : 1);
     if (!grid)
         return hipSuccess;
     if (grid > 0x7FFFFFFFull)
@@ -850,6 +851,12 @@ constexpr uint32_t sub_round_max_blocks = 40;
 // Shortest key range of a windowed f32 tile, in blocks.
 constexpr uint32_t window_min_blocks_f32 = 2;
 
+uint32_t prefill_window_rows(const pool_view& p, uint32_t q_heads)
+{
+    const uint32_t group = q_heads / p.kv_heads;
+    return p.dtype == CKV_F32 ? 256 / group : 128 / std::min(group, 4u);
+}
+
 prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t q_heads,
                                 int cu_count)
 {
@@ -863,7 +870,7 @@ prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t
     if (p.dtype == CKV_F32) {
         // f32 pools: 8-wave workgroups, two to a compute unit; a launch that
         // gives at most one to each splits its long tiles' keys to fill them
-        const uint64_t grid = (uint64_t)m.n_tiles * group * p.kv_heads;
+        const uint64_t grid = (uint64_t)m.n_tiles * (windowed ? 1 : group) * p.kv_heads;
         uint64_t split = grid && cu_count > 0 && grid <= (uint64_t)cu_count
             ? 2 * (uint64_t)cu_count / grid
             : 1;
@@ -881,17 +888,15 @@ prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t
     if (windowed) {
         // 4-wave workgroups, two to a compute unit; a launch that leaves some idle splits
         // each tile's keys between as many as fill them
-        const uint32_t G = std::min(group, 4u), passes = group / G;
-        const uint64_t busy = (uint64_t)m.row_blocks[G == 4 ? 0 : G == 2 ? 1 : 2] * passes * p.kv_heads;
-        const uint64_t pairs = (uint64_t)m.n_tiles * (2 * G) * passes * p.kv_heads;
+        const uint64_t busy = (uint64_t)m.n_tiles * (group / std::min(group, 4u)) * p.kv_heads;
         uint64_t split = busy && cu_count > 0 ? 2 * (uint64_t)cu_count / busy : 1;
         if (const char* forced = std::getenv("CKV_PREFILL_SPLIT"))
             split = (uint64_t)std::max(1L, std::strtol(forced, nullptr, 10));
         plan.waves = 4;
         plan.n_split = (uint32_t)std::clamp<uint64_t>(split, 1, split_max);
         if (plan.n_split > 1) {
-            plan.records_floats = pairs * plan.n_split * 128 * prefill_record_floats;
-            plan.counters = pairs;
+            plan.records_floats = busy * plan.n_split * 128 * prefill_record_floats;
+            plan.counters = busy;
         }
         return plan;
     }

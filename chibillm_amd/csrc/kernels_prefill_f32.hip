@@ -74,11 +74,12 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
     const uint32_t kvh = blockIdx.x % kv_heads;
     // key ranges vary slowest: every tile's first range is dispatched first
     const uint32_t n_split = split_scratch.n_split;
-    const uint32_t n_rest = md.n_tiles * G;
+    constexpr uint32_t subs = WINDOW ? 1 : G; // a window's tiles are of a workgroup's rows
+    const uint32_t n_rest = md.n_tiles * subs;
     const uint32_t rest = blockIdx.x / kv_heads % n_rest;
     const uint32_t part = blockIdx.x / kv_heads / n_rest; // this workgroup's range of the keys
-    const uint32_t sub = rest % G;
-    const uint32_t tile = rest / G;
+    const uint32_t sub = rest % subs;
+    const uint32_t tile = rest / subs;
     // the tile: first row, rows, first position, table offset
     const uint4 te = *reinterpret_cast<const uint4*>(md.tiles + tile_entry_words * tile);
     const uint32_t count = te.y;
@@ -419,7 +420,8 @@ hipError_t launch_prefill_f32(hipStream_t s, const pool_view& p, const meta_view
     if (split.n_split < 1 || split.min_blocks < 1
         || (split.n_split > 1 && (!split.records || !split.arrivals)))
         return hipErrorInvalidValue;
-    const uint64_t grid = (uint64_t)m.n_tiles * group * p.kv_heads * split.n_split;
+    const bool windowed = m.window.window != all_keys.window;
+    const uint64_t grid = (uint64_t)m.n_tiles * (windowed ? 1 : group) * p.kv_heads * split.n_split;
     if (!grid)
         return hipSuccess;
     if (grid > 0x7FFFFFFFull)
@@ -441,8 +443,7 @@ hipError_t launch_prefill_f32(hipStream_t s, const pool_view& p, const meta_view
             return hipErrorInvalidValue;
         }
     };
-    return m.window.window != all_keys.window ? launch(std::true_type {})
-                                              : launch(std::false_type {});
+    return windowed ? launch(std::true_type {}) : launch(std::false_type {});
 }
 
 } // namespace ckv

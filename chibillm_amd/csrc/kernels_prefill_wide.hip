@@ -110,7 +110,8 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
     __shared__ __attribute__((aligned(16))) uint8_t lds[n_stages * (k_stage_bytes + v_stage_bytes)];
     constexpr int terms = p_terms<WINDOW>;
     constexpr uint32_t tile_rows = 32 * waves / G;
-    constexpr uint32_t subs = prefill_tile_rows / tile_rows; // workgroups per (tile, head pass, kv head)
+    // workgroups per (tile, head pass, kv head); a window's tiles are of a workgroup's rows
+    constexpr uint32_t subs = WINDOW ? 1 : prefill_tile_rows / tile_rows;
 
     const uint32_t kv_heads = p.kv_heads;
     const uint32_t group = q_heads / kv_heads;
@@ -623,14 +624,16 @@ prefill_shape_info prefill_wide_plan(const pool_view& p, const meta_view& m, uin
     prefill_shape_info plan { waves, 1, min_blocks, 0, 0 };
     const uint32_t group = q_heads / p.kv_heads, G = wide_heads(group);
     // row_blocks[i]: the tiles' workgroups of 32 << i rows
-    const uint64_t busy = (uint64_t)m.row_blocks[G == 4 ? 0 : G == 2 ? 1 : 2] * (group / G) * p.kv_heads;
+    const bool windowed = m.window.window != all_keys.window;
+    const uint32_t workgroups = windowed ? m.n_tiles : m.row_blocks[G == 4 ? 0 : G == 2 ? 1 : 2];
+    const uint64_t busy = (uint64_t)workgroups * (group / G) * p.kv_heads;
     uint64_t split = busy && cu_count > 0 ? (uint64_t)cu_count / busy : 1;
     if (const char* forced = std::getenv("CKV_PREFILL_SPLIT"))
         split = (uint64_t)std::max(1L, std::strtol(forced, nullptr, 10));
     // records are kept for every workgroup of the grid, those past a short
     // tile's rows included: within 128 MiB
-    const uint64_t grid = (uint64_t)m.n_tiles * (prefill_tile_rows * G / (32 * waves)) * (group / G)
-        * p.kv_heads;
+    const uint64_t grid = (uint64_t)m.n_tiles * (windowed ? 1 : prefill_tile_rows * G / (32 * waves))
+        * (group / G) * p.kv_heads;
     const uint64_t floats = grid * (32 * waves) * (dim + 4);
     const uint64_t room = std::max<uint64_t>(1, ((uint64_t)128 << 20) / sizeof(float) / std::max<uint64_t>(floats, 1));
     plan.n_split = (uint32_t)std::clamp<uint64_t>(std::min(split, room), 1, split_max);
@@ -646,8 +649,9 @@ hipError_t launch_prefill_wide(hipStream_t s, const pool_view& p, const meta_vie
                                void* out, const void* gate, prefill_split split)
 {
     const uint32_t group = q_heads / p.kv_heads, G = wide_heads(group);
-    const uint64_t grid = (uint64_t)m.n_tiles * (prefill_tile_rows * G / (32 * waves)) * (group / G)
-        * p.kv_heads * split.n_split;
+    const bool windowed = m.window.window != all_keys.window;
+    const uint64_t grid = (uint64_t)m.n_tiles * (windowed ? 1 : prefill_tile_rows * G / (32 * waves))
+        * (group / G) * p.kv_heads * split.n_split;
     if (!grid)
         return hipSuccess;
     if (grid > 0x7FFFFFFFull)
@@ -665,8 +669,7 @@ hipError_t launch_prefill_wide(hipStream_t s, const pool_view& p, const meta_vie
             return launch_g<4, WINDOW>(s, p, m, layer, q, q_heads, c, out, gate, n, split);
         }
     };
-    return m.window.window != all_keys.window ? launch(std::true_type {})
-                                              : launch(std::false_type {});
+    return windowed ? launch(std::true_type {}) : launch(std::false_type {});
 }
 
 } // namespace ckv
