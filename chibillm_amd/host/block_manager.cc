@@ -80,6 +80,20 @@ block_manager::release(seq_id id) noexcept
     tables_.erase(it);
 }
 
+result<void, state_error>
+block_manager::truncate(seq_id id, std::size_t tokens)
+{
+    const auto it = tables_.find(id);
+    if (it == tables_.end() || tokens == 0 || (tokens - 1) / size_ >= it->second.size())
+        return fail(state_errc::invalid_reservation);
+    auto& table = it->second;
+    const std::size_t keep = (tokens - 1) / size_ + 1;
+    for (std::size_t i = keep; i < table.size(); ++i)
+        unref(table[i]);
+    table.resize(keep);
+    return {};
+}
+
 std::uint32_t
 block_manager::refcount(block_id block) const noexcept
 {

@@ -51,6 +51,11 @@ public:
     // zero return to the back of the free list in table order.
     void release(seq_id id) noexcept override;
 
+    // Gives back the sequence's pages past those of its first `tokens` (> 0), as
+    // release() does: the end of a compaction. invalid_reservation for an unknown
+    // sequence or more tokens than it has pages for.
+    result<void, state_error> truncate(seq_id id, std::size_t tokens);
+
     // ---- sharing ------------------------------------------------------------
     std::uint32_t refcount(block_id block) const noexcept;
     // Adds a reference to each page (all must be allocated).

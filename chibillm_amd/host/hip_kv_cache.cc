@@ -304,6 +304,25 @@ hip_kv_cache::import_prefix(std::span<const block_id> blocks, const host_kv_chec
 }
 
 result<void, state_error>
+hip_kv_cache::compact(std::span<const std::uint32_t> from, std::span<const std::uint32_t> to,
+                      std::span<const std::int32_t> shift, std::span<const std::uint32_t> counts,
+                      float theta, std::size_t rotary)
+{
+    std::size_t moves = 0;
+    for (const std::uint32_t n : counts)
+        moves += n;
+    if (from.size() != moves || to.size() != moves || (!shift.empty() && shift.size() != moves))
+        return fail(state_errc::invalid_reservation);
+    const int rc = ckv_compact(pool_, from.data(), to.data(), shift.empty() ? nullptr : shift.data(),
+                               counts.data(), counts.size(), theta, rotary);
+    if (rc && rc != CKV_E_HIP_FAILURE)
+        return fail(state_errc::invalid_reservation, ctx_->last(rc), "compaction");
+    if (rc)
+        return fail(state_errc::backend_failure, ctx_->last(rc), "compaction");
+    return {};
+}
+
+result<void, state_error>
 hip_kv_cache::copy_pages(std::span<const block_id> from, std::span<const block_id> to)
 {
     if (from.size() != to.size())

@@ -236,6 +236,15 @@ public:
     export_prefix(std::span<const block_id> blocks, std::size_t tokens) const;
     result<void, state_error> import_prefix(std::span<const block_id> blocks,
                                             const host_kv_checkpoint& saved);
+    // Kept tokens' rows of all layers to other slots, their keys turned by `shift`
+    // positions (empty: not at all), as ckv_compact, whose moves and rules these are:
+    // counts[q] consecutive moves of sequence q. invalid_reservation where they are
+    // refused.
+    result<void, state_error> compact(std::span<const std::uint32_t> from,
+                                      std::span<const std::uint32_t> to,
+                                      std::span<const std::int32_t> shift,
+                                      std::span<const std::uint32_t> counts, float theta,
+                                      std::size_t rotary_dimension = 0);
     // Page copies on the device, all layers, keys and values.
     result<void, state_error> copy_pages(std::span<const block_id> from,
                                          std::span<const block_id> to);

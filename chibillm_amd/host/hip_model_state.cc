@@ -1,5 +1,8 @@
 #include "hip_model_state.h"
 
+#include <algorithm>
+#include <limits>
+
 namespace chibillm {
 
 result<std::unique_ptr<hip_model_state>, state_error>
@@ -63,6 +66,58 @@ try {
     return pages_->free_block_count() >= pages;
 } catch (const std::bad_alloc&) {
     return false;
+}
+
+result<void, state_error>
+hip_model_state::compact(seq_id id, std::span<const std::uint32_t> kept, float theta,
+                         std::size_t rotary)
+{
+    const std::size_t bs = cache_.block_size();
+    const auto held = resources(id).blocks;
+    if (kept.empty() || kept.back() / bs >= held.size())
+        return fail(state_errc::invalid_reservation);
+    for (std::size_t i = 1; i < kept.size(); ++i)
+        if (kept[i] <= kept[i - 1])
+            return fail(state_errc::invalid_reservation);
+    const std::size_t width = rotary ? rotary : cache_.head_dimension();
+    if (!(theta >= 0.0f) || theta == std::numeric_limits<float>::infinity()
+        || (theta > 0.0f && (width % 2 || width > cache_.head_dimension() || width > 512)))
+        return fail(state_errc::invalid_reservation);
+    // the pages that change, or that later tokens will fill, have to be the sequence's own
+    const std::vector<block_id> old(held.begin(), held.end());
+    const std::size_t n = kept.size(), pages = (n - 1) / bs + 1;
+    const auto shared = [&] {
+        std::vector<std::size_t> found;
+        for (std::size_t j = 0; j < pages; ++j) {
+            const std::size_t last = std::min(n, (j + 1) * bs) - 1;
+            // tokens ascend: a page's last one moves if any does
+            if (pages_->refcount(old[j]) > 1 && (kept[last] != last || last % bs != bs - 1))
+                found.push_back(j);
+        }
+        return found;
+    };
+    std::vector<std::size_t> forks = shared();
+    if (forks.size() > pages_->free_block_count() && spill_) {
+        spill_for(forks.size()); // which may leave pages to this sequence alone
+        forks = shared();
+    }
+    if (forks.size() > pages_->free_block_count())
+        return fail(state_errc::capacity_exhausted);
+    for (const std::size_t j : forks)
+        if (auto fresh = pages_->fork(id, j); !fresh)
+            return fail(fresh.error());
+    const auto table = resources(id).blocks;
+    const std::uint32_t size = static_cast<std::uint32_t>(bs), count = static_cast<std::uint32_t>(n);
+    std::vector<std::uint32_t> from(n), to(n);
+    std::vector<std::int32_t> shift(theta > 0.0f ? n : 0);
+    for (std::uint32_t i = 0; i < count; ++i) {
+        from[i] = old[kept[i] / size] * size + kept[i] % size;
+        to[i] = table[i / size] * size + i % size;
+        if (!shift.empty())
+            shift[i] = static_cast<std::int32_t>(i - kept[i]);
+    }
+    CL_TRY(cache_.compact(from, to, shift, std::span(&count, 1), theta, rotary));
+    return pages_->truncate(id, n);
 }
 
 std::size_t

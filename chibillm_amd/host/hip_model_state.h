@@ -93,6 +93,18 @@ public:
                                                                       std::size_t tokens) const override;
     result<void, state_error> restore(seq_id id, const model_checkpoint& saved) override;
 
+    // Drops the sequence's tokens but for `kept` (ascending): those move together, to
+    // positions 0 .. kept.size() - 1, on the device, and the pages behind them are given
+    // back. With theta (> 0) their keys, cached as rotated at their old positions, turn to
+    // the new ones (ckv_compact); 0 leaves them as they are. Pages that others share
+    // (checkpoints, other sequences) are not written: a private page takes their place,
+    // also that of a shared last page which later tokens will fill. The next batch of the
+    // sequence starts at position kept.size(). Errors, before anything changes:
+    // invalid_reservation (no token, one out of order or past the sequence's pages, a
+    // rotary width or theta that ckv_compact refuses), capacity_exhausted.
+    result<void, state_error> compact(seq_id id, std::span<const std::uint32_t> kept,
+                                      float theta = 0.0f, std::size_t rotary_dimension = 0);
+
     // Keeps the sequences' block tables on the device (device_tables); the
     // rows of released sequences are returned to it.
     result<void, tensor_op_error> enable_device_tables(std::size_t max_sequences,

@@ -387,4 +387,110 @@ store_kv_rotated(hip_kv_cache& cache, const device_tensor& keys, const device_te
     return {};
 }
 
+result<void, tensor_op_error>
+paged_attention_window(hip_kv_cache& cache, const device_tensor& queries, std::size_t layer,
+                       std::size_t q_heads, std::size_t window, std::size_t sinks,
+                       device_tensor& output, const device_tensor* gate)
+{
+    std::size_t rows = 0;
+    CL_TRY_ASSIGN(rows, validate_attention(cache, queries, layer, q_heads, output));
+    if (gate)
+        CL_TRY(validate_gate(cache, *gate, output));
+    const int rc = ckv_attention_window(cache.pool(), layer, queries.data, q_heads,
+                                        attention_scale(cache), window, sinks,
+                                        gate ? gate->data : nullptr, output.data, rows);
+    if (rc)
+        return from_ckv(cache, rc);
+    return {};
+}
+
+result<void, tensor_op_error>
+store_kv_and_attend_window(hip_kv_cache& cache, const device_tensor& keys,
+                           const device_tensor& values, const device_tensor& queries,
+                           std::size_t layer, std::size_t q_heads, std::size_t window,
+                           std::size_t sinks, device_tensor& output, const device_tensor* gate)
+{
+    std::size_t rows = 0;
+    CL_TRY_ASSIGN(rows, validate_store(cache, keys, values, layer));
+    std::size_t q_rows = 0;
+    CL_TRY_ASSIGN(q_rows, validate_attention(cache, queries, layer, q_heads, output));
+    if (q_rows != rows)
+        return fail(tensor_op_errc::position_count_mismatch);
+    if (gate)
+        CL_TRY(validate_gate(cache, *gate, output));
+    const int rc = ckv_append_decode_window(cache.pool(), layer, keys.data, values.data,
+                                            queries.data, q_heads, attention_scale(cache), window,
+                                            sinks, gate ? gate->data : nullptr, output.data, rows);
+    if (rc)
+        return from_ckv(cache, rc);
+    return {};
+}
+
+result<void, tensor_op_error>
+upload_rope_axes(hip_kv_cache& cache, std::span<const std::uint32_t> positions, std::size_t axes)
+{
+    if (!axes || positions.size() % axes)
+        return fail(tensor_op_errc::position_count_mismatch);
+    const int rc = ckv_rope_axes_upload(cache.pool(), positions.data(), axes, positions.size() / axes);
+    if (rc)
+        return from_ckv(cache, rc);
+    return {};
+}
+
+namespace {
+
+result<void, tensor_op_error>
+validate_pair_axis(const hip_kv_cache& cache, std::span<const std::uint8_t> pair_axis,
+                   std::size_t rotary)
+{
+    if (pair_axis.size() != (rotary ? rotary : cache.head_dimension()) / 2)
+        return fail(tensor_op_errc::invalid_head_dimension);
+    return {};
+}
+
+} // namespace
+
+result<void, tensor_op_error>
+rope_axes(hip_kv_cache& cache, const device_tensor& input, std::size_t head_count, float theta,
+          std::span<const std::uint8_t> pair_axis, device_tensor& output, std::size_t rotary)
+{
+    const dtype t = cache_dtype(cache);
+    CL_TRY(validate_layouts({ { input, 2, t }, { output, 2, t } }));
+    if (output.dims != input.dims)
+        return fail(tensor_op_errc::output_shape_mismatch);
+    if (head_count && input.dims[1] != head_count * cache.head_dimension())
+        return fail(tensor_op_errc::invalid_head_dimension);
+    CL_TRY(validate_pair_axis(cache, pair_axis, rotary));
+    const int rc = ckv_rope_axes(cache.pool(), input.data, output.data, head_count, theta, rotary,
+                                 pair_axis.data(), input.dims[0]);
+    if (rc)
+        return from_ckv(cache, rc);
+    return {};
+}
+
+result<void, tensor_op_error>
+store_kv_rotated_axes(hip_kv_cache& cache, const device_tensor& queries, device_tensor& rotated,
+                      std::size_t q_heads, const device_tensor& keys, const device_tensor& values,
+                      std::size_t layer, float theta, std::span<const std::uint8_t> pair_axis,
+                      std::size_t rotary)
+{
+    std::size_t rows = 0;
+    CL_TRY_ASSIGN(rows, validate_store(cache, keys, values, layer));
+    const dtype t = cache_dtype(cache);
+    CL_TRY(validate_layouts({ { queries, 2, t }, { rotated, 2, t } }));
+    if (rotated.dims != queries.dims)
+        return fail(tensor_op_errc::output_shape_mismatch);
+    if (queries.dims[0] != rows)
+        return fail(tensor_op_errc::position_count_mismatch);
+    if (queries.dims[1] != q_heads * cache.head_dimension())
+        return fail(tensor_op_errc::invalid_head_dimension);
+    CL_TRY(validate_pair_axis(cache, pair_axis, rotary));
+    const int rc = ckv_rope_axes_append(cache.pool(), layer, queries.data, rotated.data, q_heads,
+                                        keys.data, values.data, theta, rotary, pair_axis.data(),
+                                        rows);
+    if (rc)
+        return from_ckv(cache, rc);
+    return {};
+}
+
 } // namespace chibillm

@@ -187,6 +187,49 @@ result<void, tensor_op_error> rope(hip_kv_cache& cache, const device_tensor& inp
                                    std::size_t head_count, float theta, device_tensor& output,
                                    std::size_t rotary_dimension = 0);
 
+// paged_attention of rows that attend their last `window` tokens and the sequence's
+// first `sinks` (ckv_attention_window), and store_kv of decode rows before it in one
+// pass where possible (ckv_append_decode_window); gate may be null, otherwise as
+// paged_attention_gated's. New: the reference attends to every token.
+result<void, tensor_op_error> paged_attention_window(hip_kv_cache& cache,
+                                                     const device_tensor& queries,
+                                                     std::size_t layer,
+                                                     std::size_t query_head_count,
+                                                     std::size_t window, std::size_t sinks,
+                                                     device_tensor& output,
+                                                     const device_tensor* gate = nullptr);
+result<void, tensor_op_error> store_kv_and_attend_window(hip_kv_cache& cache,
+                                                         const device_tensor& keys,
+                                                         const device_tensor& values,
+                                                         const device_tensor& queries,
+                                                         std::size_t layer,
+                                                         std::size_t query_head_count,
+                                                         std::size_t window, std::size_t sinks,
+                                                         device_tensor& output,
+                                                         const device_tensor* gate = nullptr);
+
+// Positions of the uploaded batch's rows on several axes ([axes][rows], host), the
+// rotation of [rows, heads * head_dim] rows by them and that of a layer's queries and
+// keys with store_kv, in one launch (ckv_rope_axes_upload, ckv_rope_axes,
+// ckv_rope_axes_append). pair_axis: the axis of each of rotary_dimension / 2 pairs
+// (invalid_head_dimension otherwise); rotary_dimension 0 means the whole head. New.
+result<void, tensor_op_error> upload_rope_axes(hip_kv_cache& cache,
+                                               std::span<const std::uint32_t> positions,
+                                               std::size_t axes);
+result<void, tensor_op_error> rope_axes(hip_kv_cache& cache, const device_tensor& input,
+                                        std::size_t head_count, float theta,
+                                        std::span<const std::uint8_t> pair_axis,
+                                        device_tensor& output, std::size_t rotary_dimension = 0);
+result<void, tensor_op_error> store_kv_rotated_axes(hip_kv_cache& cache,
+                                                    const device_tensor& queries,
+                                                    device_tensor& rotated,
+                                                    std::size_t query_head_count,
+                                                    const device_tensor& keys,
+                                                    const device_tensor& values,
+                                                    std::size_t layer, float theta,
+                                                    std::span<const std::uint8_t> pair_axis,
+                                                    std::size_t rotary_dimension = 0);
+
 // rope of the key rows fused into store_kv (ckv_rope_append): the
 // apply_rope + store_kv pair of src/qwen/qwen_layer.cc:20-30, :43.
 result<void, tensor_op_error> store_kv_rotated(hip_kv_cache& cache, const device_tensor& keys,
