@@ -601,7 +601,7 @@ int ensure_window_plan(ckv_pool* pool)
     const uint32_t bs = (uint32_t)pool->block_size;
     const std::vector<uint32_t>& left = close_window_gaps(pool, bs);
     const decode_plan_shape shape =
-        shape_decode_plan(left, bs, (uint32_t)pool->kv_heads, ctx->cu_count,
+        shape_window_plan(left, bs, (uint32_t)pool->kv_heads, ctx->cu_count,
                           decode_form_of(pool->dtype, (uint32_t)pool->head_dim));
     const size_t words = std::max<size_t>(plan_words(shape, left.size()), 4);
     void* host = nullptr;

@@ -1009,6 +1009,31 @@ uint32_t fast_waves(uint32_t group, int dtype, uint32_t units, int cu_count,
     return limit;
 }
 
+// The same for rows behind a window, which are short and mostly equally long: 8 waves,
+// two workgroups to a compute unit, for one or two q heads per KV head; 4 waves where
+// the units or the chunks of halved rows (shape_window_plan) are more than two for each,
+// and for more q heads, whose lanes let one workgroup of 8 waves or two of 4 reside
+// (8 q heads: while all units reside at once). 128-wide heads, whole rows, us at 10, 8 and
+// 4 waves: 48 rows behind 1,024 tokens 45.3, 41.9 and 43.4; 64 50.8, 49.4 and 48.3; 80 69.0,
+// 67.0 and 62.6; 4 q heads per KV head, at 8 and 4 waves: 80 rows behind 256 30.7 and
+// 22.2, 64 behind 1,024 54.4 and 50.3; 8: 64 behind 1,024 75.2 and 68.2, 80 109 and 115.
+uint32_t window_waves(uint32_t head_dim, uint32_t group, int dtype, uint32_t units, int cu_count,
+                      uint32_t mean_pages, uint32_t split_pages)
+{
+    const uint32_t waves = fast_waves(group, dtype, units, cu_count, mean_pages, split_pages);
+    const uint32_t cus = (uint32_t)std::max(cu_count, 1);
+    if (std::getenv("CKV_DECODE_WAVES") || dtype == CKV_F32 || units < cus)
+        return waves;
+    const bool many = units > 2 * cus;
+    if (split_pages)
+        return many && group <= 4 ? 4 : waves;
+    if (head_dim != 128)
+        return waves;
+    if (group > 2)
+        return group == 8 && many ? waves : 4;
+    return units >= 2 * cus ? 4 : 8;
+}
+
 template <bool WINDOW, int D, int G>
 hipError_t launch_fast(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
                        const void* q, uint32_t q_heads, float scale_log2, void* out, int dt,
@@ -1032,7 +1057,9 @@ hipError_t launch_fast(hipStream_t s, const pool_view& p, const meta_view& m, ui
         }
     }
     const uint32_t units = m.n_plan * p.kv_heads;
-    const uint32_t waves = fast_waves(G, dt, units, cu_count, m.mean_pages, m.split_pages);
+    const uint32_t waves = WINDOW
+        ? window_waves(D, G, dt, units, cu_count, m.mean_pages, m.split_pages)
+        : fast_waves(G, dt, units, cu_count, m.mean_pages, m.split_pages);
     const dim3 grid(units), block(64 * waves);
     // the merge's (acc, max, denominator) per wave, the rope angle table, a flag
     const size_t lds = ((size_t)waves * G * (D + 2) + (rope ? rotary : 0) + 1) * sizeof(float);

@@ -426,7 +426,8 @@ decode_form decode_form_of(int dtype, uint32_t head_dim)
 }
 
 decode_plan_shape shape_decode_plan(const std::vector<uint32_t>& positions, uint32_t block_size,
-                                    uint32_t kv_heads, int cu_count, const decode_form& form)
+                                    uint32_t kv_heads, int cu_count, const decode_form& form,
+                                    uint64_t chunk)
 {
     const uint32_t rows = (uint32_t)positions.size();
     decode_plan_shape shape { 0, rows, 0, 0, rows, 0, 0, false };
@@ -435,6 +436,10 @@ decode_plan_shape shape_decode_plan(const std::vector<uint32_t>& positions, uint
     bool fixed_set, balanced_set;
     uint64_t span = forced_pages("CKV_DECODE_SPLIT", fixed_set);
     const uint64_t target = forced_pages("CKV_DECODE_BALANCE", balanced_set);
+    if (chunk && !fixed_set && !balanced_set) {
+        span = chunk;
+        fixed_set = true;
+    }
     uint64_t deal = 0; // workgroups per kv head the balanced plan deals the pages to
     if (balanced_set) {
         deal = target ? (total + target - 1) / target : 0;
@@ -533,6 +538,31 @@ decode_plan_shape shape_decode_plan(const std::vector<uint32_t>& positions, uint
     shape.n_cut = (uint32_t)cut;
     shape.n_wgs = (uint32_t)wgs;
     return shape;
+}
+
+// Rows behind a window are mostly equally long. With one to one and a half (row, kv
+// head) units per compute unit, some hold two whole rows and most one; halves, four
+// waves each (decode_wg.h), even them out. Measured on MI355X (8 kv heads, 2 q heads
+// per kv head, bf16, us, whole rows at 8 waves and halves at 4): 34 rows behind a window
+// of 4,096 tokens 130 and 107, of 2,048 67.7 and 58.4, of 1,024 36.6 and 32.7, of 512
+// 21.0 and 19.9, of 256 12.3 and 13.0; 48 rows behind 2,048 75.0 and 69.7, behind 512
+// 24.0 and 24.0; 52 rows behind 2,048 78.9 and 83.0. 256-wide heads hold one workgroup
+// to a compute unit: 40 rows of 8 kv heads, 4 q heads each, behind 1,024 tokens 91 and
+// 65, behind 256 30.7 and 24.5; 160 of 2 kv heads, 2 each, 67.7 and 61.1, 21.8 and 22.4.
+constexpr uint64_t window_half_pages = 33, window_half_pages_wide = 17;
+
+decode_plan_shape shape_window_plan(const std::vector<uint32_t>& positions, uint32_t block_size,
+                                    uint32_t kv_heads, int cu_count, const decode_form& form)
+{
+    uint64_t total, longest;
+    batch_pages(positions, block_size, total, longest);
+    const uint64_t rows = positions.size(), cus = (uint64_t)std::max(cu_count, 1);
+    const bool even = 8 * total >= 7 * longest * rows;
+    const uint64_t least = form.per_cu == 1 ? window_half_pages_wide : window_half_pages;
+    const bool halves = !form.few_waves && even && longest >= least
+        && rows * kv_heads > cus && 2 * rows * kv_heads <= 3 * cus;
+    return shape_decode_plan(positions, block_size, kv_heads, cu_count, form,
+                             halves ? (longest + 1) / 2 : 0);
 }
 
 void write_decode_plan(const std::vector<uint32_t>& positions,
