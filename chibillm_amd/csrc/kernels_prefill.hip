@@ -853,8 +853,7 @@ constexpr uint32_t window_min_blocks_f32 = 2;
 
 uint32_t prefill_window_rows(const pool_view& p, uint32_t q_heads)
 {
-    const uint32_t group = q_heads / p.kv_heads;
-    return p.dtype == CKV_F32 ? 256 / group : 128 / std::min(group, 4u);
+    return 128 / std::min(q_heads / p.kv_heads, 4u);
 }
 
 prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t q_heads,
@@ -870,7 +869,8 @@ prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t
     if (p.dtype == CKV_F32) {
         // f32 pools: 8-wave workgroups, two to a compute unit; a launch that
         // gives at most one to each splits its long tiles' keys to fill them
-        const uint64_t grid = (uint64_t)m.n_tiles * (windowed ? 1 : group) * p.kv_heads;
+        const uint64_t per_tile = windowed ? group / std::min(group, 4u) : group;
+        const uint64_t grid = (uint64_t)m.n_tiles * per_tile * p.kv_heads;
         uint64_t split = grid && cu_count > 0 && grid <= (uint64_t)cu_count
             ? 2 * (uint64_t)cu_count / grid
             : 1;
@@ -880,7 +880,7 @@ prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t
         if (windowed && !std::getenv("CKV_PREFILL_SPLIT_MIN"))
             plan.min_blocks = window_min_blocks_f32;
         if (plan.n_split > 1) {
-            plan.records_floats = grid * plan.n_split * 256 * prefill_record_floats;
+            plan.records_floats = grid * plan.n_split * (windowed ? 128 : 256) * prefill_record_floats;
             plan.counters = grid;
         }
         return plan;

@@ -37,6 +37,7 @@
 // between up to 8 workgroups, as the 16-bit kernel does (kernels_prefill.hip):
 // each stores its unnormalised state as 16-byte records, and the last to
 // arrive folds them in range order.
+#include <algorithm>
 #include <type_traits>
 
 #include "attend_alone.h"
@@ -49,7 +50,6 @@ namespace {
 constexpr uint32_t dim = 128;
 constexpr uint32_t page_tokens = 16;
 constexpr uint32_t block_keys = 32;
-constexpr uint32_t waves = 8;
 constexpr uint32_t row_pitch = dim * 4 + 16;              // bytes per staged key row
 constexpr uint32_t tensor_bytes = block_keys * row_pitch; // one block of K (or V)
 constexpr uint32_t stage_bytes = 2 * tensor_bytes;        // K, then V
@@ -60,24 +60,32 @@ __device__ __forceinline__ f32x16_t mfma(float a, float b, const f32x16_t& c)
     return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
 }
 
-// WINDOW: rows attend through md.window, as in kernels_prefill.hip.
-template <int G, bool WINDOW>
+// WINDOW (4 waves): rows attend through md.window, as in kernels_prefill.hip. A window's
+// tiles are short chains of dear blocks: workgroups of half the rows have half the chain
+// to a block and two share a compute unit (2 chunks of 220 and 300 rows behind 1,000
+// tokens, window 512: 65 us with 8 waves, 45 with 4).
+template <int G, bool WINDOW, int waves = WINDOW ? 4 : 8>
 __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
     pool_view p, meta_view md, uint32_t layer, const float* __restrict__ q,
     float* __restrict__ out, uint32_t q_heads, float c, const float* __restrict__ gate,
     prefill_split split_scratch)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[n_stages * stage_bytes];
-    constexpr uint32_t tile_rows = 256 / G;
+    static_assert(waves == 8 || G <= 4, "a workgroup covers every q head of its group, or 4 of 8");
+    constexpr uint32_t tile_rows = 32 * waves / G;
 
     const uint32_t kv_heads = p.kv_heads;
     const uint32_t kvh = blockIdx.x % kv_heads;
+    const uint32_t group = WINDOW ? q_heads / kv_heads : G;
+    const uint32_t passes = WINDOW ? group / G : 1; // workgroups a GQA group takes
+    const uint32_t pass = WINDOW ? blockIdx.x / kv_heads % passes : 0;
+    const uint32_t of_pass = blockIdx.x / (kv_heads * passes);
     // key ranges vary slowest: every tile's first range is dispatched first
     const uint32_t n_split = split_scratch.n_split;
     constexpr uint32_t subs = WINDOW ? 1 : G; // a window's tiles are of a workgroup's rows
     const uint32_t n_rest = md.n_tiles * subs;
-    const uint32_t rest = blockIdx.x / kv_heads % n_rest;
-    const uint32_t part = blockIdx.x / kv_heads / n_rest; // this workgroup's range of the keys
+    const uint32_t rest = of_pass % n_rest;
+    const uint32_t part = of_pass / n_rest; // this workgroup's range of the keys
     const uint32_t sub = rest % subs;
     const uint32_t tile = rest / subs;
     // the tile: first row, rows, first position, table offset
@@ -114,7 +122,7 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
     const uint64_t q_stride = (uint64_t)q_heads * dim;
 
     // this wave's q-block: head kvh * G + wave % G, tile rows 32 * (wave / G) + n
-    const uint32_t head = kvh * G + wave % G;
+    const uint32_t head = kvh * group + pass * G + wave % G;
     const uint32_t row = (wave / G) * 32 + n;
     const bool valid = row < nrows;
     const uint32_t qpos = pos0 + min(row, nrows - 1);
@@ -135,36 +143,46 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
         qr[4 * t + 3] = v.w;
     }
 
-    // Staging: thread t moves 16 bytes of key rows t/32 and t/32 + 16 of the
-    // block (one of each page), of K and of V.
+    // Staging: thread t moves 16 bytes of key rows t/32, t/32 + 2 waves, ... of each page
+    // of the block, of K and of V.
     const uint64_t page_bytes = (uint64_t)page_tokens * p.features * 4;
     const uint64_t layer_bytes = p.layer_elems * 4;
     const uint8_t* kbase = static_cast<const uint8_t*>(p.keys) + layer * layer_bytes + kvh * dim * 4;
     const uint8_t* vbase = static_cast<const uint8_t*>(p.values) + layer * layer_bytes + kvh * dim * 4;
+    constexpr uint32_t step = 2 * waves, each = page_tokens / step; // rows of a page a thread moves
     const uint32_t sr = tid >> 5;
     const uint32_t scol = (tid & 31) * 16;
     const uint64_t srow = (uint64_t)sr * p.features * 4 + scol;
-    uint4 k_a, k_b, v_a, v_b; // the staged 16 bytes of each page's K and V row
+    const uint64_t srow_step = (uint64_t)step * p.features * 4;
+    // the staged 16 bytes of each page's K and V rows
+    uint4 k_a[each], k_b[each], v_a[each], v_b[each];
     auto fetch = [&](uint32_t kb) __attribute__((always_inline)) {
         const uint32_t key0 = in_table(kb) * block_keys;
         const uint64_t pa = table[2 * in_table(kb)];
         const uint64_t pb = table[min(2 * in_table(kb) + 1, last_entry)];
-        k_a = k_b = v_a = v_b = make_uint4(0, 0, 0, 0);
-        if (some_row_attends(key0 + sr)) {
-            k_a = *reinterpret_cast<const uint4*>(kbase + pa * page_bytes + srow);
-            v_a = *reinterpret_cast<const uint4*>(vbase + pa * page_bytes + srow);
-        }
-        if (some_row_attends(key0 + 16 + sr)) {
-            k_b = *reinterpret_cast<const uint4*>(kbase + pb * page_bytes + srow);
-            v_b = *reinterpret_cast<const uint4*>(vbase + pb * page_bytes + srow);
+#pragma unroll
+        for (uint32_t i = 0; i < each; ++i) {
+            const uint64_t at = srow + i * srow_step;
+            k_a[i] = k_b[i] = v_a[i] = v_b[i] = make_uint4(0, 0, 0, 0);
+            if (some_row_attends(key0 + sr + i * step)) {
+                k_a[i] = *reinterpret_cast<const uint4*>(kbase + pa * page_bytes + at);
+                v_a[i] = *reinterpret_cast<const uint4*>(vbase + pa * page_bytes + at);
+            }
+            if (some_row_attends(key0 + 16 + sr + i * step)) {
+                k_b[i] = *reinterpret_cast<const uint4*>(kbase + pb * page_bytes + at);
+                v_b[i] = *reinterpret_cast<const uint4*>(vbase + pb * page_bytes + at);
+            }
         }
     };
     auto store = [&](uint32_t kb) __attribute__((always_inline)) {
         uint8_t* st = lds + (kb % n_stages) * stage_bytes + sr * row_pitch + scol;
-        *reinterpret_cast<uint4*>(st) = k_a;
-        *reinterpret_cast<uint4*>(st + 16 * row_pitch) = k_b;
-        *reinterpret_cast<uint4*>(st + tensor_bytes) = v_a;
-        *reinterpret_cast<uint4*>(st + tensor_bytes + 16 * row_pitch) = v_b;
+#pragma unroll
+        for (uint32_t i = 0; i < each; ++i, st += step * row_pitch) {
+            *reinterpret_cast<uint4*>(st) = k_a[i];
+            *reinterpret_cast<uint4*>(st + 16 * row_pitch) = k_b[i];
+            *reinterpret_cast<uint4*>(st + tensor_bytes) = v_a[i];
+            *reinterpret_cast<uint4*>(st + tensor_bytes + 16 * row_pitch) = v_b[i];
+        }
     };
 
     f32x16_t o[4];
@@ -283,7 +301,7 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
         // workgroup's 256 query vectors consecutive. The range that arrives
         // last folds every range's record in range order, two per round trip,
         // with weights 2^(m_s - M).
-        const uint32_t pair = rest * kv_heads + kvh;
+        const uint32_t pair = (rest * passes + pass) * kv_heads + kvh;
         const uint32_t qv = wave * 32 + n;
         constexpr uint32_t QV = 32 * waves, chunks = prefill_record_floats / 4;
         const __amdgpu_buffer_rsrc_t rs = record_rsrc(
@@ -404,7 +422,7 @@ hipError_t launch_g(hipStream_t s, const pool_view& p, const meta_view& m, uint3
                     const void* q, uint32_t q_heads, float c, void* out, uint32_t grid,
                     const void* gate, prefill_split split)
 {
-    hipLaunchKernelGGL((prefill_f32_kernel<G, WINDOW>), dim3(grid), dim3(64 * waves), 0, s, p, m, layer,
+    hipLaunchKernelGGL((prefill_f32_kernel<G, WINDOW>), dim3(grid), dim3(WINDOW ? 256 : 512), 0, s, p, m, layer,
                        static_cast<const float*>(q), static_cast<float*>(out), q_heads, c,
                        static_cast<const float*>(gate), split);
     return hipGetLastError();
@@ -421,7 +439,8 @@ hipError_t launch_prefill_f32(hipStream_t s, const pool_view& p, const meta_view
         || (split.n_split > 1 && (!split.records || !split.arrivals)))
         return hipErrorInvalidValue;
     const bool windowed = m.window.window != all_keys.window;
-    const uint64_t grid = (uint64_t)m.n_tiles * (windowed ? 1 : group) * p.kv_heads * split.n_split;
+    const uint64_t per_tile = windowed ? group / std::min(group, 4u) : group;
+    const uint64_t grid = (uint64_t)m.n_tiles * per_tile * p.kv_heads * split.n_split;
     if (!grid)
         return hipSuccess;
     if (grid > 0x7FFFFFFFull)
@@ -438,7 +457,10 @@ hipError_t launch_prefill_f32(hipStream_t s, const pool_view& p, const meta_view
         case 4:
             return launch_g<4, WINDOW>(s, p, m, layer, q, q_heads, c, out, n, gate, split);
         case 8:
-            return launch_g<8, WINDOW>(s, p, m, layer, q, q_heads, c, out, n, gate, split);
+            if constexpr (WINDOW) // two workgroups of 4 heads
+                return launch_g<4, WINDOW>(s, p, m, layer, q, q_heads, c, out, n, gate, split);
+            else
+                return launch_g<8, WINDOW>(s, p, m, layer, q, q_heads, c, out, n, gate, split);
         default:
             return hipErrorInvalidValue;
         }
