@@ -662,6 +662,7 @@ int ensure_window_tiles(ckv_pool* pool, uint32_t rows)
         return status;
     pool->window_meta.tiles = pool->d_window_tiles;
     pool->window_meta.n_tiles = (uint32_t)parts.size();
+    pool->window_meta.tile_blocks = parts.empty() ? 0 : parts.front().first;
     pool->window_tile_rows = rows;
     return CKV_OK;
 }

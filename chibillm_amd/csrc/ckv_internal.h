@@ -83,7 +83,8 @@ struct meta_view {
     uint32_t n_items;
     uint32_t chunk; // tokens per decode work item, a multiple of 16
     uint32_t n_tiles;
-    uint32_t tile_blocks; // 32-key blocks the batch's shortest query tile attends (host side)
+    uint32_t tile_blocks; // 32-key blocks the batch's shortest query tile attends (host side);
+                          // behind a window those of its longest
     uint32_t row_blocks[3]; // runs of 32, 64 and 128 rows the tiles fall into (host side)
     uint32_t mean_pages; // pages attended per row, mean over the batch (host side)
     uint32_t n_plan;      // workgroups per kv head of the fast decode (the entries they start at)

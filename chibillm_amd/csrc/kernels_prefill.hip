@@ -837,6 +837,64 @@ bool prefill_supported(const pool_view& p, uint32_t q_heads, const void* q, cons
     return aligned16(p.keys) && aligned16(p.values) && aligned16(q) && aligned16(out);
 }
 
+namespace {
+
+// Key ranges of a windowed launch. One that gives every compute unit a workgroup takes
+// one range (3 split 408 workgroups of 35 bf16 blocks in 66 us, 1 in 55). A smaller one
+// takes the n of least time by an estimate: the compute unit with the most workgroups has
+// blocks / n of block us to go, and `shared` of that again for each workgroup more; n
+// ranges hand over in base + n * range us, and each record in record us. Fitted on MI355X,
+// us at n = 1, 2, 3, 4, 6, 8: bf16, 64 workgroups of 36 blocks, 39, 27, 23, 21, 23, 24,
+// and 192 of 23, 29, 30, 37, 35, 42, 47; 256 wide, 32 of 34, 70, 51, 44, 42, 43, 45; f32,
+// 72 of 20, 103, 60, 47, 58, 51, 55. The n taken comes within a tenth of the best but for
+// f32's launches of short tiles (144 workgroups of 7 blocks take 42 us, in 2 ranges 32).
+struct window_cost {
+    double block, shared, base, range, record;
+};
+constexpr window_cost cost_16bit { 0.85, 0.6, 2.0, 0.4, 0.01 }, cost_wide { 1.45, 1.0, 4.0, 2.0, 0.02 },
+    cost_f32 { 4.4, 0.8, 0.0, 0.8, 0.02 };
+constexpr uint32_t window_min_blocks = 2; // of a range
+
+prefill_shape_info window_plan(const pool_view& p, const meta_view& m, uint32_t q_heads,
+                               int cu_count)
+{
+    prefill_shape_info plan { 4, 1, window_min_blocks, 0, 0 };
+    if (const char* forced = std::getenv("CKV_PREFILL_SPLIT_MIN"))
+        plan.min_blocks = (uint32_t)std::max(1L, std::strtol(forced, nullptr, 10));
+    const uint32_t group = q_heads / p.kv_heads;
+    const uint64_t grid = (uint64_t)m.n_tiles * (group / std::min(group, 4u)) * p.kv_heads;
+    const uint64_t cus = (uint64_t)std::max(cu_count, 1);
+    const window_cost& cost = p.dtype == CKV_F32 ? cost_f32 : p.head_dim == 256 ? cost_wide : cost_16bit;
+    const uint64_t floats = grid * 128 * (p.head_dim + 4); // of a range's records, within 128 MiB in all
+    double best = 0.0;
+    for (uint32_t n = 1; n <= split_max; ++n) {
+        if (n > 1 && (grid >= cus || prefill_range_count(m.tile_blocks, n, plan.min_blocks) < n
+                      || floats * n > ((uint64_t)128 << 20) / sizeof(float)))
+            break;
+        const double more = (double)((grid * n + cus - 1) / cus) - 1.0;
+        const double us = (1.0 + more * cost.shared) * m.tile_blocks / n * cost.block
+            + (n > 1 ? cost.base + n * (cost.range + grid * cost.record) : 0.0);
+        if (n == 1 || us < best) {
+            best = us;
+            plan.n_split = n;
+        }
+    }
+    if (const char* forced = std::getenv("CKV_PREFILL_SPLIT"))
+        plan.n_split = (uint32_t)std::clamp(std::strtol(forced, nullptr, 10), 1L, (long)split_max);
+    if (plan.n_split > 1) {
+        plan.records_floats = floats * plan.n_split;
+        plan.counters = grid;
+    }
+    return plan;
+}
+
+} // namespace
+
+uint32_t prefill_window_rows(const pool_view& p, uint32_t q_heads)
+{
+    return 128 / std::min(q_heads / p.kv_heads, 4u);
+}
+
 // A launch of 8-wave workgroups (one per compute unit: their LDS stages take
 // 135 KB) that would not give every compute unit one, or would end on a
 // partial round, takes 4-wave workgroups instead, two to a compute unit (GQA
@@ -848,13 +906,6 @@ bool prefill_supported(const pool_view& p, uint32_t q_heads, const void* q, cons
 // a launch of more than half a round of 8-wave workgroups, and less than one,
 // takes 4-wave workgroups unless its shortest tile attends more 32-key blocks
 constexpr uint32_t sub_round_max_blocks = 40;
-// Shortest key range of a windowed f32 tile, in blocks.
-constexpr uint32_t window_min_blocks_f32 = 2;
-
-uint32_t prefill_window_rows(const pool_view& p, uint32_t q_heads)
-{
-    return 128 / std::min(q_heads / p.kv_heads, 4u);
-}
 
 prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t q_heads,
                                 int cu_count)
@@ -863,40 +914,23 @@ prefill_shape_info prefill_plan(const pool_view& p, const meta_view& m, uint32_t
     const uint32_t group = p.kv_heads ? q_heads / p.kv_heads : 0;
     if (const char* forced = std::getenv("CKV_PREFILL_SPLIT_MIN"))
         plan.min_blocks = (uint32_t)std::max(1L, std::strtol(forced, nullptr, 10));
+    if (m.window.window != all_keys.window)
+        return window_plan(p, m, q_heads, cu_count);
     if (p.head_dim == 256)
         return prefill_wide_plan(p, m, q_heads, cu_count, plan.min_blocks);
-    const bool windowed = m.window.window != all_keys.window;
     if (p.dtype == CKV_F32) {
         // f32 pools: 8-wave workgroups, two to a compute unit; a launch that
         // gives at most one to each splits its long tiles' keys to fill them
-        const uint64_t per_tile = windowed ? group / std::min(group, 4u) : group;
-        const uint64_t grid = (uint64_t)m.n_tiles * per_tile * p.kv_heads;
+        const uint64_t grid = (uint64_t)m.n_tiles * group * p.kv_heads;
         uint64_t split = grid && cu_count > 0 && grid <= (uint64_t)cu_count
             ? 2 * (uint64_t)cu_count / grid
             : 1;
         if (const char* forced = std::getenv("CKV_PREFILL_SPLIT"))
             split = (uint64_t)std::max(1L, std::strtol(forced, nullptr, 10));
         plan.n_split = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(split, 1), split_max);
-        if (windowed && !std::getenv("CKV_PREFILL_SPLIT_MIN"))
-            plan.min_blocks = window_min_blocks_f32;
         if (plan.n_split > 1) {
-            plan.records_floats = grid * plan.n_split * (windowed ? 128 : 256) * prefill_record_floats;
+            plan.records_floats = grid * plan.n_split * 256 * prefill_record_floats;
             plan.counters = grid;
-        }
-        return plan;
-    }
-    if (windowed) {
-        // 4-wave workgroups, two to a compute unit; a launch that leaves some idle splits
-        // each tile's keys between as many as fill them
-        const uint64_t busy = (uint64_t)m.n_tiles * (group / std::min(group, 4u)) * p.kv_heads;
-        uint64_t split = busy && cu_count > 0 ? 2 * (uint64_t)cu_count / busy : 1;
-        if (const char* forced = std::getenv("CKV_PREFILL_SPLIT"))
-            split = (uint64_t)std::max(1L, std::strtol(forced, nullptr, 10));
-        plan.waves = 4;
-        plan.n_split = (uint32_t)std::clamp<uint64_t>(split, 1, split_max);
-        if (plan.n_split > 1) {
-            plan.records_floats = busy * plan.n_split * 128 * prefill_record_floats;
-            plan.counters = busy;
         }
         return plan;
     }

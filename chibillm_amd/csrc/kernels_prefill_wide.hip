@@ -624,16 +624,14 @@ prefill_shape_info prefill_wide_plan(const pool_view& p, const meta_view& m, uin
     prefill_shape_info plan { waves, 1, min_blocks, 0, 0 };
     const uint32_t group = q_heads / p.kv_heads, G = wide_heads(group);
     // row_blocks[i]: the tiles' workgroups of 32 << i rows
-    const bool windowed = m.window.window != all_keys.window;
-    const uint32_t workgroups = windowed ? m.n_tiles : m.row_blocks[G == 4 ? 0 : G == 2 ? 1 : 2];
-    const uint64_t busy = (uint64_t)workgroups * (group / G) * p.kv_heads;
+    const uint64_t busy = (uint64_t)m.row_blocks[G == 4 ? 0 : G == 2 ? 1 : 2] * (group / G) * p.kv_heads;
     uint64_t split = busy && cu_count > 0 ? (uint64_t)cu_count / busy : 1;
     if (const char* forced = std::getenv("CKV_PREFILL_SPLIT"))
         split = (uint64_t)std::max(1L, std::strtol(forced, nullptr, 10));
     // records are kept for every workgroup of the grid, those past a short
     // tile's rows included: within 128 MiB
-    const uint64_t grid = (uint64_t)m.n_tiles * (windowed ? 1 : prefill_tile_rows * G / (32 * waves))
-        * (group / G) * p.kv_heads;
+    const uint64_t grid = (uint64_t)m.n_tiles * (prefill_tile_rows * G / (32 * waves)) * (group / G)
+        * p.kv_heads;
     const uint64_t floats = grid * (32 * waves) * (dim + 4);
     const uint64_t room = std::max<uint64_t>(1, ((uint64_t)128 << 20) / sizeof(float) / std::max<uint64_t>(floats, 1));
     plan.n_split = (uint32_t)std::clamp<uint64_t>(std::min(split, room), 1, split_max);
