@@ -153,11 +153,32 @@ hipError_t host_free(ckv_context* ctx, void* ptr)
     return hipHostFree(ptr);
 }
 
+// Whether the context's stream is being captured into a graph (or cannot be asked
+// while another is): a launch there takes no upload and no allocation, whose replays
+// would read staging memory of other uploads or free what a graph uses.
+bool capturing(const ckv_context* ctx)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing(ctx->stream, &status);
+    if (e != hipSuccess)
+        (void)hipGetLastError();
+    return e != hipSuccess || status != hipStreamCaptureStatusNone;
+}
+
+int refuse_captured(ckv_context* ctx)
+{
+    return set_error(ctx, CKV_E_INVALID_ARGUMENT,
+                     "the stream is being captured and the call has something to upload or "
+                     "allocate: make it once on this batch before the capture");
+}
+
 // Returns pinned staging memory of at least `bytes`: the ring's next slot,
 // after the copy last made from it has completed. upload_staged copies from
 // this slot and advances the ring.
 int stage(ckv_context* ctx, size_t bytes, void** host)
 {
+    if (ctx->in_capture)
+        return refuse_captured(ctx);
     auto& slot = ctx->staging[ctx->staging_next];
     if (slot.pending) {
         const hipError_t e = hipEventSynchronize(slot.done);
@@ -194,18 +215,25 @@ int upload_staged(ckv_context* ctx, void* device, size_t bytes)
     return CKV_OK;
 }
 
-// Grow-only device buffer; the stream is drained before an old buffer is freed.
+// Grow-only device buffer; the stream is drained before an old buffer is freed. One
+// that a graph may use is kept.
 template <class T>
 int ensure_device(ckv_context* ctx, T** ptr, size_t* capacity, size_t needed, const char* what)
 {
     if (needed <= *capacity)
         return CKV_OK;
+    if (ctx->in_capture)
+        return refuse_captured(ctx);
     // grow by half again at least: a batch a little larger than the last
     // must not reallocate (and drain the stream) every step
     const size_t count = std::max({ needed, *capacity + *capacity / 2, (size_t)1024 });
     if (*ptr) {
-        (void)hipStreamSynchronize(ctx->stream);
-        (void)dev_free(ctx, *ptr);
+        if (ctx->captured) {
+            ctx->retired.push_back(*ptr);
+        } else {
+            (void)hipStreamSynchronize(ctx->stream);
+            (void)dev_free(ctx, *ptr);
+        }
         *ptr = nullptr;
         *capacity = 0;
     }
@@ -410,25 +438,6 @@ int ensure_plan(ckv_pool* pool)
     return CKV_OK;
 }
 
-// Whether the context's stream is being captured into a graph (or cannot be asked
-// while another is): a launch there takes no upload and no allocation, whose replays
-// would read staging memory of other uploads or free what a graph uses.
-bool capturing(const ckv_context* ctx)
-{
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    const hipError_t e = hipStreamIsCapturing(ctx->stream, &status);
-    if (e != hipSuccess)
-        (void)hipGetLastError();
-    return e != hipSuccess || status != hipStreamCaptureStatusNone;
-}
-
-int refuse_captured(ckv_context* ctx)
-{
-    return set_error(ctx, CKV_E_INVALID_ARGUMENT,
-                     "the stream is being captured and the call has something to upload or "
-                     "allocate: make it once on this batch before the capture");
-}
-
 // Scratch of the fast decode when its plan cuts rows into chunks: a partial
 // record for every (record, q head) and an arrival counter for every
 // (record, kv head). The counters have a buffer of their own (the generic
@@ -443,10 +452,6 @@ int ensure_split(ckv_pool* pool, const meta_view& m, size_t q_heads, split_scrat
     size_t capacity_floats = pool->d_partials_bytes / sizeof(float);
     const size_t floats = (size_t)m.n_records * q_heads
         * partial_record_floats((uint32_t)pool->head_dim);
-    if (m.window.window != all_keys.window
-        && (floats > capacity_floats || m.n_records * pool->kv_heads > pool->d_arrivals_words)
-        && capturing(ctx))
-        return refuse_captured(ctx);
     int status = ensure_device(ctx, &pool->d_partials, &capacity_floats, floats,
                                "decode partials");
     pool->d_partials_bytes = capacity_floats * sizeof(float);
@@ -547,28 +552,30 @@ key_window window_of(const ckv_pool* pool, size_t window, size_t sinks)
     return window_low(pool->last_position, w) > w.sinks ? w : all_keys;
 }
 
-// Selects the batch's window; its plan and work list are derived anew unless they
-// are this window's already.
-void select_window(ckv_pool* pool, key_window w)
+// The batch through a window, in tiles of at most `tile_rows` rows (0: decode rows).
+window_batch& select_window(ckv_pool* pool, key_window w, uint32_t tile_rows = 0)
 {
-    meta_view& m = pool->window_meta;
-    if (m.window.window == w.window && m.window.sinks == w.sinks
-        && pool->window_positions.size() == pool->positions.size())
-        return;
-    pool->window_positions.clear(); // stays so if what follows throws
-    pool->window_plan_ready = pool->window_work_ready = false;
-    pool->window_tile_rows = 0;
-    pool->window_positions.resize(pool->positions.size());
-    m = pool->meta;
-    m.window = w;
+    auto& all = pool->windows;
+    for (size_t i = 0; i < pool->n_windows; ++i)
+        if (all[i]->meta.window.window == w.window && all[i]->meta.window.sinks == w.sinks
+            && all[i]->tile_rows == tile_rows)
+            return *all[i];
+    if (pool->n_windows == all.size())
+        all.push_back(std::make_unique<window_batch>());
+    window_batch& made = *all[pool->n_windows++];
+    made.tile_rows = tile_rows;
+    made.plan_ready = made.work_ready = made.tiles_ready = false;
+    made.meta = pool->meta;
+    made.meta.window = w;
+    return made;
 }
 
 // The rows' positions less the tokens of the units (of `unit` tokens) that the
 // window skips.
-const std::vector<uint32_t>& close_window_gaps(ckv_pool* pool, uint32_t unit)
+const std::vector<uint32_t>& close_window_gaps(ckv_pool* pool, key_window w, uint32_t unit)
 {
-    const key_window w = pool->window_meta.window;
     std::vector<uint32_t>& left = pool->window_positions;
+    left.resize(pool->positions.size());
     for (size_t r = 0; r < left.size(); ++r) {
         const uint32_t p = pool->positions[r];
         left[r] = p - window_gap_of(window_low(p, w), w.sinks, unit).skip * unit;
@@ -577,29 +584,24 @@ const std::vector<uint32_t>& close_window_gaps(ckv_pool* pool, uint32_t unit)
 }
 
 // The window's work list of the generic decode, in tokens, at its first launch.
-int ensure_window_work(ckv_pool* pool)
+int ensure_window_work(ckv_pool* pool, window_batch& b)
 {
-    if (pool->window_work_ready)
+    if (b.work_ready)
         return CKV_OK;
-    if (capturing(pool->ctx))
-        return refuse_captured(pool->ctx);
-    const int status = put_work(pool, close_window_gaps(pool, 1), pool->window_meta,
-                                &pool->d_window_work, &pool->d_window_work_words,
-                                pool->window_work_multi);
-    pool->window_work_ready = status == CKV_OK;
+    const int status = put_work(pool, close_window_gaps(pool, b.meta.window, 1), b.meta, &b.d_work,
+                                &b.d_work_words, b.work_multi);
+    b.work_ready = status == CKV_OK;
     return status;
 }
 
 // The window's plan of the fast decode, in pages, at its first launch.
-int ensure_window_plan(ckv_pool* pool)
+int ensure_window_plan(ckv_pool* pool, window_batch& b)
 {
-    if (pool->window_plan_ready)
+    if (b.plan_ready)
         return CKV_OK;
     ckv_context* ctx = pool->ctx;
-    if (capturing(ctx))
-        return refuse_captured(ctx);
     const uint32_t bs = (uint32_t)pool->block_size;
-    const std::vector<uint32_t>& left = close_window_gaps(pool, bs);
+    const std::vector<uint32_t>& left = close_window_gaps(pool, b.meta.window, bs);
     const decode_plan_shape shape =
         shape_window_plan(left, bs, (uint32_t)pool->kv_heads, ctx->cu_count,
                           decode_form_of(pool->dtype, (uint32_t)pool->head_dim));
@@ -607,34 +609,32 @@ int ensure_window_plan(ckv_pool* pool)
     void* host = nullptr;
     int status = stage(ctx, words * sizeof(uint32_t), &host);
     if (!status)
-        status = ensure_device(ctx, &pool->d_window_plan, &pool->d_window_plan_words, words,
-                               "decode plan");
+        status = ensure_device(ctx, &b.d_plan, &b.d_plan_words, words, "decode plan");
     if (status)
         return status;
     auto* w = static_cast<uint32_t*>(host);
-    put_plan(pool, left, pool->window_meta, shape, w, pool->d_window_plan);
+    put_plan(pool, left, b.meta, shape, w, b.d_plan);
     place_window_plan(pool->positions, shape, w);
     uint64_t pages = 0;
     for (const uint32_t p : left)
         pages += p / bs + 1;
-    pool->window_meta.mean_pages = left.empty() ? 0 : (uint32_t)(pages / left.size());
-    status = upload_staged(ctx, pool->d_window_plan, words * sizeof(uint32_t));
-    pool->window_plan_ready = status == CKV_OK;
+    b.meta.mean_pages = left.empty() ? 0 : (uint32_t)(pages / left.size());
+    status = upload_staged(ctx, b.d_plan, words * sizeof(uint32_t));
+    b.plan_ready = status == CKV_OK;
     return status;
 }
 
-// The window's tiles of at most `rows` rows, one for each workgroup (tiles of up to 256
+// The window's tiles of at most b.tile_rows rows, one for each workgroup (tiles of up to 256
 // rows whose empty places return at once left those that work on a quarter of the
 // compute units: 32 sequences of 64 rows behind a window of 512 took 59 us, twice
 // what 16 took), those with the most key blocks first, at their first launch.
-int ensure_window_tiles(ckv_pool* pool, uint32_t rows)
+int ensure_window_tiles(ckv_pool* pool, window_batch& b)
 {
-    if (pool->window_tile_rows == rows)
+    if (b.tiles_ready)
         return CKV_OK;
     ckv_context* ctx = pool->ctx;
-    if (capturing(ctx))
-        return refuse_captured(ctx);
-    const key_window w = pool->window_meta.window;
+    const key_window w = b.meta.window;
+    const uint32_t rows = b.tile_rows;
     const std::vector<uint32_t>& all = pool->tiles;
     std::vector<std::pair<uint32_t, std::array<uint32_t, tile_entry_words>>> parts;
     for (size_t t = 0; t < all.size(); t += tile_entry_words)
@@ -650,78 +650,86 @@ int ensure_window_tiles(ckv_pool* pool, uint32_t rows)
     void* host = nullptr;
     int status = stage(ctx, words * sizeof(uint32_t), &host);
     if (!status)
-        status = ensure_device(ctx, &pool->d_window_tiles, &pool->d_window_tiles_words, words,
-                               "window tiles");
+        status = ensure_device(ctx, &b.d_tiles, &b.d_tiles_words, words, "window tiles");
     if (status)
         return status;
     auto* to = static_cast<uint32_t*>(host);
     for (const auto& part : parts)
         to = std::copy(part.second.begin(), part.second.end(), to);
-    status = upload_staged(ctx, pool->d_window_tiles, words * sizeof(uint32_t));
+    status = upload_staged(ctx, b.d_tiles, words * sizeof(uint32_t));
+    b.meta.tiles = b.d_tiles;
+    b.meta.n_tiles = (uint32_t)parts.size();
+    b.meta.tile_blocks = parts.empty() ? 0 : parts.front().first;
+    b.tiles_ready = status == CKV_OK;
+    return status;
+}
+
+// The batch through a window that leaves something out; null: the batch itself.
+window_batch* decode_window(ckv_pool* pool, key_window window)
+{
+    return window.window == all_keys.window ? nullptr : &select_window(pool, window);
+}
+
+// The plan and scratch of a fast decode launch, over the batch or through a window.
+int ensure_fast(ckv_pool* pool, window_batch* through, size_t q_heads, split_scratch& split)
+{
+    const int status = through ? ensure_window_plan(pool, *through) : ensure_plan(pool);
+    return status ? status
+                  : ensure_split(pool, through ? through->meta : pool->meta, q_heads, split);
+}
+
+// Everything of a decode launch but the launch: its plan or work list, and scratch.
+struct decode_setup {
+    window_batch* through = nullptr;
+    bool needs_merge = false;
+    split_scratch split {};
+    float* partials = nullptr;
+};
+
+int setup_decode(ckv_pool* pool, const void* queries, size_t q_heads, const void* output,
+                 key_window window, decode_setup& d)
+{
+    ckv_context* ctx = pool->ctx;
+    const bool fast = decode_fast_applies(view_of(pool), (uint32_t)q_heads, queries, output);
+    d.through = decode_window(pool, window);
+    int status = fast ? ensure_fast(pool, d.through, q_heads, d.split)
+        : d.through   ? ensure_window_work(pool, *d.through)
+                      : ensure_work(pool);
     if (status)
         return status;
-    pool->window_meta.tiles = pool->d_window_tiles;
-    pool->window_meta.n_tiles = (uint32_t)parts.size();
-    pool->window_meta.tile_blocks = parts.empty() ? 0 : parts.front().first;
-    pool->window_tile_rows = rows;
-    return CKV_OK;
-}
-
-// What a decode launch runs over: the batch, or the batch through a window.
-meta_view& decode_meta(ckv_pool* pool, key_window window)
-{
-    if (window.window == all_keys.window)
-        return pool->meta;
-    select_window(pool, window);
-    return pool->window_meta;
-}
-
-// The plan and scratch of a fast decode launch over `m` (decode_meta).
-int ensure_fast(ckv_pool* pool, const meta_view& m, size_t q_heads, split_scratch& split)
-{
-    const int status = &m == &pool->meta ? ensure_plan(pool) : ensure_window_plan(pool);
-    return status ? status : ensure_split(pool, m, q_heads, split);
+    d.needs_merge = !fast && (d.through ? d.through->work_multi : pool->work_multi);
+    if (d.needs_merge) {
+        size_t capacity_floats = pool->d_partials_bytes / sizeof(float);
+        const size_t needed = (size_t)(d.through ? d.through->meta : pool->meta).n_items * q_heads
+            * partial_record_floats((uint32_t)pool->head_dim);
+        status = ensure_device(ctx, &pool->d_partials, &capacity_floats, needed,
+                               "decode partials");
+        // stored whatever the outcome: a failed regrow leaves no buffer and
+        // must leave no capacity either
+        pool->d_partials_bytes = capacity_floats * sizeof(float);
+        d.partials = pool->d_partials;
+    }
+    return status;
 }
 
 int run_decode(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale,
                void* output, const void* gate = nullptr, key_window window = all_keys)
 {
     ckv_context* ctx = pool->ctx;
-    const pool_view view = view_of(pool);
-    float* partials = nullptr;
-    split_scratch split {};
-    const bool fast = decode_fast_applies(view, (uint32_t)q_heads, queries, output);
-    meta_view& m = decode_meta(pool, window);
-    const bool windowed = &m != &pool->meta;
-    int status = fast ? ensure_fast(pool, m, q_heads, split)
-        : windowed    ? ensure_window_work(pool)
-                      : ensure_work(pool);
+    decode_setup d;
+    int status = setup_decode(pool, queries, q_heads, output, window, d);
     if (status)
         return status;
-    const bool needs_merge = !fast && (windowed ? pool->window_work_multi : pool->work_multi);
-    if (needs_merge) {
-        size_t capacity_floats = pool->d_partials_bytes / sizeof(float);
-        const size_t needed = (size_t)m.n_items * q_heads
-            * partial_record_floats((uint32_t)pool->head_dim);
-        if (windowed && needed > capacity_floats && capturing(ctx))
-            return refuse_captured(ctx);
-        status = ensure_device(ctx, &pool->d_partials, &capacity_floats, needed,
-                               "decode partials");
-        // stored whatever the outcome: a failed regrow leaves no buffer and
-        // no capacity, so the next launch allocates again
-        pool->d_partials_bytes = capacity_floats * sizeof(float);
-        if (status)
-            return status;
-        partials = pool->d_partials;
-    }
-    status = run_kernel(ctx, windowed ? "window_attention_decode" : "paged_attention_decode", [&] {
+    const pool_view view = view_of(pool);
+    const meta_view& m = d.through ? d.through->meta : pool->meta;
+    status = run_kernel(ctx, d.through ? "window_attention_decode" : "paged_attention_decode", [&] {
         return launch_decode(ctx->stream, view, m, (uint32_t)layer, queries, (uint32_t)q_heads,
-                             scale, output, partials, ctx->cu_count, gate, split);
+                             scale, output, d.partials, ctx->cu_count, gate, d.split);
     });
-    if (status || !needs_merge)
+    if (status || !d.needs_merge)
         return status;
     return run_kernel(ctx, "paged_attention_merge", [&] {
-        return launch_merge(ctx->stream, view, m, (uint32_t)q_heads, output, partials, gate);
+        return launch_merge(ctx->stream, view, m, (uint32_t)q_heads, output, d.partials, gate);
     });
 }
 
@@ -927,8 +935,9 @@ int create_pool(ckv_context* ctx, size_t layers, size_t blocks, size_t block_siz
     return CKV_OK;
 }
 
-// Entry points through this make their context's device current while they run, and
-// give a status for what the host code throws.
+// Entry points through this make their context's device current while they run, take
+// a capture of its stream into account (ckv_context::in_capture) and give a status for
+// what the host code throws.
 struct device_scope {
     int before = -1;
     explicit device_scope(int device)
@@ -945,6 +954,17 @@ struct device_scope {
     }
 };
 
+struct capture_scope {
+    ckv_context* ctx;
+    explicit capture_scope(ckv_context* c)
+        : ctx(c)
+    {
+        ctx->in_capture = capturing(ctx);
+        ctx->captured |= ctx->in_capture;
+    }
+    ~capture_scope() { ctx->in_capture = false; }
+};
+
 template <class Call>
 int guarded(ckv_pool* pool, Call&& call) noexcept
 {
@@ -952,6 +972,7 @@ int guarded(ckv_pool* pool, Call&& call) noexcept
         return CKV_E_INVALID_ARGUMENT;
     try {
         const device_scope scope(pool->ctx->device);
+        const capture_scope capture(pool->ctx);
         return call();
     } catch (const std::exception&) {
         pool->ctx->last_error.assign("host memory"); // within the string's reserve
@@ -1097,6 +1118,8 @@ int ckv_context_destroy(ckv_context* ctx)
             (void)host_free(ctx, slot.pinned);
         (void)hipEventDestroy(slot.done);
     }
+    for (void* buffer : ctx->retired)
+        (void)dev_free(ctx, buffer);
     (void)hipStreamDestroy(ctx->own_stream);
     delete ctx;
     return CKV_OK;
@@ -1315,12 +1338,10 @@ int ckv_pool_destroy(ckv_pool* pool)
         (void)dev_free(ctx, pool->d_spill);
     if (pool->d_rope_q)
         (void)dev_free(ctx, pool->d_rope_q);
-    if (pool->d_window_plan)
-        (void)dev_free(ctx, pool->d_window_plan);
-    if (pool->d_window_work)
-        (void)dev_free(ctx, pool->d_window_work);
-    if (pool->d_window_tiles)
-        (void)dev_free(ctx, pool->d_window_tiles);
+    for (const auto& w : pool->windows)
+        for (uint32_t* buffer : { w->d_plan, w->d_work, w->d_tiles })
+            if (buffer)
+                (void)dev_free(ctx, buffer);
     if (pool->d_axes)
         (void)dev_free(ctx, pool->d_axes);
     delete pool;
@@ -1394,9 +1415,7 @@ void adopt_batch(ckv_pool* pool, size_t rows, size_t n_entries, bool with_slots,
     pool->fusable = fusable;
     pool->plan_ready = plan_uploaded;
     pool->work_ready = false;
-    pool->window_positions.clear();
-    pool->window_plan_ready = pool->window_work_ready = false;
-    pool->window_tile_rows = 0;
+    pool->n_windows = 0;
     pool->axes = 0;
     pool->uploaded = true;
 }
@@ -1530,9 +1549,9 @@ int ckv_tables_upload(ckv_pool* pool, const uint32_t* block_table, size_t n_entr
     m.slots = pool->d_meta + s_slots;
     m.tiles = pool->d_meta + s_tiles;
     m.n_tiles = (uint32_t)(tiles.size() / tile_entry_words);
-    pool->tiles = tiles;
     m.tile_blocks = shortest_tile_blocks(tiles);
     count_row_blocks(tiles, m.row_blocks);
+    pool->tiles.swap(tiles);
     adopt_batch(pool, rows, n_entries, slots != nullptr, shared, fusable, with_plan, false);
     return CKV_OK;
 }
@@ -1821,9 +1840,9 @@ int ckv_batch_upload(ckv_pool* pool, const uint32_t* seq, const uint32_t* first_
     m.slots = d + s_slots;
     m.tiles = d + s_tiles;
     m.n_tiles = (uint32_t)(tiles.size() / tile_entry_words);
-    pool->tiles = tiles;
     m.tile_blocks = shortest_tile_blocks(tiles);
     count_row_blocks(tiles, m.row_blocks);
+    pool->tiles.swap(tiles);
     adopt_batch(pool, rows, pool->seq_max * pool->seq_cap, with_slots != 0, shared, fusable,
                 with_plan, true);
     return CKV_OK;
@@ -2020,14 +2039,20 @@ int run_append_decode(ckv_pool* pool, size_t layer, const void* keys, const void
     if (pool->fusable && decode_fast_applies(view, (uint32_t)q_heads, queries, output)
         && aligned(keys) && aligned(values)) {
         split_scratch split {};
-        const meta_view& m = decode_meta(pool, window);
-        if (const int status = ensure_fast(pool, m, q_heads, split))
+        window_batch* through = decode_window(pool, window);
+        if (const int status = ensure_fast(pool, through, q_heads, split))
             return status;
-        return run_kernel(ctx, &m == &pool->meta ? "append_decode" : "append_decode_window", [&] {
+        const meta_view& m = through ? through->meta : pool->meta;
+        return run_kernel(ctx, through ? "append_decode_window" : "append_decode", [&] {
             return launch_append_decode(ctx->stream, view, m, (uint32_t)layer, keys, values,
                                         queries, (uint32_t)q_heads, scale, output, gate,
                                         ctx->cu_count, split);
         });
+    }
+    if (ctx->in_capture) { // refused, if at all, before the append is captured
+        decode_setup setup;
+        if (const int status = setup_decode(pool, queries, q_heads, output, window, setup))
+            return status;
     }
     if (const int status = ckv_append(pool, layer, keys, values, rows))
         return status;
@@ -2059,11 +2084,6 @@ int run_prefill(ckv_pool* pool, size_t layer, const void* queries, size_t q_head
     const prefill_shape_info plan = prefill_plan(view, m, (uint32_t)q_heads, ctx->cu_count);
     prefill_split split { nullptr, nullptr, plan.n_split, plan.min_blocks };
     if (plan.n_split > 1) {
-        if (windowed
-            && (plan.records_floats > pool->d_pre_records_floats
-                || plan.counters > pool->d_pre_arrivals_words)
-            && capturing(ctx))
-            return refuse_captured(ctx);
         int status = ensure_device(ctx, &pool->d_pre_records, &pool->d_pre_records_floats,
                                    (size_t)plan.records_floats, "prefill split records");
         if (status)
@@ -2196,16 +2216,16 @@ int run_rope_append_decode(ckv_pool* pool, size_t layer, const void* keys, const
     ckv_context* ctx = pool->ctx;
     const pool_view view = view_of(pool);
     const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    const bool windowed = window.window != all_keys.window;
     // the fused kernel rotates 16-bit pages in lane pairs part ^ (rotary / 16)
     const bool lane_pairs = view.dtype != CKV_F32 && rotary >= 16 && (rotary & (rotary - 1)) == 0;
     if (pool->fusable && lane_pairs && decode_fast_applies(view, (uint32_t)q_heads, queries, output)
         && aligned(keys) && aligned(values) && (!gate || aligned(gate))) {
         split_scratch split {};
-        const meta_view& m = decode_meta(pool, window);
-        if (const int status = ensure_fast(pool, m, q_heads, split))
+        window_batch* through = decode_window(pool, window);
+        if (const int status = ensure_fast(pool, through, q_heads, split))
             return status;
-        return run_kernel(ctx, windowed ? "rope_append_decode_window" : "rope_append_decode", [&] {
+        const meta_view& m = through ? through->meta : pool->meta;
+        return run_kernel(ctx, through ? "rope_append_decode_window" : "rope_append_decode", [&] {
             return launch_append_decode(ctx->stream, view, m, (uint32_t)layer, keys, values,
                                         queries, (uint32_t)q_heads, scale, output, gate,
                                         ctx->cu_count, split, &freq, rotary);
@@ -2214,10 +2234,12 @@ int run_rope_append_decode(ckv_pool* pool, size_t layer, const void* keys, const
     // unfused: queries rotated into a pool buffer, keys rotated into their
     // slots, then the attention over the rotated queries
     const size_t q_bytes = rows * q_heads * pool->head_dim * pool->elem_size;
-    if (windowed && q_bytes > pool->d_rope_q_bytes && capturing(ctx))
-        return refuse_captured(ctx);
     int status = ensure_device(ctx, &pool->d_rope_q, &pool->d_rope_q_bytes, q_bytes,
                                "rotated queries");
+    if (!status && ctx->in_capture) { // refused, if at all, before the append is captured
+        decode_setup setup;
+        status = setup_decode(pool, pool->d_rope_q, q_heads, output, window, setup);
+    }
     if (status)
         return status;
     status = ckv_rope(pool, queries, pool->d_rope_q, q_heads, theta, rotary_dim, rows);
@@ -2373,11 +2395,13 @@ int ckv_attention_window(ckv_pool* pool, size_t layer, const void* queries, size
             || !prefill_takes(pool, queries, q_heads, scale, output, gate))
             return run_decode(pool, layer, queries, q_heads, scale, output, gate, w);
         // also a window that leaves nothing out: its kernels hold probabilities in more bits
-        select_window(pool, w.window != all_keys.window ? w : key_window { UINT32_MAX - 1, 0 });
-        status = ensure_window_tiles(pool, prefill_window_rows(view_of(pool), (uint32_t)q_heads));
+        window_batch& through =
+            select_window(pool, w.window != all_keys.window ? w : key_window { UINT32_MAX - 1, 0 },
+                          prefill_window_rows(view_of(pool), (uint32_t)q_heads));
+        status = ensure_window_tiles(pool, through);
         if (status)
             return status;
-        return run_prefill(pool, layer, queries, q_heads, scale, output, gate, pool->window_meta);
+        return run_prefill(pool, layer, queries, q_heads, scale, output, gate, through.meta);
     });
 }
 
@@ -2436,8 +2460,6 @@ int ckv_rope_axes_upload(ckv_pool* pool, const uint32_t* positions, size_t axes,
             return set_error(ctx, CKV_E_NO_TABLES, "axes before ckv_tables_upload");
         if (rows != pool->positions.size())
             return set_error(ctx, CKV_E_POSITION_COUNT_MISMATCH, "rows != uploaded positions");
-        if (capturing(ctx))
-            return refuse_captured(ctx);
         const size_t words = std::max<size_t>(axes * rows, 4);
         void* host = nullptr;
         int status = stage(ctx, words * sizeof(uint32_t), &host);
@@ -2593,8 +2615,6 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
         const std::vector<uint32_t>&kept = plan.kept, &runs = plan.runs;
         if (kept.empty())
             return CKV_OK;
-        if (capturing(ctx))
-            return refuse_captured(ctx);
         // up: runs | from | to | shift
         const size_t s_from = round4(runs.size()), s_to = s_from + round4(kept.size());
         const size_t s_shift = s_to + round4(kept.size()), words = s_shift + kept.size();

@@ -6,6 +6,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <map>
+#include <memory>
 #include <string>
 #include <vector>
 
@@ -194,6 +195,19 @@ struct move_marks {
     uint32_t generation = 0;
 };
 
+// A batch through a window: the same rows with the plan, the work list or the tiles of
+// what the window leaves of them, each derived at the first launch that takes it and
+// kept, in buffers of their own, until the next batch: a model's layers of several
+// windows, and graphs that captured them, find theirs.
+struct window_batch {
+    uint32_t tile_rows = 0; // the tiles' rows at most; 0: decode rows
+    bool plan_ready = false, work_ready = false, tiles_ready = false;
+    bool work_multi = false;
+    meta_view meta {};
+    uint32_t *d_plan = nullptr, *d_work = nullptr, *d_tiles = nullptr;
+    size_t d_plan_words = 0, d_work_words = 0, d_tiles_words = 0;
+};
+
 struct pending_timing {
     const char* name;
     hipEvent_t start;
@@ -252,6 +266,15 @@ struct ckv_context {
     // device and pinned host allocations and frees made by the library on
     // this context (ckv_debug_allocations)
     uint64_t allocations = 0;
+
+    // A captured launch keeps reading what it was given whenever its graph is replayed.
+    // in_capture: a call that takes launches under capture into account runs on a stream
+    // being captured, and is refused what it would upload or allocate. captured: some
+    // such call was captured; buffers that grow from then on leave the old one to the
+    // graphs, until the context goes.
+    bool in_capture = false;
+    bool captured = false;
+    std::vector<void*> retired;
 
     bool profile = false;
     std::vector<ckv::pending_timing> pending;
@@ -319,21 +342,10 @@ struct ckv_pool {
     std::vector<uint32_t> seq_len, seq_host, dirty;
     std::vector<uint8_t> seq_dirty;
 
-    // The current batch through a window: the same rows with the plan and work
-    // list of what the window leaves of them, derived at the first launch with it
-    // and kept until another window or batch comes.
-    bool window_plan_ready = false;
-    bool window_work_ready = false;
-    bool window_work_multi = false;
-    std::vector<uint32_t> window_positions; // positions less the tokens of the skipped pages
-    ckv::meta_view window_meta {};
-    uint32_t* d_window_plan = nullptr;
-    size_t d_window_plan_words = 0;
-    uint32_t* d_window_work = nullptr;
-    size_t d_window_work_words = 0;
-    uint32_t window_tile_rows = 0; // rows of window_meta's tiles at most; 0: none yet
-    uint32_t* d_window_tiles = nullptr;
-    size_t d_window_tiles_words = 0;
+    // the current batch through each window it was attended through, then spare ones
+    std::vector<std::unique_ptr<ckv::window_batch>> windows;
+    size_t n_windows = 0;
+    std::vector<uint32_t> window_positions; // positions less the tokens of the skipped units
 
     // the batch rows' positions on several axes ([axes][rows], ckv_rope_axes_upload)
     uint32_t axes = 0;

@@ -296,3 +296,100 @@ def test_captured_decode_replays_and_cold_capture_is_refused(ctx):
             assert torch.equal(out, want)
     pool.close()
     own.close()
+
+
+@pytest.mark.parametrize("dtype,d,chunks", [("bf16", 128, False), ("f32", 128, False), ("bf16", 64, False),
+                                            ("bf16", 128, True), ("f32", 128, True), ("f16", 256, True)])
+def test_captured_windows_keep_what_they_read(ctx, dtype, d, chunks):
+    """Layers of two windows and more query heads captured into one graph: calls of other windows
+    and of more heads afterwards, which take lists of their own and larger scratch, leave its
+    replays as they were, on new inputs."""
+    print(f"captured windows {dtype} d {d} chunks {chunks}", flush=True)
+    from chibillm_amd import ckv
+    stream = torch.cuda.Stream()
+    own = ckv.Context(0, stream=stream)
+    first, counts = ([900, 40, 0], [100, 1, 33]) if chunks else ([1500, 89, 0, 700], [1] * 4)
+    rows, heads = sum(counts), 2
+    cache = Cache(own, dtype, [f + c for f, c in zip(first, counts)], heads, d, seed=12)
+    with torch.cuda.stream(stream):
+        pool = cache.to_device()
+        cache.upload(first, counts, slots=not chunks)
+        q, k, v = (cache.randn(rows, n * heads, d).cuda().flatten(1) for n in (8, 1, 1))
+        scale = 1 / math.sqrt(d)
+
+        def layer(group, window, out):
+            rows_q = q[:, :group * heads * d].contiguous() if group < 8 else q
+            if chunks or group == 4:
+                pool.attention_window(0, rows_q, group * heads, scale, window, out, sinks=4)
+            else:
+                pool.rope_append_decode_window(0, k, v, rows_q, group * heads, scale, 1e4, window, out, sinks=4)
+
+        calls = [(2, 700), (2, 60), (4, 700), (2, 5000)]
+        outs = [torch.empty(rows, g * heads * d, dtype=cache.dtype, device="cuda") for g, _ in calls]
+
+        def layers():
+            for (group, window), out in zip(calls, outs):
+                layer(group, window, out)
+
+        layers()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            layers()
+        wide = torch.empty(rows, 8 * heads * d, dtype=cache.dtype, device="cuda")
+        for turn in range(3):
+            for window in (33 + turn, 800 + turn, 400):
+                layer(8, window, wide)
+                layer(2, window, outs[0])
+            for x in (q, k, v):
+                x.normal_()
+            layers()
+            stream.synchronize()
+            want = [out.clone() for out in outs]
+            for out in outs:
+                out.fill_(math.nan)
+            graph.replay()
+            stream.synchronize()
+            for out, w, call in zip(outs, want, calls):
+                assert torch.equal(out, w), f"replay {turn} of group {call[0]} window {call[1]}"
+    pool.close()
+    own.close()
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("bf16", 64), ("f32", 128)])
+@pytest.mark.parametrize("window", [40, 10_000])
+def test_a_refused_call_captures_nothing(ctx, dtype, d, window):
+    """Under capture and before any eager call, also where the window covers every row: refused
+    before the append, so that the graph leaves the cache as it was."""
+    from chibillm_amd import ckv
+    stream = torch.cuda.Stream()
+    own = ckv.Context(0, stream=stream)
+    lengths = [300, 7, 801]
+    cache = Cache(own, dtype, lengths, 2, d, seed=13)
+    with torch.cuda.stream(stream):
+        pool = cache.to_device()
+        _, _, at = cache.upload([n - 1 for n in lengths], [1] * 3)
+        q, k, v = (cache.randn(3, n, d).cuda().flatten(1) for n in (16, 2, 2))
+        out, scale, refused = torch.zeros_like(q), 1 / math.sqrt(d), 0
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out.add_(1)  # a graph has to hold something
+            for call in (lambda: pool.append_decode_window(0, k, v, q, 16, scale, window, out, sinks=4),
+                         lambda: pool.rope_append_decode_window(0, k, v, q, 16, scale, 1e4, window, out, sinks=4)):
+                try:
+                    call()
+                except ckv.CkvError as e:
+                    assert e.name == "ckv.invalid_argument"
+                    refused += 1
+        # rows of a plan that came with the batch and cuts none have nothing to upload
+        assert refused == 2 or (window > 1000 and refused < 2)
+        graph.replay()
+        stream.synchronize()
+        if refused == 2:
+            cache.unchanged()
+            assert torch.all(out == 1)
+        else:
+            cache.unchanged(but=at)
+    pool.close()
+    own.close()
