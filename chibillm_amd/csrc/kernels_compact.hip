@@ -9,7 +9,12 @@
 // In place, a move may overwrite a slot that another move reads. A run's moves are
 // done in order, a chunk at a time: a workgroup reads a chunk's rows into registers,
 // waits until all of them have arrived, and writes them. One workgroup walks a run
-// for one head of one layer of K or V, so nothing else touches the bytes it reads.
+// for some heads of one layer of K or V, so nothing else touches the bytes it reads.
+//
+// Bound by HBM, each row read and written once. Measured on MI355X, 8 kv heads of 128,
+// bf16: 28 layers of 1,010 moves (the newer half of 2,011 tokens to behind the first
+// four) 58.6 us, 3.9 TB/s; 12 layers of 7,500 moves of six sequences to fresh pages
+// 169 us, 4.4 TB/s, where a device copy runs at 4.76.
 #include "ckv_internal.h"
 #include "prefill_records.h"
 #include "rope_turns.h"
@@ -23,10 +28,10 @@ constexpr uint32_t block_threads = 256;
 
 // Rows whose rotary and head widths are whole pairs of 16-byte words: a thread moves a
 // word of a head's first half and the one it is turned with (or two words past the
-// rotary width, of its halves likewise) for `ahead` tokens at a time. The workgroup goes through `heads` heads of
-// a chunk of tokens, whose angles it computes once, then to the next chunk; the next
-// head's rows are in flight while this one's are turned and written. Rows are read and
-// written once: past the caches, as checkpoints are.
+// rotary width, of its halves likewise) for `ahead` tokens at a time. The workgroup goes
+// through `heads` heads of a chunk of tokens, whose angles it computes once, then to the
+// next chunk; the next head's rows are in flight while this one's are turned and
+// written. Rows are read and written once: past the caches, as checkpoints are.
 constexpr uint32_t ahead = 2;
 
 template <int DT>

@@ -6,6 +6,12 @@
 // position; elements past the rotary width are copied. Queries, keys and values of a
 // layer go through one launch: rotated queries to a buffer, rotated keys and the
 // values into the rows' slots.
+//
+// Bound by HBM from a few hundred rows on: each row is read and written once. Measured
+// on MI355X, 16 q and 8 kv heads of 128, bf16: 4,096 rows 14.9 us, 4.5 TB/s read and
+// written (an element a thread with every angle computed for each head, 24.6 us); 1,531
+// fp16 rows of 8 q and 2 kv heads of 256, 64 of them rotated, 6.7 to 7.7 us by the host;
+// 6 rows take 3.3 us on the GPU, a launch's own time.
 #include "ckv_internal.h"
 #include "rope_turns.h"
 
@@ -18,8 +24,8 @@ constexpr uint32_t block_threads = 256;
 
 // Rows whose rotary and head widths are whole pairs of 16-byte words: a thread takes
 // one word of a head's first half and the one it is turned with (or two words past the
-// rotary width, of its halves likewise) in `per` heads of a row, whose angles it computes once, with the rows'
-// words in flight meanwhile.
+// rotary width, of its halves likewise) in PER heads of a row, whose angles it computes
+// once, with the rows' words in flight meanwhile.
 template <int DT, int PER>
 __global__ __launch_bounds__(block_threads) void rope_axes_words_kernel(
     pool_view p, const uint32_t* __restrict__ slots, uint32_t layer, axes_rows x, uint32_t rows,
@@ -96,8 +102,8 @@ __global__ __launch_bounds__(block_threads) void rope_axes_words_kernel(
     }
 }
 
-// Any other geometry: one thread per (head, pair) and grid row per row: heads 0 .. q_heads - 1 are the
-// query row's, the next kv_heads the key's and value's.
+// Any other geometry: one thread per (head, pair) and grid row per row: heads
+// 0 .. q_heads - 1 are the query row's, the next kv_heads the key's and value's.
 template <int DT>
 __global__ __launch_bounds__(block_threads) void rope_axes_kernel(
     pool_view p, const uint32_t* __restrict__ slots, uint32_t layer, axes_rows x, uint32_t rows,

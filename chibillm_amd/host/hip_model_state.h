@@ -99,9 +99,11 @@ public:
     // the new ones (ckv_compact); 0 leaves them as they are. Pages that others share
     // (checkpoints, other sequences) are not written: a private page takes their place,
     // also that of a shared last page which later tokens will fill. The next batch of the
-    // sequence starts at position kept.size(). Errors, before anything changes:
-    // invalid_reservation (no token, one out of order or past the sequence's pages, a
-    // rotary width or theta that ckv_compact refuses), capacity_exhausted.
+    // sequence starts at position kept.size(), and a checkpoint of it from then on holds
+    // the kept tokens. Errors, before anything changes: invalid_reservation (no token, one
+    // out of order or past the sequence's pages, a rotary width or theta that ckv_compact
+    // refuses), capacity_exhausted. Not to be called under stream capture; after any other
+    // error (the device's) the sequence is to be released.
     result<void, state_error> compact(seq_id id, std::span<const std::uint32_t> kept,
                                       float theta = 0.0f, std::size_t rotary_dimension = 0);
 

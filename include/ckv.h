@@ -378,10 +378,11 @@ int ckv_sigmoid_mul(ckv_context* ctx, int dtype, const void* gate, const void* i
  * sequence may give them back, as long as its table keeps some page id of the
  * pool in their place. Keys outside the window in pages that are read weigh
  * nothing, whatever their values.
- * Each batch keeps the work lists of one window at a time; a layer's calls with
- * the same window reuse them, a call with another replaces them (one small
- * upload). A call on a stream under capture is refused (invalid_argument) when
- * it would upload or allocate: make it once on the batch before the capture.
+ * The first call of a window on a batch makes its work lists (one small upload);
+ * later ones, of any layer, reuse them. A call on a stream under capture is refused
+ * (invalid_argument), before anything is captured, when it would upload or
+ * allocate: make it once on the batch before the capture. A captured call holds for
+ * the batch it was captured on, whatever other calls follow it there.
  * gate may be NULL; otherwise as ckv_attention_gated's, and it must not be the
  * queries' or the output's memory (unsupported_aliasing). */
 
