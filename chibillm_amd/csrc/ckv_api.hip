@@ -604,7 +604,7 @@ int ensure_window_plan(ckv_pool* pool, window_batch& b)
     const std::vector<uint32_t>& left = close_window_gaps(pool, b.meta.window, bs);
     const decode_plan_shape shape =
         shape_window_plan(left, bs, (uint32_t)pool->kv_heads, ctx->cu_count,
-                          decode_form_of(pool->dtype, (uint32_t)pool->head_dim));
+                          window_form_of(pool->dtype, (uint32_t)pool->head_dim));
     const size_t words = std::max<size_t>(plan_words(shape, left.size()), 4);
     void* host = nullptr;
     int status = stage(ctx, words * sizeof(uint32_t), &host);

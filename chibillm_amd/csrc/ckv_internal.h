@@ -431,6 +431,7 @@ decode_plan_shape shape_decode_plan(const std::vector<uint32_t>& positions, uint
                                     const decode_form& form = decode_form_of(CKV_BF16, 128),
                                     uint64_t chunk = 0); // fixed chunks of so many pages
 // The plan of rows through a window, from their positions without its gaps.
+decode_form window_form_of(int dtype, uint32_t head_dim);
 decode_plan_shape shape_window_plan(const std::vector<uint32_t>& positions, uint32_t block_size,
                                     uint32_t kv_heads, int cu_count, const decode_form& form);
 // Waves per workgroup of the fast decode for a launch of `units` (plan

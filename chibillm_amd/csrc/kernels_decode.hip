@@ -551,6 +551,17 @@ decode_plan_shape shape_decode_plan(const std::vector<uint32_t>& positions, uint
 // 65, behind 256 30.7 and 24.5; 160 of 2 kv heads, 2 each, 67.7 and 61.1, 21.8 and 22.4.
 constexpr uint64_t window_half_pages = 33, window_half_pages_wide = 17;
 
+decode_form window_form_of(int dtype, uint32_t head_dim)
+{
+    decode_form form = decode_form_of(dtype, head_dim);
+    // f32 rows behind a window are few pages: pieces of 4 rather than 8 fill more of the
+    // GPU where they have room (3 rows behind 300 tokens: 128-wide heads 6.6 and 6.0 us,
+    // 256-wide 12.7 and 9.4; 12 behind 600: 256-wide 15.4 and 11.7)
+    if (dtype == CKV_F32)
+        form.min_pages = std::min(form.min_pages, 4u);
+    return form;
+}
+
 decode_plan_shape shape_window_plan(const std::vector<uint32_t>& positions, uint32_t block_size,
                                     uint32_t kv_heads, int cu_count, const decode_form& form)
 {
