@@ -215,6 +215,21 @@ int upload_staged(ckv_context* ctx, void* device, size_t bytes)
     return CKV_OK;
 }
 
+// upload_staged by a kernel that reads the staging memory (launch_fetch).
+int fetch_staged(ckv_context* ctx, uint32_t* device, size_t words)
+{
+    auto& slot = ctx->staging[ctx->staging_next];
+    hipError_t e = launch_fetch(ctx->stream, device, slot.pinned, words);
+    if (e != hipSuccess)
+        return hip_error(ctx, e, "staged words");
+    e = hipEventRecord(slot.done, ctx->stream);
+    if (e != hipSuccess)
+        return hip_error(ctx, e, "staged words event");
+    slot.pending = true;
+    ctx->staging_next = (ctx->staging_next + 1) % ckv_context::staging_slots;
+    return CKV_OK;
+}
+
 // Grow-only device buffer; the stream is drained before an old buffer is freed. One
 // that a graph may use is kept.
 template <class T>
@@ -2617,7 +2632,7 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
             return CKV_OK;
         // up: runs | from | to | shift
         const size_t s_from = round4(runs.size()), s_to = s_from + round4(kept.size());
-        const size_t s_shift = s_to + round4(kept.size()), words = s_shift + kept.size();
+        const size_t s_shift = s_to + round4(kept.size()), words = s_shift + round4(kept.size());
         void* host = nullptr;
         status = stage(ctx, words * sizeof(uint32_t), &host);
         if (status)
@@ -2631,7 +2646,7 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
         }
         status = ensure_device(ctx, &pool->d_pairs, &pool->d_pairs_words, words, "move lists");
         if (!status)
-            status = upload_staged(ctx, pool->d_pairs, words * sizeof(uint32_t));
+            status = fetch_staged(ctx, pool->d_pairs, words);
         if (status)
             return status;
         const uint32_t* d = pool->d_pairs;

@@ -198,7 +198,31 @@ __global__ __launch_bounds__(block_threads) void compact_kernel(pool_view p, com
     }
 }
 
+// Words from pinned host memory, 16 bytes a thread.
+__global__ __launch_bounds__(block_threads) void fetch_kernel(uint4* __restrict__ to,
+                                                              const uint4* __restrict__ from,
+                                                              uint32_t n)
+{
+    const uint32_t i = blockIdx.x * block_threads + threadIdx.x;
+    if (i < n)
+        to[i] = from[i];
+}
+
 } // namespace
+
+hipError_t launch_fetch(hipStream_t s, uint32_t* to, const void* pinned, size_t words)
+{
+    void* from = nullptr;
+    if (const hipError_t e = hipHostGetDevicePointer(&from, const_cast<void*>(pinned), 0))
+        return e;
+    const uint64_t n = words / 4, blocks = (n + block_threads - 1) / block_threads;
+    if (words % 4 || n > 0xFFFFFFFFull)
+        return hipErrorInvalidValue;
+    fetch_kernel<<<(uint32_t)blocks, block_threads, 0, s>>>(reinterpret_cast<uint4*>(to),
+                                                            static_cast<const uint4*>(from),
+                                                            (uint32_t)n);
+    return hipGetLastError();
+}
 
 // Measured on MI355X: bytes pass at 4.5 TB/s, a run's chunk takes 2.9 us, and a launch
 // more costs 8 us where bytes are moving (28 layers of 1,206 scattered moves: one run
