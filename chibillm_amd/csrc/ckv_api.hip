@@ -1359,6 +1359,8 @@ int ckv_pool_destroy(ckv_pool* pool)
                 (void)dev_free(ctx, buffer);
     if (pool->d_axes)
         (void)dev_free(ctx, pool->d_axes);
+    if (pool->d_spare)
+        (void)dev_free(ctx, pool->d_spare);
     delete pool;
     return CKV_OK;
 }
@@ -2606,6 +2608,8 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
             return set_error(ctx, CKV_E_INVALID_ARGUMENT, "slots are required");
         if (n > pool->blocks * pool->block_size)
             return set_error(ctx, CKV_E_UNSUPPORTED_ALIASING, "two moves share a target");
+        if (pool->blocks * pool->block_size > spare_slot)
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT, "a pool of more than 2^31 slots");
         ckv::turn_table turns;
         uint32_t rotary = 0;
         if (shift) {
@@ -2630,9 +2634,10 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
         const std::vector<uint32_t>&kept = plan.kept, &runs = plan.runs;
         if (kept.empty())
             return CKV_OK;
-        // up: runs | from | to | shift
-        const size_t s_from = round4(runs.size()), s_to = s_from + round4(kept.size());
-        const size_t s_shift = s_to + round4(kept.size()), words = s_shift + round4(kept.size());
+        // up: runs | from | to | shift, the saved moves' after the others'
+        const size_t lists = kept.size() + plan.saved.size();
+        const size_t s_from = round4(runs.size()), s_to = s_from + round4(lists);
+        const size_t s_shift = s_to + round4(lists), words = s_shift + round4(lists);
         void* host = nullptr;
         status = stage(ctx, words * sizeof(uint32_t), &host);
         if (status)
@@ -2640,11 +2645,19 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
         auto* w = static_cast<uint32_t*>(host);
         std::copy(runs.begin(), runs.end(), w);
         for (size_t k = 0; k < kept.size(); ++k) {
-            w[s_from + k] = from[kept[k]];
+            w[s_from + k] = plan.spare[k] == UINT32_MAX ? from[kept[k]] : spare_slot + plan.spare[k];
             w[s_to + k] = to[kept[k]];
             w[s_shift + k] = shift ? (uint32_t)shift[kept[k]] : 0;
         }
-        status = ensure_device(ctx, &pool->d_pairs, &pool->d_pairs_words, words, "move lists");
+        for (size_t j = 0; j < plan.saved.size(); ++j) {
+            w[s_from + kept.size() + j] = from[plan.saved[j]];
+            w[s_to + kept.size() + j] = spare_slot + (uint32_t)j;
+            w[s_shift + kept.size() + j] = 0;
+        }
+        const size_t spare_bytes = plan.saved.size() * pool->layers * 2 * view.features * pool->elem_size;
+        status = ensure_device(ctx, &pool->d_spare, &pool->d_spare_bytes, spare_bytes, "saved rows");
+        if (!status)
+            status = ensure_device(ctx, &pool->d_pairs, &pool->d_pairs_words, words, "move lists");
         if (!status)
             status = fetch_staged(ctx, pool->d_pairs, words);
         if (status)
@@ -2655,7 +2668,8 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
             const uint32_t* first = d;
             for (const uint32_t n_runs : plan.launches) {
                 const compact_moves moves { first, d + s_from, d + s_to,
-                                            reinterpret_cast<const int32_t*>(d + s_shift), n_runs };
+                                            reinterpret_cast<const int32_t*>(d + s_shift), n_runs,
+                                            pool->d_spare, (uint32_t)plan.saved.size() };
                 if (e == hipSuccess)
                     e = launch_compact(ctx->stream, view, (uint32_t)pool->layers, moves, rotary,
                                        turns);

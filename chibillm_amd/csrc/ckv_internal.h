@@ -188,10 +188,10 @@ __device__ __forceinline__ void rope_pair(float a, float b, float c, float s, fl
     rb = __builtin_fmaf(b, c, a * s);
 }
 
-// The moves of a compaction that read each slot (the first and the last), and
-// whether one writes it, by the generation of the call that marked them.
+// The moves of a compaction that read each slot (the first and the last) and the one
+// that writes it, by the generation of the call that marked them.
 struct move_marks {
-    std::vector<uint32_t> read, first, last, written;
+    std::vector<uint32_t> read, first, last, written, writer;
     uint32_t generation = 0;
 };
 
@@ -353,6 +353,8 @@ struct ckv_pool {
     size_t d_axes_words = 0;
 
     ckv::move_marks marks; // of ckv_compact's slots
+    uint8_t* d_spare = nullptr; // rows it saves
+    size_t d_spare_bytes = 0;
 
     // device scratch
     float* d_partials = nullptr;
@@ -553,28 +555,31 @@ hipError_t launch_rope_axes(hipStream_t s, const pool_view& p, const meta_view& 
 // Moves of a compaction on the device: `runs` holds n_runs (first move, moves), each
 // run's moves in order, and the moves' source slots, target slots and position
 // shifts. A run's moves may overwrite what the same run reads at or before them;
-// nothing a run reads or writes is written by another.
+// nothing a run reads or writes is written by another. Slots from spare_slot on are rows
+// of `spare`, n_spare for each layer of K, then of V.
+constexpr uint32_t spare_slot = 0x80000000u;
 struct compact_moves {
     const uint32_t* runs;
     const uint32_t* from;
     const uint32_t* to;
     const int32_t* shift;
     uint32_t n_runs;
+    void* spare;
+    uint32_t n_spare;
 };
-// Checks the moves of ckv_compact and cuts them into runs. `kept` are the moves that
-// change something, `runs` pairs (first of kept, how many), in the order of their
-// launches, whose numbers of runs `launches` holds. The runs of one launch depend on
-// each other in no way. A sequence's moves fall into waves, in none of which a move
-// overwrites what another reads; a wave is cut into runs of at most compact_run moves
-// and has a launch of its own, but for a sequence's first ones, where going through them
-// in one run, in order, is estimated to take less than their launches. Returns null, or
-// why the moves are refused, with the status.
+// Checks the moves of ckv_compact (of at most spare_slot slots) and cuts them into runs.
+// `kept` are the moves that change something, run by run; `runs` pairs (first of kept,
+// how many), in the order of their launches, whose numbers of runs `launches` holds. The
+// runs of one launch depend on each other in no way. Where some of kept read what another
+// run writes, `saved` are those moves and `spare` the place in it of each of kept
+// (UINT32_MAX: none): the first of two launches copies their sources to spare rows, its
+// runs counting on from the end of kept. Returns null, or why the moves are refused, with
+// the status.
 constexpr uint32_t compact_run = 64;
-constexpr uint32_t compact_launches = 6;
 struct compact_plan {
-    std::vector<uint32_t> kept, runs, launches;
+    std::vector<uint32_t> kept, spare, saved, runs, launches;
 };
-// What a move costs, in microseconds: its bytes, its share of a run done in order, and
+// What a move costs, in microseconds: its bytes and its share of a run done in order; and
 // a launch.
 struct compact_cost {
     double move_bytes, move_in_run, launch;

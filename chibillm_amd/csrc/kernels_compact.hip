@@ -10,6 +10,11 @@
 // done in order, a chunk at a time: a workgroup reads a chunk's rows into registers,
 // waits until all of them have arrived, and writes them. One workgroup walks a run
 // for some heads of one layer of K or V, so nothing else touches the bytes it reads.
+// Runs are made so that a move and the one that overwrites its source share a run: kept
+// tokens that move towards the front form chains, the writer of a slot after its reader,
+// short where many tokens leave (a fraction f kept: log n / log 1/f moves). A long chain,
+// where few leave, is cut into several runs once it would take longer than one launch
+// more, which saves the sources that other runs overwrite to spare rows first.
 //
 // Bound by HBM, each row read and written once. Measured on MI355X, 8 kv heads of 128,
 // bf16: 28 layers of 1,010 moves (the newer half of 2,011 tokens to behind the first
@@ -25,6 +30,21 @@ namespace ckv {
 namespace {
 
 constexpr uint32_t block_threads = 256;
+
+// A workgroup's saved rows: those of its layer of K or V.
+template <class T>
+__device__ __forceinline__ T* spare_rows(const pool_view& p, const compact_moves& m)
+{
+    return static_cast<T*>(m.spare)
+        + ((uint64_t)blockIdx.z * gridDim.y + blockIdx.y) * m.n_spare * p.features;
+}
+
+// The row of a slot, or of spare_slot + a saved row.
+template <class T>
+__device__ __forceinline__ T* moved_row(T* base, T* spare, uint32_t slot, uint32_t features)
+{
+    return (slot & spare_slot ? spare : base) + (uint64_t)(slot & ~spare_slot) * features;
+}
 
 // Rows whose rotary and head widths are whole pairs of 16-byte words: a thread moves a
 // word of a head's first half and the one it is turned with (or two words past the
@@ -63,6 +83,8 @@ __global__ __launch_bounds__(block_threads) void compact_rows_kernel(pool_view p
     const uint32_t run = blockIdx.x / parts, head0 = blockIdx.x % parts * heads;
     const bool keys = blockIdx.z == 0;
     T* base = static_cast<T*>(keys ? p.keys : p.values) + blockIdx.y * p.layer_elems + head0 * d + at;
+    T* spare = spare_rows<T>(p, m) + head0 * d + at;
+    auto row_of = [&](uint32_t slot) { return moved_row(base, spare, slot, p.features); };
     const uint32_t first = m.runs[2 * run], count = m.runs[2 * run + 1];
     const uint32_t chunk = ahead * step;
 
@@ -82,7 +104,7 @@ __global__ __launch_bounds__(block_threads) void compact_rows_kernel(pool_view p
         rows x;
 #pragma unroll
         for (uint32_t k = 0; k < ahead; ++k) {
-            const T* src = base + (uint64_t)s.from[k] * p.features + h * d;
+            const T* src = row_of(s.from[k]) + h * d;
             x.a[k].v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(src));
             x.b[k].v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(src + apart));
         }
@@ -131,7 +153,7 @@ __global__ __launch_bounds__(block_threads) void compact_rows_kernel(pool_view p
                     }
                 }
                 if (now.live[k]) {
-                    T* dst = base + (uint64_t)now.to[k] * p.features + h * d;
+                    T* dst = row_of(now.to[k]) + h * d;
                     __builtin_nontemporal_store(x.a[k].v, reinterpret_cast<u32x4_t*>(dst));
                     __builtin_nontemporal_store(x.b[k].v, reinterpret_cast<u32x4_t*>(dst + apart));
                 }
@@ -157,6 +179,7 @@ __global__ __launch_bounds__(block_threads) void compact_kernel(pool_view p, com
     const uint64_t base = blockIdx.y * p.layer_elems + (uint64_t)head * d;
     const bool keys = blockIdx.z == 0;
     T* rows = static_cast<T*>(keys ? p.keys : p.values) + base;
+    T* spare = spare_rows<T>(p, m) + head * d;
     const uint32_t first = m.runs[2 * run], count = m.runs[2 * run + 1];
     const uint64_t total = (uint64_t)count * pairs;
     for (uint64_t i0 = 0; i0 < total; i0 += items * block_threads) {
@@ -169,7 +192,7 @@ __global__ __launch_bounds__(block_threads) void compact_kernel(pool_view p, com
             const uint32_t move = first + (uint32_t)(i / pairs), pair = (uint32_t)(i % pairs);
             const uint32_t a = pair < half ? pair : rotary + 2 * (pair - half);
             const uint32_t b = pair < half ? pair + half : min(a + 1, d - 1);
-            const T* src = rows + (uint64_t)m.from[move] * p.features;
+            const T* src = moved_row(rows, spare, m.from[move], p.features);
             x[k] = src[a];
             y[k] = src[b];
         }
@@ -183,7 +206,7 @@ __global__ __launch_bounds__(block_threads) void compact_kernel(pool_view p, com
             const uint32_t move = first + (uint32_t)(i / pairs), pair = (uint32_t)(i % pairs);
             const uint32_t a = pair < half ? pair : rotary + 2 * (pair - half);
             const uint32_t b = pair < half ? pair + half : min(a + 1, d - 1);
-            T* dst = rows + (uint64_t)m.to[move] * p.features;
+            T* dst = moved_row(rows, spare, m.to[move], p.features);
             const int32_t shift = m.shift[move];
             if (keys && shift && pair < half) {
                 float s, c, r1, r2;
@@ -225,8 +248,7 @@ hipError_t launch_fetch(hipStream_t s, uint32_t* to, const void* pinned, size_t 
 }
 
 // Measured on MI355X: bytes pass at 4.5 TB/s, a run's chunk takes 2.9 us, and a launch
-// more costs 8 us where bytes are moving (28 layers of 1,206 scattered moves: one run
-// 68 us, six launches 101; 4 layers of 2,100 moves: one run 103 us, six launches 69).
+// more costs 8 us where bytes are moving.
 compact_cost compact_cost_of(const pool_view& p, uint32_t layers)
 {
     const double row = (double)p.features * p.elem_size;
@@ -247,7 +269,7 @@ const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* fro
         if (from[i] >= slots || to[i] >= slots)
             return "a move's slot is outside the pool";
     if (marks.written.size() < slots) {
-        for (auto* v : { &marks.read, &marks.first, &marks.last, &marks.written })
+        for (auto* v : { &marks.read, &marks.first, &marks.last, &marks.written, &marks.writer })
             v->assign(slots, 0);
         marks.generation = 0;
     }
@@ -264,64 +286,87 @@ const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* fro
         marks.last[from[i]] = (uint32_t)i;
     }
     status = CKV_E_UNSUPPORTED_ALIASING;
-    plan.kept.reserve(n);
-    std::vector<uint32_t> runs[compact_launches];
-    std::vector<size_t> waves; // where a sequence's waves begin, in kept
-    for (size_t q = 0, begin = 0; q < n_sequences; begin += counts[q], ++q) {
-        const size_t end = begin + counts[q];
-        size_t wave = begin; // the wave's first move
-        waves.assign(1, plan.kept.size());
-        for (size_t i = begin; i < end; ++i) {
+    for (size_t q = 0, begin = 0; q < n_sequences; begin += counts[q], ++q)
+        for (size_t i = begin; i < begin + counts[q]; ++i) {
             if (marks.written[to[i]] == g)
                 return "two moves share a target";
             marks.written[to[i]] = g;
-            if (marks.read[to[i]] == g) {
-                const size_t first = marks.first[to[i]], last = marks.last[to[i]];
-                if (first < begin || last > i)
-                    return "a move's target is read by a later move or another sequence";
-                if (last == i ? first < i : last >= wave) { // read in this wave (or perhaps)
-                    wave = i;
-                    if (plan.kept.size() > waves.back())
-                        waves.push_back(plan.kept.size());
-                }
-            }
-            if (from[i] != to[i] || (shift && shift[i]))
-                plan.kept.push_back((uint32_t)i);
-        }
-        const size_t moves = plan.kept.size();
-        if (waves.size() > 1 && waves.back() == moves)
-            waves.pop_back();
-        // The last `split` waves with launches of their own, those before in one run,
-        // which goes on while other sequences' bytes move.
-        const size_t all = waves.size(), mine = moves - waves[0];
-        const double bytes = cost.move_bytes * (double)n / std::max<size_t>(counts[q], 1);
-        size_t split = 0;
-        double best = 0.0;
-        for (size_t c = 0; c < std::min<size_t>(all, compact_launches); ++c) {
-            const size_t before = (c ? waves[all - c] : moves) - waves[0];
-            const double run = all - c > 1 ? cost.move_in_run * before : 0.0;
-            const double us = std::max(run, bytes * before) + bytes * (mine - before) + cost.launch * c;
-            if (!c || us < best) {
-                best = us;
-                split = c;
-            }
-        }
-        auto cut = [&](std::vector<uint32_t>& into, size_t first, size_t last, size_t each) {
-            for (size_t at = first; at < last; at += each)
-                into.insert(into.end(), { (uint32_t)at, (uint32_t)std::min(each, last - at) });
-        };
-        const size_t tail = split ? waves[all - split] : moves;
-        cut(runs[0], waves[0], tail, all - split > 1 ? std::max<size_t>(tail, 1) : compact_run);
-        for (size_t c = 0; c < split; ++c)
-            cut(runs[1 + c], waves[all - split + c], c + 1 < split ? waves[all - split + c + 1] : moves,
-                compact_run);
-    }
-    for (const auto& r : runs)
-        if (!r.empty()) {
-            plan.launches.push_back((uint32_t)(r.size() / 2));
-            plan.runs.insert(plan.runs.end(), r.begin(), r.end());
+            marks.writer[to[i]] = (uint32_t)i;
+            if (marks.read[to[i]] == g && (marks.first[to[i]] < begin || marks.last[to[i]] > i))
+                return "a move's target is read by a later move or another sequence";
         }
     status = CKV_OK;
+    auto changes = [&](size_t i) { return from[i] != to[i] || (shift && shift[i]); };
+    // Chains: a move joins the chain of the move that reads its target first, if that
+    // chain has fewer than `most` moves.
+    std::vector<uint32_t> chain(n, UINT32_MAX), sizes;
+    auto follow = [&](uint32_t most) {
+        sizes.clear();
+        for (size_t i = 0; i < n; ++i) {
+            if (!changes(i))
+                continue;
+            const uint32_t reader = marks.read[to[i]] == g ? marks.first[to[i]] : (uint32_t)i;
+            if (reader < i && sizes[chain[reader]] < most) {
+                chain[i] = chain[reader];
+            } else {
+                chain[i] = (uint32_t)sizes.size();
+                sizes.push_back(0);
+            }
+            ++sizes[chain[i]];
+        }
+    };
+    follow(UINT32_MAX);
+    if (sizes.empty())
+        return nullptr;
+    const double longest = cost.move_in_run * *std::max_element(sizes.begin(), sizes.end());
+    const double others = std::max(cost.move_bytes * (double)n, cost.move_in_run * compact_run);
+    if (longest > others + cost.launch)
+        follow(compact_run);
+    // Chains in the order of their first moves, as many to a run as it takes; a longer one
+    // has a run of its own.
+    std::vector<uint32_t> run_of(sizes.size()), begins { 0 };
+    uint32_t held = 0; // moves of the run that takes chains, the last of them
+    bool open = false;
+    uint32_t taking = 0;
+    for (size_t c = 0; c < sizes.size(); ++c) {
+        if (sizes[c] <= compact_run && open && held + sizes[c] <= compact_run) {
+            run_of[c] = taking;
+            held += sizes[c];
+        } else {
+            run_of[c] = (uint32_t)begins.size() - 1;
+            begins.push_back(0);
+            if (sizes[c] <= compact_run) {
+                taking = run_of[c];
+                held = sizes[c];
+                open = true;
+            }
+        }
+        begins[run_of[c] + 1] += sizes[c];
+    }
+    for (size_t r = 1; r < begins.size(); ++r)
+        begins[r] += begins[r - 1];
+    plan.kept.resize(begins.back());
+    plan.spare.assign(plan.kept.size(), UINT32_MAX);
+    std::vector<uint32_t> next(begins.begin(), begins.end() - 1);
+    for (size_t i = 0; i < n; ++i) {
+        if (chain[i] == UINT32_MAX)
+            continue;
+        const uint32_t run = run_of[chain[i]], at = next[run]++;
+        plan.kept[at] = (uint32_t)i;
+        const uint32_t writer = marks.written[from[i]] == g ? marks.writer[from[i]] : (uint32_t)i;
+        if (chain[writer] != UINT32_MAX && run_of[chain[writer]] != run) {
+            plan.spare[at] = (uint32_t)plan.saved.size();
+            plan.saved.push_back((uint32_t)i);
+        }
+    }
+    const uint32_t kept = (uint32_t)plan.kept.size(), saved = (uint32_t)plan.saved.size();
+    for (uint32_t at = 0; at < saved; at += compact_run)
+        plan.runs.insert(plan.runs.end(), { kept + at, std::min(compact_run, saved - at) });
+    if (saved)
+        plan.launches.push_back((uint32_t)plan.runs.size() / 2);
+    for (size_t r = 0; r + 1 < begins.size(); ++r)
+        plan.runs.insert(plan.runs.end(), { begins[r], begins[r + 1] - begins[r] });
+    plan.launches.push_back((uint32_t)begins.size() - 1);
     return nullptr;
 }
 

@@ -487,8 +487,8 @@ int ckv_rope_axes_append(ckv_pool* pool, size_t layer, const void* queries, void
  * slot may be both read and written (in place) if its write comes at or after every
  * move that reads it, within one sequence: kept tokens moving towards the front, in
  * order, are such moves. Nothing else is changed; the tables are the caller's.
- * Checks, before anything changes: invalid_argument (a null array, a stream under
- * capture), invalid_head_dimension and invalid_rope_theta (with shift),
+ * Checks, before anything changes: invalid_argument (a null array, a pool of more than
+ * 2^31 slots, a stream under capture), invalid_head_dimension and invalid_rope_theta (with shift),
  * cache_slot_out_of_range, unsupported_aliasing (a repeated target, or one that a later
  * move or another sequence reads). Profile name "compact". */
 int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const int32_t* shift,

@@ -97,7 +97,9 @@ void run_and_compare(const plan& p, uint32_t slots, const std::vector<uint32_t>&
         want[to[i]] = 1000 + from[i];
     std::vector<int> done(from.size(), 0);
     size_t first = 0;
-    REQUIRE(p.launches.size() <= compact_launches);
+    REQUIRE(p.launches.size() == (p.kept.empty() ? 0 : p.saved.empty() ? 1 : 2));
+    REQUIRE(p.spare.size() == p.kept.size());
+    std::vector<uint32_t> spare(p.saved.size(), 0);
     for (const uint32_t n : p.launches) {
         struct walk {
             uint32_t at, end;
@@ -112,10 +114,18 @@ void run_and_compare(const plan& p, uint32_t slots, const std::vector<uint32_t>&
             walk& w = runs[r];
             const uint32_t k = std::min<uint32_t>(32, w.end - w.at);
             if (w.held.empty()) {
-                for (uint32_t j = 0; j < k; ++j)
-                    w.held.push_back(got[from[p.kept[w.at + j]]]);
+                for (uint32_t j = 0; j < k; ++j) {
+                    const uint32_t at = w.at + j, kept = (uint32_t)p.kept.size();
+                    w.held.push_back(at >= kept                 ? got[from[p.saved.at(at - kept)]]
+                                         : p.spare[at] != UINT32_MAX ? spare.at(p.spare[at])
+                                                                     : got[from[p.kept[at]]]);
+                }
             } else {
                 for (uint32_t j = 0; j < k; ++j) {
+                    if (w.at + j >= p.kept.size()) {
+                        spare.at(w.at + j - p.kept.size()) = w.held[j];
+                        continue;
+                    }
                     const uint32_t i = p.kept[w.at + j];
                     REQUIRE(!done[i]);
                     done[i] = 1;
@@ -162,7 +172,7 @@ TEST("compaction: concurrent runs leave what reads before writes do")
             }
             counts.push_back(n);
         }
-        // rates that favour launches, one run, and either
+        // rates that favour cutting chains, none, and either
         const compact_cost costs[] = { { 0.0, 1.0, 0.1 }, { 1.0, 0.0, 9.0 }, { 0.007, 0.05, 8.0 } };
         run_and_compare(compaction(marks, slots, from, to, counts, nullptr, costs[trial % 3]), slots, from,
                         to, rng);
@@ -181,7 +191,7 @@ TEST("compaction: concurrent runs leave what reads before writes do")
     }
 }
 
-TEST("compaction: a middle that leaves takes two launches, one token one run")
+TEST("compaction: chains share runs, and one that is too long is cut")
 {
     move_marks marks;
     std::vector<uint32_t> from, to;
@@ -191,8 +201,9 @@ TEST("compaction: a middle that leaves takes two launches, one token one run")
             from.push_back(t);
         }
     plan p = compaction(marks, 2000, from, to, { (uint32_t)to.size() });
-    CHECK(p.launches.size() == 2);
-    CHECK(p.kept.size() == 1000 && p.launches[0] == (996 + 63) / 64 && p.launches[1] == 1);
+    // 1004 tokens but for the first 4, 8 of them in chains of two
+    CHECK(p.launches.size() == 1 && p.kept.size() == 1000 && p.saved.empty());
+    CHECK(p.launches[0] == (1000 + 63) / 64);
     from.clear();
     to.clear();
     for (uint32_t t = 0; t < 2000; ++t)
@@ -200,8 +211,12 @@ TEST("compaction: a middle that leaves takes two launches, one token one run")
             to.push_back((uint32_t)to.size());
             from.push_back(t);
         }
-    p = compaction(marks, 2000, from, to, { (uint32_t)to.size() });
+    // one chain: in one run where launches cost more, else cut where each run ends
+    p = compaction(marks, 2000, from, to, { (uint32_t)to.size() }, nullptr, { 0.007, 0.05, 100.0 });
     CHECK(p.launches.size() == 1 && p.launches[0] == 1 && p.kept.size() == 1995);
+    p = compaction(marks, 2000, from, to, { (uint32_t)to.size() });
+    CHECK(p.launches.size() == 2 && p.kept.size() == 1995 && p.saved.size() == (1995 + 63) / 64 - 1);
+    CHECK(p.launches[0] == 1 && p.launches[1] == (1995 + 63) / 64);
 }
 
 TEST("compaction: unsafe moves are refused")
