@@ -189,9 +189,13 @@ __device__ __forceinline__ void rope_pair(float a, float b, float c, float s, fl
 }
 
 // The moves of a compaction that read each slot (the first and the last) and the one
-// that writes it, by the generation of the call that marked them.
+// that writes it, by the generation of the call that marked them; and its moves' chains.
 struct move_marks {
-    std::vector<uint32_t> read, first, last, written, writer;
+    struct mark {
+        uint32_t read = 0, first = 0, last = 0, written = 0, writer = 0;
+    };
+    std::vector<mark> at_slot;
+    std::vector<uint32_t> chain, reader, sizes;
     uint32_t generation = 0;
 };
 

@@ -18,8 +18,9 @@
 //
 // Bound by HBM, each row read and written once. Measured on MI355X, 8 kv heads of 128,
 // bf16: 28 layers of 1,010 moves (the newer half of 2,011 tokens to behind the first
-// four) 58.6 us, 3.9 TB/s; 12 layers of 7,500 moves of six sequences to fresh pages
-// 169 us, 4.4 TB/s, where a device copy runs at 4.76.
+// four) 54.5 us, 4.2 TB/s; 12 layers of 7,600 moves of six sequences to fresh pages or in
+// place 157 us, a device copy's 4.76 TB/s; one of 2,000 tokens leaving 4 layers, a chain
+// that is cut, 39 us where its bytes take 14, leaving 28 layers, uncut, 108 and 96.
 #include "ckv_internal.h"
 #include "prefill_records.h"
 #include "rope_turns.h"
@@ -264,64 +265,74 @@ const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* fro
     size_t n = 0;
     for (size_t q = 0; q < n_sequences; ++q)
         n += counts[q];
-    status = CKV_E_CACHE_SLOT_OUT_OF_RANGE;
-    for (size_t i = 0; i < n; ++i)
-        if (from[i] >= slots || to[i] >= slots)
-            return "a move's slot is outside the pool";
-    if (marks.written.size() < slots) {
-        for (auto* v : { &marks.read, &marks.first, &marks.last, &marks.written, &marks.writer })
-            v->assign(slots, 0);
+    auto& at_slot = marks.at_slot;
+    if (at_slot.size() < slots) {
+        at_slot.assign(slots, {});
         marks.generation = 0;
     }
     if (++marks.generation == 0) {
-        std::fill(marks.read.begin(), marks.read.end(), 0);
-        std::fill(marks.written.begin(), marks.written.end(), 0);
+        std::fill(at_slot.begin(), at_slot.end(), move_marks::mark {});
         marks.generation = 1;
     }
     const uint32_t g = marks.generation;
+    status = CKV_E_CACHE_SLOT_OUT_OF_RANGE;
     for (size_t i = 0; i < n; ++i) {
-        if (marks.read[from[i]] != g)
-            marks.first[from[i]] = (uint32_t)i;
-        marks.read[from[i]] = g;
-        marks.last[from[i]] = (uint32_t)i;
+        if (from[i] >= slots || to[i] >= slots)
+            return "a move's slot is outside the pool";
+        auto& m = at_slot[from[i]];
+        if (m.read != g) {
+            m.read = g;
+            m.first = (uint32_t)i;
+        }
+        m.last = (uint32_t)i;
     }
+    // Chains: a move joins the chain of the move that reads its target first, if that
+    // chain has fewer than `most` moves.
+    std::vector<uint32_t> &chain = marks.chain, &reader = marks.reader, &sizes = marks.sizes;
+    chain.resize(n);
+    reader.resize(n);
+    sizes.assign(n, 0);
+    uint32_t n_chains = 0;
+    auto follow = [&](uint32_t i, uint32_t most) { // (selects: no branch would guess it)
+        const uint32_t r = reader[i];
+        chain[i] = n_chains;
+        const uint32_t other = chain[r];
+        const bool joins = r < i && sizes[other] < most;
+        chain[i] = joins ? other : n_chains;
+        n_chains += !joins;
+        ++sizes[chain[i]];
+    };
     status = CKV_E_UNSUPPORTED_ALIASING;
     for (size_t q = 0, begin = 0; q < n_sequences; begin += counts[q], ++q)
         for (size_t i = begin; i < begin + counts[q]; ++i) {
-            if (marks.written[to[i]] == g)
+            auto& m = at_slot[to[i]];
+            if (m.written == g)
                 return "two moves share a target";
-            marks.written[to[i]] = g;
-            marks.writer[to[i]] = (uint32_t)i;
-            if (marks.read[to[i]] == g && (marks.first[to[i]] < begin || marks.last[to[i]] > i))
+            m.written = g;
+            m.writer = (uint32_t)i;
+            const bool read = m.read == g;
+            if (read & ((m.first < begin) | (m.last > i)))
                 return "a move's target is read by a later move or another sequence";
+            reader[i] = read ? m.first : (uint32_t)i; // the move itself: none
+            if (from[i] != to[i] || (shift && shift[i]))
+                follow((uint32_t)i, UINT32_MAX);
+            else
+                chain[i] = UINT32_MAX; // changes nothing
         }
     status = CKV_OK;
-    auto changes = [&](size_t i) { return from[i] != to[i] || (shift && shift[i]); };
-    // Chains: a move joins the chain of the move that reads its target first, if that
-    // chain has fewer than `most` moves.
-    std::vector<uint32_t> chain(n, UINT32_MAX), sizes;
-    auto follow = [&](uint32_t most) {
-        sizes.clear();
-        for (size_t i = 0; i < n; ++i) {
-            if (!changes(i))
-                continue;
-            const uint32_t reader = marks.read[to[i]] == g ? marks.first[to[i]] : (uint32_t)i;
-            if (reader < i && sizes[chain[reader]] < most) {
-                chain[i] = chain[reader];
-            } else {
-                chain[i] = (uint32_t)sizes.size();
-                sizes.push_back(0);
-            }
-            ++sizes[chain[i]];
-        }
-    };
-    follow(UINT32_MAX);
-    if (sizes.empty())
+    if (!n_chains)
         return nullptr;
+    sizes.resize(n_chains);
     const double longest = cost.move_in_run * *std::max_element(sizes.begin(), sizes.end());
     const double others = std::max(cost.move_bytes * (double)n, cost.move_in_run * compact_run);
-    if (longest > others + cost.launch)
-        follow(compact_run);
+    if (longest > others + cost.launch) {
+        sizes.assign(n, 0);
+        n_chains = 0;
+        for (uint32_t i = 0; i < n; ++i)
+            if (chain[i] != UINT32_MAX)
+                follow(i, compact_run);
+        sizes.resize(n_chains);
+    }
     // Chains in the order of their first moves, as many to a run as it takes; a longer one
     // has a run of its own.
     std::vector<uint32_t> run_of(sizes.size()), begins { 0 };
@@ -353,7 +364,8 @@ const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* fro
             continue;
         const uint32_t run = run_of[chain[i]], at = next[run]++;
         plan.kept[at] = (uint32_t)i;
-        const uint32_t writer = marks.written[from[i]] == g ? marks.writer[from[i]] : (uint32_t)i;
+        const auto& m = at_slot[from[i]];
+        const uint32_t writer = m.written == g ? m.writer : (uint32_t)i;
         if (chain[writer] != UINT32_MAX && run_of[chain[writer]] != run) {
             plan.spare[at] = (uint32_t)plan.saved.size();
             plan.saved.push_back((uint32_t)i);
