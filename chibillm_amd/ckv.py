@@ -25,7 +25,6 @@ _lib = None
 _sz = C.c_size_t
 _vp = C.c_void_p
 _u32p = C.POINTER(C.c_uint32)
-_i32p = C.POINTER(C.c_int32)
 _f = C.c_float
 _i = C.c_int
 
@@ -87,7 +86,7 @@ _SIGNATURES = [
     ("ckv_rope_axes_upload", _i, [_vp, _u32p, _sz, _sz]),
     ("ckv_rope_axes", _i, [_vp, _vp, _vp, _sz, _f, _sz, C.c_char_p, _sz]),
     ("ckv_rope_axes_append", _i, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _f, _sz, C.c_char_p, _sz]),
-    ("ckv_compact", _i, [_vp, _u32p, _u32p, _i32p, _u32p, _sz, _f, _sz]),
+    ("ckv_compact", _i, [_vp, _vp, _vp, _vp, _vp, _sz, _f, _sz]),
 ]
 SYMBOLS = [name for name, _, _ in _SIGNATURES]
 
@@ -468,12 +467,12 @@ class Pool:
         positions (ckv_compact); counts are the moves of each sequence."""
         f, t, c = _u32(from_slots), _u32(to_slots), _u32(counts)
         s = None if shift is None else np.ascontiguousarray(shift, dtype=np.int32)
-        if f.size != t.size or int(c.sum(dtype=np.uint64)) != f.size \
-                or (s is not None and s.size != f.size):
+        if f.size != t.size or sum(c.tolist()) != f.size or (s is not None and s.size != f.size):
             raise ValueError("from_slots, to_slots and shift have an entry for each counted move")
+        # (addresses: typed pointers take twice as long to make)
         self.ctx.check(load().ckv_compact(
-            self.handle, _p(f), _p(t), None if s is None else s.ctypes.data_as(_i32p), _p(c),
-            c.size, theta, rotary_dim))
+            self.handle, f.ctypes.data, t.ctypes.data, None if s is None else s.ctypes.data,
+            c.ctypes.data, c.size, theta, rotary_dim))
 
     def copy_blocks(self, src, dst) -> None:
         s, d = _u32(src), _u32(dst)
