@@ -351,6 +351,12 @@ TEST("entry points: what is refused")
     // nothing to do
     const uint32_t none[] = { 0 };
     CHECK(ckv_compact(&pool, nullptr, nullptr, nullptr, none, 1, 0.0f, 0) == CKV_OK);
+    {
+        const size_t blocks = pool.blocks;
+        pool.blocks = (size_t(1) << 31) / pool.block_size + 1; // a slot past what the move lists hold
+        CHECK(ckv_compact(&pool, from, to, nullptr, counts, 1, 0.0f, 0) == CKV_E_INVALID_ARGUMENT);
+        pool.blocks = blocks;
+    }
     CHECK(ckv_compact(&pool, from, from, nullptr, counts, 1, 0.0f, 0) == CKV_OK);
     pool.positions.clear();
     CHECK(attend(0, nullptr, 4, 8, nullptr, nullptr, 0) == CKV_OK);

@@ -167,3 +167,66 @@ def test_on_another_stream_and_back(ctx, rows):
         assert torch.equal(rotated, outs[0][0]) and torch.equal(out, outs[0][1])
     pool.close()
     own.close()
+
+
+def test_captured_axes_and_what_capture_refuses(ctx):
+    """A captured rotation with append replays on new inputs; uploads of positions and compactions are
+    refused under capture and leave it going."""
+    stream = torch.cuda.Stream()
+    own = ckv.Context(0, stream=stream)
+    n, heads, d = 37, 2, 128
+    cache = Cache(own, "bf16", [60], heads, d, seed=61)
+    with torch.cuda.stream(stream):
+        pool = cache.to_device()
+        _, _, at = cache.upload([60 - n], [n])
+        positions = np.stack([np.arange(n), 7 * np.arange(n), 3 + 0 * np.arange(n)])
+        pool.upload_axes(positions)
+        axis = ckv.rope_pair_axes([24, 20, 20], True)
+        q, k, v = (cache.randn(n, x, d).cuda().flatten(1) for x in (2 * heads, heads, heads))
+        rotated = torch.empty_like(q)
+        slots = cache.slots(cache.tables[0], np.arange(20))
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            pool.rope_axes_append(0, q, rotated, 2 * heads, k, v, 1e4, axis)
+            for call in (lambda: pool.upload_axes(positions), lambda: pool.compact(slots[10:], slots[:10], [10])):
+                with pytest.raises(ckv.CkvError) as refused:
+                    call()
+                assert refused.value.name == "ckv.invalid_argument"
+        for _ in range(3):
+            for x in (q, k, v):
+                x.normal_()
+            pool.rope_axes_append(0, q, rotated, 2 * heads, k, v, 1e4, axis)
+            stream.synchronize()
+            want = rotated.clone(), cache.kd[0, at].clone(), cache.vd[0, at].clone()
+            rotated.zero_()
+            cache.kd[0, at] = 0
+            cache.vd[0, at] = 0
+            graph.replay()
+            stream.synchronize()
+            for got, w in zip((rotated, cache.kd[0, at], cache.vd[0, at]), want):
+                assert torch.equal(got, w)
+        pool.compact(slots[10:], slots[:10], [10])
+        stream.synchronize()
+    pool.close()
+    own.close()
+
+
+@pytest.mark.parametrize("dtype,heads,d,layers", [("bf16", 8, 128, 3), ("f32", 1, 33, 2), ("f16", 2, 256, 1)])
+def test_a_chain_that_is_cut_and_one_that_is_not(ctx, dtype, heads, d, layers):
+    """One token leaves long sequences: every move's source is the target of the next, cut into runs
+    whose first reads were saved, in place and with keys turned."""
+    lengths = [2000, 700, 70]
+    print(f"chains {dtype} {heads} x {d} layers {layers}", flush=True)
+    cache = Cache(ctx, dtype, lengths, heads, d, layers=layers, seed=71)
+    pool = cache.to_device()
+    gone = [5, 300, 68]
+    source = np.concatenate([cache.slots(t, np.delete(np.arange(n), x)) for t, n, x in zip(cache.tables, lengths, gone)])
+    target = np.concatenate([cache.slots(t, np.arange(n - 1)) for t, n in zip(cache.tables, lengths)])
+    for _ in range(2):  # twice the same moves, over what the first left
+        pool.compact(source, target, [n - 1 for n in lengths])
+        for x in (cache.k, cache.v):
+            x[:, target] = x[:, source].clone()
+    ctx.sync()
+    cache.unchanged()
+    pool.close()
