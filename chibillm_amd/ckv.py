@@ -436,7 +436,7 @@ class Pool:
         self.ctx.check(load().ckv_rope_axes_upload(self.handle, _p(p), p.shape[0], p.shape[1]))
 
     def _pair_axis(self, pair_axis, rotary_dim: int) -> bytes:
-        axes = np.asarray(pair_axis, dtype=np.uint8).tobytes()
+        axes = np.asarray(pair_axis).astype(np.uint8).tobytes()
         if len(axes) != (rotary_dim or self.geometry[4]) // 2:
             raise ValueError("pair_axis has an axis for each of rotary_dim / 2 pairs")
         return axes

@@ -950,6 +950,17 @@ int create_pool(ckv_context* ctx, size_t layers, size_t blocks, size_t block_siz
     return CKV_OK;
 }
 
+// The turns of a rotation, made anew where it is not the last one's.
+const ckv::turn_table& turns_of(ckv_pool* pool, float theta, uint32_t rotary)
+{
+    if (pool->turns_theta != theta || pool->turns_rotary != rotary) {
+        ckv::turn_steps(theta, rotary, pool->turns);
+        pool->turns_theta = theta;
+        pool->turns_rotary = rotary;
+    }
+    return pool->turns;
+}
+
 // Entry points through this make their context's device current while they run, take
 // a capture of its stream into account (ckv_context::in_capture) and give a status for
 // what the host code throws.
@@ -2496,10 +2507,9 @@ int ckv_rope_axes_upload(ckv_pool* pool, const uint32_t* positions, size_t axes,
 
 namespace {
 
-// The checks of rope on several axes after the row count; fills the tables.
+// The checks of rope on several axes after the row count; fills the axes.
 int check_rope_axes(ckv_pool* pool, size_t heads, float theta, size_t rotary_dim,
-                    const uint8_t* pair_axis, ckv::turn_table& turns, ckv::axis_table& axes,
-                    uint32_t& rotary)
+                    const uint8_t* pair_axis, ckv::axis_table& axes, uint32_t& rotary)
 {
     ckv_context* ctx = pool->ctx;
     if (heads == 0)
@@ -2527,7 +2537,6 @@ int check_rope_axes(ckv_pool* pool, size_t heads, float theta, size_t rotary_dim
                              "axis of pair " + std::to_string(j) + " was not uploaded");
         axes.axis[j] = pair_axis[j];
     }
-    ckv::turn_steps(theta, rotary, turns);
     return CKV_OK;
 }
 
@@ -2544,17 +2553,17 @@ int ckv_rope_axes(ckv_pool* pool, const void* input, void* output, size_t heads,
             return set_error(ctx, CKV_E_NO_TABLES, "rope before ckv_tables_upload");
         if (rows != pool->positions.size())
             return set_error(ctx, CKV_E_POSITION_COUNT_MISMATCH, "rows != uploaded positions");
-        ckv::turn_table turns;
         ckv::axis_table axes;
         uint32_t rotary = 0;
-        if (const int status = check_rope_axes(pool, heads, theta, rotary_dim, pair_axis, turns,
-                                               axes, rotary))
+        if (const int status = check_rope_axes(pool, heads, theta, rotary_dim, pair_axis, axes,
+                                               rotary))
             return status;
         const pool_view view = view_of(pool);
         return run_kernel(ctx, "rope_axes", [&] {
             return launch_rope_axes(ctx->stream, view, pool->meta, 0,
                                     { input, output, nullptr, nullptr }, (uint32_t)rows,
-                                    (uint32_t)heads, rotary, turns, axes, pool->d_axes);
+                                    (uint32_t)heads, rotary, turns_of(pool, theta, rotary), axes,
+                                    pool->d_axes);
         });
     });
 }
@@ -2574,18 +2583,18 @@ int ckv_rope_axes_append(ckv_pool* pool, size_t layer, const void* queries, void
             return set_error(ctx, CKV_E_INVALID_ARGUMENT, "queries and rotated are required");
         if (rows && (rotated == keys || rotated == values))
             return set_error(ctx, CKV_E_UNSUPPORTED_ALIASING, "rotated overlaps keys or values");
-        ckv::turn_table turns;
         ckv::axis_table axes;
         uint32_t rotary = 0;
         status = check_rope_axes(pool, q_heads + pool->kv_heads, theta, rotary_dim, pair_axis,
-                                 turns, axes, rotary);
+                                 axes, rotary);
         if (status)
             return status;
         const pool_view view = view_of(pool);
         return run_kernel(ctx, "rope_axes_append", [&] {
             return launch_rope_axes(ctx->stream, view, pool->meta, (uint32_t)layer,
                                     { queries, rotated, keys, values }, (uint32_t)rows,
-                                    (uint32_t)q_heads, rotary, turns, axes, pool->d_axes);
+                                    (uint32_t)q_heads, rotary, turns_of(pool, theta, rotary), axes,
+                                    pool->d_axes);
         });
     });
 }
@@ -2610,7 +2619,6 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
             return set_error(ctx, CKV_E_UNSUPPORTED_ALIASING, "two moves share a target");
         if (pool->blocks * pool->block_size > spare_slot)
             return set_error(ctx, CKV_E_INVALID_ARGUMENT, "a pool of more than 2^31 slots");
-        ckv::turn_table turns;
         uint32_t rotary = 0;
         if (shift) {
             const size_t width = rotary_dim ? rotary_dim : pool->head_dim;
@@ -2622,7 +2630,6 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
                 return set_error(ctx, CKV_E_INVALID_ROPE_THETA,
                                  "theta must be positive and finite");
             rotary = (uint32_t)width;
-            ckv::turn_steps(theta, rotary, turns);
         }
         compact_plan plan;
         int status = CKV_OK;
@@ -2672,7 +2679,7 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
                                             pool->d_spare, (uint32_t)plan.saved.size() };
                 if (e == hipSuccess)
                     e = launch_compact(ctx->stream, view, (uint32_t)pool->layers, moves, rotary,
-                                       turns);
+                                       rotary ? turns_of(pool, theta, rotary) : pool->turns);
                 first += 2 * n_runs;
             }
             return e;

@@ -356,6 +356,10 @@ struct ckv_pool {
     uint32_t* d_axes = nullptr;
     size_t d_axes_words = 0;
 
+    ckv::turn_table turns {}; // of the last theta and rotary width (turns_of)
+    float turns_theta = 0.0f;
+    uint32_t turns_rotary = 0;
+
     ckv::move_marks marks; // of ckv_compact's slots
     uint8_t* d_spare = nullptr; // rows it saves
     size_t d_spare_bytes = 0;

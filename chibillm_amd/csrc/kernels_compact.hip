@@ -18,7 +18,7 @@
 //
 // Bound by HBM, each row read and written once. Measured on MI355X, 8 kv heads of 128,
 // bf16: 28 layers of 1,010 moves (the newer half of 2,011 tokens to behind the first
-// four) 54.5 us, 4.2 TB/s; 12 layers of 7,600 moves of six sequences to fresh pages or in
+// four) 53.5 us, 4.3 TB/s; 12 layers of 7,600 moves of six sequences to fresh pages or in
 // place 157 us, a device copy's 4.76 TB/s; one of 2,000 tokens leaving 4 layers, a chain
 // that is cut, 39 us where its bytes take 14, leaving 28 layers, uncut, 108 and 96.
 #include "ckv_internal.h"

@@ -10,8 +10,8 @@
 // Bound by HBM from a few hundred rows on: each row is read and written once. Measured
 // on MI355X, 16 q and 8 kv heads of 128, bf16: 4,096 rows 14.9 us, 4.5 TB/s read and
 // written (an element a thread with every angle computed for each head, 24.6 us); 1,531
-// fp16 rows of 8 q and 2 kv heads of 256, 64 of them rotated, 6.7 to 7.7 us by the host;
-// 6 rows take 3.3 us on the GPU, a launch's own time.
+// fp16 rows of 8 q and 2 kv heads of 256, 64 of them rotated, 6.5 us; 6 rows take 3.3 us
+// on the GPU, a launch's own time, and a call 6.1.
 #include "ckv_internal.h"
 #include "rope_turns.h"
 
