@@ -125,6 +125,46 @@ struct prefill_shape {
     static constexpr uint32_t dmas = 2 * regions;        // DMA loads per block and wave
 };
 
+// The results of a wave's 32 rows on their way to memory, behind a window. An
+// accumulator holds four features of each row: stored from there, an instruction writes
+// 16 bytes (two lanes) of each of 32 rows 4 KB apart, and the L2 takes a request for every
+// one. So the floats go through LDS, a wave's own part of the stages, and leave as whole
+// rows, 16 bytes a lane (32 prompts of 128 rows, half of whose bytes are outputs, 19.0
+// and 15.5 us; 64 of 64 14.6 and 13.3).
+constexpr uint32_t row_floats = dim + 4; // a row's pitch in LDS: 16 rows on other banks
+
+// Rows 0 .. n_rows - 1 but those of `skip`, from `tile` [32][row_floats], times
+// sigmoid(gate), rounded once, to out[row * stride + feature]. (Unrolled no further: the
+// code that follows the key blocks is fetched cold.)
+template <bool F16>
+__device__ __forceinline__ void store_rows(const float* tile, uint32_t lane, uint32_t n_rows,
+                                           uint32_t skip, uint16_t* out, size_t stride,
+                                           const uint16_t* gate)
+{
+    constexpr uint32_t lanes = dim / 8, rows = 64 / lanes; // of a row, at a time
+    const uint32_t f = lane % lanes * 8;
+#pragma unroll 2
+    for (uint32_t i = 0; i < 32 / rows; ++i) {
+        const uint32_t r = i * rows + lane / lanes;
+        const float4 a = *reinterpret_cast<const float4*>(tile + r * row_floats + f);
+        const float4 b = *reinterpret_cast<const float4*>(tile + r * row_floats + f + 4);
+        float x[8] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
+        if (r >= n_rows || skip >> r & 1)
+            continue;
+        const size_t at = r * stride + f;
+        if (gate) { // sigmoid_mul (src/qwen/qwen_layer.cc:204) in the epilogue
+            const uint4 v = *reinterpret_cast<const uint4*>(gate + at);
+            const uint32_t w[4] = { v.x, v.y, v.z, v.w };
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[e] *= sigmoid(half_value<F16>((uint16_t)(w[e / 2] >> (16 * (e % 2)))));
+        }
+        *reinterpret_cast<uint4*>(out + at) =
+            make_uint4(pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(x[4], x[5]),
+                       pack2<F16>(x[6], x[7]));
+    }
+}
+
 // WINDOW (4 waves): rows attend through md.window. Blocks that no row of the
 // workgroup attends are left out of the count (in_table gives a block's place in the
 // sequence); keys that none attends in the blocks at the gap's edges are staged from
@@ -138,7 +178,7 @@ struct prefill_shape {
 // cores and each block's dependence chain, with 24 products a block in place of 16: 16
 // chunks of 1,024 rows behind 4,000 tokens through 2,048 of them take 405 to 450 us by
 // the box's clock and issue 1.02 PFLOP/s (an 8,192-wide library product: 1.23); one
-// chunk of 512 behind 6,000 through 1,024 takes 20.9 us, a chain of 9 blocks and the
+// chunk of 512 behind 6,000 through 1,024 takes 20.6 us, a chain of 9 blocks and the
 // fold of 4 ranges.
 template <int G, bool F16, bool WIDE, int W, bool WINDOW>
 __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
@@ -737,7 +777,24 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
         const uint64_t odd_lanes = __ballot(valid && odd != 0.0f);
         alone = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
     }
-    if (active && valid && !(alone >> n & 1)) {
+    if constexpr (WINDOW) {
+        wait_vector_memory();
+        __syncthreads(); // every wave is past its LDS reads
+        static_assert(W * 32 * row_floats * sizeof(float) <= n_stages * stage_bytes);
+        float* tile_out = reinterpret_cast<float*>(lds) + wave * (32 * row_floats);
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int quad = 0; quad < 4; ++quad) {
+                const f32x16_t& acc = o[mt];
+                *reinterpret_cast<float4*>(tile_out + n * row_floats + 32 * mt + 8 * quad + 4 * g) =
+                    make_float4(acc[4 * quad] * inv, acc[4 * quad + 1] * inv, acc[4 * quad + 2] * inv,
+                                acc[4 * quad + 3] * inv);
+            }
+        const size_t first = (size_t)(row0 + rb * 32) * q_stride + (size_t)head * dim;
+        store_rows<F16>(tile_out, lane, active ? nrows - rb * 32 : 0, alone, out + first, q_stride,
+                        gate ? gate + first : nullptr);
+    } else if (active && valid) {
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
