@@ -45,6 +45,7 @@
 #include "ckv_internal.h"
 #include "prefill_records.h"
 #include "prefill_tile.h"
+#include "store_rows.h"
 
 #include <algorithm>
 #include <cstdlib>
@@ -125,46 +126,6 @@ struct prefill_shape {
     static constexpr uint32_t dmas = 2 * regions;        // DMA loads per block and wave
 };
 
-// The results of a wave's 32 rows on their way to memory, behind a window. An
-// accumulator holds four features of each row: stored from there, an instruction writes
-// 16 bytes (two lanes) of each of 32 rows 4 KB apart, and the L2 takes a request for every
-// one. So the floats go through LDS, a wave's own part of the stages, and leave as whole
-// rows, 16 bytes a lane (32 prompts of 128 rows, half of whose bytes are outputs, 19.0
-// and 15.5 us; 64 of 64 14.6 and 13.3).
-constexpr uint32_t row_floats = dim + 4; // a row's pitch in LDS: 16 rows on other banks
-
-// Rows 0 .. n_rows - 1 but those of `skip`, from `tile` [32][row_floats], times
-// sigmoid(gate), rounded once, to out[row * stride + feature]. (Unrolled no further: the
-// code that follows the key blocks is fetched cold.)
-template <bool F16>
-__device__ __forceinline__ void store_rows(const float* tile, uint32_t lane, uint32_t n_rows,
-                                           uint32_t skip, uint16_t* out, size_t stride,
-                                           const uint16_t* gate)
-{
-    constexpr uint32_t lanes = dim / 8, rows = 64 / lanes; // of a row, at a time
-    const uint32_t f = lane % lanes * 8;
-#pragma unroll 2
-    for (uint32_t i = 0; i < 32 / rows; ++i) {
-        const uint32_t r = i * rows + lane / lanes;
-        const float4 a = *reinterpret_cast<const float4*>(tile + r * row_floats + f);
-        const float4 b = *reinterpret_cast<const float4*>(tile + r * row_floats + f + 4);
-        float x[8] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
-        if (r >= n_rows || skip >> r & 1)
-            continue;
-        const size_t at = r * stride + f;
-        if (gate) { // sigmoid_mul (src/qwen/qwen_layer.cc:204) in the epilogue
-            const uint4 v = *reinterpret_cast<const uint4*>(gate + at);
-            const uint32_t w[4] = { v.x, v.y, v.z, v.w };
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                x[e] *= sigmoid(half_value<F16>((uint16_t)(w[e / 2] >> (16 * (e % 2)))));
-        }
-        *reinterpret_cast<uint4*>(out + at) =
-            make_uint4(pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(x[4], x[5]),
-                       pack2<F16>(x[6], x[7]));
-    }
-}
-
 // WINDOW (4 waves): rows attend through md.window. Blocks that no row of the
 // workgroup attends are left out of the count (in_table gives a block's place in the
 // sequence); keys that none attends in the blocks at the gap's edges are staged from
@@ -177,10 +138,11 @@ __device__ __forceinline__ void store_rows(const float* tile, uint32_t lane, uin
 // workgroups of 4 heads each. Large launches are bound as the others are, by the matrix
 // cores and each block's dependence chain, with 24 products a block in place of 16: 16
 // chunks of 1,024 rows behind 4,000 tokens through 2,048 of them take 405 to 450 us by
-// the box's clock and issue 1.02 PFLOP/s (an 8,192-wide library product: 1.23); one
+// the clock and issue 1.02 PFLOP/s (an 8,192-wide library product: 1.23); one
 // chunk of 512 behind 6,000 through 1,024 takes 20.6 us, a chain of 9 blocks and the
-// fold of 4 ranges.
-template <int G, bool F16, bool WIDE, int W, bool WINDOW>
+// fold of 4 ranges. RANGES: the launch may cut a tile's keys (without the code for it,
+// what follows the blocks is shorter to fetch).
+template <int G, bool F16, bool WIDE, int W, bool WINDOW, bool RANGES = true>
 __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     pool_view p, meta_view md, uint32_t layer, const uint16_t* __restrict__ q,
     uint16_t* __restrict__ out, uint32_t q_heads, float c, const uint16_t* __restrict__ gate,
@@ -240,7 +202,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     // into n_parts ranges of at least min_blocks (uniform over the tile's
     // workgroups), range `part`.
     uint32_t n_parts = 1, kb_begin = 0, kb_end = n_blocks;
-    if constexpr (SPLIT) {
+    if constexpr (SPLIT && RANGES) {
         n_parts = prefill_range_count(n_blocks, n_split, split_scratch.min_blocks);
         if (part >= n_parts)
             return;
@@ -681,7 +643,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     }
 
     float lt = l + __shfl_xor(l, 32); // the query's denominator (both lane halves)
-    if (SPLIT && n_parts > 1) {
+    if (SPLIT && RANGES && n_parts > 1) {
         // A share of a split tile: its record is 33 chunks of 4 floats per
         // query vector, chunk 0 = [max, denominator, 0, 0] and chunk 1 + j =
         // acc[4j .. 4j + 3], chunk-major with the workgroup's 128 query vectors
@@ -780,19 +742,20 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     if constexpr (WINDOW) {
         wait_vector_memory();
         __syncthreads(); // every wave is past its LDS reads
-        static_assert(W * 32 * row_floats * sizeof(float) <= n_stages * stage_bytes);
-        float* tile_out = reinterpret_cast<float*>(lds) + wave * (32 * row_floats);
+        static_assert(W * 32 * row_floats<dim> * sizeof(float) <= n_stages * stage_bytes);
+        float* tile_out = reinterpret_cast<float*>(lds) + wave * (32 * row_floats<dim>);
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
             for (int quad = 0; quad < 4; ++quad) {
                 const f32x16_t& acc = o[mt];
-                *reinterpret_cast<float4*>(tile_out + n * row_floats + 32 * mt + 8 * quad + 4 * g) =
+                *reinterpret_cast<float4*>(tile_out + n * row_floats<dim> + 32 * mt + 8 * quad + 4 * g) =
                     make_float4(acc[4 * quad] * inv, acc[4 * quad + 1] * inv, acc[4 * quad + 2] * inv,
                                 acc[4 * quad + 3] * inv);
             }
         const size_t first = (size_t)(row0 + rb * 32) * q_stride + (size_t)head * dim;
-        store_rows<F16>(tile_out, lane, active ? nrows - rb * 32 : 0, alone, out + first, q_stride,
+        store_rows<dim, F16 ? CKV_F16 : CKV_BF16>(
+            tile_out, lane, active ? nrows - rb * 32 : 0, alone, out + first, q_stride,
                         gate ? gate + first : nullptr);
     } else if (active && valid) {
 #pragma unroll
@@ -849,6 +812,15 @@ hipError_t launch_gw(hipStream_t s, const pool_view& p, const meta_view& m, uint
     const bool wide = p.layer_elems * 2 > 0xFFFFFFFFull;
     const bool f16 = p.dtype == CKV_F16;
     const dim3 g((uint32_t)grid), b(64 * W);
+    if constexpr (WINDOW)
+        if (split.n_split == 1) {
+            auto* kernel = f16 ? (wide ? prefill_kernel<G, true, true, W, true, false>
+                                       : prefill_kernel<G, true, false, W, true, false>)
+                               : (wide ? prefill_kernel<G, false, true, W, true, false>
+                                       : prefill_kernel<G, false, false, W, true, false>);
+            kernel<<<g, b, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
+            return hipGetLastError();
+        }
     if (f16 && wide)
         hipLaunchKernelGGL((prefill_kernel<G, true, true, W, WINDOW>), g, b, 0, s, p, m, layer, qq, oo,
                            q_heads, c, gg, split);

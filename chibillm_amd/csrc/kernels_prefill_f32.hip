@@ -43,6 +43,7 @@
 #include "attend_alone.h"
 #include "ckv_internal.h"
 #include "prefill_records.h"
+#include "store_rows.h"
 
 namespace ckv {
 namespace {
@@ -64,7 +65,9 @@ __device__ __forceinline__ f32x16_t mfma(float a, float b, const f32x16_t& c)
 // tiles are short chains of dear blocks: workgroups of half the rows have half the chain
 // to a block and two share a compute unit (2 chunks of 220 and 300 rows behind 1,000
 // tokens, window 512: 65 us with 8 waves, 45 with 4).
-template <int G, bool WINDOW, int waves = WINDOW ? 4 : 8>
+// RANGES: the launch may cut a tile's keys; a window's launch that does not stores its
+// results as whole rows (store_rows.h).
+template <int G, bool WINDOW, bool RANGES = true, int waves = WINDOW ? 4 : 8>
 __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
     pool_view p, meta_view md, uint32_t layer, const float* __restrict__ q,
     float* __restrict__ out, uint32_t q_heads, float c, const float* __restrict__ gate,
@@ -110,7 +113,8 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
     const uint32_t n_blocks = pos_last / block_keys + 1 - gap.skip;
     const uint32_t last_entry = pos_last / page_tokens;
     // key blocks [kb_begin, kb_end) of this workgroup
-    const uint32_t n_parts = prefill_range_count(n_blocks, n_split, split_scratch.min_blocks);
+    const uint32_t n_parts =
+        RANGES ? prefill_range_count(n_blocks, n_split, split_scratch.min_blocks) : 1;
     if (part >= n_parts)
         return;
     uint32_t kb_begin, kb_end;
@@ -293,7 +297,7 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
     }
 
     float lt = l + __shfl_xor(l, 32); // the query's denominator (both lane halves)
-    if (n_parts > 1) {
+    if (RANGES && n_parts > 1) {
         // A range of a split tile: its record is 33 chunks of 4 floats per query
         // vector, chunk 0 = [max (log2 units), denominator, 0, 0] and chunk
         // 1 + j = features 4j .. 4j + 3 (lane half h, element r of the four
@@ -383,7 +387,20 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
         const uint64_t odd_lanes = __ballot(valid && odd != 0.0f);
         alone = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
     }
-    if (valid && !(alone >> n & 1)) {
+    if constexpr (!RANGES) {
+        wait_vector_memory();
+        __syncthreads(); // every wave is past its LDS reads
+        static_assert(waves * 32 * row_floats<dim> * sizeof(float) <= n_stages * stage_bytes);
+        float* tile_out = reinterpret_cast<float*>(lds) + wave * (32 * row_floats<dim>);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            *reinterpret_cast<float4*>(tile_out + n * row_floats<dim> + 32 * (r >> 2) + 16 * h + 4 * (r & 3)) =
+                make_float4(o[0][r] * inv, o[1][r] * inv, o[2][r] * inv, o[3][r] * inv);
+        const uint32_t before = (wave / G) * 32;
+        const size_t first = (size_t)(row0 + before) * q_stride + (size_t)head * dim;
+        store_rows<dim, CKV_F32>(tile_out, lane, nrows > before ? nrows - before : 0, alone, out + first,
+                                 q_stride, gate ? gate + first : nullptr);
+    } else if (valid && !(alone >> n & 1)) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             // features 4 * (8 * (r / 4) + 4h + r % 4) + 0..3: accumulators 0..3
@@ -422,9 +439,13 @@ hipError_t launch_g(hipStream_t s, const pool_view& p, const meta_view& m, uint3
                     const void* q, uint32_t q_heads, float c, void* out, uint32_t grid,
                     const void* gate, prefill_split split)
 {
-    hipLaunchKernelGGL((prefill_f32_kernel<G, WINDOW>), dim3(grid), dim3(WINDOW ? 256 : 512), 0, s, p, m, layer,
-                       static_cast<const float*>(q), static_cast<float*>(out), q_heads, c,
-                       static_cast<const float*>(gate), split);
+    auto* kernel = prefill_f32_kernel<G, WINDOW>;
+    if constexpr (WINDOW)
+        if (split.n_split == 1)
+            kernel = prefill_f32_kernel<G, true, false>;
+    kernel<<<grid, WINDOW ? 256 : 512, 0, s>>>(p, m, layer, static_cast<const float*>(q),
+                                               static_cast<float*>(out), q_heads, c,
+                                               static_cast<const float*>(gate), split);
     return hipGetLastError();
 }
 

@@ -45,6 +45,7 @@
 #include "ckv_internal.h"
 #include "prefill_records.h"
 #include "prefill_tile.h"
+#include "store_rows.h"
 
 #include <algorithm>
 #include <cstdlib>
@@ -100,8 +101,10 @@ __device__ __forceinline__ void wait_all_but(uint32_t loads)
 // FAR: a layer spans more than 4 GiB, so page offsets take 64 bits. WINDOW: blocks
 // that no row of the workgroup attends are left out of the count (in_table gives a
 // block's place); keys that none attends in the blocks at the gap's edges are staged
-// from the zero row, so what they hold never enters a product.
-template <int G, bool F16, bool FAR, bool WINDOW>
+// from the zero row, so what they hold never enters a product. RANGES: the launch may cut
+// a tile's keys; a window's launch that does not stores its results as whole rows
+// (store_rows.h), which beside the fold's code made that slower.
+template <int G, bool F16, bool FAR, bool WINDOW, bool RANGES = true>
 __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
     pool_view p, meta_view md, uint32_t layer, const uint16_t* __restrict__ q,
     uint16_t* __restrict__ out, uint32_t q_heads, float c, const uint16_t* __restrict__ gate,
@@ -148,7 +151,8 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
         return end <= pos_last && (!WINDOW || key0 >= low || end < window.sinks);
     };
     const uint32_t n_blocks = pos_last / block_keys + 1 - gap.skip;
-    const uint32_t n_parts = prefill_range_count(n_blocks, n_split, split_scratch.min_blocks);
+    const uint32_t n_parts =
+        RANGES ? prefill_range_count(n_blocks, n_split, split_scratch.min_blocks) : 1;
     if (part >= n_parts)
         return;
     uint32_t kb_begin, kb_end;
@@ -469,7 +473,7 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
     }
 
     float lt = l + __shfl_xor(l, 32); // the query's denominator (both lane halves)
-    if (n_parts > 1) {
+    if (RANGES && n_parts > 1) {
         // The hand-over of kernels_prefill.hip, with 65 chunks of four floats per
         // (range, query vector): [max, denominator, 0, 0], then acc[4j .. 4j + 3].
         const uint32_t pair = (rest * passes + pass) * kv_heads + kvh;
@@ -549,7 +553,23 @@ __global__ __launch_bounds__(64 * waves, 1) void prefill_wide_kernel(
     const uint64_t odd_lanes = __ballot(valid && odd != 0.0f);
     const uint32_t alone = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
     uint16_t* dst = out + qoff;
-    if (valid && !(alone >> n & 1)) {
+    if constexpr (!RANGES) {
+        wait_vector_memory();
+        __syncthreads(); // every wave is past its LDS reads
+        static_assert(waves * 32 * row_floats<dim> * sizeof(float) <= sizeof(lds));
+        float* tile_out = reinterpret_cast<float*>(lds) + wave * (32 * row_floats<dim>);
+#pragma unroll
+        for (uint32_t mt = 0; mt < tiles_o; ++mt)
+#pragma unroll
+            for (uint32_t quad = 0; quad < 4; ++quad)
+                *reinterpret_cast<float4*>(tile_out + n * row_floats<dim> + 32 * mt + 8 * quad + 4 * g) =
+                    make_float4(o[mt][4 * quad] * inv, o[mt][4 * quad + 1] * inv,
+                                o[mt][4 * quad + 2] * inv, o[mt][4 * quad + 3] * inv);
+        const size_t first = (size_t)(row0 + rb * 32) * q_stride + (size_t)head * dim;
+        store_rows<dim, F16 ? CKV_F16 : CKV_BF16>(tile_out, lane, nrows > rb * 32 ? nrows - rb * 32 : 0,
+                                                  alone, out + first, q_stride,
+                                                  gate ? gate + first : nullptr);
+    } else if (valid && !(alone >> n & 1)) {
 #pragma unroll
         for (uint32_t mt = 0; mt < tiles_o; ++mt)
 #pragma unroll
@@ -596,6 +616,15 @@ hipError_t launch_g(hipStream_t s, const pool_view& p, const meta_view& m, uint3
     auto* oo = static_cast<uint16_t*>(out);
     const auto* gg = static_cast<const uint16_t*>(gate);
     const dim3 blocks(grid), threads(64 * waves);
+    if constexpr (WINDOW)
+        if (split.n_split == 1) {
+            auto* kernel = f16 ? (far ? prefill_wide_kernel<G, true, true, true, false>
+                                      : prefill_wide_kernel<G, true, false, true, false>)
+                               : (far ? prefill_wide_kernel<G, false, true, true, false>
+                                      : prefill_wide_kernel<G, false, false, true, false>);
+            kernel<<<blocks, threads, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
+            return hipGetLastError();
+        }
     if (f16 && far)
         prefill_wide_kernel<G, true, true, WINDOW><<<blocks, threads, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
     else if (f16)
