@@ -597,7 +597,7 @@ const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* fro
                             const uint32_t* to, const int32_t* shift, const uint32_t* counts,
                             size_t n_sequences, const compact_cost& cost, compact_plan& plan,
                             int& status);
-// Words (a multiple of 4, both arrays aligned to 16 bytes) from pinned host memory, read
+// Words (an even number, both arrays aligned to 8 bytes) from pinned host memory, read
 // by a kernel: between two kernels a copy of 120 KB takes 14 us on MI355X, of 16 KB 5.
 hipError_t launch_fetch(hipStream_t s, uint32_t* to, const void* pinned, size_t words);
 hipError_t launch_compact(hipStream_t s, const pool_view& p, uint32_t layers,

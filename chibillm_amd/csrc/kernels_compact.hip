@@ -19,8 +19,8 @@
 // Bound by HBM, each row read and written once. Measured on MI355X, 8 kv heads of 128,
 // bf16: 28 layers of 1,010 moves (the newer half of 2,011 tokens to behind the first
 // four) 53.5 us, 4.3 TB/s; 12 layers of 7,600 moves of six sequences to fresh pages or in
-// place 157 us, a device copy's 4.76 TB/s; one of 2,000 tokens leaving 4 layers, a chain
-// that is cut, 39 us where its bytes take 14, leaving 28 layers, uncut, 108 and 96.
+// place 156 us, a device copy's 4.76 TB/s; one of 2,000 tokens leaving 4 layers, a chain
+// that is cut, 32 us where its bytes take 14, leaving 28 layers, uncut, 109 and 96.
 #include "ckv_internal.h"
 #include "prefill_records.h"
 #include "rope_turns.h"
@@ -222,14 +222,15 @@ __global__ __launch_bounds__(block_threads) void compact_kernel(pool_view p, com
     }
 }
 
-// Words from pinned host memory, 16 bytes a thread.
-__global__ __launch_bounds__(block_threads) void fetch_kernel(uint4* __restrict__ to,
-                                                              const uint4* __restrict__ from,
+// Words from pinned host memory, 8 bytes a thread, past every cache: the host wrote them
+// since the GPU last read there.
+__global__ __launch_bounds__(block_threads) void fetch_kernel(uint64_t* __restrict__ to,
+                                                              const uint64_t* __restrict__ from,
                                                               uint32_t n)
 {
     const uint32_t i = blockIdx.x * block_threads + threadIdx.x;
     if (i < n)
-        to[i] = from[i];
+        to[i] = __hip_atomic_load(from + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
 } // namespace
@@ -239,11 +240,11 @@ hipError_t launch_fetch(hipStream_t s, uint32_t* to, const void* pinned, size_t 
     void* from = nullptr;
     if (const hipError_t e = hipHostGetDevicePointer(&from, const_cast<void*>(pinned), 0))
         return e;
-    const uint64_t n = words / 4, blocks = (n + block_threads - 1) / block_threads;
-    if (words % 4 || n > 0xFFFFFFFFull)
+    const uint64_t n = words / 2, blocks = (n + block_threads - 1) / block_threads;
+    if (words % 2 || n > 0xFFFFFFFFull)
         return hipErrorInvalidValue;
-    fetch_kernel<<<(uint32_t)blocks, block_threads, 0, s>>>(reinterpret_cast<uint4*>(to),
-                                                            static_cast<const uint4*>(from),
+    fetch_kernel<<<(uint32_t)blocks, block_threads, 0, s>>>(reinterpret_cast<uint64_t*>(to),
+                                                            static_cast<const uint64_t*>(from),
                                                             (uint32_t)n);
     return hipGetLastError();
 }
