@@ -443,7 +443,7 @@ decode_plan_shape shape_decode_plan(const std::vector<uint32_t>& positions, uint
 // The plan of rows through a window, from their positions without its gaps.
 decode_form window_form_of(int dtype, uint32_t head_dim);
 decode_plan_shape shape_window_plan(const std::vector<uint32_t>& positions, uint32_t block_size,
-                                    uint32_t kv_heads, int cu_count, const decode_form& form);
+                                    uint32_t kv_heads, int cu_count, decode_form form);
 // Waves per workgroup of the fast decode for a launch of `units` (plan
 // workgroup, kv head) workgroups: a plan's split_pages (0 when no row is cut)
 // and the batch's mean row pages decide it; CKV_DECODE_WAVES overrides.

@@ -1017,12 +1017,18 @@ uint32_t fast_waves(uint32_t group, int dtype, uint32_t units, int cu_count,
 // 4 waves: 48 rows behind 1,024 tokens 45.3, 41.9 and 43.4; 64 50.8, 49.4 and 48.3; 80 69.0,
 // 67.0 and 62.6; 4 q heads per KV head, at 8 and 4 waves: 80 rows behind 256 30.7 and
 // 22.2, 64 behind 1,024 54.4 and 50.3; 8: 64 behind 1,024 75.2 and 68.2, 80 109 and 115.
+// Pieces of 4 pages, at 8 and 4 waves: 4 rows behind 512 6.8 and 6.4, 1 behind 256 6.2
+// and 6.0.
 uint32_t window_waves(uint32_t head_dim, uint32_t group, int dtype, uint32_t units, int cu_count,
                       uint32_t mean_pages, uint32_t split_pages)
 {
     const uint32_t waves = fast_waves(group, dtype, units, cu_count, mean_pages, split_pages);
     const uint32_t cus = (uint32_t)std::max(cu_count, 1);
-    if (std::getenv("CKV_DECODE_WAVES") || dtype == CKV_F32 || units < cus)
+    if (std::getenv("CKV_DECODE_WAVES") || dtype == CKV_F32)
+        return waves;
+    if (head_dim == 128 && split_pages && split_pages <= 4) // a page for each wave
+        return std::min(waves, 4u);
+    if (units < cus)
         return waves;
     const bool many = units > 2 * cus;
     if (split_pages)

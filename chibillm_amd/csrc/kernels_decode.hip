@@ -551,6 +551,12 @@ decode_plan_shape shape_decode_plan(const std::vector<uint32_t>& positions, uint
 // 65, behind 256 30.7 and 24.5; 160 of 2 kv heads, 2 each, 67.7 and 61.1, 21.8 and 22.4.
 constexpr uint64_t window_half_pages = 33, window_half_pages_wide = 17;
 
+// Small batches of 128-wide 16-bit rows are cut into pieces of an eighth of the longest
+// row, 4 to 12 pages, where all others are of at least 12: us at 12 and now (8 kv heads,
+// bf16), 4 rows behind 512 tokens 7.0 and 6.4, 1 behind 256 6.8 and 6.0, 8 behind 256 6.6
+// and 6.1. Rows of up to 16 pages stay whole (16 behind 128, 6.1 and 6.5 in halves).
+constexpr uint64_t window_whole_pages = 16;
+
 decode_form window_form_of(int dtype, uint32_t head_dim)
 {
     decode_form form = decode_form_of(dtype, head_dim);
@@ -563,10 +569,12 @@ decode_form window_form_of(int dtype, uint32_t head_dim)
 }
 
 decode_plan_shape shape_window_plan(const std::vector<uint32_t>& positions, uint32_t block_size,
-                                    uint32_t kv_heads, int cu_count, const decode_form& form)
+                                    uint32_t kv_heads, int cu_count, decode_form form)
 {
     uint64_t total, longest;
     batch_pages(positions, block_size, total, longest);
+    if (form.min_pages == form_narrow.min_pages && longest > window_whole_pages)
+        form.min_pages = (uint32_t)std::clamp<uint64_t>(longest / 8, 4, form_narrow.min_pages);
     const uint64_t rows = positions.size(), cus = (uint64_t)std::max(cu_count, 1);
     const bool even = 8 * total >= 7 * longest * rows;
     const uint64_t least = form.per_cu == 1 ? window_half_pages_wide : window_half_pages;

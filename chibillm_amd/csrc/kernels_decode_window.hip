@@ -5,7 +5,7 @@
 // and 16 q heads of 128, behind 1,024 tokens and 4 sinks, 39.5 us, 5.1 TB/s (one wave
 // for each chunk of tokens and kv head, then a merge, took 334); 24 gated rows of 2 kv
 // and 8 q heads of 256 behind 2,048 and 16 sinks 27.9 us, 3.2 TB/s (493); 4 rows of 60
-// to 1,900 tokens behind 512 7.5 us (82.6).
+// to 1,900 tokens behind 512 6.6 us (82.6).
 #include "decode_wg.h"
 
 namespace ckv {
