@@ -382,7 +382,8 @@ int ckv_sigmoid_mul(ckv_context* ctx, int dtype, const void* gate, const void* i
  * later ones, of any layer, reuse them. A call on a stream under capture is refused
  * (invalid_argument), before anything is captured, when it would upload or
  * allocate: make it once on the batch before the capture. A captured call holds for
- * the batch it was captured on, whatever other calls follow it there.
+ * the batch it was captured on, whatever other calls follow it there; replays of one
+ * pool's calls run one after another, as its calls do (they share its scratch).
  * gate may be NULL; otherwise as ckv_attention_gated's, and it must not be the
  * queries' or the output's memory (unsupported_aliasing). */
 
