@@ -1,6 +1,7 @@
 #include "block_manager.h"
 
 #include <limits>
+#include <utility>
 
 namespace chibillm {
 
@@ -78,6 +79,35 @@ block_manager::release(seq_id id) noexcept
     for (const block_id b : it->second)
         unref(b);
     tables_.erase(it);
+}
+
+result<std::vector<block_id>, state_error>
+block_manager::borrow(std::size_t count)
+{
+    if (count > free_.size())
+        return fail(state_errc::capacity_exhausted);
+    std::vector<block_id> pages(count);
+    for (block_id& b : pages)
+        b = take();
+    return pages;
+}
+
+void
+block_manager::put(seq_id id, std::size_t index, block_id page) noexcept
+{
+    const auto it = tables_.find(id);
+    if (it == tables_.end() || index >= it->second.size())
+        return;
+    unref(std::exchange(it->second[index], page));
+}
+
+void
+block_manager::give_back(std::span<const block_id> borrowed) noexcept
+{
+    for (auto it = borrowed.rbegin(); it != borrowed.rend(); ++it) {
+        refs_[*it] = 0;
+        free_.push_front(*it);
+    }
 }
 
 result<void, state_error>

@@ -51,6 +51,15 @@ public:
     // zero return to the back of the free list in table order.
     void release(seq_id id) noexcept override;
 
+    // Takes `count` free pages that no table names yet (one reference each): for a caller that
+    // writes them before it puts them into one. capacity_exhausted where there are fewer.
+    result<std::vector<block_id>, state_error> borrow(std::size_t count);
+    // The sequence's page `index` becomes the borrowed `page`; its former one loses a reference.
+    void put(seq_id id, std::size_t index, block_id page) noexcept;
+    // Borrowed pages that were put nowhere, all of one borrow(), go back to the front of the
+    // free list, as if never taken.
+    void give_back(std::span<const block_id> borrowed) noexcept;
+
     // Gives back the sequence's pages past those of its first `tokens` (> 0), as
     // release() does: the end of a compaction. invalid_reservation for an unknown
     // sequence or more tokens than it has pages for.

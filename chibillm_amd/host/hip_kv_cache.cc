@@ -315,10 +315,11 @@ hip_kv_cache::compact(std::span<const std::uint32_t> from, std::span<const std::
         return fail(state_errc::invalid_reservation);
     const int rc = ckv_compact(pool_, from.data(), to.data(), shift.empty() ? nullptr : shift.data(),
                                counts.data(), counts.size(), theta, rotary);
-    if (rc && rc != CKV_E_HIP_FAILURE)
-        return fail(state_errc::invalid_reservation, ctx_->last(rc), "compaction");
     if (rc)
-        return fail(state_errc::backend_failure, ctx_->last(rc), "compaction");
+        return fail(rc == CKV_E_HIP_FAILURE                ? state_errc::backend_failure
+                        : rc == CKV_E_TENSOR_ALLOCATION_FAILED ? state_errc::allocation_failed
+                                                               : state_errc::invalid_reservation,
+                    ctx_->last(rc), "compaction");
     return {};
 }
 

@@ -239,7 +239,7 @@ public:
     // Kept tokens' rows of all layers to other slots, their keys turned by `shift`
     // positions (empty: not at all), as ckv_compact, whose moves and rules these are:
     // counts[q] consecutive moves of sequence q. invalid_reservation where they are
-    // refused.
+    // refused, allocation_failed where host memory runs out, both before anything changes.
     result<void, state_error> compact(std::span<const std::uint32_t> from,
                                       std::span<const std::uint32_t> to,
                                       std::span<const std::int32_t> shift,

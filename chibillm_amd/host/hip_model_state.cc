@@ -101,15 +101,20 @@ hip_model_state::compact(seq_id id, std::span<const std::uint32_t> kept, float t
         spill_for(forks.size()); // which may leave pages to this sequence alone
         forks = shared();
     }
-    if (forks.size() > pages_->free_block_count())
-        return fail(state_errc::capacity_exhausted);
-    for (const std::size_t j : forks)
-        if (auto fresh = pages_->fork(id, j); !fresh)
-            return fail(fresh.error());
-    const auto table = resources(id).blocks;
     const std::uint32_t size = static_cast<std::uint32_t>(bs), count = static_cast<std::uint32_t>(n);
     std::vector<std::uint32_t> from(n), to(n);
     std::vector<std::int32_t> shift(theta > 0.0f ? n : 0);
+    std::vector<block_id> table = old;
+    // the pages that take the shared ones' place enter the sequence's table once the moves
+    // are accepted; until then a failure gives them back
+    struct borrowed_pages {
+        block_manager& owner;
+        std::vector<block_id> pages;
+        ~borrowed_pages() { owner.give_back(pages); }
+    } fresh { *pages_, {} };
+    CL_TRY_ASSIGN(fresh.pages, pages_->borrow(forks.size()));
+    for (std::size_t k = 0; k < forks.size(); ++k)
+        table[forks[k]] = fresh.pages[k];
     for (std::uint32_t i = 0; i < count; ++i) {
         from[i] = old[kept[i] / size] * size + kept[i] % size;
         to[i] = table[i / size] * size + i % size;
@@ -117,6 +122,9 @@ hip_model_state::compact(seq_id id, std::span<const std::uint32_t> kept, float t
             shift[i] = static_cast<std::int32_t>(i - kept[i]);
     }
     CL_TRY(cache_.compact(from, to, shift, std::span(&count, 1), theta, rotary));
+    for (std::size_t k = 0; k < forks.size(); ++k)
+        pages_->put(id, forks[k], fresh.pages[k]);
+    fresh.pages.clear();
     return pages_->truncate(id, n);
 }
 

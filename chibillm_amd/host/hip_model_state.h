@@ -102,8 +102,9 @@ public:
     // sequence starts at position kept.size(), and a checkpoint of it from then on holds
     // the kept tokens. Errors, before anything changes: invalid_reservation (no token, one
     // out of order or past the sequence's pages, a rotary width or theta that ckv_compact
-    // refuses), capacity_exhausted. Not to be called under stream capture; after any other
-    // error (the device's) the sequence is to be released.
+    // refuses, a stream under capture), capacity_exhausted (for want of a page, though
+    // checkpoints were spilled), allocation_failed (host memory). After backend_failure (the
+    // device's) the table is as it was but rows may have moved: the sequence is to be released.
     result<void, state_error> compact(seq_id id, std::span<const std::uint32_t> kept,
                                       float theta = 0.0f, std::size_t rotary_dimension = 0);
 

@@ -27,6 +27,10 @@ def test_host_layer_cpu():
     _run("host_tests", 120)
 
 
+def test_model_state_cpu():
+    _run("host_state_tests", 60)
+
+
 def test_decode_planner_cpu():
     """libckv's fast decode planner on the CPU (tests/cpp/plan_tests.cc): every
     plan covers each row's pages once, its workgroups' entries link up, and
