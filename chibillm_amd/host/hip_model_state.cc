@@ -3,6 +3,8 @@
 #include <algorithm>
 #include <limits>
 
+#include "model_batch.h"
+
 namespace chibillm {
 
 result<std::unique_ptr<hip_model_state>, state_error>
@@ -74,7 +76,9 @@ hip_model_state::compact(seq_id id, std::span<const std::uint32_t> kept, float t
 {
     const std::size_t bs = cache_.block_size();
     const auto held = resources(id).blocks;
-    if (kept.empty() || kept.back() / bs >= held.size())
+    if (in_batch_ || kept.empty() || kept.back() / bs >= held.size())
+        return fail(state_errc::invalid_reservation);
+    if (const auto at = next_.find(id); at != next_.end() && at->second == no_position)
         return fail(state_errc::invalid_reservation);
     for (std::size_t i = 1; i < kept.size(); ++i)
         if (kept[i] <= kept[i - 1])
@@ -121,11 +125,55 @@ hip_model_state::compact(seq_id id, std::span<const std::uint32_t> kept, float t
         if (!shift.empty())
             shift[i] = static_cast<std::int32_t>(i - kept[i]);
     }
-    CL_TRY(cache_.compact(from, to, shift, std::span(&count, 1), theta, rotary));
+    std::size_t& next = next_.try_emplace(id, no_position).first->second;
+    const std::size_t before = std::exchange(next, no_position);
+    if (auto done = cache_.compact(from, to, shift, std::span(&count, 1), theta, rotary); !done) {
+        if (done.error() != state_errc::backend_failure) {
+            if (before == no_position)
+                next_.erase(id);
+            else
+                next = before;
+        }
+        return fail(std::move(done.error()));
+    }
+    next = n;
     for (std::size_t k = 0; k < forks.size(); ++k)
         pages_->put(id, forks[k], fresh.pages[k]);
     fresh.pages.clear();
     return pages_->truncate(id, n);
+}
+
+result<void, state_error>
+hip_model_state::begin_batch(const model_batch& batch)
+{
+    begun_.clear();
+    if (!next_.empty())
+        for (const model_batch_item& item : batch.items) {
+            const auto at = next_.find(item.id);
+            if (at == next_.end())
+                continue;
+            if (at->second == no_position || batch.positions[item.token_offset] != at->second)
+                return fail(state_errc::invalid_reservation);
+            begun_.emplace_back(item.id, at->second + item.token_count);
+        }
+    in_batch_ = true;
+    return {};
+}
+
+void
+hip_model_state::commit_batch() noexcept
+{
+    for (const auto& [id, next] : begun_)
+        if (const auto at = next_.find(id); at != next_.end())
+            at->second = next;
+    abort_batch();
+}
+
+void
+hip_model_state::abort_batch() noexcept
+{
+    begun_.clear();
+    in_batch_ = false;
 }
 
 std::size_t

@@ -21,6 +21,9 @@
 
 #include <list>
 #include <memory>
+#include <unordered_map>
+#include <utility>
+#include <vector>
 
 #include "block_manager.h"
 #include "hip_kv_cache.h"
@@ -79,6 +82,7 @@ public:
     void release(seq_id id) noexcept override
     {
         pages_->release(id);
+        next_.erase(id);
         if (tables_)
             tables_->release(id);
     }
@@ -99,14 +103,19 @@ public:
     // the new ones (ckv_compact); 0 leaves them as they are. Pages that others share
     // (checkpoints, other sequences) are not written: a private page takes their place,
     // also that of a shared last page which later tokens will fill. The next batch of the
-    // sequence starts at position kept.size(), and a checkpoint of it from then on holds
-    // the kept tokens. Errors, before anything changes: invalid_reservation (no token, one
+    // sequence starts at position kept.size() (a scheduler that holds the sequence knows if
+    // the call goes through its compact()): begin_batch refuses one that does not, with
+    // invalid_reservation. A checkpoint of it from then on holds the kept tokens. Errors, before anything changes: invalid_reservation (no token, one
     // out of order or past the sequence's pages, a rotary width or theta that ckv_compact
-    // refuses, a stream under capture), capacity_exhausted (for want of a page, though
+    // refuses, a batch begun, a stream under capture), capacity_exhausted (for want of a page, though
     // checkpoints were spilled), allocation_failed (host memory). After backend_failure (the
     // device's) the table is as it was but rows may have moved: the sequence is to be released.
     result<void, state_error> compact(seq_id id, std::span<const std::uint32_t> kept,
-                                      float theta = 0.0f, std::size_t rotary_dimension = 0);
+                                      float theta = 0.0f,
+                                      std::size_t rotary_dimension = 0) override;
+    result<void, state_error> begin_batch(const model_batch& batch) override;
+    void commit_batch() noexcept override;
+    void abort_batch() noexcept override;
 
     // Keeps the sequences' block tables on the device (device_tables); the
     // rows of released sequences are returned to it.
@@ -150,6 +159,12 @@ private:
     std::size_t cow_copies_ = 0;
     std::unique_ptr<device_tables> tables_;
     std::shared_ptr<shared_checkpoint_list> live_ = std::make_shared<shared_checkpoint_list>();
+    // Where the next batch of a sequence that was compacted starts; no_position after a
+    // compaction that the device failed.
+    static constexpr std::size_t no_position = static_cast<std::size_t>(-1);
+    std::unordered_map<seq_id, std::size_t> next_;
+    std::vector<std::pair<seq_id, std::size_t>> begun_; // of next_, once the batch is committed
+    bool in_batch_ = false;
     bool spill_ = true;
     std::size_t spills_ = 0, spilled_pages_ = 0;
 };

@@ -132,4 +132,13 @@ inference_engine::remove(seq_id id)
     return {};
 }
 
+result<void, inference_engine_error>
+inference_engine::compact(seq_id id, std::span<const std::uint32_t> kept, float theta,
+                          std::size_t rotary)
+{
+    if (auto done = scheduler_.compact(id, kept, theta, rotary); !done)
+        return fail(inference_engine_errc::sequence_compact_failed, done.error());
+    return {};
+}
+
 } // namespace chibillm

@@ -18,12 +18,13 @@ enum class inference_engine_errc : std::uint8_t {
     batch_completion_failed,
     sequence_cancel_failed,
     sequence_remove_failed,
+    sequence_compact_failed,
 };
 
 [[nodiscard]] inline std::string_view
 error_name(inference_engine_errc code) noexcept
 {
-    static constexpr std::array<std::string_view, 10> names {
+    static constexpr std::array<std::string_view, 11> names {
         "inference_engine.scheduler_creation_failed",
         "inference_engine.sequence_add_failed",
         "inference_engine.scheduling_failed",
@@ -34,6 +35,7 @@ error_name(inference_engine_errc code) noexcept
         "inference_engine.batch_completion_failed",
         "inference_engine.sequence_cancel_failed",
         "inference_engine.sequence_remove_failed",
+        "inference_engine.sequence_compact_failed",
     };
     const auto i = static_cast<std::size_t>(code);
     return i < names.size() ? names[i] : "inference_engine.unknown_error";
@@ -69,6 +71,12 @@ public:
     [[nodiscard]] result<std::vector<sequence_update>, inference_engine_error> step();
     [[nodiscard]] result<void, inference_engine_error> cancel(seq_id id);
     [[nodiscard]] result<void, inference_engine_error> remove(seq_id id);
+
+    // scheduler::compact, between steps.
+    [[nodiscard]] result<void, inference_engine_error> compact(seq_id id,
+                                                               std::span<const std::uint32_t> kept,
+                                                               float theta = 0.0f,
+                                                               std::size_t rotary_dimension = 0);
 
     // Host time spent in each stage of the steps so far (no reference
     // counterpart): scheduling, building the model batch, the runner's

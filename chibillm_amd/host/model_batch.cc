@@ -8,7 +8,7 @@
 // scheduled count differs from the item's, or whose tokens or positions would
 // leave the sequence or the u32 position range. It then lays the items'
 // unprocessed tokens end to end in batch order, each at its position
-// (processed + i), with a copy of the sequence's block table, and marks the
+// (next_position + i: processed + i but behind a compaction), with a copy of the sequence's block table, and marks the
 // last row of each sampling item as its logits row.
 //
 // prepare_paged_batch turns a model batch into the arrays the KV path takes:
@@ -40,7 +40,7 @@ namespace {
 // What build_model_batch takes from the scheduler for one item.
 struct item_source {
     const seq* sequence;
-    std::size_t first; // position of the item's first token
+    std::size_t first; // the item's first token in the sequence's history
 };
 
 std::optional<model_batch_errc>
@@ -56,7 +56,8 @@ item_fault(const scheduled_item& item, const seq* s, seq_status wanted)
     const std::size_t first = s->processed_token_count();
     if (first > s->token_count() || s->token_count() - first < item.token_count)
         return model_batch_errc::token_range_out_of_bounds;
-    if (first > last_position || item.token_count - 1 > last_position - first)
+    const std::size_t position = s->next_position();
+    if (position > last_position || item.token_count - 1 > last_position - position)
         return model_batch_errc::position_out_of_range;
     return std::nullopt;
 }
@@ -109,7 +110,7 @@ build_model_batch(const scheduled_batch& scheduled, const scheduler& engine)
         const auto unprocessed = s->tokens().subspan(first, item.token_count);
         std::copy(unprocessed.begin(), unprocessed.end(), out.tokens.begin() + row);
         for (std::size_t t = 0; t < item.token_count; ++t)
-            out.positions[row + t] = static_cast<position_id>(first + t);
+            out.positions[row + t] = static_cast<position_id>(s->next_position() + t);
         const auto table = engine.state().resources(item.id).blocks;
         model_batch_item built { item.id, row, item.token_count, std::nullopt,
                                  std::vector<block_id>(table.begin(), table.end()) };

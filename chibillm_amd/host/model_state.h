@@ -73,6 +73,15 @@ public:
         return fail(state_errc::invalid_reservation);
     }
 
+    // Drops the sequence's tokens but for `kept` (ascending positions), which move to
+    // positions 0 .. kept.size() - 1, between batches; with theta (> 0) their keys turn to
+    // them. invalid_reservation where a state cannot. New.
+    virtual result<void, state_error> compact(seq_id, std::span<const std::uint32_t> /* kept */,
+                                              float /* theta */, std::size_t /* rotary */)
+    {
+        return fail(state_errc::invalid_reservation);
+    }
+
     virtual std::size_t block_size() const noexcept { return 0; }
     virtual sequence_resources resources(seq_id) const noexcept { return {}; }
 

@@ -25,7 +25,8 @@
 // its sample (a prefill item first becomes running), then either finishes on
 // EOS or the length limit (its pages released, its budget returned) or joins
 // the back of the running queue. abort() undoes the batch's scheduling but
-// keeps its pages for the retry; cancel() finishes a live sequence.
+// keeps its pages for the retry; cancel() finishes a live sequence; compact()
+// drops some of its cached tokens, whose places its next ones take.
 #include "scheduler.h"
 
 #include <algorithm>
@@ -224,6 +225,8 @@ scheduler::checkpoint_cut(const seq& s, std::size_t tokens) const noexcept
 {
     const std::size_t from = s.processed_token_count();
     const auto prompt = s.prompt_tokens();
+    if (s.dropped_token_count())
+        return tokens; // its prefixes are not in the state any more
     for (const std::size_t boundary : s.checkpoints()) {
         if (boundary <= from)
             continue;
@@ -273,7 +276,7 @@ scheduler::reserve(const std::vector<planned>& items, scheduled_batch& batch)
 {
     for (const planned& p : items) {
         seq& s = members_.at(p.id).sequence;
-        auto room = state_->reserve(p.id, s.processed_token_count() + p.tokens);
+        auto room = state_->reserve(p.id, s.next_position() + p.tokens);
         if (!room) {
             unschedule(batch); // pages already reserved stay with their sequences
             if (room.error() == state_errc::capacity_exhausted)
@@ -338,7 +341,8 @@ scheduler::publish_prefix(const seq& s) noexcept
 {
     const std::size_t count = s.processed_token_count();
     const auto boundaries = s.checkpoints();
-    if (!std::binary_search(boundaries.begin(), boundaries.end(), count) || !worth_caching(count))
+    if (s.dropped_token_count()
+        || !std::binary_search(boundaries.begin(), boundaries.end(), count) || !worth_caching(count))
         return;
     const auto prefix = s.prompt_tokens().first(count);
     if (prefixes_.contains(prefix))
@@ -461,6 +465,30 @@ scheduler::cancel(seq_id id)
     if (auto finished = m->sequence.finish(finish_reason::cancelled); !finished)
         return fail(scheduler_errc::sequence_failure, finished.error());
     leave(id, *m);
+    check_invariants();
+    return {};
+}
+
+result<void, scheduler_error>
+scheduler::compact(seq_id id, std::span<const std::uint32_t> kept, float theta, std::size_t rotary)
+{
+    if (active_)
+        return fail(scheduler_errc::batch_in_flight);
+    member* m = find_member(id);
+    if (!m)
+        return fail(scheduler_errc::unknown_sequence);
+    seq& s = m->sequence;
+    if (s.is_finished())
+        return fail(scheduler_errc::invalid_sequence_state);
+    if (kept.empty() || kept.back() >= s.next_position())
+        return fail(scheduler_errc::sequence_failure, seq_errc::invalid_cached_prefix, "compact");
+    if (auto done = state_->compact(id, kept, theta, rotary); !done)
+        return fail(done.error() == state_errc::capacity_exhausted
+                        ? scheduler_errc::cache_capacity_exhausted
+                        : scheduler_errc::block_manager_failure,
+                    done.error(), "compact sequence " + std::to_string(id));
+    [[maybe_unused]] auto counted = s.keep_positions(kept.size());
+    assert(counted);
     check_invariants();
     return {};
 }

@@ -145,6 +145,16 @@ public:
     [[nodiscard]] result<void, scheduler_error> abort(batch_id id);
 
     [[nodiscard]] result<void, scheduler_error> cancel(seq_id id);
+    // Compacts a live sequence in the state (model_state::compact), between batches: of the
+    // tokens at positions 0 .. next_position() - 1 those at `kept` stay, and its next batch
+    // goes on behind them. Its prefixes are published no more. Errors: batch_in_flight,
+    // unknown_sequence, invalid_sequence_state (finished), sequence_failure (no kept position
+    // or one that holds no token yet), cache_capacity_exhausted, block_manager_failure; after
+    // a device's failure the sequence is to be cancelled. New: the reference drops nothing.
+    [[nodiscard]] result<void, scheduler_error> compact(seq_id id,
+                                                        std::span<const std::uint32_t> kept,
+                                                        float theta = 0.0f,
+                                                        std::size_t rotary_dimension = 0);
     [[nodiscard]] result<void, scheduler_error> remove(seq_id id);
 
 private:

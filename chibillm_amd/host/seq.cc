@@ -115,6 +115,20 @@ seq::restore_prefix(std::size_t count)
 }
 
 result<void, seq_errc>
+seq::keep_positions(std::size_t count)
+{
+    if (auto bad = check({ { is_finished(), seq_errc::already_finished },
+                           { scheduled_ != 0, seq_errc::work_already_scheduled },
+                           { count == 0 || count > next_position(),
+                             seq_errc::invalid_cached_prefix } });
+        !bad)
+        return bad;
+    dropped_ = processed_ - count;
+    check_invariants();
+    return {};
+}
+
+result<void, seq_errc>
 seq::append_token(token_id token)
 {
     if (auto bad = check({ { is_finished(), seq_errc::already_finished },
@@ -205,7 +219,7 @@ void
 seq::check_invariants() const noexcept
 {
     assert(prompt_size_ > 0 && prompt_size_ <= tokens_.size());
-    assert(scheduled_ <= tokens_.size() - processed_);
+    assert(scheduled_ <= tokens_.size() - processed_ && dropped_ <= processed_);
     assert(is_finished() == (reason_ != finish_reason::none));
     assert(!is_finished() || scheduled_ == 0);
 }

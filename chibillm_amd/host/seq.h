@@ -101,6 +101,14 @@ public:
     [[nodiscard]] std::size_t processed_token_count() const noexcept { return processed_; }
     [[nodiscard]] std::size_t cached_token_count() const noexcept { return cached_; }
     [[nodiscard]] std::span<const std::size_t> checkpoints() const noexcept { return checkpoints_; }
+    // The place in the KV cache of the next token: the processed ones are at positions
+    // 0 .. next_position() - 1, less those that compactions dropped. New: the reference's
+    // caches drop nothing.
+    [[nodiscard]] std::size_t next_position() const noexcept { return processed_ - dropped_; }
+    [[nodiscard]] std::size_t dropped_token_count() const noexcept { return dropped_; }
+    // After a compaction that kept `count` of them (> 0, at most next_position();
+    // invalid_cached_prefix otherwise), between batches.
+    [[nodiscard]] result<void, seq_errc> keep_positions(std::size_t count);
     // Marks a restored proper prefix of the prompt as processed.
     [[nodiscard]] result<void, seq_errc> restore_prefix(std::size_t count);
 
@@ -132,6 +140,7 @@ private:
     std::size_t prompt_size_;
     std::size_t processed_ = 0;
     std::size_t cached_ = 0;
+    std::size_t dropped_ = 0;
     std::vector<std::size_t> checkpoints_;
     std::size_t scheduled_ = 0;
     generation_params params_;

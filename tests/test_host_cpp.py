@@ -28,6 +28,8 @@ def test_host_layer_cpu():
 
 
 def test_model_state_cpu():
+    """Compaction of a sequence in the state and under the engine, on host arrays
+    (tests/cpp/host_state_tests.cc)."""
     _run("host_state_tests", 60)
 
 
