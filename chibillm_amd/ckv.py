@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import warnings
 from typing import Optional, Sequence
 
 import numpy as np
@@ -161,13 +162,18 @@ def _p(a: Optional[np.ndarray]):
 def rope_pair_axes(sections, interleaved: bool = False) -> np.ndarray:
     """pair_axis of the rope_axes calls from the rotary pairs each axis turns
     (sections[a]; their sum is rotary_dim / 2): one section after another, or
-    interleaved, the axes taken in turn while they have pairs left and the rest
-    by the first."""
+    interleaved: of n axes the a-th (a > 0) has the pairs a, a + n, a + 2n, ..., its first
+    sections[a] of them, and the first axis has the rest. Where the pairs end before
+    an axis has its own ([8, 12, 12] leaves the second 11 and the third 10) the first has
+    more than its section says, and a UserWarning gives the counts."""
     if not interleaved:
         return np.repeat(np.arange(len(sections)), sections).astype(np.uint8)
     axes = np.zeros(sum(sections), np.uint8)
     for a in range(1, len(sections)):
         axes[a:sections[a] * len(sections):len(sections)] = a
+    counts = np.bincount(axes, minlength=len(sections)).tolist()
+    if counts != list(sections):
+        warnings.warn(f"interleaved sections {list(sections)} turn {counts} pairs", stacklevel=2)
     return axes
 
 

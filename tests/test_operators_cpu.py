@@ -3,6 +3,7 @@
 moves are cut into and what the entry points refuse; and the binding's own checks."""
 import os
 import subprocess
+import warnings
 
 import numpy as np
 import pytest
@@ -32,6 +33,22 @@ def test_rope_pair_axes(sections):
         if axis:
             assert np.flatnonzero(mixed == axis).tolist() == [
                 j for j in range(sum(sections)) if j % len(sections) == axis and j < pairs * len(sections)]
+
+
+@pytest.mark.parametrize("sections,turned", [([8, 12, 12], [11, 11, 10]), ([4, 20], [12, 12]), ([20, 20, 4], [25, 15, 4])])
+def test_interleaved_sections_that_do_not_fit_are_told(sections, turned):
+    with pytest.warns(UserWarning, match=r"turn \[{}\] pairs".format(", ".join(map(str, turned)))):
+        axes = ckv.rope_pair_axes(sections, interleaved=True)
+    assert np.bincount(axes).tolist() == turned
+
+
+@pytest.mark.parametrize("sections", [[32], [24, 20, 20], [11, 11, 10], [5, 3], [2, 1, 1, 1], [5, 0, 2]])
+def test_interleaved_sections_turn_what_they_say(sections):
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        axes = ckv.rope_pair_axes(sections, interleaved=True)
+        ckv.rope_pair_axes([8, 12, 12])  # one after another any sections do
+    assert np.bincount(axes, minlength=len(sections)).tolist() == sections
 
 
 class _Stub:
