@@ -2422,7 +2422,8 @@ int ckv_attention_window(ckv_pool* pool, size_t layer, const void* queries, size
         if (!batch_has_tiles(pool)
             || !prefill_takes(pool, queries, q_heads, scale, output, gate))
             return run_decode(pool, layer, queries, q_heads, scale, output, gate, w);
-        // also a window that leaves nothing out: its kernels hold probabilities in more bits
+        // also a window that leaves nothing out: its kernels hold probabilities in as many
+        // bits as the others or more (16 to 8 in 128-wide bf16)
         window_batch& through =
             select_window(pool, w.window != all_keys.window ? w : key_window { UINT32_MAX - 1, 0 },
                           prefill_window_rows(view_of(pool), (uint32_t)q_heads));

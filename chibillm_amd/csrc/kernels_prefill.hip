@@ -879,13 +879,13 @@ namespace {
 // blocks / n of block us to go, and `shared` of that again for each workgroup more; n
 // ranges hand over in base + n * range us, and each record in record us. Fitted on MI355X,
 // us at n = 1, 2, 3, 4, 6, 8: bf16, 64 workgroups of 36 blocks, 39, 27, 23, 21, 23, 24,
-// and 192 of 23, 29, 30, 37, 35, 42, 47; 256 wide, 32 of 34, 70, 51, 44, 42, 43, 45; f32,
+// and 192 of 23, 29, 30, 37, 35, 42, 47; 256 wide, 32 of 34, 68, 46, 39, 36, 35, 37; f32,
 // 72 of 20, 103, 60, 47, 58, 51, 55. The n taken comes within a tenth of the best but for
 // f32's launches of short tiles (144 workgroups of 7 blocks take 42 us, in 2 ranges 32).
 struct window_cost {
     double block, shared, base, range, record;
 };
-constexpr window_cost cost_16bit { 0.85, 0.6, 2.0, 0.4, 0.01 }, cost_wide { 1.45, 1.0, 4.0, 2.0, 0.02 },
+constexpr window_cost cost_16bit { 0.85, 0.6, 2.0, 0.4, 0.01 }, cost_wide { 1.65, 1.0, 4.0, 2.0, 0.02 },
     cost_f32 { 4.4, 0.8, 0.0, 0.8, 0.02 };
 constexpr uint32_t window_min_blocks = 2; // of a range
 

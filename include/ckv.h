@@ -372,7 +372,8 @@ int ckv_sigmoid_mul(ckv_context* ctx, int dtype, const void* gate, const void* i
  * layer reads of them. A row at position p attends key t when t <= p and
  * (t > p - window or t < sinks): the last `window` tokens, itself among them,
  * and the sequence's first `sinks`. output = softmax(q . k * scale) . v over
- * those, with fp32 accumulation. window must be at least 1 (invalid_argument);
+ * those, with fp32 accumulation; where the matrix cores multiply probabilities and 16-bit
+ * values, probabilities keep at least 16 bits (256-wide heads: all 24). window must be at least 1 (invalid_argument);
  * any larger value, and any sinks from 0 on, are taken.
  * Pages that hold no key a row attends are not read, whatever is in them: a
  * sequence may give them back, as long as its table keeps some page id of the
