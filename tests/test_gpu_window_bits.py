@@ -1,20 +1,20 @@
 """How many bits of a probability enter the product with V in the windowed prefill.
 
 Outputs are rounded to the pool's type, which hides the rounding of probabilities where outputs
-are as large as values. Here a row attends two keys of nearly equal scores whose values are v
-and -v: the output is v tanh(d / 2), d the difference of the scores, small enough that its
-own rounding is far below a probability's. Scores are exact in 32 bits: one product of two numbers
-of eight bits, and a scale of a power of two."""
+are as large as values. Here a row attends a sink of score 0 and value 0 and two keys of nearly equal
+scores below it whose values are v and -v: the output is the difference of their probabilities,
+small enough that its own rounding is far below theirs. Scores are exact in 32 bits: sums of two
+products of numbers of eight bits, and a scale of a power of two."""
 import numpy as np
 import pytest
 import torch
 
 from tests.gpu_util import new_context
-from tests.operator_ref import STEP32, Cache, assert_within
+from tests.operator_ref import ROUND, STEP32, Cache, assert_within
 
 pytestmark = pytest.mark.gpu
 
-SCALE, UNIT = 2.0 ** -4, 2.0 ** -19  # UNIT: the scores' grid, after the scale
+SCALE, ROWS = 2.0 ** -4, 600
 
 
 @pytest.fixture(scope="module")
@@ -25,32 +25,47 @@ def ctx():
     c.close()
 
 
-def rounded(x, bits):
-    """x in 64 bits rounded to `bits` significant ones."""
-    m, e = np.frexp(x)
-    return np.ldexp(np.round(m * 2.0 ** bits) / 2.0 ** bits, e)
+def numbers():
+    """Of each token its score's own part, r 2^-19 with r below 256; of each row what it takes from
+    the scores of both, j 2^-8 with j below 256: probabilities from 0.36 to 1 of the sink's."""
+    rng = np.random.RandomState(1)
+    return rng.randint(0, 256, ROWS) * 2.0 ** -19, rng.randint(0, 256, ROWS) * 2.0 ** -8
 
 
-def scores(n):
-    return np.random.RandomState(n).randint(0, 256, n).astype(np.float64) * UNIT
+def outputs(weight):
+    """Of rows 2 on, for values of 1 at even tokens and -1 at odd ones, with weight(p) of each of
+    the two entering the product with V."""
+    own, taken = numbers()
+    a, b = np.exp(own[1:-1] - taken[2:]), np.exp(own[2:] - taken[2:]) # tokens i - 1 and i of row i
+    return (1 - 2 * (np.arange(2, ROWS) % 2)) * (weight(b) - weight(a)) / (1 + a + b)
 
 
 def room(p_bits):
-    """What the definition allows besides the output's rounding, of |v| = 1: scores are exact and
-    below 1, so that their exponential, the sum of two and the division are each within two steps
-    of 2^-23 (fp16's, taken at 2^6 times, in an exponent that is rounded at 2^-22: 1.4 steps of the
-    probability), a key range's weight within two; a probability of p_bits bits is off by at most
-    2^-p_bits of itself in either of two keys."""
-    return 8 * STEP32 + 2.0 ** -p_bits
+    """What 32-bit arithmetic may add to an output's rounding, of |v| = 1. Scores are exact. A
+    probability's exponent is a product and a sum rounded at 2^-24 of at most 2 (fp16's, taken at 2^6
+    times, at 2^-22), its exponential within two steps of 2^-23, a key range's weight within two, the
+    sums and the division within two: 8 steps of each of two probabilities that make up at most
+    2/3 of the sum. Rounded to p_bits bits a probability is off by 2^-p_bits of itself at most."""
+    return (8 * STEP32 + 2.0 ** -p_bits) * 2 / 3
+
+
+def bf16_terms(p, n):
+    """p as the sum of n roundings to bf16, each of what those before it left."""
+    left, total = torch.from_numpy(p).float(), torch.zeros(p.size)
+    for _ in range(n):
+        term = left.bfloat16().float()
+        left, total = left - term, total + term
+    return total.double().numpy()
 
 
 def test_the_bound_tells_bits_apart():
-    """On the CPU: probabilities rounded to 16 bits pass the bound of 16 and fail that of 22."""
-    s = scores(300)
-    d = s[1:] - s[:-1]
-    p = rounded(np.exp(-np.abs(d)), 16)
-    off = np.abs((1 - p) / (1 + np.exp(-np.abs(d))) - np.tanh(np.abs(d) / 2)).max()
-    assert room(22) < off < room(16)
+    """On the CPU: probabilities as two bf16 terms pass the bound of 16 bits and fail that of 22 by
+    more than the output's rounding; as three they pass that of 24."""
+    exact = outputs(lambda p: p)
+    slack = np.abs(exact) * ROUND[torch.bfloat16] * (1 + 1e-3)
+    for terms, bits, passes in ((1, 8, True), (1, 16, False), (2, 16, True), (2, 22, False), (3, 24, True)):
+        off = np.abs(outputs(lambda p: bf16_terms(p, terms)) - exact)
+        assert (np.all(off <= room(bits))) if passes else np.any(off > room(bits) + 2 * slack)
 
 
 @pytest.mark.parametrize("dtype,group,d,p_bits", [
@@ -62,24 +77,25 @@ def test_probabilities_keep_their_bits(ctx, dtype, group, d, p_bits, split, monk
     print(f"bits {dtype} group {group} d {d}: {p_bits}, {split} key ranges", flush=True)
     monkeypatch.setenv("CKV_PREFILL_SPLIT", split)
     monkeypatch.setenv("CKV_PREFILL_SPLIT_MIN", "1")
-    n, first = 300, 0
-    cache = Cache(ctx, dtype, [n], 1, d, seed=1)
-    at = cache.slots(cache.tables[0], np.arange(n))
-    s = scores(n)
-    sign = torch.from_numpy(1.0 - 2.0 * (np.arange(n) % 2))
+    own, taken = numbers()
+    cache = Cache(ctx, dtype, [ROWS], 1, d, seed=1)
+    at = cache.slots(cache.tables[0], np.arange(ROWS))
     side = torch.where(torch.arange(d) % 3 == 0, -1.0, 1.0).double()
-    cache.k[0, at] = 0
-    cache.k[0, at, :, 0] = torch.from_numpy(s / SCALE * 2.0 ** 8).to(cache.dtype)[:, None]
-    assert torch.equal(cache.k[0, at, 0, 0].double(), torch.from_numpy(s / SCALE * 2.0 ** 8))
-    cache.v[0, at] = (sign[:, None] * side).to(cache.dtype)[:, None]
+    sign = torch.from_numpy(1.0 - 2.0 * (np.arange(ROWS) % 2))
+    k, v = torch.zeros(ROWS, d, dtype=torch.float64), sign[:, None] * side
+    k[1:, 0], k[1:, 1] = torch.from_numpy(own[1:] / SCALE * 2.0 ** 8), 1.0
+    v[0] = 0
+    q = torch.zeros(ROWS, group, d, dtype=torch.float64)
+    q[..., 0], q[..., 1] = 2.0 ** -8, torch.from_numpy(-taken / SCALE)[:, None]
+    cache.k[0, at], cache.v[0, at] = k.to(cache.dtype)[:, None], v.to(cache.dtype)[:, None]
+    qt = q.to(cache.dtype)
+    assert torch.equal(cache.k[0, at, 0].double(), k) and torch.equal(qt.double(), q)
     pool = cache.to_device()
-    cache.upload([first], [n], slots=False)
-    q = torch.zeros(n, group, d, dtype=cache.dtype)
-    q[..., 0] = 2.0 ** -8
-    out = torch.empty(n, group * d, dtype=cache.dtype, device="cuda")
-    pool.attention_window(0, q.cuda().flatten(1), group, SCALE, 2, out, sinks=0)
+    cache.upload([0], [ROWS], slots=False)
+    out = torch.empty(ROWS, group * d, dtype=cache.dtype, device="cuda")
+    pool.attention_window(0, qt.cuda().flatten(1), group, SCALE, 2, out, sinks=1)
     ctx.sync()
-    mean = torch.cat([sign[:1], sign[1:] * torch.tanh(torch.from_numpy(s[1:] - s[:-1]) / 2)])
-    want = (mean[:, None] * side)[:, None].expand(n, group, d)
-    assert_within(out.view(n, group, d), want, torch.full((n, group, d), room(p_bits), dtype=torch.float64), "two keys")
+    want = torch.from_numpy(outputs(lambda p: p))[:, None] * side
+    want = want[:, None].expand(-1, group, d)
+    assert_within(out.view(ROWS, group, d)[2:], want, torch.full(want.shape, room(p_bits), dtype=torch.float64), "rows")
     pool.close()
