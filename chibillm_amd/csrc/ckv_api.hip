@@ -230,11 +230,12 @@ int fetch_staged(ckv_context* ctx, uint32_t* device, size_t words)
     return CKV_OK;
 }
 
-// Grow-only device buffer; the stream is drained before an old buffer is freed. One
-// that a graph may use is kept.
+// Grow-only device buffer of a pool; the stream is drained before an old buffer is freed.
+// One that a graph may use is kept as long as the pool.
 template <class T>
-int ensure_device(ckv_context* ctx, T** ptr, size_t* capacity, size_t needed, const char* what)
+int ensure_device(ckv_pool* pool, T** ptr, size_t* capacity, size_t needed, const char* what)
 {
+    ckv_context* ctx = pool->ctx;
     if (needed <= *capacity)
         return CKV_OK;
     if (ctx->in_capture)
@@ -243,8 +244,8 @@ int ensure_device(ckv_context* ctx, T** ptr, size_t* capacity, size_t needed, co
     // must not reallocate (and drain the stream) every step
     const size_t count = std::max({ needed, *capacity + *capacity / 2, (size_t)1024 });
     if (*ptr) {
-        if (ctx->captured) {
-            ctx->retired.push_back(*ptr);
+        if (pool->captured) {
+            pool->retired.push_back(*ptr);
         } else {
             (void)hipStreamSynchronize(ctx->stream);
             (void)dev_free(ctx, *ptr);
@@ -442,7 +443,7 @@ int ensure_plan(ckv_pool* pool)
     int status = stage(ctx, words * sizeof(uint32_t), &host);
     if (status)
         return status;
-    status = ensure_device(ctx, &pool->d_plan, &pool->d_plan_words, words, "decode plan");
+    status = ensure_device(pool, &pool->d_plan, &pool->d_plan_words, words, "decode plan");
     if (status)
         return status;
     put_plan(pool, pool->positions, pool->meta, shape, static_cast<uint32_t*>(host), pool->d_plan);
@@ -467,14 +468,14 @@ int ensure_split(ckv_pool* pool, const meta_view& m, size_t q_heads, split_scrat
     size_t capacity_floats = pool->d_partials_bytes / sizeof(float);
     const size_t floats = (size_t)m.n_records * q_heads
         * partial_record_floats((uint32_t)pool->head_dim);
-    int status = ensure_device(ctx, &pool->d_partials, &capacity_floats, floats,
+    int status = ensure_device(pool, &pool->d_partials, &capacity_floats, floats,
                                "decode partials");
     pool->d_partials_bytes = capacity_floats * sizeof(float);
     if (status)
         return status;
     const size_t counters = (size_t)m.n_records * pool->kv_heads;
     if (counters > pool->d_arrivals_words) {
-        status = ensure_device(ctx, &pool->d_arrivals, &pool->d_arrivals_words, counters,
+        status = ensure_device(pool, &pool->d_arrivals, &pool->d_arrivals_words, counters,
                                "decode arrival counters");
         if (status)
             return status;
@@ -531,7 +532,7 @@ int put_work(ckv_pool* pool, const std::vector<uint32_t>& positions, meta_view& 
             w[2 * item + 1] = c;
         }
     }
-    status = ensure_device(ctx, device, device_words, words, "decode work list");
+    status = ensure_device(pool, device, device_words, words, "decode work list");
     if (status)
         return status;
     status = upload_staged(ctx, *device, words * sizeof(uint32_t));
@@ -624,7 +625,7 @@ int ensure_window_plan(ckv_pool* pool, window_batch& b)
     void* host = nullptr;
     int status = stage(ctx, words * sizeof(uint32_t), &host);
     if (!status)
-        status = ensure_device(ctx, &b.d_plan, &b.d_plan_words, words, "decode plan");
+        status = ensure_device(pool, &b.d_plan, &b.d_plan_words, words, "decode plan");
     if (status)
         return status;
     auto* w = static_cast<uint32_t*>(host);
@@ -665,7 +666,7 @@ int ensure_window_tiles(ckv_pool* pool, window_batch& b)
     void* host = nullptr;
     int status = stage(ctx, words * sizeof(uint32_t), &host);
     if (!status)
-        status = ensure_device(ctx, &b.d_tiles, &b.d_tiles_words, words, "window tiles");
+        status = ensure_device(pool, &b.d_tiles, &b.d_tiles_words, words, "window tiles");
     if (status)
         return status;
     auto* to = static_cast<uint32_t*>(host);
@@ -704,7 +705,6 @@ struct decode_setup {
 int setup_decode(ckv_pool* pool, const void* queries, size_t q_heads, const void* output,
                  key_window window, decode_setup& d)
 {
-    ckv_context* ctx = pool->ctx;
     const bool fast = decode_fast_applies(view_of(pool), (uint32_t)q_heads, queries, output);
     d.through = decode_window(pool, window);
     int status = fast ? ensure_fast(pool, d.through, q_heads, d.split)
@@ -717,7 +717,7 @@ int setup_decode(ckv_pool* pool, const void* queries, size_t q_heads, const void
         size_t capacity_floats = pool->d_partials_bytes / sizeof(float);
         const size_t needed = (size_t)(d.through ? d.through->meta : pool->meta).n_items * q_heads
             * partial_record_floats((uint32_t)pool->head_dim);
-        status = ensure_device(ctx, &pool->d_partials, &capacity_floats, needed,
+        status = ensure_device(pool, &pool->d_partials, &capacity_floats, needed,
                                "decode partials");
         // stored whatever the outcome: a failed regrow leaves no buffer and
         // must leave no capacity either
@@ -760,7 +760,7 @@ int stage_pairs(ckv_pool* pool, const uint32_t* a, const uint32_t* b, size_t n)
         words[2 * i] = a[i];
         words[2 * i + 1] = b[i];
     }
-    status = ensure_device(ctx, &pool->d_pairs, &pool->d_pairs_words, 2 * n, "pair buffer");
+    status = ensure_device(pool, &pool->d_pairs, &pool->d_pairs_words, 2 * n, "pair buffer");
     if (status)
         return status;
     return upload_staged(ctx, pool->d_pairs, 2 * n * sizeof(uint32_t));
@@ -775,7 +775,7 @@ int stage_list(ckv_pool* pool, const uint32_t* list, size_t n)
     if (status)
         return status;
     std::memcpy(host, list, n * sizeof(uint32_t));
-    status = ensure_device(ctx, &pool->d_pairs, &pool->d_pairs_words, n, "block list");
+    status = ensure_device(pool, &pool->d_pairs, &pool->d_pairs_words, n, "block list");
     if (status)
         return status;
     return upload_staged(ctx, pool->d_pairs, n * sizeof(uint32_t));
@@ -842,7 +842,7 @@ int run_transfer(ckv_pool* pool, const uint32_t* blocks, size_t n_blocks, size_t
     const size_t layer_bytes = tokens * pool->kv_heads * pool->head_dim * pool->elem_size;
     const size_t per_chunk = std::clamp<size_t>(spill_chunk_bytes / layer_bytes, 1, pool->layers);
     const size_t chunk_bytes = per_chunk * layer_bytes;
-    status = ensure_device(ctx, &pool->d_spill, &pool->d_spill_bytes, 2 * chunk_bytes,
+    status = ensure_device(pool, &pool->d_spill, &pool->d_spill_bytes, 2 * chunk_bytes,
                            "spill staging");
     if (status)
         return status;
@@ -982,11 +982,11 @@ struct device_scope {
 
 struct capture_scope {
     ckv_context* ctx;
-    explicit capture_scope(ckv_context* c)
-        : ctx(c)
+    explicit capture_scope(ckv_pool* pool)
+        : ctx(pool->ctx)
     {
         ctx->in_capture = capturing(ctx);
-        ctx->captured |= ctx->in_capture;
+        pool->captured |= ctx->in_capture;
     }
     ~capture_scope() { ctx->in_capture = false; }
 };
@@ -998,7 +998,7 @@ int guarded(ckv_pool* pool, Call&& call) noexcept
         return CKV_E_INVALID_ARGUMENT;
     try {
         const device_scope scope(pool->ctx->device);
-        const capture_scope capture(pool->ctx);
+        const capture_scope capture(pool);
         return call();
     } catch (const std::exception&) {
         pool->ctx->last_error.assign("host memory"); // within the string's reserve
@@ -1144,8 +1144,6 @@ int ckv_context_destroy(ckv_context* ctx)
             (void)host_free(ctx, slot.pinned);
         (void)hipEventDestroy(slot.done);
     }
-    for (void* buffer : ctx->retired)
-        (void)dev_free(ctx, buffer);
     (void)hipStreamDestroy(ctx->own_stream);
     delete ctx;
     return CKV_OK;
@@ -1372,6 +1370,8 @@ int ckv_pool_destroy(ckv_pool* pool)
         (void)dev_free(ctx, pool->d_axes);
     if (pool->d_spare)
         (void)dev_free(ctx, pool->d_spare);
+    for (void* buffer : pool->retired)
+        (void)dev_free(ctx, buffer);
     delete pool;
     return CKV_OK;
 }
@@ -1560,7 +1560,7 @@ int ckv_tables_upload(ckv_pool* pool, const uint32_t* block_table, size_t n_entr
     if (slots)
         put(s_slots, slots, rows);
     put(s_tiles, tiles.data(), tiles.size());
-    status = ensure_device(ctx, &pool->d_meta, &pool->d_meta_words, words, "metadata buffer");
+    status = ensure_device(pool, &pool->d_meta, &pool->d_meta_words, words, "metadata buffer");
     if (status)
         return status;
     if (with_plan)
@@ -1658,7 +1658,7 @@ int ckv_seq_tables_reserve(ckv_pool* pool, size_t max_sequences, size_t pages_pe
     const size_t words = max_sequences * pages_per_sequence;
     if (pool->device_tables)
         pool->uploaded = false; // the batch indexes the arena, which may be replaced
-    int status = ensure_device(ctx, &pool->d_seq, &pool->d_seq_words, words, "sequence tables");
+    int status = ensure_device(pool, &pool->d_seq, &pool->d_seq_words, words, "sequence tables");
     if (status)
         return status;
     // every entry starts as page 0: a valid page id, whatever a range reads
@@ -1829,7 +1829,7 @@ int ckv_batch_upload(ckv_pool* pool, const uint32_t* seq, const uint32_t* first_
     }
     if (!tiles.empty())
         std::memcpy(section(s_tiles), tiles.data(), tiles.size() * sizeof(uint32_t));
-    status = ensure_device(ctx, &pool->d_meta, &pool->d_meta_words, s_pairs + up_words,
+    status = ensure_device(pool, &pool->d_meta, &pool->d_meta_words, s_pairs + up_words,
                            "metadata buffer");
     if (status)
         return status;
@@ -2112,12 +2112,12 @@ int run_prefill(ckv_pool* pool, size_t layer, const void* queries, size_t q_head
     const prefill_shape_info plan = prefill_plan(view, m, (uint32_t)q_heads, ctx->cu_count);
     prefill_split split { nullptr, nullptr, plan.n_split, plan.min_blocks };
     if (plan.n_split > 1) {
-        int status = ensure_device(ctx, &pool->d_pre_records, &pool->d_pre_records_floats,
+        int status = ensure_device(pool, &pool->d_pre_records, &pool->d_pre_records_floats,
                                    (size_t)plan.records_floats, "prefill split records");
         if (status)
             return status;
         if (plan.counters > pool->d_pre_arrivals_words) {
-            status = ensure_device(ctx, &pool->d_pre_arrivals, &pool->d_pre_arrivals_words,
+            status = ensure_device(pool, &pool->d_pre_arrivals, &pool->d_pre_arrivals_words,
                                    (size_t)plan.counters, "prefill split counters");
             if (status)
                 return status;
@@ -2262,7 +2262,7 @@ int run_rope_append_decode(ckv_pool* pool, size_t layer, const void* keys, const
     // unfused: queries rotated into a pool buffer, keys rotated into their
     // slots, then the attention over the rotated queries
     const size_t q_bytes = rows * q_heads * pool->head_dim * pool->elem_size;
-    int status = ensure_device(ctx, &pool->d_rope_q, &pool->d_rope_q_bytes, q_bytes,
+    int status = ensure_device(pool, &pool->d_rope_q, &pool->d_rope_q_bytes, q_bytes,
                                "rotated queries");
     if (!status && ctx->in_capture) { // refused, if at all, before the append is captured
         decode_setup setup;
@@ -2497,7 +2497,7 @@ int ckv_rope_axes_upload(ckv_pool* pool, const uint32_t* positions, size_t axes,
         if (rows)
             std::memcpy(host, positions, axes * rows * sizeof(uint32_t));
         pool->axes = 0; // until the copy is on its way
-        status = ensure_device(ctx, &pool->d_axes, &pool->d_axes_words, words, "axis positions");
+        status = ensure_device(pool, &pool->d_axes, &pool->d_axes_words, words, "axis positions");
         if (!status)
             status = upload_staged(ctx, pool->d_axes, words * sizeof(uint32_t));
         if (!status)
@@ -2663,9 +2663,9 @@ int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const 
             w[s_shift + kept.size() + j] = 0;
         }
         const size_t spare_bytes = plan.saved.size() * pool->layers * 2 * view.features * pool->elem_size;
-        status = ensure_device(ctx, &pool->d_spare, &pool->d_spare_bytes, spare_bytes, "saved rows");
+        status = ensure_device(pool, &pool->d_spare, &pool->d_spare_bytes, spare_bytes, "saved rows");
         if (!status)
-            status = ensure_device(ctx, &pool->d_pairs, &pool->d_pairs_words, words, "move lists");
+            status = ensure_device(pool, &pool->d_pairs, &pool->d_pairs_words, words, "move lists");
         if (!status)
             status = fetch_staged(ctx, pool->d_pairs, words);
         if (status)

@@ -271,14 +271,9 @@ struct ckv_context {
     // this context (ckv_debug_allocations)
     uint64_t allocations = 0;
 
-    // A captured launch keeps reading what it was given whenever its graph is replayed.
-    // in_capture: a call that takes launches under capture into account runs on a stream
-    // being captured, and is refused what it would upload or allocate. captured: some
-    // such call was captured; buffers that grow from then on leave the old one to the
-    // graphs, until the context goes.
+    // A call that takes launches under capture into account runs on a stream being
+    // captured: it is refused what it would upload or allocate.
     bool in_capture = false;
-    bool captured = false;
-    std::vector<void*> retired;
 
     bool profile = false;
     std::vector<ckv::pending_timing> pending;
@@ -363,6 +358,13 @@ struct ckv_pool {
     ckv::move_marks marks; // of ckv_compact's slots
     uint8_t* d_spare = nullptr; // rows it saves
     size_t d_spare_bytes = 0;
+
+    // A captured launch keeps reading what it was given whenever its graph is replayed.
+    // captured: a call of the pool that takes launches under capture into account was
+    // made under one; buffers that grow from then on leave the old one to the graphs,
+    // until the pool goes.
+    bool captured = false;
+    std::vector<void*> retired;
 
     // device scratch
     float* d_partials = nullptr;
