@@ -298,6 +298,8 @@ int check_attention(const ckv_pool* pool, size_t layer, const void* queries, siz
         return set_error(ctx, CKV_E_INVALID_KV_HEAD_MAPPING, "q_heads % kv_heads != 0");
     if (layer >= pool->layers)
         return set_error(ctx, CKV_E_CACHE_LAYER_OUT_OF_RANGE, "layer >= layers");
+    if (q_heads > UINT32_MAX / pool->head_dim)
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "row too wide");
     return CKV_OK;
 }
 
@@ -1937,7 +1939,7 @@ int check_rope(ckv_pool* pool, size_t heads, float theta, size_t rotary_dim,
                          "rotary_dim must be at most " + std::to_string(2 * ckv::max_rope_pairs));
     if (!std::isfinite(theta) || theta <= 0.0f)
         return set_error(ctx, CKV_E_INVALID_ROPE_THETA, "theta must be positive and finite");
-    if ((uint64_t)heads * head_dim > UINT32_MAX)
+    if (heads > UINT32_MAX / head_dim)
         return set_error(ctx, CKV_E_INVALID_ARGUMENT, "row too wide");
     rotary = (uint32_t)rotary_dim;
     ckv::rope_frequencies(theta, rotary, freq);
@@ -2340,6 +2342,8 @@ int ckv_append_decode_noalloc(ckv_pool* pool, size_t layer, const void* keys, co
         return fail_fixed(ctx, CKV_E_INVALID_KV_HEAD_MAPPING, "q_heads % kv_heads != 0");
     if (layer >= pool->layers)
         return fail_fixed(ctx, CKV_E_CACHE_LAYER_OUT_OF_RANGE, "layer >= layers");
+    if (q_heads > UINT32_MAX / pool->head_dim)
+        return fail_fixed(ctx, CKV_E_INVALID_ARGUMENT, "row too wide");
     if (!rows)
         return CKV_OK;
     // what only this entry point requires
@@ -2525,7 +2529,7 @@ int check_rope_axes(ckv_pool* pool, size_t heads, float theta, size_t rotary_dim
                              + std::to_string(2 * ckv::max_turn_pairs));
     if (!std::isfinite(theta) || theta <= 0.0f)
         return set_error(ctx, CKV_E_INVALID_ROPE_THETA, "theta must be positive and finite");
-    if ((uint64_t)heads * head_dim > UINT32_MAX)
+    if (heads > UINT32_MAX / head_dim)
         return set_error(ctx, CKV_E_INVALID_ARGUMENT, "row too wide");
     if (!pair_axis)
         return set_error(ctx, CKV_E_INVALID_ARGUMENT, "pair_axis is required");
@@ -2586,8 +2590,9 @@ int ckv_rope_axes_append(ckv_pool* pool, size_t layer, const void* queries, void
             return set_error(ctx, CKV_E_UNSUPPORTED_ALIASING, "rotated overlaps keys or values");
         ckv::axis_table axes;
         uint32_t rotary = 0;
-        status = check_rope_axes(pool, q_heads + pool->kv_heads, theta, rotary_dim, pair_axis,
-                                 axes, rotary);
+        // (the sum past the largest count is one of a row too wide)
+        const size_t heads = std::min(q_heads, SIZE_MAX - pool->kv_heads) + pool->kv_heads;
+        status = check_rope_axes(pool, heads, theta, rotary_dim, pair_axis, axes, rotary);
         if (status)
             return status;
         const pool_view view = view_of(pool);

@@ -287,7 +287,8 @@ int ckv_gather(ckv_pool* pool, size_t layer, size_t table_offset, size_t table_l
  * paged_attention_partial_f32 / paged_attention_reduce_f32
  * (src/metal/kernels/attention.metal:446-615), generalised to every row.
  * Checks: invalid_head_count, invalid_kv_head_mapping (q_heads % kv_heads),
- * cache_layer_out_of_range, position_count_mismatch (rows != uploaded rows). */
+ * cache_layer_out_of_range, position_count_mismatch (rows != uploaded rows),
+ * invalid_argument (a null array, rows of 2^32 elements or more). */
 int ckv_decode_attention(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads,
                          float scale, void* output, size_t rows);
 /* store_kv followed by the decode form, in one launch where possible: the

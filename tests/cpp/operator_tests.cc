@@ -362,4 +362,39 @@ TEST("entry points: what is refused")
     CHECK(attend(0, nullptr, 4, 8, nullptr, nullptr, 0) == CKV_OK);
 }
 
+// Head counts whose rows pass 32 bits, or that wrap once kv heads are added, reach no launch.
+TEST("entry points: rows too wide for 32 bits are refused")
+{
+    ckv_context ctx;
+    ckv_pool pool;
+    pool.ctx = &ctx;
+    pool.layers = 1;
+    pool.blocks = 8;
+    pool.block_size = 16;
+    pool.kv_heads = 2;
+    pool.head_dim = 128;
+    pool.uploaded = pool.has_slots = true;
+    pool.positions = { 40, 50 };
+    pool.last_position = 50;
+    pool.slot_rows = 2;
+    pool.axes = 1;
+    int x[4]; // never read
+    const uint8_t axis[64] = {};
+    for (const size_t heads : { (size_t)1 << 25, (size_t)1 << 32, (size_t)1 << 57, ((size_t)1 << 57) + 2,
+                                SIZE_MAX - 1, SIZE_MAX - 3 }) {
+        CHECK(ckv_rope_axes(&pool, x, x + 1, heads, 1e4f, 0, axis, 2) == CKV_E_INVALID_ARGUMENT);
+        CHECK(ckv_rope_axes_append(&pool, 0, x, x, heads, x + 1, x + 2, 1e4f, 0, axis, 2)
+              == CKV_E_INVALID_ARGUMENT);
+        CHECK(ckv_rope(&pool, x, x + 1, heads, 1e4f, 0, 2) == CKV_E_INVALID_ARGUMENT);
+        CHECK(ckv_attention_window(&pool, 0, x, heads, 1.0f, 8, 0, nullptr, x + 1, 2)
+              == CKV_E_INVALID_ARGUMENT);
+        CHECK(ckv_append_decode_window(&pool, 0, x, x + 1, x + 2, heads, 1.0f, 8, 0, nullptr, x + 3, 2)
+              == CKV_E_INVALID_ARGUMENT);
+        CHECK(ckv_attention(&pool, 0, x, heads, 1.0f, x + 1, 2) == CKV_E_INVALID_ARGUMENT);
+        CHECK(ckv_append_decode(&pool, 0, x, x + 1, x + 2, heads, 1.0f, x + 3, 2) == CKV_E_INVALID_ARGUMENT);
+        CHECK(ckv_append_decode_noalloc(&pool, 0, x, x + 1, x + 2, heads, 1.0f, x + 3, 2)
+              == CKV_E_INVALID_ARGUMENT);
+    }
+}
+
 } // namespace
