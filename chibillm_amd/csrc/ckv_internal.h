@@ -556,6 +556,10 @@ struct axes_rows {
     const void* keys;
     const void* values;
 };
+// Heads of a row that a thread of the launch takes in 16-byte words: four, unless that
+// leaves fewer than two workgroups per compute unit; 0: the rows go pair by pair.
+uint32_t rope_axes_heads(const pool_view& p, const axes_rows& x, uint32_t rows, uint32_t heads,
+                         uint32_t rotary);
 hipError_t launch_rope_axes(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
                             const axes_rows& x, uint32_t rows, uint32_t q_heads, uint32_t rotary,
                             const turn_table& turns, const axis_table& axes,
@@ -602,6 +606,10 @@ const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* fro
 // Words (an even number, both arrays aligned to 8 bytes) from pinned host memory, read
 // by a kernel: between two kernels a copy of 120 KB takes 14 us on MI355X, of 16 KB 5.
 hipError_t launch_fetch(hipStream_t s, uint32_t* to, const void* pinned, size_t words);
+// The kv heads that a workgroup of the compaction in 16-byte words goes through: all of
+// them, unless that leaves fewer workgroups than keep the memory busy; 0: the geometry is
+// moved an element at a time.
+uint32_t compact_heads(const pool_view& p, uint32_t layers, uint32_t n_runs, uint32_t rotary);
 hipError_t launch_compact(hipStream_t s, const pool_view& p, uint32_t layers,
                           const compact_moves& moves, uint32_t rotary, const turn_table& turns);
 

@@ -383,25 +383,31 @@ const char* plan_compaction(move_marks& marks, size_t slots, const uint32_t* fro
     return nullptr;
 }
 
+uint32_t compact_heads(const pool_view& p, uint32_t layers, uint32_t n_runs, uint32_t rotary)
+{
+    const uint32_t each = 16 / p.elem_size;
+    const auto aligned = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
+    if (p.head_dim % (2 * each) || rotary % (2 * each) || p.head_dim / (2 * each) > block_threads
+        || !aligned(p.keys) || !aligned(p.values))
+        return 0;
+    uint32_t heads = p.kv_heads;
+    while (heads % 2 == 0 && (uint64_t)n_runs * layers * 2 * (p.kv_heads / heads) < 2048)
+        heads /= 2;
+    return heads;
+}
+
 hipError_t launch_compact(hipStream_t s, const pool_view& p, uint32_t layers,
                           const compact_moves& moves, uint32_t rotary, const turn_table& turns)
 {
     if (!moves.n_runs)
         return hipSuccess;
-    const uint32_t each = 16 / p.elem_size;
-    const auto aligned = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
-    const bool words = p.head_dim % (2 * each) == 0 && rotary % (2 * each) == 0
-        && p.head_dim / (2 * each) <= block_threads && aligned(p.keys) && aligned(p.values);
-    // heads a workgroup goes through: all of them, unless that leaves fewer workgroups
-    // than keep the memory busy
-    uint32_t heads = words ? p.kv_heads : 1;
-    while (heads % 2 == 0 && (uint64_t)moves.n_runs * layers * 2 * (p.kv_heads / heads) < 2048)
-        heads /= 2;
+    const uint32_t in_words = compact_heads(p, layers, moves.n_runs, rotary);
+    const uint32_t heads = std::max(in_words, 1u);
     const uint64_t blocks = (uint64_t)moves.n_runs * (p.kv_heads / heads);
     if (blocks > 0x7FFFFFFFull || layers > 65535)
         return hipErrorInvalidValue;
     const dim3 grid((uint32_t)blocks, layers, 2);
-    if (words) {
+    if (in_words) {
         auto* kernel = p.dtype == CKV_F32 ? compact_rows_kernel<CKV_F32>
             : p.dtype == CKV_BF16         ? compact_rows_kernel<CKV_BF16>
                                           : compact_rows_kernel<CKV_F16>;

@@ -60,7 +60,7 @@ __global__ __launch_bounds__(block_threads) void rope_axes_words_kernel(
         a[i].v = *reinterpret_cast<const uint4*>(src);
         b[i].v = *reinterpret_cast<const uint4*>(src + apart);
     }
-    const uint64_t slot_row = head0 + PER > q_heads
+    const uint64_t slot_row = heads > q_heads && head0 + PER > q_heads // rotated alone, rows have no slots
         ? layer * p.layer_elems + (uint64_t)slots[row] * p.features
         : 0;
     float c[each], s[each];
@@ -163,6 +163,19 @@ void turn_steps(float theta, uint32_t rotary, turn_table& out)
     }
 }
 
+uint32_t rope_axes_heads(const pool_view& p, const axes_rows& x, uint32_t rows, uint32_t heads,
+                         uint32_t rotary)
+{
+    const uint32_t each = 16 / p.elem_size;
+    const auto aligned = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
+    if (p.head_dim % (2 * each) || rotary % (2 * each) || !aligned(x.queries) || !aligned(x.rotated)
+        || !aligned(x.keys) || !aligned(x.values)
+        || (x.keys && (!aligned(p.keys) || !aligned(p.values))))
+        return 0;
+    const uint64_t words = (uint64_t)rows * (p.head_dim / (2 * each)); // of a head's halves
+    return words * heads / 4 >= 512 * block_threads ? 4 : 1;
+}
+
 hipError_t launch_rope_axes(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
                             const axes_rows& x, uint32_t rows, uint32_t q_heads, uint32_t rotary,
                             const turn_table& turns, const axis_table& axes,
@@ -171,14 +184,9 @@ hipError_t launch_rope_axes(hipStream_t s, const pool_view& p, const meta_view& 
     const uint32_t heads = q_heads + (x.keys ? p.kv_heads : 0);
     if (!rows || !heads)
         return hipSuccess;
-    const uint32_t each = 16 / p.elem_size;
-    const auto aligned = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
-    if (p.head_dim % (2 * each) == 0 && rotary % (2 * each) == 0 && aligned(x.queries)
-        && aligned(x.rotated) && aligned(x.keys) && aligned(x.values)
-        && (!x.keys || (aligned(p.keys) && aligned(p.values)))) {
-        const uint64_t words = (uint64_t)rows * (p.head_dim / (2 * each)); // of a head's halves
-        // four heads a thread, unless that leaves fewer than two workgroups per compute unit
-        const bool four = words * heads / 4 >= 512 * block_threads;
+    if (const uint32_t per = rope_axes_heads(p, x, rows, heads, rotary)) {
+        const uint64_t words = (uint64_t)rows * (p.head_dim / (32 / p.elem_size)); // of a head's halves
+        const bool four = per == 4;
         const uint64_t parts = four ? (heads + 3) / 4 : heads;
         const uint64_t blocks = (words * parts + block_threads - 1) / block_threads;
         if (blocks > 0x7FFFFFFFull)

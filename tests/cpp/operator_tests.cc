@@ -397,4 +397,42 @@ TEST("entry points: rows too wide for 32 bits are refused")
     }
 }
 
+// The forms that the device tests of large batches mean to reach, at their sizes
+// (tests/test_gpu_operators_large.py).
+TEST("launch forms: heads a workgroup of a compaction and a thread of a rotation take")
+{
+    auto pool = [](int dtype, uint32_t kv_heads, uint32_t head_dim) {
+        pool_view p {};
+        p.dtype = dtype;
+        p.elem_size = dtype == CKV_F32 ? 4 : 2;
+        p.kv_heads = kv_heads;
+        p.head_dim = head_dim;
+        p.features = kv_heads * head_dim;
+        return p;
+    };
+    auto runs = [](uint32_t moves) { return (moves + compact_run - 1) / compact_run; };
+    CHECK(compact_heads(pool(CKV_BF16, 8, 64), 12, runs(6000), 64) == 8);
+    CHECK(compact_heads(pool(CKV_BF16, 8, 64), 12, runs(3500), 64) == 4);
+    CHECK(compact_heads(pool(CKV_F32, 8, 64), 12, runs(1800), 32) == 2);
+    CHECK(compact_heads(pool(CKV_F16, 8, 64), 12, runs(1000), 0) == 1);
+    CHECK(compact_heads(pool(CKV_F32, 4, 128), 16, runs(4200), 128) == 4);
+    CHECK(compact_heads(pool(CKV_F16, 3, 256), 2, runs(900), 64) == 3); // an odd number never halves
+    CHECK(compact_heads(pool(CKV_F16, 6, 256), 2, runs(900), 64) == 3);
+    CHECK(compact_heads(pool(CKV_F32, 3, 33), 12, runs(6000), 0) == 0);
+    CHECK(compact_heads(pool(CKV_BF16, 8, 64), 12, runs(6000), 24) == 0);
+    pool_view odd = pool(CKV_BF16, 8, 64);
+    odd.values = reinterpret_cast<void*>(8);
+    CHECK(compact_heads(odd, 12, runs(6000), 64) == 0);
+    const axes_rows x {};
+    CHECK(rope_axes_heads(pool(CKV_BF16, 8, 128), x, 4200, 16, 128) == 4);
+    CHECK(rope_axes_heads(pool(CKV_BF16, 7, 128), x, 4700, 14, 48) == 4);
+    CHECK(rope_axes_heads(pool(CKV_F16, 3, 256), x, 5500, 6, 64) == 4);
+    CHECK(rope_axes_heads(pool(CKV_F32, 5, 64), x, 13200, 5, 64) == 4);
+    CHECK(rope_axes_heads(pool(CKV_BF16, 8, 128), x, 4000, 16, 128) == 1);
+    CHECK(rope_axes_heads(pool(CKV_BF16, 8, 128), x, 4200, 16, 24) == 0);
+    axes_rows unaligned {};
+    unaligned.rotated = reinterpret_cast<void*>(2);
+    CHECK(rope_axes_heads(pool(CKV_BF16, 8, 128), unaligned, 4200, 16, 128) == 0);
+}
+
 } // namespace
