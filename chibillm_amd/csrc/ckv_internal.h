@@ -493,6 +493,9 @@ hipError_t launch_window_fast(hipStream_t s, const pool_view& p, const meta_view
                               void* out, const void* k_in, const void* v_in, const void* gate,
                               int cu_count, split_scratch split, const rope_table* rope,
                               uint32_t rotary);
+// Waves per workgroup of the fast decode through a window (decode_fast_waves's arguments).
+uint32_t decode_window_waves(uint32_t head_dim, uint32_t group, int dtype, uint32_t units,
+                             int cu_count, uint32_t mean_pages, uint32_t split_pages);
 // Sets every entry of a plan written from the window's positions to its row's position.
 void place_window_plan(const std::vector<uint32_t>& positions, const decode_plan_shape& shape,
                        uint32_t* plan);

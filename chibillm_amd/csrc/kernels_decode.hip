@@ -554,8 +554,9 @@ constexpr uint64_t window_half_pages = 33, window_half_pages_wide = 17;
 // Small batches of 128-wide 16-bit rows are cut into pieces of an eighth of the longest
 // row, 4 to 12 pages, where all others are of at least 12: us at 12 and now (8 kv heads,
 // bf16), 4 rows behind 512 tokens 7.0 and 6.4, 1 behind 256 6.8 and 6.0, 8 behind 256 6.6
-// and 6.1. Rows of up to 16 pages stay whole (16 behind 128, 6.1 and 6.5 in halves).
-constexpr uint64_t window_whole_pages = 16;
+// and 6.1. Where the longest row has up to 16 pages, pieces stay at 12 or more (16 rows
+// behind 128, whole 6.1 and in halves 6.5).
+constexpr uint64_t window_long_pages = 16;
 
 decode_form window_form_of(int dtype, uint32_t head_dim)
 {
@@ -573,7 +574,7 @@ decode_plan_shape shape_window_plan(const std::vector<uint32_t>& positions, uint
 {
     uint64_t total, longest;
     batch_pages(positions, block_size, total, longest);
-    if (form.min_pages == form_narrow.min_pages && longest > window_whole_pages)
+    if (form.min_pages == form_narrow.min_pages && longest > window_long_pages)
         form.min_pages = (uint32_t)std::clamp<uint64_t>(longest / 8, 4, form_narrow.min_pages);
     const uint64_t rows = positions.size(), cus = (uint64_t)std::max(cu_count, 1);
     const bool even = 8 * total >= 7 * longest * rows;

@@ -10,6 +10,12 @@
 
 namespace ckv {
 
+uint32_t decode_window_waves(uint32_t head_dim, uint32_t group, int dtype, uint32_t units,
+                             int cu_count, uint32_t mean_pages, uint32_t split_pages)
+{
+    return window_waves(head_dim, group, dtype, units, cu_count, mean_pages, split_pages);
+}
+
 hipError_t launch_window_fast(hipStream_t s, const pool_view& p, const meta_view& m,
                               uint32_t layer, const void* q, uint32_t q_heads, float scale_log2,
                               void* out, const void* k_in, const void* v_in, const void* gate,

@@ -4,6 +4,7 @@
 // a GPU: every call here ends in its checks).
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <random>
 
 #include "check.h"
@@ -433,6 +434,158 @@ TEST("launch forms: heads a workgroup of a compaction and a thread of a rotation
     axes_rows unaligned {};
     unaligned.rotated = reinterpret_cast<void*>(2);
     CHECK(rope_axes_heads(pool(CKV_BF16, 8, 128), unaligned, 4200, 16, 128) == 0);
+}
+
+constexpr uint32_t page = 16;
+
+// The plan of rows at `positions` behind a window, its structure checked: a row's chunks
+// cover the pages that hold a key it attends, each once and in order, with the row's own
+// position, its records behind one another, and workgroups linked through every entry.
+decode_plan_shape window_plan_of(const std::vector<uint32_t>& positions, key_window w, uint32_t kv_heads,
+                                 int cus, int dtype, uint32_t head_dim)
+{
+    const size_t rows = positions.size();
+    std::vector<uint32_t> left(rows), offsets(rows);
+    for (size_t r = 0, at = 0; r < rows; at += positions[r] / page + 1, ++r) {
+        left[r] = positions[r] - window_gap_of(window_low(positions[r], w), w.sinks, page).skip * page;
+        offsets[r] = (uint32_t)at;
+    }
+    const decode_plan_shape s = shape_window_plan(left, page, kv_heads, cus, window_form_of(dtype, head_dim));
+    std::vector<uint32_t> plan(plan_entry_words * s.n_items, 0xDEADBEEFu), first(rows, 0xDEADBEEFu),
+        cut(s.n_cut, 0xDEADBEEFu);
+    std::vector<uint64_t> scratch;
+    write_decode_plan(left, offsets, page, s, scratch, plan.data(), first.data(), cut.data());
+    place_window_plan(positions, s, plan.data());
+    REQUIRE(s.n_wgs >= 1 && s.n_wgs <= s.n_items);
+    std::vector<int> reached(s.n_items, 0);
+    struct piece {
+        uint32_t chunk, first, end, of;
+    };
+    std::vector<std::vector<piece>> pieces(rows);
+    for (uint32_t wg = 0; wg < s.n_wgs; ++wg)
+        for (uint32_t at = wg; at != plan_last;) {
+            REQUIRE(at < s.n_items && !reached[at]++);
+            const uint32_t* e = &plan[plan_entry_words * at];
+            REQUIRE(e[0] < rows);
+            CHECK(e[2] == positions[e[0]] && e[3] == offsets[e[0]] + e[4]);
+            pieces[e[0]].push_back({ e[1], e[4], e[5], e[6] });
+            at = e[7];
+        }
+    CHECK(std::count(reached.begin(), reached.end(), 1) == (std::ptrdiff_t)s.n_items);
+    uint32_t records = 0, cuts = 0;
+    std::vector<int> taken(s.n_records, 0);
+    for (size_t r = 0; r < rows; ++r) {
+        auto& of = pieces[r];
+        std::sort(of.begin(), of.end(), [](const piece& a, const piece& b) { return a.chunk < b.chunk; });
+        const window_gap gap = window_gap_of(window_low(positions[r], w), w.sinks, page);
+        std::vector<uint32_t> read;
+        uint32_t at = 0;
+        for (size_t c = 0; c < of.size(); ++c) {
+            REQUIRE(of[c].chunk == c && of[c].of == of.size() && of[c].first == at && of[c].end > at);
+            at = of[c].end;
+            for (uint32_t u = of[c].first; u < of[c].end; ++u)
+                read.push_back(u < gap.kept ? u : u + gap.skip);
+        }
+        std::vector<uint32_t> want;
+        for (uint32_t u = 0; u <= positions[r] / page; ++u) {
+            bool some = false;
+            for (uint32_t t = u * page; t < (u + 1) * page; ++t)
+                some = some || attends(positions[r], t, w);
+            if (some)
+                want.push_back(u);
+        }
+        CHECK(read == want);
+        if (of.size() > 1) {
+            ++cuts;
+            records += (uint32_t)of.size();
+            for (size_t c = 0; c < of.size(); ++c) {
+                REQUIRE(first[r] + c < s.n_records);
+                CHECK(!taken[first[r] + c]++);
+            }
+            CHECK(std::count(cut.begin(), cut.end(), (uint32_t)r) == 1);
+        }
+    }
+    CHECK(records == s.n_records && cuts == s.n_cut);
+    return s;
+}
+
+TEST("window plan: every row's attended pages once, at any size")
+{
+    std::mt19937_64 rng(11);
+    for (int trial = 0; trial < 600; ++trial) {
+        const uint32_t kv_heads = 1u << rng() % 4, rows = 1 + rng() % (trial % 5 ? 40 : 200);
+        const int cus = trial % 3 ? 256 : 1 + (int)(rng() % 300);
+        const key_window w { 1 + (uint32_t)(rng() % (trial % 2 ? 2100 : 90)), (uint32_t)(rng() % 3 * (rng() % 70)) };
+        const uint32_t high = 40 + rng() % 5000;
+        std::vector<uint32_t> positions(rows);
+        for (auto& p : positions)
+            p = rng() % high;
+        const int dtype = (int)(rng() % 3);
+        window_plan_of(positions, w, kv_heads, cus, dtype, rng() % 2 ? 128 : 256);
+    }
+}
+
+TEST("window plan: halves of rows of equal length, from one to one and a half units per compute unit")
+{
+    const key_window w { 1024, 4 };
+    auto rows = [](size_t n) {
+        std::vector<uint32_t> p(n);
+        for (size_t r = 0; r < n; ++r)
+            p[r] = 1500 + 211 * (uint32_t)r % 9000;
+        return p;
+    };
+    for (const size_t n : { 33u, 40u, 48u }) { // 8 kv heads: 264 to 384 units
+        const decode_plan_shape s = window_plan_of(rows(n), w, 8, 256, CKV_BF16, 128);
+        CHECK(s.n_cut == n && s.n_records == 2 * n && (s.split_pages == 33 || s.split_pages == 34));
+    }
+    // one unit per compute unit or fewer is cut as any small batch is, more than one and a half stay whole
+    CHECK(window_plan_of(rows(49), w, 8, 256, CKV_BF16, 128).n_cut == 0);
+    CHECK(window_plan_of(rows(64), w, 8, 256, CKV_BF16, 128).n_cut == 0);
+    CHECK(window_plan_of(rows(80), w, 8, 256, CKV_F16, 128).n_cut == 0);
+    CHECK(window_plan_of(rows(32), w, 8, 256, CKV_BF16, 128).n_records != 64);
+    // 32 pages behind 512 tokens are too few to halve, 256-wide rows of 17 are not
+    CHECK(window_plan_of(rows(40), { 490, 0 }, 8, 256, CKV_BF16, 128).n_records == 0);
+    CHECK(window_plan_of(rows(40), { 272, 4 }, 8, 256, CKV_BF16, 256).n_records == 80);
+    CHECK(window_plan_of(rows(40), w, 8, 256, CKV_F32, 128).n_records != 80);
+    // rows of unequal length are not halved
+    std::vector<uint32_t> uneven = rows(40);
+    for (size_t r = 0; r < 20; ++r)
+        uneven[r] = 100;
+    CHECK(window_plan_of(uneven, w, 8, 256, CKV_BF16, 128).n_records != 80);
+}
+
+TEST("window plan: pieces of small batches, an eighth of the longest row")
+{
+    auto pieces = [](size_t n, uint32_t window, int dtype, uint32_t head_dim) {
+        return window_plan_of(std::vector<uint32_t>(n, 4000), { window, 0 }, 8, 256, dtype, head_dim).split_pages;
+    };
+    CHECK(pieces(4, 512, CKV_BF16, 128) == 4 || pieces(4, 512, CKV_BF16, 128) == 5);
+    CHECK(pieces(1, 256, CKV_BF16, 128) == 4); // 17 pages
+    CHECK(pieces(1, 241, CKV_BF16, 128) == 12); // 16: the pieces of a batch without a window
+    CHECK(window_plan_of({ 4000 }, { 177, 0 }, 8, 256, CKV_BF16, 128).n_records == 0); // 12 stay whole
+    CHECK(pieces(2, 2000, CKV_BF16, 128) >= 12);
+    CHECK(pieces(3, 300, CKV_F32, 128) >= 4 && pieces(3, 300, CKV_F32, 128) < 8);
+}
+
+TEST("window decode: waves of a workgroup")
+{
+    if (std::getenv("CKV_DECODE_WAVES"))
+        return;
+    auto waves = [](uint32_t head_dim, uint32_t group, int dtype, uint32_t units, uint32_t split) {
+        return decode_window_waves(head_dim, group, dtype, units, 256, 65, split);
+    };
+    CHECK(waves(128, 2, CKV_F32, 400, 0) == 4);
+    CHECK(waves(128, 2, CKV_BF16, 40, 4) == 4);    // pieces of four pages
+    CHECK(waves(128, 2, CKV_BF16, 200, 0) == 16);  // a workgroup to a compute unit and to spare
+    CHECK(waves(128, 4, CKV_BF16, 200, 0) == 8);
+    CHECK(waves(128, 2, CKV_BF16, 768, 33) == 4);  // halves of 48 rows
+    CHECK(waves(128, 8, CKV_BF16, 768, 33) == 8);
+    CHECK(waves(128, 2, CKV_BF16, 400, 0) == 8);   // whole rows, one to two units per compute unit
+    CHECK(waves(128, 2, CKV_BF16, 640, 0) == 4);   // more
+    CHECK(waves(128, 4, CKV_BF16, 640, 0) == 4);
+    CHECK(waves(128, 8, CKV_BF16, 512, 0) == 4);
+    CHECK(waves(128, 8, CKV_BF16, 640, 0) == 8);
+    CHECK(waves(256, 4, CKV_BF16, 640, 0) == 8);
 }
 
 } // namespace
