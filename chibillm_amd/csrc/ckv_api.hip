@@ -677,7 +677,7 @@ int ensure_window_tiles(ckv_pool* pool, window_batch& b)
     status = upload_staged(ctx, b.d_tiles, words * sizeof(uint32_t));
     b.meta.tiles = b.d_tiles;
     b.meta.n_tiles = (uint32_t)parts.size();
-    b.meta.tile_blocks = parts.empty() ? 0 : parts.front().first;
+    b.meta.longest_blocks = parts.empty() ? 0 : parts.front().first;
     b.tiles_ready = status == CKV_OK;
     return status;
 }

@@ -84,8 +84,7 @@ struct meta_view {
     uint32_t n_items;
     uint32_t chunk; // tokens per decode work item, a multiple of 16
     uint32_t n_tiles;
-    uint32_t tile_blocks; // 32-key blocks the batch's shortest query tile attends (host side);
-                          // behind a window those of its longest
+    uint32_t tile_blocks; // 32-key blocks the batch's shortest query tile attends (host side)
     uint32_t row_blocks[3]; // runs of 32, 64 and 128 rows the tiles fall into (host side)
     uint32_t mean_pages; // pages attended per row, mean over the batch (host side)
     uint32_t n_plan;      // workgroups per kv head of the fast decode (the entries they start at)
@@ -94,6 +93,7 @@ struct meta_view {
     uint32_t n_records;   // partial records of the rows cut into chunks
     uint32_t n_cut;       // rows cut into chunks
     key_window window = all_keys;
+    uint32_t longest_blocks; // 32-key blocks the longest of a window's tiles attends (host side)
 };
 
 // Device scratch of the fast decode's cut rows: a partial record
@@ -139,7 +139,8 @@ __host__ __device__ inline uint32_t prefill_range_count(uint32_t n_blocks, uint3
 }
 
 // The key blocks [begin, end) of range `part` of n ranges. Range 0 starts at
-// block 0, so every query of the tile attends some key of it. 32-bit:
+// block 0, of which every query attends some key where there is no window; through
+// one it may attend none there, but itself in some range. 32-bit:
 // n_blocks < 2^27 (positions are 32-bit) and part < split_max.
 __host__ __device__ inline void prefill_range_bounds(uint32_t n_blocks, uint32_t n, uint32_t part,
                                                      uint32_t& begin, uint32_t& end)

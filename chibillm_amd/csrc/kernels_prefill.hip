@@ -722,7 +722,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
                     o[j / 4][4 * (j % 4) + e] = acc + __uint_as_float(vb[j][e]) * wb;
                 }
         }
-        // lt > 0 for a valid row: the tile's first share attends key 0
+        // lt > 0 for a valid row: some share holds the row's own key
     }
 
     const float inv = 1.0f / lt;
@@ -902,11 +902,11 @@ prefill_shape_info window_plan(const pool_view& p, const meta_view& m, uint32_t 
     const uint64_t floats = grid * 128 * (p.head_dim + 4); // of a range's records, within 128 MiB in all
     double best = 0.0;
     for (uint32_t n = 1; n <= split_max; ++n) {
-        if (n > 1 && (grid >= cus || prefill_range_count(m.tile_blocks, n, plan.min_blocks) < n
+        if (n > 1 && (grid >= cus || prefill_range_count(m.longest_blocks, n, plan.min_blocks) < n
                       || floats * n > ((uint64_t)128 << 20) / sizeof(float)))
             break;
         const double more = (double)((grid * n + cus - 1) / cus) - 1.0;
-        const double us = (1.0 + more * cost.shared) * m.tile_blocks / n * cost.block
+        const double us = (1.0 + more * cost.shared) * m.longest_blocks / n * cost.block
             + (n > 1 ? cost.base + n * (cost.range + grid * cost.record) : 0.0);
         if (n == 1 || us < best) {
             best = us;

@@ -370,7 +370,7 @@ __global__ __launch_bounds__(64 * waves, 2) void prefill_f32_kernel(
                     o[a][r] = acc + __uint_as_float(vb[r][a]) * wb;
                 }
         }
-        // lt > 0 for a valid row: the tile's first range attends key 0
+        // lt > 0 for a valid row: some range holds the row's own key
     }
 
     const float inv = 1.0f / lt;
