@@ -373,19 +373,21 @@ int ckv_sigmoid_mul(ckv_context* ctx, int dtype, const void* gate, const void* i
  * layer reads of them. A row at position p attends key t when t <= p and
  * (t > p - window or t < sinks): the last `window` tokens, itself among them,
  * and the sequence's first `sinks`. output = softmax(q . k * scale) . v over
- * those, with fp32 accumulation; where the matrix cores multiply probabilities and 16-bit
- * values, probabilities keep at least 16 bits (256-wide heads: all 24). window must be at least 1 (invalid_argument);
- * any larger value, and any sinks from 0 on, are taken.
+ * those, with fp32 accumulation; where the matrix cores multiply probabilities and
+ * 16-bit values, probabilities keep at least 16 bits (256-wide heads: all 24).
+ * window must be at least 1 (invalid_argument); any larger value, and any sinks from
+ * 0 on, are taken.
  * Pages that hold no key a row attends are not read, whatever is in them: a
- * sequence may give them back, as long as its table keeps some page id of the
- * pool in their place. Keys outside the window in pages that are read weigh
+ * caller may give them back, as long as the sequence's table keeps some page id of
+ * the pool in their place. Keys outside the window in pages that are read weigh
  * nothing, whatever their values.
  * The first call of a window on a batch makes its work lists (one small upload);
  * later ones, of any layer, reuse them. A call on a stream under capture is refused
  * (invalid_argument), before anything is captured, when it would upload or
  * allocate: make it once on the batch before the capture. A captured call holds for
- * the batch it was captured on, whatever other calls follow it there; replays of one
- * pool's calls run one after another, as its calls do (they share its scratch).
+ * the batch it was captured on (and no longer than its pool), whatever other calls
+ * follow it there; replays of one pool's calls run one after another, as its calls do
+ * (they share its scratch).
  * gate may be NULL; otherwise as ckv_attention_gated's, and it must not be the
  * queries' or the output's memory (unsupported_aliasing). */
 
