@@ -152,7 +152,8 @@ hip_model_state::begin_batch(const model_batch& batch)
             const auto at = next_.find(item.id);
             if (at == next_.end())
                 continue;
-            if (at->second == no_position || batch.positions[item.token_offset] != at->second)
+            if (at->second == no_position || item.token_offset >= batch.positions.size()
+                || batch.positions[item.token_offset] != at->second)
                 return fail(state_errc::invalid_reservation);
             begun_.emplace_back(item.id, at->second + item.token_count);
         }
