@@ -155,6 +155,20 @@ def _u32(a) -> Optional[np.ndarray]:
     return np.ascontiguousarray(np.asarray(a), dtype=np.uint32)
 
 
+def _exact(a, dtype) -> np.ndarray:
+    """a as a contiguous array of `dtype`; ValueError where its numbers are others there."""
+    x = np.asarray(a)
+    y = np.ascontiguousarray(x, dtype=dtype)
+    if x.dtype != y.dtype and not np.array_equal(x, y):
+        raise ValueError(f"numbers outside {y.dtype}")
+    return y
+
+
+def _window(window: int, sinks: int) -> None:
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks are counts of tokens")
+
+
 def _p(a: Optional[np.ndarray]):
     return None if a is None else a.ctypes.data_as(_u32p)
 
@@ -412,6 +426,7 @@ class Pool:
         """Attention to the last `window` tokens and the first `sinks`
         (* sigmoid(gate)) (ckv_attention_window)."""
         rows = queries.shape[0] if rows is None else rows
+        _window(window, sinks)
         self.ctx.check(load().ckv_attention_window(self.handle, layer, _ptr(queries), q_heads,
                                                    scale, window, sinks, _ptr(gate), _ptr(output),
                                                    rows))
@@ -420,6 +435,7 @@ class Pool:
                              output, sinks: int = 0, gate=None, rows=None) -> None:
         """append, then attention_window of decode rows (ckv_append_decode_window)."""
         rows = queries.shape[0] if rows is None else rows
+        _window(window, sinks)
         self.ctx.check(load().ckv_append_decode_window(
             self.handle, layer, _ptr(keys), _ptr(values), _ptr(queries), q_heads, scale, window,
             sinks, _ptr(gate), _ptr(output), rows))
@@ -430,19 +446,20 @@ class Pool:
         """append_decode_window from unrotated queries and keys
         (ckv_rope_append_decode_window)."""
         rows = queries.shape[0] if rows is None else rows
+        _window(window, sinks)
         self.ctx.check(load().ckv_rope_append_decode_window(
             self.handle, layer, _ptr(keys), _ptr(values), _ptr(queries), q_heads, scale, theta,
             rotary_dim, window, sinks, _ptr(gate), _ptr(output), rows))
 
     def upload_axes(self, positions) -> None:
         """The batch's positions on several axes, [axes, rows] (ckv_rope_axes_upload)."""
-        p = _u32(positions)
+        p = _exact(positions, np.uint32)
         if p.ndim != 2:
             raise ValueError("positions are [axes, rows]")
         self.ctx.check(load().ckv_rope_axes_upload(self.handle, _p(p), p.shape[0], p.shape[1]))
 
     def _pair_axis(self, pair_axis, rotary_dim: int) -> bytes:
-        axes = np.asarray(pair_axis).astype(np.uint8).tobytes()
+        axes = _exact(pair_axis, np.uint8).tobytes()
         if len(axes) != (rotary_dim or self.geometry[4]) // 2:
             raise ValueError("pair_axis has an axis for each of rotary_dim / 2 pairs")
         return axes
@@ -471,8 +488,8 @@ class Pool:
                 rotary_dim: int = 0) -> None:
         """Kept tokens' K and V of every layer to other slots, keys turned by `shift`
         positions (ckv_compact); counts are the moves of each sequence."""
-        f, t, c = _u32(from_slots), _u32(to_slots), _u32(counts)
-        s = None if shift is None else np.ascontiguousarray(shift, dtype=np.int32)
+        f, t, c = (_exact(a, np.uint32) for a in (from_slots, to_slots, counts))
+        s = None if shift is None else _exact(shift, np.int32)
         if f.size != t.size or sum(c.tolist()) != f.size or (s is not None and s.size != f.size):
             raise ValueError("from_slots, to_slots and shift have an entry for each counted move")
         # (addresses: typed pointers take twice as long to make)

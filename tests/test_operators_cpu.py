@@ -69,3 +69,25 @@ def test_binding_refuses_arrays_of_other_sizes():
     for moves in (([1, 2], [3], [2], None), ([1, 2], [3, 4], [1], None), ([1, 2], [3, 4], [2], [0])):
         with pytest.raises(ValueError):
             pool.compact(*moves)
+
+
+def test_binding_refuses_numbers_that_wrap():
+    """Slots, shifts, positions and axes that 32 or 8 bits do not hold, and negative windows and sinks
+    (size_t to the library), would be other numbers there."""
+    pool, rows = _Stub(), np.zeros((2, 256))
+    with pytest.raises(ValueError):
+        pool.upload_axes(np.array([[1, -1]]))
+    with pytest.raises(ValueError):
+        pool.upload_axes(np.array([[1, 2 ** 32]]))
+    for axis in (-1, 256, 257):
+        with pytest.raises(ValueError):
+            pool.rope_axes(rows, rows, 2, 1e4, [axis] * 64)
+    for moves in (([2 ** 32 + 5], [3], [1], None), ([5], [-3], [1], None), ([5], [3], [1], [2 ** 31]), ([5], [3], [1], [0.5])):
+        with pytest.raises(ValueError):
+            pool.compact(*moves)
+    for window, sinks in ((-1, 0), (8, -1)):
+        for call in (lambda: ckv.Pool.attention_window(pool, 0, rows, 2, 1.0, window, rows, sinks=sinks),
+                     lambda: ckv.Pool.append_decode_window(pool, 0, rows, rows, rows, 2, 1.0, window, rows, sinks=sinks),
+                     lambda: ckv.Pool.rope_append_decode_window(pool, 0, rows, rows, rows, 2, 1.0, 1e4, window, rows, sinks=sinks)):
+            with pytest.raises(ValueError, match="counts of tokens"):
+                call()
