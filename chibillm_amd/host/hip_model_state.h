@@ -105,11 +105,12 @@ public:
     // also that of a shared last page which later tokens will fill. The next batch of the
     // sequence starts at position kept.size() (a scheduler that holds the sequence knows if
     // the call goes through its compact()): begin_batch refuses one that does not, with
-    // invalid_reservation. A checkpoint of it from then on holds the kept tokens. Errors, before anything changes: invalid_reservation (no token, one
-    // out of order or past the sequence's pages, a rotary width or theta that ckv_compact
-    // refuses, a batch begun, a stream under capture), capacity_exhausted (for want of a page, though
-    // checkpoints were spilled), allocation_failed (host memory). After backend_failure (the
-    // device's) the table is as it was but rows may have moved: the sequence is to be released.
+    // invalid_reservation. A checkpoint of it from then on holds the kept tokens. Errors,
+    // before anything changes: invalid_reservation (no token, one out of order or past the
+    // sequence's pages, a rotary width or theta that ckv_compact refuses, a batch begun, a
+    // stream under capture), capacity_exhausted (for want of a page, though checkpoints were
+    // spilled), allocation_failed (host memory). After backend_failure (the device's) the
+    // table is as it was but rows may have moved: the sequence is to be released.
     result<void, state_error> compact(seq_id id, std::span<const std::uint32_t> kept,
                                       float theta = 0.0f,
                                       std::size_t rotary_dimension = 0) override;

@@ -8,8 +8,9 @@
 // scheduled count differs from the item's, or whose tokens or positions would
 // leave the sequence or the u32 position range. It then lays the items'
 // unprocessed tokens end to end in batch order, each at its position
-// (next_position + i: processed + i but behind a compaction), with a copy of the sequence's block table, and marks the
-// last row of each sampling item as its logits row.
+// (next_position + i: processed + i, less what a compaction dropped), with a copy of
+// the sequence's block table, and marks the last row of each sampling item as its
+// logits row.
 //
 // prepare_paged_batch turns a model batch into the arrays the KV path takes:
 // the items' block tables concatenated, and per row its slot

@@ -1,7 +1,7 @@
 // One request's token history and its progress through prefill and decode
 // (the interface of src/seq.h:12-150). Tokens are [prompt | completion];
-// `processed` tokens are in the KV cache, `scheduled` tokens belong to the
-// batch in flight, and there is always a one-token gap between a running
+// `processed` tokens are in the KV cache (but for those that a compaction
+// dropped), `scheduled` tokens belong to the batch in flight, and there is always a one-token gap between a running
 // sequence's last sample and the cache.
 #pragma once
 
