@@ -87,6 +87,12 @@ _SIGNATURES = [
     ("ckv_rope_axes_upload", _i, [_vp, _u32p, _sz, _sz]),
     ("ckv_rope_axes", _i, [_vp, _vp, _vp, _sz, _f, _sz, C.c_char_p, _sz]),
     ("ckv_rope_axes_append", _i, [_vp, _sz, _vp, _vp, _sz, _vp, _vp, _f, _sz, C.c_char_p, _sz]),
+    ("ckv_pool_create_fp4", _i, [_vp, _sz, _sz, _sz, _sz, _sz, _i, C.POINTER(_vp)]),
+    ("ckv_pool_wrap_fp4", _i, [_vp, _sz, _sz, _sz, _sz, _sz, _i, _vp, _vp, C.POINTER(_vp)]),
+    ("ckv_rotate", _i, [_vp, _vp, _vp, _vp, _sz, _sz]),
+    ("ckv_rotate_append", _i, [_vp, _sz, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _sz]),
+    ("ckv_rotate_append_decode", _i, [_vp, _sz, _vp, _vp, _vp, _vp, _sz, _f, _vp, _vp, _vp, _vp, _sz]),
+    ("ckv_prompt_attention", _i, [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _f, _vp, _vp, _sz]),
     ("ckv_compact", _i, [_vp, _vp, _vp, _vp, _vp, _sz, _f, _sz]),
 ]
 SYMBOLS = [name for name, _, _ in _SIGNATURES]
@@ -191,6 +197,37 @@ def rope_pair_axes(sections, interleaved: bool = False) -> np.ndarray:
     return axes
 
 
+class Rotation(C.Structure):
+    """How rows are rotated (ckv_rotation): layout "halves" or "pairs" (neighbours), scaling
+    "none", "linear", "bands" or "yarn" with its factor, low, high and original."""
+
+    _fields_ = [("theta", _f), ("rotary_dim", C.c_uint32), ("layout", C.c_int32), ("scaling", C.c_int32),
+                ("factor", _f), ("low", _f), ("high", _f), ("original", C.c_uint32), ("magnitude", _f)]
+    LAYOUTS = {"halves": 0, "pairs": 1}
+    SCALINGS = {"none": 0, "linear": 1, "bands": 2, "yarn": 3}
+
+    def __init__(self, theta: float, rotary_dim: int = 0, layout: str = "halves", scaling: str = "none",
+                 factor: float = 1.0, low: float = 1.0, high: float = 32.0, original: int = 0,
+                 magnitude: float = 0.0):
+        if not 0 <= rotary_dim < 1 << 32 or not 0 <= original < 1 << 32:
+            raise ValueError("rotary_dim and original are counts")
+        super().__init__(theta, rotary_dim, self.LAYOUTS[layout], self.SCALINGS[scaling], factor, low, high,
+                         original, magnitude)
+
+
+def _rotation(rotation: Optional[Rotation]):
+    return None if rotation is None else C.addressof(rotation)
+
+
+def _rows(x):
+    """(address, elements from one row to the next) of a 2-D device tensor of whole rows."""
+    if not x.is_cuda:
+        raise ValueError("device arrays must be GPU tensors")
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError("rows are [rows, features] with features side by side")
+    return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else 0
+
+
 class Context:
     """A device and the stream ckv enqueues on (ckv_context)."""
 
@@ -277,21 +314,24 @@ class Context:
 
 
 class Pool:
-    """Paged K/V tensors [layer, block, token, kv_head, feature] (ckv_pool)."""
+    """Paged K/V tensors [layer, block, token, kv_head, feature] (ckv_pool), or, with fp4, in 4
+    bits (ckv_pool_create_fp4; dtype is the rows')."""
 
     def __init__(self, ctx: Context, layers: int, blocks: int, block_size: int, kv_heads: int,
-                 head_dim: int, dtype=BF16, keys=None, values=None):
+                 head_dim: int, dtype=BF16, keys=None, values=None, fp4: bool = False):
         lib = load()
         self.ctx = ctx
         self.geometry = (layers, blocks, block_size, kv_heads, head_dim)
         self.dtype = _dtype_code(dtype)
         h = _vp()
         if keys is None:
-            rc = lib.ckv_pool_create(ctx.handle, layers, blocks, block_size, kv_heads, head_dim,
-                                     self.dtype, C.byref(h))
+            create = lib.ckv_pool_create_fp4 if fp4 else lib.ckv_pool_create
+            rc = create(ctx.handle, layers, blocks, block_size, kv_heads, head_dim, self.dtype,
+                        C.byref(h))
         else:
-            rc = lib.ckv_pool_wrap(ctx.handle, layers, blocks, block_size, kv_heads, head_dim,
-                                   self.dtype, _ptr(keys), _ptr(values), C.byref(h))
+            wrap = lib.ckv_pool_wrap_fp4 if fp4 else lib.ckv_pool_wrap
+            rc = wrap(ctx.handle, layers, blocks, block_size, kv_heads, head_dim, self.dtype,
+                      _ptr(keys), _ptr(values), C.byref(h))
         ctx.check(rc)
         self.handle = h
         self._keep = (keys, values)
@@ -483,6 +523,42 @@ class Pool:
         self.ctx.check(load().ckv_rope_axes_append(
             self.handle, layer, _ptr(queries), _ptr(rotated), q_heads, _ptr(keys), _ptr(values),
             theta, rotary_dim, a, rows))
+
+    def rotate(self, rotation: Rotation, inputs, outputs, heads: int, rows: Optional[int] = None) -> None:
+        """Rows rotated by their positions (ckv_rotate)."""
+        rows = inputs.shape[0] if rows is None else rows
+        self.ctx.check(load().ckv_rotate(self.handle, _rotation(rotation), _ptr(inputs), _ptr(outputs),
+                                         heads, rows))
+
+    def rotate_append(self, layer: int, rotation: Optional[Rotation], queries, rotated, q_heads: int,
+                      keys, values, held_keys=None, held_values=None,
+                      rows: Optional[int] = None) -> None:
+        """Queries rotated into `rotated`, keys rotated and appended with the values, which
+        held_keys and held_values take as the cache holds them (ckv_rotate_append)."""
+        rows = keys.shape[0] if rows is None else rows
+        self.ctx.check(load().ckv_rotate_append(
+            self.handle, layer, _rotation(rotation), _ptr(queries), _ptr(rotated), q_heads, _ptr(keys),
+            _ptr(values), _ptr(held_keys), _ptr(held_values), rows))
+
+    def rotate_append_decode(self, layer: int, rotation: Optional[Rotation], keys, values, queries,
+                             q_heads: int, scale: float, output, gate=None, held_keys=None,
+                             held_values=None, rows: Optional[int] = None) -> None:
+        """A decode step from unrotated rows (ckv_rotate_append_decode)."""
+        rows = queries.shape[0] if rows is None else rows
+        self.ctx.check(load().ckv_rotate_append_decode(
+            self.handle, layer, _rotation(rotation), _ptr(keys), _ptr(values), _ptr(queries), q_heads,
+            scale, _ptr(gate), _ptr(held_keys), _ptr(held_values), _ptr(output), rows))
+
+    def prompt_attention(self, queries, keys, values, q_heads: int, scale: float, output, gate=None,
+                         rows: Optional[int] = None) -> None:
+        """Whole prompts' attention from their rows (ckv_prompt_attention); queries, and keys
+        and values, may be parts of wider rows."""
+        rows = queries.shape[0] if rows is None else rows
+        (q, q_stride), (k, k_stride), (v, v_stride) = _rows(queries), _rows(keys), _rows(values)
+        if k_stride != v_stride:
+            raise ValueError("keys and values have rows of one stride")
+        self.ctx.check(load().ckv_prompt_attention(
+            self.handle, q, q_stride, k, v, k_stride, q_heads, scale, _ptr(gate), _ptr(output), rows))
 
     def compact(self, from_slots, to_slots, counts, shift=None, theta: float = 0.0,
                 rotary_dim: int = 0) -> None:

@@ -5,6 +5,7 @@
 // enqueues HIP work on the context stream. Metadata goes up with one pinned
 // host-to-device copy per call.
 #include "ckv_internal.h"
+#include "fp4.h"
 
 #include <cmath>
 
@@ -430,6 +431,17 @@ void put_plan(ckv_pool* pool, const std::vector<uint32_t>& positions, meta_view&
     m.n_cut = shape.n_cut;
 }
 
+decode_form form_of(const ckv_pool* pool)
+{
+    return pool->fp4 ? fp4_decode_form() : decode_form_of(pool->dtype, (uint32_t)pool->head_dim);
+}
+
+// Pools held in 4 bits are refused by what reads or writes elements of the rows' type.
+int refuse_fp4(const ckv_pool* pool)
+{
+    return pool->fp4 ? set_error(pool->ctx, CKV_E_UNSUPPORTED_DTYPE, "the pool is held in 4 bits") : CKV_OK;
+}
+
 // The fast decode plan of a batch uploaded without it (one served by the
 // prefill kernel), at its first decode launch.
 int ensure_plan(ckv_pool* pool)
@@ -439,7 +451,7 @@ int ensure_plan(ckv_pool* pool)
     ckv_context* ctx = pool->ctx;
     const decode_plan_shape shape = shape_decode_plan(
         pool->positions, (uint32_t)pool->block_size, (uint32_t)pool->kv_heads, ctx->cu_count,
-        decode_form_of(pool->dtype, (uint32_t)pool->head_dim));
+        form_of(pool));
     const size_t words = std::max<size_t>(plan_words(shape, pool->positions.size()), 4);
     void* host = nullptr;
     int status = stage(ctx, words * sizeof(uint32_t), &host);
@@ -458,10 +470,11 @@ int ensure_plan(ckv_pool* pool)
 
 // Scratch of the fast decode when its plan cuts rows into chunks: a partial
 // record for every (record, q head) and an arrival counter for every
-// (record, kv head). The counters have a buffer of their own (the generic
+// (record, kv head, pass). The counters have a buffer of their own (the generic
 // decode writes its partials over d_partials) and are zeroed by a fill
 // kernel whenever it is allocated; launches leave them zero.
-int ensure_split(ckv_pool* pool, const meta_view& m, size_t q_heads, split_scratch& split)
+int ensure_split(ckv_pool* pool, const meta_view& m, size_t q_heads, split_scratch& split,
+                 size_t passes = 1)
 {
     split = {};
     if (!m.n_cut)
@@ -475,7 +488,7 @@ int ensure_split(ckv_pool* pool, const meta_view& m, size_t q_heads, split_scrat
     pool->d_partials_bytes = capacity_floats * sizeof(float);
     if (status)
         return status;
-    const size_t counters = (size_t)m.n_records * pool->kv_heads;
+    const size_t counters = (size_t)m.n_records * pool->kv_heads * passes;
     if (counters > pool->d_arrivals_words) {
         status = ensure_device(pool, &pool->d_arrivals, &pool->d_arrivals_words, counters,
                                "decode arrival counters");
@@ -558,6 +571,38 @@ int ensure_work(ckv_pool* pool)
                                 &pool->d_work_words, pool->work_multi);
     pool->work_ready = status == CKV_OK;
     return status;
+}
+
+// The records and counters of a prefill launch that splits its tiles' keys.
+int ensure_prefill_split(ckv_pool* pool, const prefill_shape_info& plan, prefill_split& split)
+{
+    if (plan.n_split <= 1)
+        return CKV_OK;
+    ckv_context* ctx = pool->ctx;
+    int status = ensure_device(pool, &pool->d_pre_records, &pool->d_pre_records_floats,
+                               (size_t)plan.records_floats, "prefill split records");
+    if (status)
+        return status;
+    if (plan.counters > pool->d_pre_arrivals_words) {
+        status = ensure_device(pool, &pool->d_pre_arrivals, &pool->d_pre_arrivals_words,
+                               (size_t)plan.counters, "prefill split counters");
+        if (status)
+            return status;
+        status = run_kernel(ctx, "fill", [&] {
+            return launch_fill(ctx->stream, pool->d_pre_arrivals, 0,
+                               (uint32_t)pool->d_pre_arrivals_words);
+        });
+        if (status) {
+            // not known to be zero: allocate and clear again next time
+            (void)dev_free(ctx, pool->d_pre_arrivals);
+            pool->d_pre_arrivals = nullptr;
+            pool->d_pre_arrivals_words = 0;
+            return status;
+        }
+    }
+    split.records = pool->d_pre_records;
+    split.arrivals = pool->d_pre_arrivals;
+    return CKV_OK;
 }
 
 // ---- the batch through a window ---------------------------------------------------
@@ -803,6 +848,8 @@ int run_checkpoint(ckv_pool* pool, const uint32_t* blocks, size_t n_blocks, size
     if (!pool)
         return CKV_E_INVALID_ARGUMENT;
     ckv_context* ctx = pool->ctx;
+    if (const int refused = refuse_fp4(pool))
+        return refused;
     int status = validate_prefix(pool, blocks, n_blocks, tokens);
     if (status)
         return set_error(ctx, status, "invalid checkpoint prefix");
@@ -832,6 +879,8 @@ int run_transfer(ckv_pool* pool, const uint32_t* blocks, size_t n_blocks, size_t
     if (!pool)
         return CKV_E_INVALID_ARGUMENT;
     ckv_context* ctx = pool->ctx;
+    if (const int refused = refuse_fp4(pool))
+        return refused;
     int status = validate_prefix(pool, blocks, n_blocks, tokens);
     if (status)
         return set_error(ctx, status, "invalid checkpoint prefix");
@@ -887,7 +936,7 @@ int run_transfer(ckv_pool* pool, const uint32_t* blocks, size_t n_blocks, size_t
 
 int create_pool(ckv_context* ctx, size_t layers, size_t blocks, size_t block_size,
                 size_t kv_heads, size_t head_dim, int dtype, void* keys, void* values,
-                ckv_pool** out)
+                ckv_pool** out, bool fp4 = false)
 {
     if (!ctx || !out)
         return CKV_E_INVALID_ARGUMENT;
@@ -899,10 +948,14 @@ int create_pool(ckv_context* ctx, size_t layers, size_t blocks, size_t block_siz
         return set_error(ctx, CKV_E_INVALID_BLOCK_COUNT, "blocks == 0");
     if (block_size == 0)
         return set_error(ctx, CKV_E_INVALID_BLOCK_SIZE, "block_size == 0");
+    if (fp4 && block_size % fp4_tile)
+        return set_error(ctx, CKV_E_INVALID_BLOCK_SIZE, "4-bit pools: block_size % 16 != 0");
     if (kv_heads == 0)
         return set_error(ctx, CKV_E_INVALID_KV_HEAD_COUNT, "kv_heads == 0");
     if (head_dim == 0)
         return set_error(ctx, CKV_E_INVALID_HEAD_DIMENSION_KV, "head_dim == 0");
+    if (fp4 && !fp4_head_dim(head_dim))
+        return set_error(ctx, CKV_E_INVALID_HEAD_DIMENSION_KV, "4-bit pools: head_dim must be 64, 128 or 256");
     if (dtype != CKV_F32 && dtype != CKV_BF16 && dtype != CKV_F16)
         return set_error(ctx, CKV_E_UNSUPPORTED_DTYPE, "dtype must be f32, bf16 or f16");
     const size_t elem = dtype == CKV_F32 ? 4 : 2;
@@ -913,6 +966,8 @@ int create_pool(ckv_context* ctx, size_t layers, size_t blocks, size_t block_siz
         || slots > UINT32_MAX || !mul_fits(kv_heads, head_dim, &features)
         || features > UINT32_MAX || layers > UINT32_MAX)
         return set_error(ctx, CKV_E_LAYOUT_SIZE_OVERFLOW, "KV layout does not fit");
+    if (fp4) // 17 bytes for 32 elements
+        bytes = elements / 32 * 17;
     auto* pool = new (std::nothrow) ckv_pool;
     if (!pool)
         return set_error(ctx, CKV_E_KV_ALLOCATION_FAILED, "pool object");
@@ -925,10 +980,15 @@ int create_pool(ckv_context* ctx, size_t layers, size_t blocks, size_t block_siz
     pool->dtype = dtype;
     pool->elem_size = elem;
     pool->bytes_each = bytes;
+    pool->fp4 = fp4;
     if (keys || values) {
         if (!keys || !values) {
             delete pool;
             return set_error(ctx, CKV_E_INVALID_ARGUMENT, "both buffers are required");
+        }
+        if (fp4 && ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) & 15)) {
+            delete pool;
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT, "4-bit pools: buffers must be aligned to 16 bytes");
         }
         pool->keys = keys;
         pool->values = values;
@@ -1006,6 +1066,225 @@ int guarded(ckv_pool* pool, Call&& call) noexcept
         pool->ctx->last_error.assign("host memory"); // within the string's reserve
         return CKV_E_TENSOR_ALLOCATION_FAILED;
     }
+}
+
+// ---- rotations ----------------------------------------------------------------------
+
+constexpr ckv::rotation_table no_rotation {};
+
+// The checks of a rotation after the row count. `by` is its table: the pool's, made anew
+// where the rotation is not the last one's; none for a null rotation.
+int check_rotation(ckv_pool* pool, size_t heads, const ckv_rotation* rotation,
+                   const ckv::rotation_table*& by)
+{
+    ckv_context* ctx = pool->ctx;
+    by = &no_rotation;
+    if (heads == 0)
+        return set_error(ctx, CKV_E_INVALID_HEAD_COUNT, "heads == 0");
+    const size_t head_dim = pool->head_dim;
+    if (heads > UINT32_MAX / head_dim)
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "row too wide");
+    if (!rotation)
+        return CKV_OK;
+    ckv_rotation r = *rotation;
+    if (r.rotary_dim == 0 && head_dim <= UINT32_MAX)
+        r.rotary_dim = (uint32_t)head_dim;
+    if (head_dim % 2 != 0 || r.rotary_dim % 2 != 0 || r.rotary_dim > head_dim
+        || r.rotary_dim / 2 > ckv::max_turn_pairs)
+        return set_error(ctx, CKV_E_INVALID_HEAD_DIMENSION,
+                         "head_dim and rotary_dim must be even, rotary_dim <= head_dim and at most "
+                             + std::to_string(2 * ckv::max_turn_pairs));
+    if (!std::isfinite(r.theta) || r.theta <= 0.0f)
+        return set_error(ctx, CKV_E_INVALID_ROPE_THETA, "theta must be positive and finite");
+    if (r.layout != CKV_ROTARY_HALVES && r.layout != CKV_ROTARY_NEIGHBOURS)
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "unknown rotary layout");
+    if (r.scaling < CKV_SCALING_NONE || r.scaling > CKV_SCALING_YARN)
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "unknown rotary scaling");
+    if (r.scaling != CKV_SCALING_NONE && !(std::isfinite(r.factor) && r.factor > 0.0f))
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "factor must be positive and finite");
+    const bool by_turns = r.scaling == CKV_SCALING_BANDS || r.scaling == CKV_SCALING_YARN;
+    if (by_turns && !(std::isfinite(r.low) && std::isfinite(r.high) && 0.0f < r.low && r.low < r.high
+                      && r.original))
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "needs 0 < low < high and an original length");
+    if (r.scaling == CKV_SCALING_YARN && r.theta <= 1.0f)
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "yarn needs theta > 1");
+    if (!(std::isfinite(r.magnitude) && r.magnitude >= 0.0f))
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "magnitude must be finite and not negative");
+    by = &pool->rotation;
+    const ckv_rotation& last = pool->rotation_of;
+    if (pool->rotation_ready && last.theta == r.theta && last.rotary_dim == r.rotary_dim
+        && last.layout == r.layout && last.scaling == r.scaling && last.factor == r.factor
+        && last.low == r.low && last.high == r.high && last.original == r.original
+        && last.magnitude == r.magnitude)
+        return CKV_OK;
+    const uint32_t pairs = r.rotary_dim / 2;
+    long double turns[ckv::max_turn_pairs];
+    const long double whole = 2.0L * 3.14159265358979323846264338327950288L, theta = r.theta;
+    long double first = 0, last_pair = 0;
+    if (r.scaling == CKV_SCALING_YARN) {
+        const auto pair_of = [&](long double t) {
+            return r.rotary_dim * std::log(r.original / (t * whole)) / (2.0L * std::log(theta));
+        };
+        first = std::max(std::floor(pair_of(r.high)), 0.0L);
+        last_pair = std::min(std::ceil(pair_of(r.low)), (long double)r.rotary_dim - 1);
+    }
+    for (uint32_t j = 0; j < pairs; ++j) {
+        const long double b = std::pow(theta, -2.0L * j / r.rotary_dim) / whole; // turns a position
+        switch (r.scaling) {
+        case CKV_SCALING_LINEAR:
+            turns[j] = b / r.factor;
+            break;
+        case CKV_SCALING_BANDS: {
+            const long double k = std::clamp((r.original * b - r.low) / ((long double)r.high - r.low), 0.0L, 1.0L);
+            turns[j] = b * (k + (1 - k) / r.factor);
+            break;
+        }
+        case CKV_SCALING_YARN: {
+            const long double k = std::clamp((j - first) / std::max(last_pair - first, 0.001L), 0.0L, 1.0L);
+            turns[j] = b * (1 - k) + b / r.factor * k;
+            break;
+        }
+        default:
+            turns[j] = b;
+        }
+    }
+    ckv::rotation_steps(turns, r.rotary_dim, pool->rotation);
+    pool->rotation.magnitude64 = r.magnitude > 0.0f ? (double)r.magnitude
+        : r.scaling == CKV_SCALING_YARN && r.factor > 1.0f ? 0.1 * std::log((double)r.factor) + 1.0
+                                                           : 1.0;
+    pool->rotation.magnitude = (float)pool->rotation.magnitude64;
+    pool->rotation.rotary = r.rotary_dim;
+    pool->rotation.neighbours = r.layout == CKV_ROTARY_NEIGHBOURS;
+    pool->rotation_of = r;
+    pool->rotation_ready = true;
+    return CKV_OK;
+}
+
+// ckv_rope's rotation.
+ckv_rotation plain_rotation(float theta, size_t rotary_dim)
+{
+    ckv_rotation r {};
+    r.theta = theta;
+    r.rotary_dim = (uint32_t)rotary_dim;
+    return r;
+}
+
+// ---- pools held in 4 bits --------------------------------------------------------------
+
+// Checked rows, rotated into `rotated` and appended.
+int run_rotate_append(ckv_pool* pool, size_t layer, const rotate_rows& x, size_t q_heads, size_t rows,
+                      const ckv::rotation_table& by)
+{
+    ckv_context* ctx = pool->ctx;
+    const pool_view view = view_of(pool);
+    return run_kernel(ctx, pool->fp4 ? "fp4_append" : "rotate_append", [&] {
+        return pool->fp4 ? launch_fp4_append(ctx->stream, view, pool->meta, (uint32_t)layer, x, (uint32_t)rows,
+                                             (uint32_t)q_heads, by)
+                         : launch_rotate(ctx->stream, view, pool->meta, (uint32_t)layer, x, (uint32_t)rows,
+                                         (uint32_t)q_heads, by);
+    });
+}
+
+// The plan and scratch of a decode launch of a 4-bit pool.
+int setup_fp4_decode(ckv_pool* pool, size_t q_heads, split_scratch& split)
+{
+    const int status = ensure_plan(pool);
+    return status ? status
+                  : ensure_split(pool, pool->meta, q_heads, split,
+                                 fp4_decode_passes(view_of(pool), (uint32_t)q_heads));
+}
+
+int launch_fp4_rows(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale, void* output,
+                    const void* gate, const split_scratch& split)
+{
+    ckv_context* ctx = pool->ctx;
+    return run_kernel(ctx, "fp4_attention_decode", [&] {
+        return launch_fp4_decode(ctx->stream, view_of(pool), pool->meta, (uint32_t)layer, queries,
+                                 (uint32_t)q_heads, scale, output, gate, split);
+    });
+}
+
+int run_fp4_decode(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale, void* output,
+                   const void* gate)
+{
+    return guarded(pool, [&]() -> int {
+        split_scratch split {};
+        const int status = setup_fp4_decode(pool, q_heads, split);
+        return status ? status : launch_fp4_rows(pool, layer, queries, q_heads, scale, output, gate, split);
+    });
+}
+
+// Checked decode rows, rotated, appended and attended. What is refused under capture is
+// before anything is captured.
+int run_rotate_append_decode(ckv_pool* pool, size_t layer, const ckv::rotation_table& by, const void* keys,
+                             const void* values, const void* queries, size_t q_heads, float scale,
+                             const void* gate, void* held_keys, void* held_values, void* output, size_t rows)
+{
+    const bool turned = by.rotary != 0;
+    if (turned) {
+        const size_t bytes = rows * q_heads * pool->head_dim * pool->elem_size;
+        if (const int status = ensure_device(pool, &pool->d_rope_q, &pool->d_rope_q_bytes, bytes, "rotated queries"))
+            return status;
+    }
+    const void* rotated = turned ? pool->d_rope_q : queries;
+    split_scratch split {};
+    decode_setup setup;
+    int status = pool->fp4 ? setup_fp4_decode(pool, q_heads, split)
+                           : setup_decode(pool, rotated, q_heads, output, all_keys, setup);
+    if (!status)
+        status = run_rotate_append(pool, layer,
+                                   { queries, turned ? pool->d_rope_q : nullptr, keys, values, held_keys, held_values },
+                                   turned ? q_heads : 0, rows, by);
+    if (status)
+        return status;
+    return pool->fp4 ? launch_fp4_rows(pool, layer, rotated, q_heads, scale, output, gate, split)
+                     : run_decode(pool, layer, rotated, q_heads, scale, output, gate);
+}
+
+// The attention of the batch's tiles by kernels_prompt.hip: over a 4-bit pool's cache, or
+// over rows (whole prompts).
+int run_prompt(ckv_pool* pool, size_t layer, const prompt_rows& x, size_t q_heads, float scale, void* output,
+               const void* gate, bool rows)
+{
+    ckv_context* ctx = pool->ctx;
+    const pool_view view = view_of(pool);
+    window_batch& through = select_window(pool, { UINT32_MAX - 1, 0 }, prompt_tile_rows(view, (uint32_t)q_heads));
+    int status = ensure_window_tiles(pool, through);
+    if (status)
+        return status;
+    const prefill_shape_info plan = prompt_plan(view, through.meta, (uint32_t)q_heads, ctx->cu_count);
+    prefill_split split { nullptr, nullptr, plan.n_split, plan.min_blocks };
+    if ((status = ensure_prefill_split(pool, plan, split)))
+        return status;
+    return run_kernel(ctx, rows ? "prompt_attention" : "fp4_attention_prefill", [&] {
+        return launch_prompt(ctx->stream, view, through.meta, (uint32_t)layer, x, (uint32_t)q_heads, scale, output,
+                             gate, !rows, split);
+    });
+}
+
+int run_fp4_prefill(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale, void* output,
+                    const void* gate)
+{
+    return guarded(pool, [&]() -> int {
+        prompt_rows x {};
+        x.queries = queries;
+        x.q_stride = (uint64_t)q_heads * pool->head_dim;
+        return run_prompt(pool, layer, x, q_heads, scale, output, gate, false);
+    });
+}
+
+// Whether every row of the batch is at position 0 or follows the one before it.
+bool whole_prompts(ckv_pool* pool)
+{
+    if (pool->whole_prompts < 0) {
+        const auto& at = pool->positions;
+        bool whole = true;
+        for (size_t r = 0; r < at.size() && whole; ++r)
+            whole = at[r] == 0
+                || (r && at[r - 1] + 1 == at[r] && pool->row_offsets[r - 1] == pool->row_offsets[r]);
+        pool->whole_prompts = whole;
+    }
+    return pool->whole_prompts;
 }
 
 } // namespace
@@ -1332,6 +1611,23 @@ int ckv_pool_wrap(ckv_context* ctx, size_t layers, size_t blocks, size_t block_s
                        out);
 }
 
+int ckv_pool_create_fp4(ckv_context* ctx, size_t layers, size_t blocks, size_t block_size,
+                        size_t kv_heads, size_t head_dim, int dtype, ckv_pool** out)
+{
+    return create_pool(ctx, layers, blocks, block_size, kv_heads, head_dim, dtype, nullptr,
+                       nullptr, out, true);
+}
+
+int ckv_pool_wrap_fp4(ckv_context* ctx, size_t layers, size_t blocks, size_t block_size,
+                      size_t kv_heads, size_t head_dim, int dtype, void* keys, void* values,
+                      ckv_pool** out)
+{
+    if (!keys || !values)
+        return set_error(ctx, CKV_E_INVALID_ARGUMENT, "both buffers are required");
+    return create_pool(ctx, layers, blocks, block_size, kv_heads, head_dim, dtype, keys, values,
+                       out, true);
+}
+
 int ckv_pool_destroy(ckv_pool* pool)
 {
     if (!pool)
@@ -1396,6 +1692,8 @@ int ckv_element_offset(const ckv_pool* pool, size_t layer, size_t block, size_t 
 {
     if (!pool || !offset)
         return CKV_E_INVALID_ARGUMENT;
+    if (pool->fp4)
+        return CKV_E_UNSUPPORTED_DTYPE;
     if (layer >= pool->layers)
         return CKV_E_LAYER_OUT_OF_RANGE;
     if (block >= pool->blocks)
@@ -1447,6 +1745,7 @@ void adopt_batch(ckv_pool* pool, size_t rows, size_t n_entries, bool with_slots,
     pool->work_ready = false;
     pool->n_windows = 0;
     pool->axes = 0;
+    pool->whole_prompts = -1;
     pool->uploaded = true;
 }
 
@@ -1534,7 +1833,7 @@ int ckv_tables_upload(ckv_pool* pool, const uint32_t* block_table, size_t n_entr
     const bool with_plan = !shared;
     const decode_plan_shape plan_shape = with_plan
         ? shape_decode_plan(pool->positions, (uint32_t)bs, (uint32_t)pool->kv_heads, ctx->cu_count,
-        decode_form_of(pool->dtype, (uint32_t)pool->head_dim))
+        form_of(pool))
         : decode_plan_shape {};
 
     // pack: table | offsets | lengths | positions | slots | tiles | plan
@@ -1791,7 +2090,7 @@ int ckv_batch_upload(ckv_pool* pool, const uint32_t* seq, const uint32_t* first_
     const bool with_plan = !shared;
     const decode_plan_shape plan_shape = with_plan
         ? shape_decode_plan(positions, (uint32_t)bs, (uint32_t)pool->kv_heads, ctx->cu_count,
-        decode_form_of(pool->dtype, (uint32_t)pool->head_dim))
+        form_of(pool))
         : decode_plan_shape {};
 
     // d_meta: offsets | lengths | positions | slots (written by the expand
@@ -1910,6 +2209,9 @@ int ckv_append(ckv_pool* pool, size_t layer, const void* keys, const void* value
         return set_error(ctx, CKV_E_CACHE_SLOT_COUNT_MISMATCH, "rows != uploaded slots");
     if (layer >= pool->layers)
         return set_error(ctx, CKV_E_CACHE_LAYER_OUT_OF_RANGE, "layer >= layers");
+    if (pool->fp4)
+        return run_rotate_append(pool, layer, { nullptr, nullptr, keys, values, nullptr, nullptr }, 0, rows,
+                                 no_rotation);
     const pool_view view = view_of(pool);
     return run_kernel(ctx, "store_kv", [&] {
         return launch_store_kv(ctx->stream, view, pool->meta, (uint32_t)layer, keys, values,
@@ -1989,6 +2291,13 @@ int ckv_rope_append(ckv_pool* pool, size_t layer, const void* keys, const void* 
     uint32_t rotary = 0;
     if (const int status = check_rope(pool, pool->kv_heads, theta, rotary_dim, freq, rotary))
         return status;
+    if (pool->fp4) {
+        const ckv_rotation rotation = plain_rotation(theta, rotary_dim);
+        const ckv::rotation_table* by = nullptr;
+        const int status = check_rotation(pool, pool->kv_heads, &rotation, by);
+        return status ? status
+                      : run_rotate_append(pool, layer, { nullptr, nullptr, keys, values, nullptr, nullptr }, 0, rows, *by);
+    }
     const pool_view view = view_of(pool);
     return run_kernel(ctx, "rope_append", [&] {
         return launch_rope_append(ctx->stream, view, pool->meta, (uint32_t)layer, keys, values,
@@ -2013,6 +2322,11 @@ int ckv_gather(ckv_pool* pool, size_t layer, size_t table_offset, size_t table_l
         return set_error(ctx, CKV_E_BLOCK_TABLE_RANGE_OUT_OF_BOUNDS, "gather range");
     const pool_view view = view_of(pool);
     const uint32_t* table = pool->meta.table + table_offset;
+    if (pool->fp4)
+        return run_kernel(ctx, "fp4_gather", [&] {
+            return launch_fp4_gather(ctx->stream, view, table, (uint32_t)layer, (uint32_t)n_tokens,
+                                     out_keys, out_values);
+        });
     return run_kernel(ctx, "gather_kv", [&] {
         return launch_gather(ctx->stream, view, table, (uint32_t)layer, (uint32_t)n_tokens,
                              out_keys, out_values);
@@ -2042,6 +2356,8 @@ int decode_impl(ckv_pool* pool, size_t layer, const void* queries, size_t q_head
     const int status = check_attention(pool, layer, queries, q_heads, output, rows);
     if (status || !rows)
         return status;
+    if (pool->fp4)
+        return run_fp4_decode(pool, layer, queries, q_heads, scale, output, gate);
     return run_decode(pool, layer, queries, q_heads, scale, output, gate);
 }
 
@@ -2100,6 +2416,11 @@ int append_decode_impl(ckv_pool* pool, size_t layer, const void* keys, const voi
         status = check_attention(pool, layer, queries, q_heads, output, rows);
     if (status || !rows)
         return status;
+    if (pool->fp4)
+        return guarded(pool, [&]() -> int {
+            return run_rotate_append_decode(pool, layer, no_rotation, keys, values, queries, q_heads, scale, gate,
+                                            nullptr, nullptr, output, rows);
+        });
     return run_append_decode(pool, layer, keys, values, queries, q_heads, scale, output, rows, gate,
                              all_keys);
 }
@@ -2113,31 +2434,8 @@ int run_prefill(ckv_pool* pool, size_t layer, const void* queries, size_t q_head
     const bool windowed = &m != &pool->meta;
     const prefill_shape_info plan = prefill_plan(view, m, (uint32_t)q_heads, ctx->cu_count);
     prefill_split split { nullptr, nullptr, plan.n_split, plan.min_blocks };
-    if (plan.n_split > 1) {
-        int status = ensure_device(pool, &pool->d_pre_records, &pool->d_pre_records_floats,
-                                   (size_t)plan.records_floats, "prefill split records");
-        if (status)
-            return status;
-        if (plan.counters > pool->d_pre_arrivals_words) {
-            status = ensure_device(pool, &pool->d_pre_arrivals, &pool->d_pre_arrivals_words,
-                                   (size_t)plan.counters, "prefill split counters");
-            if (status)
-                return status;
-            status = run_kernel(ctx, "fill", [&] {
-                return launch_fill(ctx->stream, pool->d_pre_arrivals, 0,
-                                   (uint32_t)pool->d_pre_arrivals_words);
-            });
-            if (status) {
-                // not known to be zero: allocate and clear again next time
-                (void)dev_free(ctx, pool->d_pre_arrivals);
-                pool->d_pre_arrivals = nullptr;
-                pool->d_pre_arrivals_words = 0;
-                return status;
-            }
-        }
-        split.records = pool->d_pre_records;
-        split.arrivals = pool->d_pre_arrivals;
-    }
+    if (const int status = ensure_prefill_split(pool, plan, split))
+        return status;
     return run_kernel(ctx, windowed ? "window_attention_prefill" : "paged_attention_prefill", [&] {
         return launch_prefill(ctx->stream, view, m, (uint32_t)layer, queries, (uint32_t)q_heads,
                               scale, output, gate, plan, split);
@@ -2162,6 +2460,8 @@ int prefill_impl(ckv_pool* pool, size_t layer, const void* queries, size_t q_hea
     const int status = check_attention(pool, layer, queries, q_heads, output, rows);
     if (status || !rows)
         return status;
+    if (pool->fp4)
+        return run_fp4_prefill(pool, layer, queries, q_heads, scale, output, gate);
     if (!prefill_takes(pool, queries, q_heads, scale, output, gate))
         return run_decode(pool, layer, queries, q_heads, scale, output, gate);
     return run_prefill(pool, layer, queries, q_heads, scale, output, gate, pool->meta);
@@ -2302,6 +2602,15 @@ int ckv_rope_append_decode(ckv_pool* pool, size_t layer, const void* keys, const
     status = check_rope(pool, q_heads, theta, rotary_dim, freq, rotary);
     if (status || !rows)
         return status;
+    if (pool->fp4)
+        return guarded(pool, [&]() -> int {
+            const ckv_rotation rotation = plain_rotation(theta, rotary_dim);
+            const ckv::rotation_table* by = nullptr;
+            const int refused = check_rotation(pool, q_heads, &rotation, by);
+            return refused ? refused
+                           : run_rotate_append_decode(pool, layer, *by, keys, values, queries, q_heads, scale, gate,
+                                                      nullptr, nullptr, output, rows);
+        });
     return run_rope_append_decode(pool, layer, keys, values, queries, q_heads, scale, theta,
                                   rotary_dim, freq, rotary, gate, output, rows, all_keys);
 }
@@ -2344,6 +2653,8 @@ int ckv_append_decode_noalloc(ckv_pool* pool, size_t layer, const void* keys, co
         return fail_fixed(ctx, CKV_E_CACHE_LAYER_OUT_OF_RANGE, "layer >= layers");
     if (q_heads > UINT32_MAX / pool->head_dim)
         return fail_fixed(ctx, CKV_E_INVALID_ARGUMENT, "row too wide");
+    if (pool->fp4)
+        return fail_fixed(ctx, CKV_E_UNSUPPORTED_DTYPE, "the pool is held in 4 bits");
     if (!rows)
         return CKV_OK;
     // what only this entry point requires
@@ -2420,6 +2731,8 @@ int ckv_attention_window(ckv_pool* pool, size_t layer, const void* queries, size
             status = check_window(pool, window);
         if (!status)
             status = check_optional_gate(pool, gate, queries, output);
+        if (!status)
+            status = refuse_fp4(pool);
         if (status || !rows)
             return status;
         const key_window w = window_of(pool, window, sinks);
@@ -2450,6 +2763,8 @@ int ckv_append_decode_window(ckv_pool* pool, size_t layer, const void* keys, con
             status = check_window(pool, window);
         if (!status)
             status = check_optional_gate(pool, gate, queries, output);
+        if (!status)
+            status = refuse_fp4(pool);
         if (status || !rows)
             return status;
         return run_append_decode(pool, layer, keys, values, queries, q_heads, scale, output, rows,
@@ -2474,6 +2789,8 @@ int ckv_rope_append_decode_window(ckv_pool* pool, size_t layer, const void* keys
         uint32_t rotary = 0;
         if (!status)
             status = check_rope(pool, q_heads, theta, rotary_dim, freq, rotary);
+        if (!status)
+            status = refuse_fp4(pool);
         if (status || !rows)
             return status;
         return run_rope_append_decode(pool, layer, keys, values, queries, q_heads, scale, theta,
@@ -2593,6 +2910,8 @@ int ckv_rope_axes_append(ckv_pool* pool, size_t layer, const void* queries, void
         // (the sum past the largest count is one of a row too wide)
         const size_t heads = std::min(q_heads, SIZE_MAX - pool->kv_heads) + pool->kv_heads;
         status = check_rope_axes(pool, heads, theta, rotary_dim, pair_axis, axes, rotary);
+        if (!status)
+            status = refuse_fp4(pool);
         if (status)
             return status;
         const pool_view view = view_of(pool);
@@ -2605,10 +2924,135 @@ int ckv_rope_axes_append(ckv_pool* pool, size_t layer, const void* queries, void
     });
 }
 
+int ckv_rotate(ckv_pool* pool, const ckv_rotation* rotation, const void* input, void* output,
+               size_t heads, size_t rows)
+{
+    return guarded(pool, [&]() -> int {
+        ckv_context* ctx = pool->ctx;
+        if (!rotation || (rows && (!input || !output)))
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT, "a rotation, input and output are required");
+        if (!pool->uploaded)
+            return set_error(ctx, CKV_E_NO_TABLES, "rotate before ckv_tables_upload");
+        if (rows != pool->positions.size())
+            return set_error(ctx, CKV_E_POSITION_COUNT_MISMATCH, "rows != uploaded positions");
+        const ckv::rotation_table* by = nullptr;
+        if (const int status = check_rotation(pool, heads, rotation, by))
+            return status;
+        return run_kernel(ctx, "rotate", [&] {
+            return launch_rotate(ctx->stream, view_of(pool), pool->meta, 0,
+                                 { input, output, nullptr, nullptr, nullptr, nullptr }, (uint32_t)rows,
+                                 (uint32_t)heads, *by);
+        });
+    });
+}
+
+namespace {
+
+// Held rows are arrays of their own.
+int check_held(const ckv_pool* pool, const void* held_keys, const void* held_values,
+               std::initializer_list<const void*> others)
+{
+    const auto clashes = [&](const void* held) {
+        return held && std::find(others.begin(), others.end(), held) != others.end();
+    };
+    if (clashes(held_keys) || clashes(held_values) || (held_keys && held_keys == held_values))
+        return set_error(pool->ctx, CKV_E_UNSUPPORTED_ALIASING, "held rows overlap another argument");
+    return CKV_OK;
+}
+
+} // namespace
+
+int ckv_rotate_append(ckv_pool* pool, size_t layer, const ckv_rotation* rotation,
+                      const void* queries, void* rotated, size_t q_heads, const void* keys,
+                      const void* values, void* held_keys, void* held_values, size_t rows)
+{
+    return guarded(pool, [&]() -> int {
+        ckv_context* ctx = pool->ctx;
+        int status = check_append(pool, keys, values, rows);
+        if (status)
+            return status;
+        if (layer >= pool->layers)
+            return set_error(ctx, CKV_E_CACHE_LAYER_OUT_OF_RANGE, "layer >= layers");
+        if (rows && q_heads && (!queries || !rotated))
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT, "queries and rotated are required");
+        if (rows && (rotated == keys || rotated == values))
+            return set_error(ctx, CKV_E_UNSUPPORTED_ALIASING, "rotated overlaps keys or values");
+        if (rows)
+            status = check_held(pool, held_keys, held_values, { queries, rotated, keys, values });
+        // (the sum past the largest count is one of a row too wide)
+        const size_t heads = std::min(q_heads, SIZE_MAX - pool->kv_heads) + pool->kv_heads;
+        const ckv::rotation_table* by = nullptr;
+        if (!status)
+            status = check_rotation(pool, heads, rotation, by);
+        if (status || !rows)
+            return status;
+        return run_rotate_append(pool, layer, { queries, rotated, keys, values, held_keys, held_values }, q_heads,
+                                 rows, *by);
+    });
+}
+
+int ckv_rotate_append_decode(ckv_pool* pool, size_t layer, const ckv_rotation* rotation,
+                             const void* keys, const void* values, const void* queries,
+                             size_t q_heads, float scale, const void* gate, void* held_keys,
+                             void* held_values, void* output, size_t rows)
+{
+    return guarded(pool, [&]() -> int {
+        int status = check_append(pool, keys, values, rows);
+        if (!status)
+            status = check_attention(pool, layer, queries, q_heads, output, rows);
+        if (!status)
+            status = check_optional_gate(pool, gate, queries, output);
+        if (!status && rows)
+            status = check_held(pool, held_keys, held_values, { queries, keys, values, gate, output });
+        const ckv::rotation_table* by = nullptr;
+        if (!status)
+            status = check_rotation(pool, q_heads, rotation, by);
+        if (status || !rows)
+            return status;
+        return run_rotate_append_decode(pool, layer, *by, keys, values, queries, q_heads, scale, gate, held_keys,
+                                        held_values, output, rows);
+    });
+}
+
+int ckv_prompt_attention(ckv_pool* pool, const void* queries, size_t q_stride, const void* keys,
+                         const void* values, size_t kv_stride, size_t q_heads, float scale,
+                         const void* gate, void* output, size_t rows)
+{
+    return guarded(pool, [&]() -> int {
+        ckv_context* ctx = pool->ctx;
+        if (rows && (!keys || !values))
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT, "keys and values are required");
+        int status = check_attention(pool, 0, queries, q_heads, output, rows);
+        if (status)
+            return status;
+        if (rows && (output == queries || output == keys || output == values || output == gate
+                     || (gate && (gate == queries || gate == keys || gate == values))))
+            return set_error(ctx, CKV_E_UNSUPPORTED_ALIASING, "the output or the gate overlaps another argument");
+        if (!fp4_head_dim(pool->head_dim))
+            return set_error(ctx, CKV_E_INVALID_HEAD_DIMENSION, "head_dim must be 64, 128 or 256");
+        const size_t q_width = q_heads * pool->head_dim, kv_width = pool->kv_heads * pool->head_dim;
+        if ((q_stride && q_stride < q_width) || (kv_stride && kv_stride < kv_width))
+            return set_error(ctx, CKV_E_INPUT_SHAPE_MISMATCH, "a stride is shorter than its row");
+        if (!whole_prompts(pool))
+            return set_error(ctx, CKV_E_INVALID_ARGUMENT, "the batch's rows are not whole prompts");
+        if (!rows)
+            return CKV_OK;
+        prompt_rows x {};
+        x.queries = queries;
+        x.keys = keys;
+        x.values = values;
+        x.q_stride = q_stride ? q_stride : q_width;
+        x.kv_stride = kv_stride ? kv_stride : kv_width;
+        return run_prompt(pool, 0, x, q_heads, scale, output, gate, true);
+    });
+}
+
 int ckv_compact(ckv_pool* pool, const uint32_t* from, const uint32_t* to, const int32_t* shift,
                 const uint32_t* counts, size_t n_sequences, float theta, size_t rotary_dim)
 {
     return guarded(pool, [&]() -> int {
+        if (const int status = refuse_fp4(pool))
+            return status;
         ckv_context* ctx = pool->ctx;
         if (!n_sequences)
             return CKV_OK;
@@ -2726,7 +3170,11 @@ int ckv_copy_blocks(ckv_pool* pool, const uint32_t* src, const uint32_t* dst, si
     int status = stage_pairs(pool, src, dst, n);
     if (status)
         return status;
-    const pool_view view = view_of(pool);
+    pool_view view = view_of(pool);
+    if (pool->fp4) { // pages as bytes
+        view.features = (uint32_t)(pool->bytes_each / pool->layers / pool->blocks);
+        view.block_size = view.elem_size = 1;
+    }
     return run_kernel(ctx, "copy_blocks", [&] {
         return launch_copy_blocks(ctx->stream, view, (uint32_t)pool->layers, pool->d_pairs,
                                   (uint32_t)n);

@@ -180,6 +180,16 @@ struct axis_table {
     uint8_t axis[max_turn_pairs];
 };
 
+// A rotation of rows (kernels_rotate.hip): how far a position turns each pair, how the
+// pairs stand, and what turned pairs are multiplied by.
+struct rotation_table {
+    turn_table turns;
+    double magnitude64;
+    float magnitude;
+    uint32_t rotary;     // 0: no rotation
+    uint32_t neighbours; // pairs (2j, 2j + 1), else (j, j + rotary / 2)
+};
+
 // One rotary pair (a, b) -> (a cos - b sin, b cos + a sin), written once with
 // explicit fused multiply-adds for every kernel that rotates (ckv_rope,
 // ckv_rope_append, the fused decode).
@@ -291,6 +301,7 @@ struct ckv_pool {
     void* values = nullptr;
     size_t bytes_each = 0;
     bool owned = false;
+    bool fp4 = false; // keys and values held in 4 bits (fp4.h); dtype is the rows'
 
     // host state of the current batch
     bool uploaded = false;
@@ -355,6 +366,11 @@ struct ckv_pool {
     ckv::turn_table turns {}; // of the last theta and rotary width (turns_of)
     float turns_theta = 0.0f;
     uint32_t turns_rotary = 0;
+
+    ckv::rotation_table rotation {}; // of the last ckv_rotation
+    ckv_rotation rotation_of {};
+    bool rotation_ready = false;
+    int whole_prompts = -1; // whether the batch's rows are whole prompts; -1: not yet looked at
 
     ckv::move_marks marks; // of ckv_compact's slots
     uint8_t* d_spare = nullptr; // rows it saves
@@ -616,5 +632,56 @@ hipError_t launch_fetch(hipStream_t s, uint32_t* to, const void* pinned, size_t 
 uint32_t compact_heads(const pool_view& p, uint32_t layers, uint32_t n_runs, uint32_t rotary);
 hipError_t launch_compact(hipStream_t s, const pool_view& p, uint32_t layers,
                           const compact_moves& moves, uint32_t rotary, const turn_table& turns);
+
+// ---- launchers (kernels_rotate.hip) ----------------------------------------------------
+// Query rows rotated into `rotated` and, with keys, key rows rotated and value rows copied
+// into the uploaded slots of `layer`, and both also into held_keys and held_values where
+// these are given. q_heads 0: keys and values alone.
+struct rotate_rows {
+    const void* queries;
+    void* rotated;
+    const void* keys;
+    const void* values;
+    void* held_keys;
+    void* held_values;
+};
+hipError_t launch_rotate(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
+                         const rotate_rows& x, uint32_t rows, uint32_t q_heads,
+                         const rotation_table& by);
+// The same into a pool held in 4 bits; held rows are as the cache holds them.
+hipError_t launch_fp4_append(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
+                             const rotate_rows& x, uint32_t rows, uint32_t q_heads,
+                             const rotation_table& by);
+hipError_t launch_fp4_gather(hipStream_t s, const pool_view& p, const uint32_t* table,
+                             uint32_t layer, uint32_t n_tokens, void* out_keys, void* out_values);
+// The fractions of a turn of turns[j] (turns a position on pair j) as steps.
+void rotation_steps(const long double* turns, uint32_t rotary, rotation_table& out);
+
+// ---- launchers (kernels_fp4_decode.hip) -------------------------------------------------
+decode_form fp4_decode_form();
+// Workgroups that share a (plan workgroup, kv head): each takes at most eight query heads
+// (f32 rows: four).
+uint32_t fp4_decode_passes(const pool_view& p, uint32_t q_heads);
+hipError_t launch_fp4_decode(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
+                             const void* q, uint32_t q_heads, float scale, void* out,
+                             const void* gate, split_scratch split);
+
+// ---- launchers (kernels_prompt.hip) ------------------------------------------------------
+// Rows of an attention of tiles; keys and values only where they are not a 4-bit pool's.
+// Strides in elements. launch_prompt sets the alignments.
+struct prompt_rows {
+    const void* queries;
+    const void* keys;
+    const void* values;
+    uint64_t q_stride, kv_stride;
+    bool vectors, out_vectors;
+};
+// Rows of a workgroup, which the tiles' are at most.
+uint32_t prompt_tile_rows(const pool_view& p, uint32_t q_heads);
+prefill_shape_info prompt_plan(const pool_view& p, const meta_view& m, uint32_t q_heads,
+                               int cu_count);
+hipError_t launch_prompt(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
+                         const prompt_rows& rows, uint32_t q_heads, float scale, void* out,
+                         const void* gate, bool fp4, const prefill_split& split);
 
 } // namespace ckv

@@ -1,0 +1,910 @@
+// Causal attention of tiles of query rows over keys that are not 16-bit pages: a cache held
+// in 4 bits (fp4.h), or the batch's own rows (whole prompts, packed one after another).
+// gfx950 matrix cores.
+//
+// A query row at position p attends keys 0..p of its sequence, softmax(q.k * scale)
+// weighted sum of v, online over blocks of 32 keys. The shape is that of the paged prefill's
+// workgroups of four waves (kernels_prefill.hip): each wave has 32 query vectors (32 rows of
+// one head), the waves share a kv head's key blocks through LDS, and per block
+//   S^T[key][query] = K . Q^T      D/16 x v_mfma_f32_32x32x16
+//   O^T[feature][query] += V^T . P^T  D/16 of them, P^T straight from registers
+// with S(kb) on the matrix cores while the vector ALU turns S(kb - 1) into probabilities.
+// Probabilities enter P.V in the rows' type; that rounding and the result's own come to 1.27
+// times the result's own (a second term for what the first left would cost half as many
+// products again).
+//
+// Staging goes through registers, a block ahead: 4-bit codes become the rows' type on the
+// way, exactly, once for the four waves; rows of any stride and alignment are taken as they
+// are. Three LDS stages, one barrier a block. Float rows have a kernel of their own below,
+// on v_mfma_f32_32x32x2 (exact products, as the paged f32 prefill).
+//
+// Keys past the tile's last position are staged as zeros. A masked key's probability is 0,
+// which meets its value in P.V all the same: where that is infinite or NaN, the rows that
+// got something that is not finite are attended again alone, by vector arithmetic over the
+// keys they attend.
+#include "ckv_internal.h"
+#include "fp4.h"
+#include "prefill_records.h"
+#include "prefill_tile.h"
+#include "store_rows.h"
+
+#include <algorithm>
+#include <cfloat>
+#include <cstdlib>
+
+namespace ckv {
+namespace {
+
+constexpr uint32_t block_keys = 32;
+constexpr uint32_t n_waves = 4, n_threads = 64 * n_waves;
+
+// Where a tile's keys are. Sequence positions are rows of `keys` and `values` (ROWS), or go
+// through a block table to 4-bit tiles.
+struct key_source {
+    const uint8_t* keys;
+    const uint8_t* values;
+    const uint32_t* table;
+    uint64_t stride; // bytes of a row
+    uint32_t block_size, kv_heads, kvh;
+};
+
+template <int D>
+__device__ __forceinline__ uint64_t tile_offset(const key_source& s, uint32_t key)
+{
+    return fp4_tile_at(s.table[key / s.block_size] * s.block_size + key % s.block_size, s.kvh,
+                       s.block_size, s.kv_heads, D);
+}
+
+__device__ __forceinline__ float word_half(uint32_t w, int e, bool f16)
+{
+    return f16 ? half_value<true>((uint16_t)(w >> (16 * e)))
+               : __builtin_bit_cast(float, e ? w & 0xFFFF0000u : w << 16);
+}
+
+// D/16 features from `f` on of a key's (or value's) row, as floats.
+template <int D, int DT, bool FP4>
+__device__ __forceinline__ void load_features(const key_source& s, uint32_t key, uint32_t f, bool v,
+                                              float (&x)[D / 16])
+{
+    constexpr uint32_t each = D / 16;
+    if constexpr (FP4) {
+        const uint8_t* tile = (v ? s.values : s.keys) + tile_offset<D>(s, key);
+        const uint32_t t = key % fp4_tile;
+#pragma unroll
+        for (uint32_t i = 0; i < each; i += 4) { // four features: half a word
+            const uint8_t* at = tile + fp4_word_at(D, t, (f + i) / 8, v) + ((f + i) % 8 ? (v && D == 64 ? 8 : 2) : 0);
+            const uint32_t codes = *reinterpret_cast<const uint16_t*>(at);
+            const float scale = fp4_scale(tile[fp4_scale_at(D, t, (f + i) / 32, v)]);
+            const uint32_t lo = fp4_bf16_pair<0>(codes, scale), hi = fp4_bf16_pair<1>(codes, scale);
+            x[i] = word_half(lo, 0, false);
+            x[i + 1] = word_half(lo, 1, false);
+            x[i + 2] = word_half(hi, 0, false);
+            x[i + 3] = word_half(hi, 1, false);
+        }
+    } else {
+        const uint8_t* row = (v ? s.values : s.keys) + key * s.stride;
+#pragma unroll
+        for (uint32_t i = 0; i < each; ++i)
+            if constexpr (DT == CKV_F32)
+                x[i] = reinterpret_cast<const float*>(row)[f + i];
+            else
+                x[i] = half_value<DT == CKV_F16>(reinterpret_cast<const uint16_t*>(row)[f + i]);
+    }
+}
+
+// One query row by vector arithmetic, four keys a step, sixteen lanes a key.
+template <int D, int DT, bool FP4, class T>
+__device__ __forceinline__ void attend_row(const key_source& s, uint32_t position, const T* q, float c,
+                                           const T* gate, T* out, uint32_t lane)
+{
+    constexpr uint32_t each = D / 16;
+    const uint32_t f = (lane & 15) * each, sub = lane >> 4;
+    float qf[each], acc[each], m = -FLT_MAX, l = 0.0f;
+    auto element = [](const T* at) {
+        if constexpr (DT == CKV_F32)
+            return *at;
+        else
+            return half_value<DT == CKV_F16>(*at);
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < each; ++j) {
+        qf[j] = element(q + f + j);
+        acc[j] = 0.0f;
+    }
+    auto weight = [&](float a, float b) { return __builtin_amdgcn_exp2f(a - b); };
+#pragma unroll 1
+    for (uint32_t key0 = 0; key0 <= position; key0 += 4) {
+        const uint32_t key = min(key0 + sub, position);
+        float x[each], score = 0.0f;
+        load_features<D, DT, FP4>(s, key, f, false, x);
+#pragma unroll
+        for (uint32_t j = 0; j < each; ++j)
+            score = __builtin_fmaf(qf[j], x[j], score);
+#pragma unroll
+        for (uint32_t d = 1; d < 16; d *= 2)
+            score += __shfl_xor(score, d);
+        score *= c;
+        load_features<D, DT, FP4>(s, key, f, true, x);
+        if (key0 + sub <= position) {
+            const float m_new = fmaxf(m, score);
+            const float keep = weight(m, m_new), w = weight(score, m_new);
+            m = m_new;
+            l = l * keep + w;
+#pragma unroll
+            for (uint32_t j = 0; j < each; ++j)
+                acc[j] = acc[j] * keep + w * x[j];
+        }
+    }
+#pragma unroll
+    for (uint32_t d = 16; d < 64; d *= 2) {
+        const float m_other = __shfl_xor(m, d), l_other = __shfl_xor(l, d);
+        const float m_new = fmaxf(m, m_other);
+        const float keep = weight(m, m_new), w = weight(m_other, m_new);
+        m = m_new;
+        l = l * keep + l_other * w;
+#pragma unroll
+        for (uint32_t j = 0; j < each; ++j) {
+            const float other = __shfl_xor(acc[j], d);
+            acc[j] = acc[j] * keep + other * w;
+        }
+    }
+    if (sub)
+        return;
+#pragma unroll
+    for (uint32_t j = 0; j < each; ++j) {
+        float y = acc[j] / l;
+        if (gate)
+            y *= sigmoid(element(gate + f + j));
+        if constexpr (DT == CKV_F32)
+            out[f + j] = y;
+        else
+            out[f + j] = (uint16_t)pack2<DT == CKV_F16>(y, 0.0f);
+    }
+}
+
+// A workgroup's part of a launch.
+struct tile_part {
+    uint32_t pair;  // the (tile, pass, kv head)
+    uint32_t kvh, pass, part;
+    uint32_t row0, nrows, pos0, pos_last;
+    uint32_t table; // the sequence's first table entry
+    uint32_t n_blocks, n_parts, kb_begin, kb_end;
+};
+
+// Blocks run over kv heads, then passes, then tiles, then key ranges. False: no keys.
+__device__ __forceinline__ bool part_of(const meta_view& md, uint32_t kv_heads, uint32_t passes,
+                                        const prefill_split& split, tile_part& w)
+{
+    w.kvh = blockIdx.x % kv_heads;
+    const uint32_t unit = blockIdx.x / kv_heads;
+    w.pass = unit % passes;
+    const uint32_t tile = unit / passes % md.n_tiles;
+    w.part = unit / passes / md.n_tiles;
+    w.pair = (tile * passes + w.pass) * kv_heads + w.kvh;
+    const uint4 te = *reinterpret_cast<const uint4*>(md.tiles + tile_entry_words * tile);
+    w.row0 = te.x;
+    w.nrows = te.y;
+    w.pos0 = te.z;
+    w.table = te.w;
+    w.pos_last = w.pos0 + w.nrows - 1;
+    w.n_blocks = w.pos_last / block_keys + 1;
+    w.n_parts = prefill_range_count(w.n_blocks, split.n_split, split.min_blocks);
+    if (w.part >= w.n_parts)
+        return false;
+    prefill_range_bounds(w.n_blocks, w.n_parts, w.part, w.kb_begin, w.kb_end);
+    return true;
+}
+
+// The state of a query vector's range of keys, as records in chunks of four floats, chunk 0
+// [max, denominator, 0, 0], chunk-major over the workgroup's 128 vectors. The range that
+// arrives last folds all, in their order. Lane (n, g) of the accumulator layout holds
+// features 32mt + 8quad + 4g + e in o[mt][4quad + e]. Returns false for the others.
+template <int D>
+__device__ __forceinline__ bool fold_ranges(const prefill_split& split, const tile_part& w, uint32_t qv,
+                                            uint32_t g, uint32_t tid, float c, float m, float& lt,
+                                            f32x16_t (&o)[D / 32], uint32_t* last_flag)
+{
+    constexpr uint32_t QV = 32 * n_waves, chunks = (D + 4) / 4;
+    const __amdgpu_buffer_rsrc_t rs = record_rsrc(
+        split.records + (uint64_t)w.pair * split.n_split * (chunks * QV * 4), split.n_split * chunks * QV * 16);
+    auto off = [&](uint32_t share, uint32_t chunk) { return ((share * chunks + chunk) * QV + qv) * 16u; };
+#pragma unroll
+    for (int mt = 0; mt < D / 32; ++mt)
+#pragma unroll
+        for (int quad = 0; quad < 4; ++quad) {
+            const f32x16_t& acc = o[mt];
+            agent_store4(rs, off(w.part, 1 + 8 * mt + 2 * quad + g), acc[4 * quad], acc[4 * quad + 1],
+                         acc[4 * quad + 2], acc[4 * quad + 3]);
+        }
+    if (g == 0)
+        agent_store4(rs, off(w.part, 0), m, lt, 0.0f, 0.0f);
+    wait_vector_memory();
+    __syncthreads(); // also: every wave is past its LDS reads
+    if (tid == 0) {
+        const uint32_t before = __hip_atomic_fetch_add(split.arrivals + w.pair, 1u, __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t last = before == w.n_parts - 1;
+        if (last)
+            __hip_atomic_store(split.arrivals + w.pair, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *last_flag = last;
+    }
+    __syncthreads();
+    if (!*last_flag)
+        return false;
+    float M = -__builtin_inff();
+    auto weight = [&](float ms, float to) { // 0 for a range that attended nothing
+        return ms == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((ms - to) * c);
+    };
+    lt = 0.0f;
+#pragma unroll
+    for (int mt = 0; mt < D / 32; ++mt)
+        o[mt] = f32x16_t {};
+#pragma unroll 1
+    for (uint32_t s = 0; s < w.n_parts; ++s) {
+        const u32x4_t head = agent_load4(rs, off(s, 0));
+        u32x4_t v[D / 8];
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+            v[j] = agent_load4(rs, off(s, 1 + 2 * j + g));
+        const float ms = __uint_as_float(head[0]);
+        const float m_new = fmaxf(M, ms);
+        const float keep = weight(M, m_new), take = weight(ms, m_new);
+        M = m_new;
+        lt = lt * keep + __uint_as_float(head[1]) * take;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                o[j / 4][4 * (j % 4) + e] = o[j / 4][4 * (j % 4) + e] * keep + __uint_as_float(v[j][e]) * take;
+    }
+    return true;
+}
+
+// What a thread holds of a block on its way to LDS: 16-bit rows, or 4-bit codes.
+template <int D, bool FP4>
+struct staged;
+template <int D>
+struct staged<D, false> {
+    static constexpr uint32_t per = D / 64; // 16-byte words of K, and of V: 32 rows of D/8
+    uint4 k[per], v[per];
+};
+template <int D>
+struct staged<D, true> {
+    // 4-byte words of K or of V: threads below half take K, the others V
+    static constexpr uint32_t words = D / 32;
+    uint32_t code[words];
+    uint32_t scale[D == 256 ? 2 : 1];
+};
+
+// 16-bit rows. GH heads of a GQA group share a workgroup: 128 / GH rows.
+template <int D, int GH, bool F16, bool FP4>
+__global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
+    pool_view p, meta_view md, uint32_t layer, prompt_rows x, uint16_t* __restrict__ out, uint32_t q_heads,
+    float c, uint32_t q_and, uint32_t q_xor, const uint16_t* __restrict__ gate, prefill_split split)
+{
+    constexpr int KS = D / 16, MT = D / 32, DT = F16 ? CKV_F16 : CKV_BF16;
+    constexpr uint32_t n_stages = 3;
+    // K stage: chunk i (features 8i .. 8i + 7) holds the block's keys in the LDS rows of the
+    // A operand, 16 bytes each; 16 more bytes a chunk spread a key's chunks over the banks.
+    constexpr uint32_t k_chunk = block_keys * 16 + 16, k_bytes = D / 8 * k_chunk;
+    // V stage: rows as they are, read transposed; key k is row (k / 4) % 4 of group
+    // k % 4 + 4 * (k / 16), 64 bytes between groups (kernels_prefill.hip).
+    constexpr uint32_t v_row = 2 * D, v_group = 4 * v_row + 64, v_bytes = 8 * v_group;
+    constexpr uint32_t stage_bytes = k_bytes + v_bytes;
+    constexpr uint32_t out_bytes = n_waves * 32 * row_floats<D> * 4;
+    constexpr uint32_t lds_bytes = n_stages * stage_bytes > out_bytes ? n_stages * stage_bytes : out_bytes;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[lds_bytes];
+    const uint32_t group = q_heads / p.kv_heads;
+    tile_part w;
+    if (!part_of(md, p.kv_heads, group / GH, split, w))
+        return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t n = lane & 31, g = lane >> 5;
+    const uint32_t head = w.kvh * group + w.pass * GH + wave % GH, rb = wave / GH;
+    const uint32_t row = rb * 32 + n;
+    const bool valid = row < w.nrows;
+    const uint32_t qpos = w.pos0 + min(row, w.nrows - 1);
+    const uint32_t pos_lo = w.pos0 + rb * 32;
+
+    key_source s;
+    if constexpr (FP4) {
+        const uint64_t layer_bytes = (uint64_t)p.blocks * p.block_size / fp4_tile * p.kv_heads * fp4_tile_bytes(D);
+        s = { static_cast<const uint8_t*>(p.keys) + layer * layer_bytes,
+              static_cast<const uint8_t*>(p.values) + layer * layer_bytes, md.table + w.table, 0, p.block_size,
+              p.kv_heads, w.kvh };
+    } else {
+        const uint64_t first = (uint64_t)(w.row0 - w.pos0) * x.kv_stride + w.kvh * D;
+        s = { static_cast<const uint8_t*>(x.keys) + 2 * first, static_cast<const uint8_t*>(x.values) + 2 * first,
+              nullptr, 2 * x.kv_stride, 0, 0, 0 };
+    }
+    const bool k_vector = !FP4 && x.vectors;
+
+    const uint16_t* q_row = static_cast<const uint16_t*>(x.queries)
+        + (uint64_t)(w.row0 + min(row, w.nrows - 1)) * x.q_stride + (uint64_t)head * D;
+    uint4 qr[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (valid) {
+            const uint16_t* at = q_row + ks * 16 + g * 8;
+            if (x.vectors)
+                v = *reinterpret_cast<const uint4*>(at);
+            else
+                v = make_uint4(at[0] | (uint32_t)at[1] << 16, at[2] | (uint32_t)at[3] << 16,
+                               at[4] | (uint32_t)at[5] << 16, at[6] | (uint32_t)at[7] << 16);
+        }
+        // a negative scale turns the queries' sign, a scale of 0 leaves nothing of them
+        qr[ks] = make_uint4((v.x & q_and) ^ q_xor, (v.y & q_and) ^ q_xor, (v.z & q_and) ^ q_xor, (v.w & q_and) ^ q_xor);
+    }
+
+    using held = staged<D, FP4>;
+    held next;
+    // block kb's words of this thread into registers
+    auto load = [&](uint32_t kb) {
+        const uint32_t key0 = kb * block_keys;
+        if constexpr (FP4) {
+            constexpr uint32_t W = held::words;
+            const bool v = tid >= n_threads / 2;
+            const uint32_t t = tid % (n_threads / 2);
+            const uint32_t tile = t / 64, at = t % 64; // of the block's two tiles
+            const uint32_t key = min(key0 + tile * fp4_tile, w.pos_last / fp4_tile * fp4_tile);
+            const uint8_t* base = (v ? s.values : s.keys) + tile_offset<D>(s, key);
+            // lane (c, quarter) of the tile: K: token at / 4, part at % 4; V: quarter at / 16, c at % 16
+            if constexpr (D == 64) {
+                const uint2 r = *reinterpret_cast<const uint2*>(base + at * 8);
+                next.code[0] = r.x;
+                next.code[1] = r.y;
+                next.scale[0] = v ? *reinterpret_cast<const uint32_t*>(base + 8 * D + at % 16 / 8 * 16 + at / 16 * 4)
+                                  : base[8 * D + at / 4 * 2 + at % 4 / 2];
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < W / 4; ++i) {
+                    const uint32_t off = v ? i * 1024 + at * 16 : at / 4 * (D / 2) + i * 64 + at % 4 * 16;
+                    const uint4 r = *reinterpret_cast<const uint4*>(base + off);
+                    next.code[4 * i] = r.x;
+                    next.code[4 * i + 1] = r.y;
+                    next.code[4 * i + 2] = r.z;
+                    next.code[4 * i + 3] = r.w;
+                    next.scale[i] = v
+                        ? *reinterpret_cast<const uint32_t*>(base + 8 * D + (4 * i + at % 16 / 4) * 16 + at / 16 * 4)
+                        : base[8 * D + at / 4 * (D / 32) + 4 * i + at % 4];
+                }
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < held::per; ++i) {
+                const uint32_t word = i * n_threads + tid, key = key0 + word / (D / 8), f = word % (D / 8) * 8;
+                const uint64_t at = min(key, w.pos_last) * s.stride + 2 * f;
+                if (k_vector) {
+                    next.k[i] = *reinterpret_cast<const uint4*>(s.keys + at);
+                    next.v[i] = *reinterpret_cast<const uint4*>(s.values + at);
+                } else {
+                    const auto gather = [](const uint8_t* from) {
+                        const auto* e = reinterpret_cast<const uint16_t*>(from);
+                        return make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
+                                          e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+                    };
+                    next.k[i] = gather(s.keys + at);
+                    next.v[i] = gather(s.values + at);
+                }
+            }
+        }
+    };
+    auto put_k = [&](uint8_t* st, uint32_t key, uint32_t chunk, uint4 v) {
+        *reinterpret_cast<uint4*>(st + chunk * k_chunk + key_row(key) * 16) = v;
+    };
+    auto v_at = [&](uint8_t* st, uint32_t key) {
+        return st + k_bytes + (key % 4 + 4 * (key / 16)) * v_group + key / 4 % 4 * v_row;
+    };
+    // and from there into its stage, zeros past the tile's last position
+    auto store = [&](uint32_t kb) {
+        uint8_t* st = lds + kb % n_stages * stage_bytes;
+        const uint32_t key0 = kb * block_keys;
+        const bool whole = key0 + block_keys - 1 <= w.pos_last;
+        if constexpr (FP4) {
+            const uint32_t t = tid % (n_threads / 2), tile = t / 64, at = t % 64;
+            if (tid < n_threads / 2) {
+                const uint32_t key = tile * fp4_tile + at / 4;
+                const bool there = whole || key0 + key <= w.pos_last;
+                if constexpr (D == 64) {
+                    const float scale = there ? fp4_scale(next.scale[0]) : 1.0f;
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i)
+                        put_k(st, key, at % 4 * 2 + i, fp4_eight<F16>(there ? next.code[i] : 0, scale));
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < held::words; ++i) {
+                        const float scale = there ? fp4_scale(next.scale[i / 4]) : 1.0f;
+                        put_k(st, key, i / 4 * 16 + at % 4 * 4 + i % 4, fp4_eight<F16>(there ? next.code[i] : 0, scale));
+                    }
+                }
+            } else {
+                const uint32_t token0 = tile * fp4_tile + at / 16 * 4, cc = at % 16;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const bool there = whole || key0 + token0 + i <= w.pos_last;
+                    uint8_t* to = v_at(st, token0 + i);
+#pragma unroll
+                    for (uint32_t part = 0; part < (D == 256 ? 2 : 1); ++part) {
+                        const float scale = there ? fp4_scale(next.scale[part] >> (8 * i) & 255) : 1.0f;
+                        if constexpr (D == 64) {
+                            const uint32_t codes = there ? next.code[i / 2] >> (16 * (i % 2)) : 0;
+                            *reinterpret_cast<uint2*>(to + cc * 8) =
+                                make_uint2(fp4_pair<0, F16>(codes, scale), fp4_pair<1, F16>(codes, scale));
+                        } else {
+                            *reinterpret_cast<uint4*>(to + part * 256 + cc * 16) =
+                                fp4_eight<F16>(there ? next.code[4 * part + i] : 0, scale);
+                        }
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < held::per; ++i) {
+                const uint32_t word = i * n_threads + tid, key = word / (D / 8), chunk = word % (D / 8);
+                const bool there = whole || key0 + key <= w.pos_last;
+                const uint4 zero = make_uint4(0, 0, 0, 0);
+                put_k(st, key, chunk, there ? next.k[i] : zero);
+                *reinterpret_cast<uint4*>(v_at(st, key) + chunk * 16) = there ? next.v[i] : zero;
+            }
+        }
+    };
+
+    f32x16_t o[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+        o[mt] = f32x16_t {};
+    float m = -__builtin_inff(), l = 0.0f, m_limit = -__builtin_inff(), mx = 0.0f;
+    const float rescale_raw = rescale_log2 / c;
+    f32x16_t sc, sp;
+    auto scores = [&](uint32_t kb) {
+        const uint8_t* kl = lds + kb % n_stages * stage_bytes + g * k_chunk + n * 16;
+        uint4 ka[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            ka[ks] = *reinterpret_cast<const uint4*>(kl + ks * 2 * k_chunk);
+        sc = f32x16_t {};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            sc = mfma<F16>(ka[ks], qr[ks], sc);
+    };
+    auto probabilities = [&](uint4 (&pt)[2]) {
+        // a range of the keys may hold none that a row attends: its maximum stays -inf
+        const float mc = m == -__builtin_inff() ? 0.0f : m * c;
+        float sum[4];
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            sp[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sp[r], c, -mc));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            sum[i] = (sp[4 * i] + sp[4 * i + 1]) + (sp[4 * i + 2] + sp[4 * i + 3]);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            pt[h] = make_uint4(pack2<F16>(sp[8 * h], sp[8 * h + 1]), pack2<F16>(sp[8 * h + 2], sp[8 * h + 3]),
+                               pack2<F16>(sp[8 * h + 4], sp[8 * h + 5]), pack2<F16>(sp[8 * h + 6], sp[8 * h + 7]));
+    };
+    const uint32_t vr_off = ((lane & 15) >> 2) * v_group + (lane >> 5) * 2 * v_row + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+    auto values = [&](uint32_t kb, const uint4 (&pt)[2]) {
+        uint32_t vaddr = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) uint8_t*)(lds + kb % n_stages * stage_bytes + k_bytes)) + vr_off;
+        asm volatile("" : "+v"(vaddr));
+        auto* vb = (__attribute__((address_space(3))) uint8_t*)(uintptr_t)vaddr;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) i16x4_t*)(vb + 4 * h * v_group + 64 * mt));
+                const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) i16x4_t*)(vb + 4 * h * v_group + v_row + 64 * mt));
+                const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+                o[mt] = mfma<F16>(make_uint4(l2.x, l2.y, h2.x, h2.y), pt[h], o[mt]);
+            }
+    };
+    auto stats = [&](uint32_t kb) {
+        const uint32_t key0 = kb * block_keys;
+        if (key0 + block_keys - 1 > pos_lo) { // the diagonal crosses this block
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (key0 + 16 * (r >> 3) + 8 * g + (r & 7) > qpos)
+                    sc[r] = -__builtin_inff();
+        }
+        sp = sc;
+        mx = lane_max(sp);
+        if (__any(mx > m_limit)) {
+            const float m_new = fmaxf(m, pair_max(mx));
+            const float alpha = m_new == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - m_new) * c);
+            l *= alpha;
+            m = m_new;
+            m_limit = m_new + rescale_raw;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+                o[mt] *= alpha;
+        }
+    };
+
+    load(w.kb_begin);
+    store(w.kb_begin);
+    if (w.kb_begin + 1 < w.kb_end)
+        load(w.kb_begin + 1);
+    __syncthreads();
+    // Iteration kb finishes block kb - 1 and scores block kb; it stages block kb + 1, whose
+    // stage was block kb - 2's, last read in iteration kb - 1.
+    uint32_t kb = w.kb_begin;
+    scores(kb);
+    if (kb + 1 < w.kb_end)
+        store(kb + 1);
+    if (kb + 2 < w.kb_end)
+        load(kb + 2);
+    stats(kb);
+    __syncthreads();
+    for (++kb; kb < w.kb_end; ++kb) {
+        uint4 pt[2];
+        probabilities(pt);
+        scores(kb);
+        if (kb + 1 < w.kb_end)
+            store(kb + 1);
+        if (kb + 2 < w.kb_end)
+            load(kb + 2);
+        values(kb - 1, pt);
+        stats(kb);
+        __syncthreads();
+    }
+    {
+        uint4 pt[2];
+        probabilities(pt);
+        values(kb - 1, pt);
+    }
+
+    float lt = l + __shfl_xor(l, 32);
+    if (w.n_parts > 1) {
+        if (!fold_ranges<D>(split, w, wave * 32 + n, g, tid, c, m, lt, o, reinterpret_cast<uint32_t*>(lds)))
+            return;
+    }
+    const float inv = 1.0f / lt;
+    float odd = inv * 0.0f; // 0 unless some result of the query is infinite or NaN
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            odd = __builtin_fmaf(o[mt][r], 0.0f, odd);
+    const uint64_t odd_lanes = __ballot(valid && odd != 0.0f);
+    uint32_t alone = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
+    __syncthreads(); // every wave is past its LDS reads
+    float* tile_out = reinterpret_cast<float*>(lds) + wave * (32 * row_floats<D>);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int quad = 0; quad < 4; ++quad) {
+            const f32x16_t& acc = o[mt];
+            *reinterpret_cast<float4*>(tile_out + n * row_floats<D> + 32 * mt + 8 * quad + 4 * g) =
+                make_float4(acc[4 * quad] * inv, acc[4 * quad + 1] * inv, acc[4 * quad + 2] * inv, acc[4 * quad + 3] * inv);
+        }
+    const uint32_t there = rb * 32 < w.nrows ? min(w.nrows - rb * 32, 32u) : 0;
+    const size_t o_stride = (size_t)q_heads * D;
+    const size_t first = (size_t)(w.row0 + rb * 32) * o_stride + (size_t)head * D;
+    if (x.out_vectors) {
+        store_rows<D, DT>(tile_out, lane, there, alone, out + first, o_stride, gate ? gate + first : nullptr);
+    } else {
+        for (uint32_t r = 0; r < there; ++r)
+            for (uint32_t f = lane; f < D; f += 64)
+                if (!(alone >> r & 1)) {
+                    float y = tile_out[r * row_floats<D> + f];
+                    if (gate)
+                        y *= sigmoid(half_value<F16>(gate[first + r * o_stride + f]));
+                    out[first + r * o_stride + f] = (uint16_t)pack2<F16>(y, 0.0f);
+                }
+    }
+    const float cs = q_and ? (q_xor ? -c : c) : 0.0f; // the scale in log2 units
+    while (__builtin_expect(alone != 0, 0)) {
+        const uint32_t r = __builtin_ctz(alone);
+        alone &= alone - 1;
+        const size_t at = first + r * o_stride;
+        attend_row<D, DT, FP4>(s, pos_lo + r, static_cast<const uint16_t*>(x.queries) + (uint64_t)(w.row0 + rb * 32 + r) * x.q_stride + (uint64_t)head * D,
+                               cs, gate ? gate + at : nullptr, out + at, lane);
+    }
+}
+
+// Float rows: S^T and O^T on v_mfma_f32_32x32x2, D/2 and D/2 products a block. The
+// contraction over features pairs 8i + e with 8i + 4 + e, so that a lane's operands are
+// 16-byte words; that over keys pairs the two keys of an accumulator element, so that a
+// probability is an operand where it was computed. Two LDS stages of whole rows.
+template <int D, int GH, bool FP4>
+__global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel(
+    pool_view p, meta_view md, uint32_t layer, prompt_rows x, float* __restrict__ out, uint32_t q_heads,
+    float c, float q_sign, const float* __restrict__ gate, prefill_split split)
+{
+    constexpr int MT = D / 32, K4 = D / 8;
+    constexpr uint32_t pitch = D + 4, stage_floats = 2 * block_keys * pitch;
+    __shared__ __attribute__((aligned(16))) float lds[2 * stage_floats];
+    static_assert(n_waves * 32 * row_floats<D> <= 2 * stage_floats);
+    const uint32_t group = q_heads / p.kv_heads;
+    tile_part w;
+    if (!part_of(md, p.kv_heads, group / GH, split, w))
+        return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t n = lane & 31, g = lane >> 5;
+    const uint32_t head = w.kvh * group + w.pass * GH + wave % GH, rb = wave / GH;
+    const uint32_t row = rb * 32 + n;
+    const bool valid = row < w.nrows;
+    const uint32_t qpos = w.pos0 + min(row, w.nrows - 1);
+    const uint32_t pos_lo = w.pos0 + rb * 32;
+    key_source s;
+    if constexpr (FP4) {
+        const uint64_t layer_bytes = (uint64_t)p.blocks * p.block_size / fp4_tile * p.kv_heads * fp4_tile_bytes(D);
+        s = { static_cast<const uint8_t*>(p.keys) + layer * layer_bytes,
+              static_cast<const uint8_t*>(p.values) + layer * layer_bytes, md.table + w.table, 0, p.block_size,
+              p.kv_heads, w.kvh };
+    } else {
+        const uint64_t first = (uint64_t)(w.row0 - w.pos0) * x.kv_stride + w.kvh * D;
+        s = { static_cast<const uint8_t*>(x.keys) + 4 * first, static_cast<const uint8_t*>(x.values) + 4 * first,
+              nullptr, 4 * x.kv_stride, 0, 0, 0 };
+    }
+    const float* q_row = static_cast<const float*>(x.queries)
+        + (uint64_t)(w.row0 + min(row, w.nrows - 1)) * x.q_stride + (uint64_t)head * D;
+    float4 qr[K4];
+#pragma unroll
+    for (int i = 0; i < K4; ++i) {
+        float4 v = make_float4(0, 0, 0, 0);
+        if (valid) {
+            const float* at = q_row + 8 * i + 4 * g;
+            v = x.vectors ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[1], at[2], at[3]);
+        }
+        qr[i] = q_sign == 0.0f ? make_float4(0, 0, 0, 0)
+                               : make_float4(v.x * q_sign, v.y * q_sign, v.z * q_sign, v.w * q_sign);
+    }
+    constexpr uint32_t per = FP4 ? D / 64 : D / 32; // 8-feature words, or 16-byte words
+    uint32_t code_k[FP4 ? per : 1], code_v[FP4 ? per : 1], scale_k[FP4 ? per : 1], scale_v[FP4 ? per : 1];
+    float4 next_k[FP4 ? 1 : per], next_v[FP4 ? 1 : per];
+    auto load = [&](uint32_t kb) {
+        const uint32_t key0 = kb * block_keys;
+#pragma unroll
+        for (uint32_t i = 0; i < per; ++i) {
+            const uint32_t word = i * n_threads + tid;
+            if constexpr (FP4) {
+                const uint32_t key = min(key0 + word / (D / 8), w.pos_last), f8 = word % (D / 8), t = key % fp4_tile;
+                const uint64_t at = tile_offset<D>(s, key);
+                code_k[i] = *reinterpret_cast<const uint32_t*>(s.keys + at + fp4_word_at(D, t, f8, false));
+                const uint8_t* v = s.values + at + fp4_word_at(D, t, f8, true);
+                if constexpr (D == 64)
+                    code_v[i] = *reinterpret_cast<const uint16_t*>(v) | (uint32_t)*reinterpret_cast<const uint16_t*>(v + 8) << 16;
+                else
+                    code_v[i] = *reinterpret_cast<const uint32_t*>(v);
+                scale_k[i] = s.keys[at + fp4_scale_at(D, t, f8 / 4, false)];
+                scale_v[i] = s.values[at + fp4_scale_at(D, t, f8 / 4, true)];
+            } else {
+                const uint32_t key = min(key0 + word / (D / 4), w.pos_last), f = word % (D / 4) * 4;
+                const float* k = reinterpret_cast<const float*>(s.keys + key * s.stride) + f;
+                const float* v = reinterpret_cast<const float*>(s.values + key * s.stride) + f;
+                if (x.vectors) {
+                    next_k[i] = *reinterpret_cast<const float4*>(k);
+                    next_v[i] = *reinterpret_cast<const float4*>(v);
+                } else {
+                    next_k[i] = make_float4(k[0], k[1], k[2], k[3]);
+                    next_v[i] = make_float4(v[0], v[1], v[2], v[3]);
+                }
+            }
+        }
+    };
+    auto store = [&](uint32_t kb) {
+        float* st = lds + kb % 2 * stage_floats;
+        const uint32_t key0 = kb * block_keys;
+        const float4 zero = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (uint32_t i = 0; i < per; ++i) {
+            const uint32_t word = i * n_threads + tid;
+            if constexpr (FP4) {
+                const uint32_t key = word / (D / 8), f = word % (D / 8) * 8;
+                const bool there = key0 + key <= w.pos_last;
+                auto put = [&](float* to, uint32_t code, uint32_t byte) {
+                    const uint4 v = fp4_eight<false>(there ? code : 0, there ? fp4_scale(byte) : 1.0f);
+                    reinterpret_cast<float4*>(to)[0] = make_float4(word_half(v.x, 0, false), word_half(v.x, 1, false), word_half(v.y, 0, false), word_half(v.y, 1, false));
+                    reinterpret_cast<float4*>(to)[1] = make_float4(word_half(v.z, 0, false), word_half(v.z, 1, false), word_half(v.w, 0, false), word_half(v.w, 1, false));
+                };
+                put(st + key * pitch + f, code_k[i], scale_k[i]);
+                put(st + (block_keys + key) * pitch + f, code_v[i], scale_v[i]);
+            } else {
+                const uint32_t key = word / (D / 4), f = word % (D / 4) * 4;
+                const bool there = key0 + key <= w.pos_last;
+                *reinterpret_cast<float4*>(st + key * pitch + f) = there ? next_k[i] : zero;
+                *reinterpret_cast<float4*>(st + (block_keys + key) * pitch + f) = there ? next_v[i] : zero;
+            }
+        }
+    };
+
+    f32x16_t o[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+        o[mt] = f32x16_t {};
+    float m = -__builtin_inff(), l = 0.0f, m_limit = -__builtin_inff();
+    const float rescale_raw = rescale_log2 / c;
+    load(w.kb_begin);
+    store(w.kb_begin);
+    __syncthreads();
+    for (uint32_t kb = w.kb_begin; kb < w.kb_end; ++kb) {
+        if (kb + 1 < w.kb_end)
+            load(kb + 1);
+        const float* st = lds + kb % 2 * stage_floats;
+        const uint32_t key0 = kb * block_keys;
+        f32x16_t sc {};
+#pragma unroll
+        for (int i = 0; i < K4; ++i) {
+            const float4 a = *reinterpret_cast<const float4*>(st + n * pitch + 8 * i + 4 * g);
+            sc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, qr[i].x, sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, qr[i].y, sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, qr[i].z, sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, qr[i].w, sc, 0, 0, 0);
+        }
+        if (key0 + block_keys - 1 > pos_lo) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (key0 + 8 * (r >> 2) + 4 * g + (r & 3) > qpos)
+                    sc[r] = -__builtin_inff();
+        }
+        const float mx = lane_max(sc);
+        if (__any(mx > m_limit)) {
+            const float m_new = fmaxf(m, pair_max(mx));
+            const float alpha = m_new == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - m_new) * c);
+            l *= alpha;
+            m = m_new;
+            m_limit = m_new + rescale_raw;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+                o[mt] *= alpha;
+        }
+        const float mc = m == -__builtin_inff() ? 0.0f : m * c;
+        float sum[4] = {};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], c, -mc));
+            sum[r & 3] += sc[r];
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float* v = st + (block_keys + 8 * (r >> 2) + 4 * g + (r & 3)) * pitch + n;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+                o[mt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[32 * mt], sc[r], o[mt], 0, 0, 0);
+        }
+        if (kb + 1 < w.kb_end)
+            store(kb + 1); // block kb - 1's stage, last read before the barrier
+        __syncthreads();
+    }
+    float lt = l + __shfl_xor(l, 32);
+    if (w.n_parts > 1) {
+        if (!fold_ranges<D>(split, w, wave * 32 + n, g, tid, c, m, lt, o, reinterpret_cast<uint32_t*>(lds)))
+            return;
+        __syncthreads(); // the flag is read
+    }
+    const float inv = 1.0f / lt;
+    float odd = inv * 0.0f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            odd = __builtin_fmaf(o[mt][r], 0.0f, odd);
+    const uint64_t odd_lanes = __ballot(valid && odd != 0.0f);
+    uint32_t alone = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
+    float* tile_out = lds + wave * (32 * row_floats<D>);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int quad = 0; quad < 4; ++quad) {
+            const f32x16_t& acc = o[mt];
+            *reinterpret_cast<float4*>(tile_out + n * row_floats<D> + 32 * mt + 8 * quad + 4 * g) =
+                make_float4(acc[4 * quad] * inv, acc[4 * quad + 1] * inv, acc[4 * quad + 2] * inv, acc[4 * quad + 3] * inv);
+        }
+    const uint32_t there = rb * 32 < w.nrows ? min(w.nrows - rb * 32, 32u) : 0;
+    const size_t o_stride = (size_t)q_heads * D;
+    const size_t first = (size_t)(w.row0 + rb * 32) * o_stride + (size_t)head * D;
+    if (x.out_vectors) {
+        store_rows<D, CKV_F32>(tile_out, lane, there, alone, out + first, o_stride, gate ? gate + first : nullptr);
+    } else {
+        for (uint32_t r = 0; r < there; ++r)
+            for (uint32_t f = lane; f < D; f += 64)
+                if (!(alone >> r & 1)) {
+                    float y = tile_out[r * row_floats<D> + f];
+                    if (gate)
+                        y *= sigmoid(gate[first + r * o_stride + f]);
+                    out[first + r * o_stride + f] = y;
+                }
+    }
+    while (__builtin_expect(alone != 0, 0)) {
+        const uint32_t r = __builtin_ctz(alone);
+        alone &= alone - 1;
+        const size_t at = first + r * o_stride;
+        attend_row<D, CKV_F32, FP4>(s, pos_lo + r, static_cast<const float*>(x.queries) + (uint64_t)(w.row0 + rb * 32 + r) * x.q_stride + (uint64_t)head * D,
+                                    c * q_sign, gate ? gate + at : nullptr, out + at, lane);
+    }
+}
+
+bool aligned16(const void* ptr)
+{
+    return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0;
+}
+
+template <int D, int GH, bool FP4>
+hipError_t launch_gh(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer, const prompt_rows& x,
+                     uint32_t q_heads, float scale, void* out, const void* gate, const prefill_split& split)
+{
+    const uint64_t grid = (uint64_t)m.n_tiles * (q_heads / GH) * split.n_split;
+    if (!grid)
+        return hipSuccess;
+    if (grid > 0x7FFFFFFFull)
+        return hipErrorInvalidValue;
+    const float c = scale == 0.0f ? log2e : __builtin_fabsf(scale) * log2e;
+    const dim3 blocks((uint32_t)grid), threads(n_threads);
+    if (p.dtype == CKV_F32) {
+        prompt_f32_kernel<D, GH, FP4><<<blocks, threads, 0, s>>>(
+            p, m, layer, x, static_cast<float*>(out), q_heads, c, scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f,
+            static_cast<const float*>(gate), split);
+        return hipGetLastError();
+    }
+    auto* kernel = p.dtype == CKV_F16 ? prompt_kernel<D, GH, true, FP4> : prompt_kernel<D, GH, false, FP4>;
+    kernel<<<blocks, threads, 0, s>>>(p, m, layer, x, static_cast<uint16_t*>(out), q_heads, c,
+                                      scale == 0.0f ? 0u : ~0u, scale < 0.0f ? 0x80008000u : 0u,
+                                      static_cast<const uint16_t*>(gate), split);
+    return hipGetLastError();
+}
+
+template <int D, bool FP4, class... Args>
+hipError_t launch_group(uint32_t heads, const Args&... args)
+{
+    return heads == 4 ? launch_gh<D, 4, FP4>(args...) : heads == 2 ? launch_gh<D, 2, FP4>(args...)
+                                                                  : launch_gh<D, 1, FP4>(args...);
+}
+
+template <bool FP4, class... Args>
+hipError_t launch_dim(uint32_t head_dim, uint32_t heads, const Args&... args)
+{
+    return head_dim == 64 ? launch_group<64, FP4>(heads, args...)
+        : head_dim == 128 ? launch_group<128, FP4>(heads, args...)
+                          : launch_group<256, FP4>(heads, args...);
+}
+
+// Heads of a GQA group that share a workgroup's key blocks.
+uint32_t heads_of(const pool_view& p, uint32_t q_heads)
+{
+    const uint32_t group = q_heads / p.kv_heads;
+    return group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+}
+
+} // namespace
+
+uint32_t prompt_tile_rows(const pool_view& p, uint32_t q_heads)
+{
+    return 32 * n_waves / heads_of(p, q_heads);
+}
+
+prefill_shape_info prompt_plan(const pool_view& p, const meta_view& m, uint32_t q_heads, int cu_count)
+{
+    prefill_shape_info plan { n_waves, 1, 4, 0, 0 };
+    const uint64_t grid = (uint64_t)m.n_tiles * (q_heads / heads_of(p, q_heads));
+    const uint64_t cus = (uint64_t)std::max(cu_count, 1);
+    if (grid && grid < cus)
+        plan.n_split = (uint32_t)std::min<uint64_t>(split_max, 2 * cus / grid);
+    if (plan.n_split > 1 && prefill_range_count(m.longest_blocks, plan.n_split, plan.min_blocks) == 1)
+        plan.n_split = 1;
+    if (plan.n_split > 1) {
+        plan.records_floats = grid * plan.n_split * 32 * n_waves * (p.head_dim + 4);
+        plan.counters = grid;
+    }
+    return plan;
+}
+
+hipError_t launch_prompt(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
+                         const prompt_rows& rows, uint32_t q_heads, float scale, void* out, const void* gate,
+                         bool fp4, const prefill_split& split)
+{
+    prompt_rows x = rows;
+    const uint32_t each = 16 / p.elem_size;
+    x.vectors = aligned16(x.queries) && x.q_stride % each == 0
+        && (fp4 || (aligned16(x.keys) && aligned16(x.values) && x.kv_stride % each == 0));
+    x.out_vectors = aligned16(out) && aligned16(gate);
+    const uint32_t heads = heads_of(p, q_heads);
+    return fp4 ? launch_dim<true>(p.head_dim, heads, s, p, m, layer, x, q_heads, scale, out, gate, split)
+               : launch_dim<false>(p.head_dim, heads, s, p, m, layer, x, q_heads, scale, out, gate, split);
+}
+
+} // namespace ckv

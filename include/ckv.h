@@ -140,7 +140,8 @@ int ckv_copy_to_host(ckv_context* ctx, void* host_dst, const void* device_src, s
  * "rope_append", "rope_append_decode", "sigmoid_mul", "checkpoint_export",
  * "checkpoint_import", "window_attention_decode", "window_attention_prefill",
  * "append_decode_window", "rope_append_decode_window", "rope_axes",
- * "rope_axes_append", "compact". */
+ * "rope_axes_append", "compact", "rotate", "rotate_append", "fp4_append", "fp4_gather",
+ * "fp4_attention_decode", "fp4_attention_prefill", "prompt_attention". */
 int ckv_profile_enable(ckv_context* ctx, int enabled);
 int ckv_profile_query(ckv_context* ctx, const char* kernel, double* total_ms,
                       uint64_t* launches);
@@ -158,6 +159,35 @@ int ckv_pool_create(ckv_context* ctx, size_t layers, size_t blocks, size_t block
 int ckv_pool_wrap(ckv_context* ctx, size_t layers, size_t blocks, size_t block_size,
                   size_t kv_heads, size_t head_dim, int dtype, void* keys, void* values,
                   ckv_pool** out);
+/* A pool that holds keys and values in 4 bits (no counterpart in the reference): each 32
+ * consecutive features of a head as 4-bit floats (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their
+ * negatives) times a power of two of their own, 17 bytes for 64 of bf16. dtype is that of
+ * the rows: of appended keys and values, queries, gates and outputs.
+ *   scale = 2^(floor(log2 m) - 2) for the largest magnitude m of the 32, at least 2^-23
+ *           (f16 rows) or 2^-100;
+ *   x is kept as the nearest of the 16 numbers to x / scale, ties to the even code, at
+ *   most 6; a block that holds an infinity or a NaN (or, rotated, 2^128) reads as NaN.
+ * Every cached number is one of the rows' type. Rows rotated on their way in
+ * (ckv_rope_append, ckv_rotate_append and their decode forms) are turned in 64 bits and
+ * rounded once.
+ * These take such a pool as any other: metadata uploads, ckv_append, ckv_gather (the
+ * numbers it holds), the attention calls without a window and their gated forms,
+ * ckv_append_decode, ckv_rope, ckv_rope_append, ckv_rope_append_decode, ckv_rope_axes, the
+ * ckv_rotate calls, ckv_prompt_attention, ckv_copy_blocks, ckv_decode_plan. The others that
+ * touch keys and values (windows, ckv_rope_axes_append, ckv_compact,
+ * ckv_append_decode_noalloc, checkpoints, ckv_element_offset) return unsupported_dtype.
+ * Attention takes any number of query heads per kv head and any scale, with products of
+ * bf16 terms that keep at least 16 bits of queries and probabilities in decode rows, and of
+ * the rows' type in prefill tiles (f32 rows: 24 bits in both).
+ * Checks: those of ckv_pool_create, in their order, where the block size must be a multiple
+ * of 16 (invalid_block_size) and head_dim 64, 128 or 256 (invalid_head_dimension); wrapped
+ * buffers must be aligned to 16 bytes (invalid_argument) and hold the bytes_each of
+ * ckv_pool_buffers: layers * blocks * block_size * kv_heads * head_dim * 17 / 32. */
+int ckv_pool_create_fp4(ckv_context* ctx, size_t layers, size_t blocks, size_t block_size,
+                        size_t kv_heads, size_t head_dim, int dtype, ckv_pool** out);
+int ckv_pool_wrap_fp4(ckv_context* ctx, size_t layers, size_t blocks, size_t block_size,
+                      size_t kv_heads, size_t head_dim, int dtype, void* keys, void* values,
+                      ckv_pool** out);
 int ckv_pool_destroy(ckv_pool* pool);
 int ckv_pool_buffers(const ckv_pool* pool, void** keys, void** values, size_t* bytes_each);
 /* metal_kv_cache::element_offset (src/metal/metal_kv_cache.cc:150-179): the
@@ -479,6 +509,91 @@ int ckv_rope_axes(ckv_pool* pool, const void* input, void* output, size_t heads,
 int ckv_rope_axes_append(ckv_pool* pool, size_t layer, const void* queries, void* rotated,
                          size_t q_heads, const void* keys, const void* values, float theta,
                          size_t rotary_dim, const uint8_t* pair_axis, size_t rows);
+
+/* ---- Rotary positions in their forms ---------------------------------------------------
+ * No counterpart in the reference, whose rope is halves without scaling: neighbouring pairs,
+ * and frequencies scaled so that a model goes past the context it was trained on. Pair
+ * j < rotary_dim/2 of a head is elements (j, j + rotary_dim/2) or (2j, 2j + 1); a row at
+ * position p turns it by p * f[j] radians and multiplies it by the magnitude; elements from
+ * rotary_dim on are copied. With b[j] = theta^(-2j/rotary_dim) and t[j] = original * b[j] /
+ * (2 pi), the turns that pair j makes in the original context:
+ *   none    f = b
+ *   linear  f = b / factor
+ *   bands   f = b * (k + (1 - k) / factor), k = (t - low) / (high - low) within 0..1: pairs
+ *           that turn often keep their frequency, those that turn little are slowed
+ *   yarn    f = b * (1 - r) + b / factor * r, r = (j - first) / (last - first) within 0..1,
+ *           where `first` and `last` are the pairs with t = high and t = low, rounded down
+ *           and up, at least 0 and at most rotary_dim - 1
+ * Angles are reduced exactly (64-bit fractions of a turn), at any 32-bit position. */
+enum ckv_rotary_layout { CKV_ROTARY_HALVES = 0, CKV_ROTARY_NEIGHBOURS = 1 };
+enum ckv_rotary_scaling {
+    CKV_SCALING_NONE = 0,
+    CKV_SCALING_LINEAR = 1,
+    CKV_SCALING_BANDS = 2,
+    CKV_SCALING_YARN = 3,
+};
+typedef struct ckv_rotation {
+    float theta;
+    uint32_t rotary_dim; /* 0: head_dim; at most 512 */
+    int32_t layout;      /* ckv_rotary_layout */
+    int32_t scaling;     /* ckv_rotary_scaling */
+    float factor;        /* with a scaling */
+    float low, high;     /* bands and yarn: turns in the original context */
+    uint32_t original;   /* bands and yarn: its length in tokens */
+    float magnitude;     /* 0: 0.1 ln(factor) + 1 with yarn and a factor above 1, else 1 */
+} ckv_rotation;
+
+/* Device rows [rows, heads*head_dim] of the pool dtype, at the batch's positions; input may
+ * equal output (in place) but not overlap it otherwise. Checks: invalid_argument (null
+ * arrays or rotation), no_tables, position_count_mismatch, invalid_head_count,
+ * invalid_head_dimension and invalid_rope_theta as ckv_rope's (rotary_dim at most 512), then
+ * invalid_argument: an unknown layout or scaling, a factor or magnitude that is not finite
+ * and positive (magnitude: or 0), low not below high, or original 0 where they count; yarn
+ * with theta <= 1. Profile name "rotate". */
+int ckv_rotate(ckv_pool* pool, const ckv_rotation* rotation, const void* input, void* output,
+               size_t heads, size_t rows);
+/* One launch for a layer's rows before their attention: query rows rotated into `rotated`
+ * (which may be queries, but no other argument), key rows rotated and, with the value rows,
+ * appended to the uploaded slots of `layer`. held_keys and held_values ([rows,
+ * kv_heads*head_dim]; either may be NULL) take the appended rows as the cache holds them:
+ * what ckv_prompt_attention reads, so that a prompt's rows attend to what later ones will.
+ * rotation NULL: rows as they are. q_heads 0: keys and values alone. The rows' slots are
+ * distinct (of two rows in one slot the cache may hold parts of both).
+ * Checks: those of ckv_append, the queries' (invalid_argument), unsupported_aliasing
+ * (`rotated` is keys or values, or a held array any other argument), then those of
+ * ckv_rotate. Profile names "rotate_append", and "fp4_append" on a pool held in 4 bits. */
+int ckv_rotate_append(ckv_pool* pool, size_t layer, const ckv_rotation* rotation,
+                      const void* queries, void* rotated, size_t q_heads, const void* keys,
+                      const void* values, void* held_keys, void* held_values, size_t rows);
+/* ckv_rotate_append into a buffer of the pool's, then the attention of decode rows (gated
+ * with a gate, NULL: none), on pools of every kind. queries are not changed. Checks: those
+ * of ckv_append_decode, unsupported_aliasing for the gate and the held rows, then those of
+ * ckv_rotate. */
+int ckv_rotate_append_decode(ckv_pool* pool, size_t layer, const ckv_rotation* rotation,
+                             const void* keys, const void* values, const void* queries,
+                             size_t q_heads, float scale, const void* gate, void* held_keys,
+                             void* held_values, void* output, size_t rows);
+
+/* ---- Attention of whole prompts from their rows ----------------------------------------
+ * No counterpart in the reference: new prompts, packed one after another in a batch, whose
+ * keys and values are in hand as rows and need not be read back from the cache (which may
+ * hold them in 4 bits). Row r attends the rows of its sequence from position 0 to its own:
+ * output = softmax(q . k * scale) . v with fp32 accumulation; probabilities enter the
+ * matrix cores in the rows' type. The batch's tables tell the sequences: every row's
+ * position is 0 or follows the row before it, in the same table range (invalid_argument
+ * otherwise). The pool gives the geometry (head_dim 64, 128 or 256: otherwise
+ * invalid_head_dimension) and type; its cache is neither read nor written, and any number
+ * of query heads per kv head, and any scale, is taken. Rows begin q_stride (queries) and kv_stride (keys, values)
+ * elements apart, at least as many as they hold (input_shape_mismatch); 0: no gap. The
+ * output has none. What a row does not attend weighs nothing, infinities and NaN included.
+ * The first call on a batch makes its work list (one small upload); under stream capture
+ * that is refused (invalid_argument), as ckv_attention_window's.
+ * Checks: invalid_argument (null keys or values), those of ckv_attention (with layer 0),
+ * unsupported_aliasing (the output or the gate is another argument), then these. Profile name
+ * "prompt_attention". */
+int ckv_prompt_attention(ckv_pool* pool, const void* queries, size_t q_stride, const void* keys,
+                         const void* values, size_t kv_stride, size_t q_heads, float scale,
+                         const void* gate, void* output, size_t rows);
 
 /* ---- Compaction ------------------------------------------------------------------------
  * No counterpart in the reference: a cache that has to drop tokens moves those it keeps
