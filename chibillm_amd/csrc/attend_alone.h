@@ -47,16 +47,18 @@ __device__ __forceinline__ float row16_sum(float v)
 // sequence the launch below takes 1.81 ms (two at a time 2.29, eight 1.96, one
 // 5.84; the general path took 3.93 for these rows). The cost grows with the
 // rows' positions, as theirs did. (The launch is that of kernels_prefill_wide.hip.)
-// WINDOW: the keys that no row of them attends are passed over by the page.
+// WINDOW: the keys that no row of them attends are passed over by the page. ROWS: keys are
+// rows one after another, without a table. Outputs and gates are o_stride apart (0: as the
+// queries).
 constexpr uint32_t alone_queries = 4;
 
-template <int D, int DT, bool WINDOW, class T>
+template <int D, int DT, bool WINDOW, bool ROWS = false, class T>
 __device__ __forceinline__ void attend_alone(const T* __restrict__ keys,
                                              const T* __restrict__ values,
                                              const uint32_t* __restrict__ table, uint32_t F,
                                              uint32_t rows, uint32_t pos0, const T* q,
                                              size_t q_stride, float c, const T* gate, T* out,
-                                             uint32_t lane, key_window window)
+                                             uint32_t lane, key_window window, size_t o_stride = 0)
 {
     constexpr bool F32 = DT == CKV_F32, F16 = DT == CKV_F16;
     constexpr uint32_t page_tokens = 16;
@@ -105,8 +107,10 @@ __device__ __forceinline__ void attend_alone(const T* __restrict__ keys,
     const uint32_t gap_begin = gap.kept * page_tokens;
     const uint32_t gap_end = gap_begin + gap.skip * page_tokens;
     const uint32_t first = WINDOW && !gap_begin ? gap_end : 0;
-    uint32_t page = table[first / page_tokens];
+    uint32_t page = ROWS ? 0 : table[first / page_tokens];
     auto at_key = [&](uint32_t key) { // in the page at hand; past the last key, that one
+        if constexpr (ROWS)
+            return (uint64_t)min(key, last) * F;
         return ((uint64_t)page * page_tokens + min(key, last) % page_tokens) * F;
     };
     words k_next = load(keys + at_key(first + sub)), v_next = load(values + at_key(first + sub));
@@ -118,7 +122,7 @@ __device__ __forceinline__ void attend_alone(const T* __restrict__ keys,
         if (WINDOW && next == gap_begin)
             next = gap_end;
         if (next <= last) {
-            if (next % page_tokens == 0)
+            if (!ROWS && next % page_tokens == 0)
                 page = table[next / page_tokens];
             k_next = load(keys + at_key(next + sub));
             v_next = load(values + at_key(next + sub));
@@ -165,7 +169,7 @@ __device__ __forceinline__ void attend_alone(const T* __restrict__ keys,
         if (i >= count || sub)
             continue;
         const float inv = 1.0f / l[i];
-        const size_t at = row[i] * q_stride + f;
+        const size_t at = row[i] * (o_stride ? o_stride : q_stride) + f;
 #pragma unroll
         for (uint32_t j = 0; j < each; j += 2) {
             float y[2] = { acc[i][j] * inv, acc[i][j + 1] * inv };

@@ -1248,17 +1248,19 @@ int run_prompt(ckv_pool* pool, size_t layer, const prompt_rows& x, size_t q_head
 {
     ckv_context* ctx = pool->ctx;
     const pool_view view = view_of(pool);
-    window_batch& through = select_window(pool, { UINT32_MAX - 1, 0 }, prompt_tile_rows(view, (uint32_t)q_heads));
+    const prompt_form form = prompt_form_of(view, pool->meta, x, (uint32_t)q_heads, scale, output, gate, !rows,
+                                            ctx->cu_count);
+    window_batch& through = select_window(pool, { UINT32_MAX - 1, 0 }, form.tile_rows());
     int status = ensure_window_tiles(pool, through);
     if (status)
         return status;
-    const prefill_shape_info plan = prompt_plan(view, through.meta, (uint32_t)q_heads, ctx->cu_count);
+    const prefill_shape_info plan = prompt_plan(view, through.meta, form, (uint32_t)q_heads, ctx->cu_count);
     prefill_split split { nullptr, nullptr, plan.n_split, plan.min_blocks };
     if ((status = ensure_prefill_split(pool, plan, split)))
         return status;
     return run_kernel(ctx, rows ? "prompt_attention" : "fp4_attention_prefill", [&] {
-        return launch_prompt(ctx->stream, view, through.meta, (uint32_t)layer, x, (uint32_t)q_heads, scale, output,
-                             gate, !rows, split);
+        return launch_prompt(ctx->stream, view, through.meta, (uint32_t)layer, x, form, (uint32_t)q_heads, scale,
+                             output, gate, !rows, split);
     });
 }
 

@@ -676,12 +676,26 @@ struct prompt_rows {
     uint64_t q_stride, kv_stride;
     bool vectors, out_vectors;
 };
-// Rows of a workgroup, which the tiles' are at most.
-uint32_t prompt_tile_rows(const pool_view& p, uint32_t q_heads);
-prefill_shape_info prompt_plan(const pool_view& p, const meta_view& m, uint32_t q_heads,
-                               int cu_count);
+// How a launch over the batch `m` runs: its waves (8: kernels_prefill.hip's workgroups over
+// rows), and whether it is kernels_prefill.hip's at all.
+struct prompt_form {
+    uint32_t waves, heads; // of a workgroup
+    bool paged_kernel;
+    uint32_t tile_rows() const { return 32 * waves / heads; } // which the tiles' are at most
+};
+prompt_form prompt_form_of(const pool_view& p, const meta_view& m, const prompt_rows& x, uint32_t q_heads,
+                           float scale, const void* out, const void* gate, bool fp4, int cu_count);
+prefill_shape_info prompt_plan(const pool_view& p, const meta_view& m, const prompt_form& form,
+                               uint32_t q_heads, int cu_count);
 hipError_t launch_prompt(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
-                         const prompt_rows& rows, uint32_t q_heads, float scale, void* out,
-                         const void* gate, bool fp4, const prefill_split& split);
+                         const prompt_rows& rows, const prompt_form& form, uint32_t q_heads,
+                         float scale, void* out, const void* gate, bool fp4,
+                         const prefill_split& split);
+// kernels_prefill.hip's workgroups of `waves` waves over rows; the caller has checked 16-bit
+// rows of 128-wide heads in 16-byte words and scale > 0.
+hipError_t launch_prefill_rows(hipStream_t s, const pool_view& p, const meta_view& m,
+                               const prompt_rows& x, uint32_t q_heads, float scale, void* out,
+                               const void* gate, uint32_t heads, uint32_t waves,
+                               const prefill_split& split);
 
 } // namespace ckv

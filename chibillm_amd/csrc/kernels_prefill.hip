@@ -142,14 +142,21 @@ struct prefill_shape {
 // chunk of 512 behind 6,000 through 1,024 takes 20.6 us, a chain of 9 blocks and the
 // fold of 4 ranges. RANGES: the launch may cut a tile's keys (without the code for it,
 // what follows the blocks is shorter to fetch).
-template <int G, bool F16, bool WIDE, int W, bool WINDOW, bool RANGES = true>
+//
+// ROWS: whole prompts, whose keys are the batch's rows (p.keys and p.values, p.features
+// apart) before and at the tile's own; queries are q_row elements apart. A "page" is then 16
+// rows of the sequence, and where the others read the table its number is its place.
+// Tiles are of a workgroup's rows, GQA groups take passes, and rows that got something
+// that is not finite are attended again, as a window's.
+template <int G, bool F16, bool WIDE, int W, bool WINDOW, bool RANGES = true, bool ROWS = false>
 __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     pool_view p, meta_view md, uint32_t layer, const uint16_t* __restrict__ q,
     uint16_t* __restrict__ out, uint32_t q_heads, float c, const uint16_t* __restrict__ gate,
-    prefill_split split_scratch)
+    prefill_split split_scratch, uint64_t q_row)
 {
     static_assert(W == 8 || (W == 4 && G <= 4), "a workgroup covers every q head of its group");
     static_assert(!WINDOW || W == 4);
+    constexpr bool OWN_TILES = WINDOW || ROWS; // tiles of a workgroup's rows, heads in passes
     constexpr int terms = WINDOW ? 2 : 1;
     constexpr float p_scale = WINDOW && F16 ? 6.0f : 0.0f; // log2
     // 4-wave workgroups may split a tile's key blocks between workgroups
@@ -160,15 +167,15 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     __shared__ __attribute__((aligned(16))) uint8_t lds[n_stages * stage_bytes];
     constexpr uint32_t tile_rows = 32 * W / G;
     // workgroups per (tile, kv head); a window's tiles are of a workgroup's rows
-    constexpr uint32_t subs = WINDOW ? 1 : 256 / tile_rows;
+    constexpr uint32_t subs = OWN_TILES ? 1 : 256 / tile_rows;
 
     const uint32_t kv_heads = p.kv_heads;
     const uint32_t kvh = blockIdx.x % kv_heads; // consecutive workgroups: different heads/XCDs
-    const uint32_t group = WINDOW ? q_heads / kv_heads : G;
-    const uint32_t passes = WINDOW ? group / G : 1; // workgroups a GQA group takes
-    const uint32_t unit = WINDOW ? blockIdx.x / kv_heads : 0;
-    const uint32_t pass = WINDOW ? unit % passes : 0;
-    const uint32_t of_pass = WINDOW ? unit / passes : blockIdx.x / kv_heads;
+    const uint32_t group = OWN_TILES ? q_heads / kv_heads : G;
+    const uint32_t passes = OWN_TILES ? group / G : 1; // workgroups a GQA group takes
+    const uint32_t unit = OWN_TILES ? blockIdx.x / kv_heads : 0;
+    const uint32_t pass = OWN_TILES ? unit % passes : 0;
+    const uint32_t of_pass = OWN_TILES ? unit / passes : blockIdx.x / kv_heads;
     // key ranges vary slowest: every tile's first range is dispatched before
     // any second one (ranges interleaved with the rows placed the ranges that
     // find no keys, and the long ones, unevenly: +5 to +29 % launch time)
@@ -188,7 +195,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     const uint32_t row0 = te.x + r0;
     const uint32_t pos0 = te.z + r0; // positions are consecutive inside a tile
     const uint32_t pos_last = pos0 + nrows - 1;
-    const uint32_t* table = md.table + te.w;
+    const uint32_t* table = ROWS ? nullptr : md.table + te.w;
     // the first row's window begins at `low`, no later row's before it
     const key_window window = md.window;
     const uint32_t low = WINDOW ? window_low(pos0, window) : 0;
@@ -225,6 +232,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     const bool active = rb * 32 < nrows;
     const uint32_t qpos = pos0 + min(row, nrows - 1);
     const size_t qoff = (size_t)(row0 + min(row, nrows - 1)) * q_stride + (size_t)head * dim;
+    const size_t qin = ROWS ? (size_t)(row0 + min(row, nrows - 1)) * q_row + (size_t)head * dim : qoff;
     // the q-block's first position, wave-uniform: the diagonal test is a scalar branch
     const uint32_t pos_lo = __builtin_amdgcn_readfirstlane(pos0 + rb * 32);
 
@@ -232,11 +240,13 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     uint4 qr[8];
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks)
-        qr[ks] = valid ? *reinterpret_cast<const uint4*>(q + qoff + ks * 16 + g * 8)
+        qr[ks] = valid ? *reinterpret_cast<const uint4*>(q + qin + ks * 16 + g * 8)
                        : make_uint4(0, 0, 0, 0);
 
-    const uint16_t* kbase = static_cast<const uint16_t*>(p.keys) + layer * p.layer_elems + kvh * dim;
-    const uint16_t* vbase = static_cast<const uint16_t*>(p.values) + layer * p.layer_elems + kvh * dim;
+    // (ROWS: the sequence's first row)
+    const size_t key_base = (ROWS ? (size_t)(te.x - te.z) * F : layer * p.layer_elems) + kvh * dim;
+    const uint16_t* kbase = static_cast<const uint16_t*>(p.keys) + key_base;
+    const uint16_t* vbase = static_cast<const uint16_t*>(p.values) + key_base;
     // K DMA: this lane's key (LDS row lane % 32) and features in the wave's
     // regions wave, wave + W, ...
     const uint32_t k_key = key_row(lane & 31);
@@ -269,6 +279,11 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     const uint32_t last_entry = pos_last / page_tokens; // the tile's last table entry
     auto fetch_pages_unchecked = [&](uint32_t at) {
         const uint32_t kb = in_table(at);
+        if constexpr (ROWS) {
+            page_a = 2 * kb;
+            page_b = min(2 * kb + 1, last_entry);
+            return;
+        }
         using c32 = const __attribute__((address_space(4))) uint32_t;
         const auto* cb = (const __attribute__((address_space(4))) uint8_t*)(uintptr_t)table;
         page_a = *(c32*)(cb + 8 * kb);
@@ -564,6 +579,13 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
                 // the next pair's pages, carried into it: a fetch used in the
                 // same trip is moved next to its use by the compiler, its
                 // latency exposed once per pair (0.7-0.9 % slower)
+                if constexpr (ROWS) {
+                    a0 = 2 * (kb + 6);
+                    b0 = a0 + 1;
+                    a1 = a0 + 2;
+                    b1 = a0 + 3;
+                    continue;
+                }
                 using c32 = const __attribute__((address_space(4))) uint32_t;
                 const auto* cb = (const __attribute__((address_space(4))) uint8_t*)(uintptr_t)table;
                 a0 = *(c32*)(cb + 8 * (kb + 6));
@@ -728,7 +750,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     const float inv = 1.0f / lt;
     uint16_t* dst = out + qoff;
     uint32_t alone = 0; // the q-block's rows that are attended again
-    if constexpr (WINDOW) {
+    if constexpr (OWN_TILES) {
         // 0 unless some result of the query is infinite or NaN (either lane half)
         float odd = inv * 0.0f;
 #pragma unroll
@@ -739,7 +761,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
         const uint64_t odd_lanes = __ballot(valid && odd != 0.0f);
         alone = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
     }
-    if constexpr (WINDOW) {
+    if constexpr (OWN_TILES) {
         wait_vector_memory();
         __syncthreads(); // every wave is past its LDS reads
         static_assert(W * 32 * row_floats<dim> * sizeof(float) <= n_stages * stage_bytes);
@@ -777,7 +799,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
                     make_uint2(pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]));
             }
     }
-    if constexpr (WINDOW) {
+    if constexpr (OWN_TILES) {
         if (__builtin_expect(alone == 0, 1))
             return;
         const size_t first = (size_t)(row0 + rb * 32) * q_stride + (size_t)head * dim;
@@ -787,9 +809,11 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
             for (uint32_t i = 0; i < alone_queries; ++i)
                 left &= left - 1;
             some ^= left;
-            attend_alone<dim, F16 ? CKV_F16 : CKV_BF16, true>(
-                kbase, vbase, table, F, __builtin_amdgcn_readfirstlane(some), pos_lo, q + first,
-                q_stride, c, gate ? gate + first : nullptr, out + first, lane, window);
+            const size_t first_in = ROWS ? (size_t)(row0 + rb * 32) * q_row + (size_t)head * dim : first;
+            attend_alone<dim, F16 ? CKV_F16 : CKV_BF16, WINDOW, ROWS>(
+                kbase, vbase, table, F, __builtin_amdgcn_readfirstlane(some), pos_lo, q + first_in,
+                ROWS ? q_row : q_stride, c, gate ? gate + first : nullptr, out + first, lane, window,
+                q_stride);
         }
     }
 }
@@ -818,21 +842,45 @@ hipError_t launch_gw(hipStream_t s, const pool_view& p, const meta_view& m, uint
                                        : prefill_kernel<G, true, false, W, true, false>)
                                : (wide ? prefill_kernel<G, false, true, W, true, false>
                                        : prefill_kernel<G, false, false, W, true, false>);
-            kernel<<<g, b, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split);
+            kernel<<<g, b, 0, s>>>(p, m, layer, qq, oo, q_heads, c, gg, split, 0);
             return hipGetLastError();
         }
     if (f16 && wide)
         hipLaunchKernelGGL((prefill_kernel<G, true, true, W, WINDOW>), g, b, 0, s, p, m, layer, qq, oo,
-                           q_heads, c, gg, split);
+                           q_heads, c, gg, split, 0);
     else if (f16)
         hipLaunchKernelGGL((prefill_kernel<G, true, false, W, WINDOW>), g, b, 0, s, p, m, layer, qq, oo,
-                           q_heads, c, gg, split);
+                           q_heads, c, gg, split, 0);
     else if (wide)
         hipLaunchKernelGGL((prefill_kernel<G, false, true, W, WINDOW>), g, b, 0, s, p, m, layer, qq, oo,
-                           q_heads, c, gg, split);
+                           q_heads, c, gg, split, 0);
     else
         hipLaunchKernelGGL((prefill_kernel<G, false, false, W, WINDOW>), g, b, 0, s, p, m, layer, qq, oo,
-                           q_heads, c, gg, split);
+                           q_heads, c, gg, split, 0);
+    return hipGetLastError();
+}
+
+template <int G, int W>
+hipError_t launch_rows(hipStream_t s, const pool_view& p, const meta_view& m, const prompt_rows& x,
+                       uint32_t q_heads, float c, void* out, const void* gate, const prefill_split& split)
+{
+    const uint64_t grid = (uint64_t)m.n_tiles * (q_heads / G) * split.n_split;
+    if (!grid)
+        return hipSuccess;
+    if (grid > 0x7FFFFFFFull)
+        return hipErrorInvalidValue;
+    pool_view rows = p;
+    rows.keys = const_cast<void*>(x.keys);
+    rows.values = const_cast<void*>(x.values);
+    rows.features = (uint32_t)x.kv_stride;
+    const bool wide = m.rows * x.kv_stride * 2 > 0xFFFFFFFFull, f16 = p.dtype == CKV_F16;
+    auto* kernel = f16 ? (wide ? prefill_kernel<G, true, true, W, false, true, true>
+                               : prefill_kernel<G, true, false, W, false, true, true>)
+                       : (wide ? prefill_kernel<G, false, true, W, false, true, true>
+                               : prefill_kernel<G, false, false, W, false, true, true>);
+    kernel<<<(uint32_t)grid, 64 * W, 0, s>>>(rows, m, 0, static_cast<const uint16_t*>(x.queries),
+                                             static_cast<uint16_t*>(out), q_heads, c,
+                                             static_cast<const uint16_t*>(gate), split, x.q_stride);
     return hipGetLastError();
 }
 
@@ -1035,6 +1083,21 @@ hipError_t launch_prefill(hipStream_t s, const pool_view& p, const meta_view& m,
     default:
         return hipErrorInvalidValue;
     }
+}
+
+hipError_t launch_prefill_rows(hipStream_t s, const pool_view& p, const meta_view& m, const prompt_rows& x,
+                               uint32_t q_heads, float scale, void* out, const void* gate, uint32_t heads,
+                               uint32_t waves, const prefill_split& split)
+{
+    const float c = scale * log2e;
+    const auto of = [&](auto g) {
+        constexpr int G = decltype(g)::value;
+        return waves == 8 ? launch_rows<G, 8>(s, p, m, x, q_heads, c, out, gate, split)
+                          : launch_rows<G, 4>(s, p, m, x, q_heads, c, out, gate, split);
+    };
+    return heads == 4 ? of(std::integral_constant<int, 4> {})
+        : heads == 2  ? of(std::integral_constant<int, 2> {})
+                      : of(std::integral_constant<int, 1> {});
 }
 
 } // namespace ckv

@@ -872,19 +872,49 @@ uint32_t heads_of(const pool_view& p, uint32_t q_heads)
 
 } // namespace
 
-uint32_t prompt_tile_rows(const pool_view& p, uint32_t q_heads)
+namespace {
+
+// Whether rows are read and written in 16-byte words.
+void set_vectors(const pool_view& p, prompt_rows& x, const void* out, const void* gate, bool fp4)
 {
-    return 32 * n_waves / heads_of(p, q_heads);
+    const uint32_t each = 16 / p.elem_size;
+    x.vectors = aligned16(x.queries) && x.q_stride % each == 0
+        && (fp4 || (aligned16(x.keys) && aligned16(x.values) && x.kv_stride % each == 0));
+    x.out_vectors = aligned16(out) && aligned16(gate);
 }
 
-prefill_shape_info prompt_plan(const pool_view& p, const meta_view& m, uint32_t q_heads, int cu_count)
+} // namespace
+
+prompt_form prompt_form_of(const pool_view& p, const meta_view& m, const prompt_rows& rows, uint32_t q_heads,
+                           float scale, const void* out, const void* gate, bool fp4, int cu_count)
 {
-    prefill_shape_info plan { n_waves, 1, 4, 0, 0 };
-    const uint64_t grid = (uint64_t)m.n_tiles * (q_heads / heads_of(p, q_heads));
+    prompt_rows x = rows;
+    set_vectors(p, x, out, gate, fp4);
+    prompt_form form { n_waves, heads_of(p, q_heads), false };
+    form.paged_kernel = !fp4 && p.head_dim == 128 && p.dtype != CKV_F32 && x.vectors && x.out_vectors
+        && scale > 0.0f && x.kv_stride <= UINT32_MAX;
+    if (!form.paged_kernel)
+        return form;
+    const uint32_t eight = form.heads == 4 ? m.row_blocks[1] : form.heads == 2 ? m.row_blocks[2] : m.n_tiles;
+    if ((uint64_t)eight * (q_heads / form.heads) >= 2 * (uint64_t)std::max(cu_count, 1))
+        form.waves = 8;
+    if (const char* forced = std::getenv("CKV_PREFILL_WAVES"))
+        form.waves = std::strtol(forced, nullptr, 10) == 8 ? 8 : 4;
+    return form;
+}
+
+prefill_shape_info prompt_plan(const pool_view& p, const meta_view& m, const prompt_form& form,
+                               uint32_t q_heads, int cu_count)
+{
+    prefill_shape_info plan { form.waves, 1, 4, 0, 0 };
+    const uint64_t grid = (uint64_t)m.n_tiles * (q_heads / form.heads);
     const uint64_t cus = (uint64_t)std::max(cu_count, 1);
-    if (grid && grid < cus)
+    if (form.waves == n_waves && grid && grid < cus)
         plan.n_split = (uint32_t)std::min<uint64_t>(split_max, 2 * cus / grid);
-    if (plan.n_split > 1 && prefill_range_count(m.longest_blocks, plan.n_split, plan.min_blocks) == 1)
+    if (const char* forced = std::getenv("CKV_PREFILL_SPLIT"))
+        plan.n_split = (uint32_t)std::clamp(std::strtol(forced, nullptr, 10), 1L, (long)split_max);
+    if (form.waves != n_waves
+        || (plan.n_split > 1 && prefill_range_count(m.longest_blocks, plan.n_split, plan.min_blocks) == 1))
         plan.n_split = 1;
     if (plan.n_split > 1) {
         plan.records_floats = grid * plan.n_split * 32 * n_waves * (p.head_dim + 4);
@@ -894,17 +924,15 @@ prefill_shape_info prompt_plan(const pool_view& p, const meta_view& m, uint32_t 
 }
 
 hipError_t launch_prompt(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
-                         const prompt_rows& rows, uint32_t q_heads, float scale, void* out, const void* gate,
-                         bool fp4, const prefill_split& split)
+                         const prompt_rows& rows, const prompt_form& form, uint32_t q_heads, float scale,
+                         void* out, const void* gate, bool fp4, const prefill_split& split)
 {
+    if (form.paged_kernel)
+        return launch_prefill_rows(s, p, m, rows, q_heads, scale, out, gate, form.heads, form.waves, split);
     prompt_rows x = rows;
-    const uint32_t each = 16 / p.elem_size;
-    x.vectors = aligned16(x.queries) && x.q_stride % each == 0
-        && (fp4 || (aligned16(x.keys) && aligned16(x.values) && x.kv_stride % each == 0));
-    x.out_vectors = aligned16(out) && aligned16(gate);
-    const uint32_t heads = heads_of(p, q_heads);
-    return fp4 ? launch_dim<true>(p.head_dim, heads, s, p, m, layer, x, q_heads, scale, out, gate, split)
-               : launch_dim<false>(p.head_dim, heads, s, p, m, layer, x, q_heads, scale, out, gate, split);
+    set_vectors(p, x, out, gate, fp4);
+    return fp4 ? launch_dim<true>(p.head_dim, form.heads, s, p, m, layer, x, q_heads, scale, out, gate, split)
+               : launch_dim<false>(p.head_dim, form.heads, s, p, m, layer, x, q_heads, scale, out, gate, split);
 }
 
 } // namespace ckv
