@@ -948,8 +948,8 @@ int create_pool(ckv_context* ctx, size_t layers, size_t blocks, size_t block_siz
         return set_error(ctx, CKV_E_INVALID_BLOCK_COUNT, "blocks == 0");
     if (block_size == 0)
         return set_error(ctx, CKV_E_INVALID_BLOCK_SIZE, "block_size == 0");
-    if (fp4 && block_size % fp4_tile)
-        return set_error(ctx, CKV_E_INVALID_BLOCK_SIZE, "4-bit pools: block_size % 16 != 0");
+    if (fp4 && (block_size % fp4_tile || (block_size & (block_size - 1)) || block_size > 4096))
+        return set_error(ctx, CKV_E_INVALID_BLOCK_SIZE, "4-bit pools: block_size must be a power of two from 16 to 4096");
     if (kv_heads == 0)
         return set_error(ctx, CKV_E_INVALID_KV_HEAD_COUNT, "kv_heads == 0");
     if (head_dim == 0)

@@ -31,9 +31,13 @@
 #include <algorithm>
 #include <cfloat>
 #include <cstdlib>
+#include <type_traits>
 
 namespace ckv {
 namespace {
+
+// What keys and values are: a 4-bit pool's, rows in 16-byte words, or rows of any alignment.
+enum source { FROM_FP4, FROM_WORDS, FROM_ROWS };
 
 constexpr uint32_t block_keys = 32;
 constexpr uint32_t n_waves = 4, n_threads = 64 * n_waves;
@@ -45,14 +49,15 @@ struct key_source {
     const uint8_t* values;
     const uint32_t* table;
     uint64_t stride; // bytes of a row
-    uint32_t block_size, kv_heads, kvh;
+    uint32_t page_log, kv_heads, kvh; // (a page is 2^page_log tiles)
 };
 
+// The first byte of a tile of the sequence, within the layer.
 template <int D>
-__device__ __forceinline__ uint64_t tile_offset(const key_source& s, uint32_t key)
+__device__ __forceinline__ uint64_t tile_offset(const key_source& s, uint32_t tile)
 {
-    return fp4_tile_at(s.table[key / s.block_size] * s.block_size + key % s.block_size, s.kvh,
-                       s.block_size, s.kv_heads, D);
+    const uint64_t page = (uint64_t)s.table[tile >> s.page_log] * s.kv_heads + s.kvh;
+    return ((page << s.page_log) + (tile & ((1u << s.page_log) - 1))) * fp4_tile_bytes(D);
 }
 
 __device__ __forceinline__ float word_half(uint32_t w, int e, bool f16)
@@ -68,7 +73,7 @@ __device__ __forceinline__ void load_features(const key_source& s, uint32_t key,
 {
     constexpr uint32_t each = D / 16;
     if constexpr (FP4) {
-        const uint8_t* tile = (v ? s.values : s.keys) + tile_offset<D>(s, key);
+        const uint8_t* tile = (v ? s.values : s.keys) + tile_offset<D>(s, key / fp4_tile);
         const uint32_t t = key % fp4_tile;
 #pragma unroll
         for (uint32_t i = 0; i < each; i += 4) { // four features: half a word
@@ -277,11 +282,12 @@ struct staged<D, true> {
 };
 
 // 16-bit rows. GH heads of a GQA group share a workgroup: 128 / GH rows.
-template <int D, int GH, bool F16, bool FP4>
+template <int D, int GH, bool F16, source SRC>
 __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
     pool_view p, meta_view md, uint32_t layer, prompt_rows x, uint16_t* __restrict__ out, uint32_t q_heads,
     float c, uint32_t q_and, uint32_t q_xor, const uint16_t* __restrict__ gate, prefill_split split)
 {
+    constexpr bool FP4 = SRC == FROM_FP4;
     constexpr int KS = D / 16, MT = D / 32, DT = F16 ? CKV_F16 : CKV_BF16;
     constexpr uint32_t n_stages = 3;
     // K stage: chunk i (features 8i .. 8i + 7) holds the block's keys in the LDS rows of the
@@ -310,15 +316,13 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
     if constexpr (FP4) {
         const uint64_t layer_bytes = (uint64_t)p.blocks * p.block_size / fp4_tile * p.kv_heads * fp4_tile_bytes(D);
         s = { static_cast<const uint8_t*>(p.keys) + layer * layer_bytes,
-              static_cast<const uint8_t*>(p.values) + layer * layer_bytes, md.table + w.table, 0, p.block_size,
-              p.kv_heads, w.kvh };
+              static_cast<const uint8_t*>(p.values) + layer * layer_bytes, md.table + w.table, 0,
+              (uint32_t)__builtin_ctz(p.block_size / fp4_tile), p.kv_heads, w.kvh };
     } else {
         const uint64_t first = (uint64_t)(w.row0 - w.pos0) * x.kv_stride + w.kvh * D;
         s = { static_cast<const uint8_t*>(x.keys) + 2 * first, static_cast<const uint8_t*>(x.values) + 2 * first,
               nullptr, 2 * x.kv_stride, 0, 0, 0 };
     }
-    const bool k_vector = !FP4 && x.vectors;
-
     const uint16_t* q_row = static_cast<const uint16_t*>(x.queries)
         + (uint64_t)(w.row0 + min(row, w.nrows - 1)) * x.q_stride + (uint64_t)head * D;
     uint4 qr[KS];
@@ -338,44 +342,50 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
     }
 
     using held = staged<D, FP4>;
-    held next;
+    // Blocks on their way: 4-bit ones three ahead of the one that is stored (a block takes less
+    // than a load from HBM), rows one.
+    constexpr uint32_t ahead = FP4 ? 3 : 1;
+    held flight[ahead];
+    // where a lane's codes and scales are in a tile
+    const bool v_wave = wave >= 2;
+    const uint32_t code_at = v_wave ? lane * 16 : lane / 4 * (D / 2) + lane % 4 * 16;
+    const uint32_t code_part = v_wave ? 1024 : 64;
+    const uint32_t scale_at = 8 * D
+        + (v_wave ? (D == 64 ? lane % 16 / 8 : lane % 16 / 4) * 16 + lane / 16 * 4
+                  : lane / 4 * (D / 32) + (D == 64 ? lane % 4 / 2 : lane % 4));
+    const uint32_t scale_part = v_wave ? 64 : 4, k_shift = scale_at % 4 * 8;
     // block kb's words of this thread into registers
-    auto load = [&](uint32_t kb) {
+    auto load = [&](uint32_t kb, held& next) {
         const uint32_t key0 = kb * block_keys;
         if constexpr (FP4) {
-            constexpr uint32_t W = held::words;
-            const bool v = tid >= n_threads / 2;
-            const uint32_t t = tid % (n_threads / 2);
-            const uint32_t tile = t / 64, at = t % 64; // of the block's two tiles
-            const uint32_t key = min(key0 + tile * fp4_tile, w.pos_last / fp4_tile * fp4_tile);
-            const uint8_t* base = (v ? s.values : s.keys) + tile_offset<D>(s, key);
-            // lane (c, quarter) of the tile: K: token at / 4, part at % 4; V: quarter at / 16, c at % 16
+            // waves 0 and 1 take K of the block's two tiles, 2 and 3 V. Of K, lane 4t + i takes
+            // part i of token t; of V, lane 16q + c features from c on of tokens 4q .. 4q + 3.
+            const uint32_t tile = min(2 * kb + (wave & 1), w.pos_last / fp4_tile);
+            const uint8_t* base = uniform_ptr((wave < 2 ? s.keys : s.values) + tile_offset<D>(s, tile));
             if constexpr (D == 64) {
-                const uint2 r = *reinterpret_cast<const uint2*>(base + at * 8);
+                const uint2 r = *reinterpret_cast<const uint2*>(base + lane * 8);
                 next.code[0] = r.x;
                 next.code[1] = r.y;
-                next.scale[0] = v ? *reinterpret_cast<const uint32_t*>(base + 8 * D + at % 16 / 8 * 16 + at / 16 * 4)
-                                  : base[8 * D + at / 4 * 2 + at % 4 / 2];
             } else {
 #pragma unroll
-                for (uint32_t i = 0; i < W / 4; ++i) {
-                    const uint32_t off = v ? i * 1024 + at * 16 : at / 4 * (D / 2) + i * 64 + at % 4 * 16;
-                    const uint4 r = *reinterpret_cast<const uint4*>(base + off);
+                for (uint32_t i = 0; i < held::words / 4; ++i) {
+                    const uint4 r = *reinterpret_cast<const uint4*>(base + code_at + i * code_part);
                     next.code[4 * i] = r.x;
                     next.code[4 * i + 1] = r.y;
                     next.code[4 * i + 2] = r.z;
                     next.code[4 * i + 3] = r.w;
-                    next.scale[i] = v
-                        ? *reinterpret_cast<const uint32_t*>(base + 8 * D + (4 * i + at % 16 / 4) * 16 + at / 16 * 4)
-                        : base[8 * D + at / 4 * (D / 32) + 4 * i + at % 4];
                 }
             }
+            // (a K lane's byte is the lowest of its word: one load for both)
+#pragma unroll
+            for (uint32_t i = 0; i < (D == 256 ? 2 : 1); ++i)
+                next.scale[i] = *reinterpret_cast<const uint32_t*>(base + (scale_at & ~3u) + i * scale_part);
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < held::per; ++i) {
                 const uint32_t word = i * n_threads + tid, key = key0 + word / (D / 8), f = word % (D / 8) * 8;
                 const uint64_t at = min(key, w.pos_last) * s.stride + 2 * f;
-                if (k_vector) {
+                if constexpr (SRC == FROM_WORDS) {
                     next.k[i] = *reinterpret_cast<const uint4*>(s.keys + at);
                     next.v[i] = *reinterpret_cast<const uint4*>(s.values + at);
                 } else {
@@ -397,33 +407,26 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
         return st + k_bytes + (key % 4 + 4 * (key / 16)) * v_group + key / 4 % 4 * v_row;
     };
     // and from there into its stage, zeros past the tile's last position
-    auto store = [&](uint32_t kb) {
-        uint8_t* st = lds + kb % n_stages * stage_bytes;
+    auto store_keys = [&](uint32_t kb, const held& next, uint8_t* st, auto all) {
+        constexpr bool ALL = decltype(all)::value;
         const uint32_t key0 = kb * block_keys;
-        const bool whole = key0 + block_keys - 1 <= w.pos_last;
         if constexpr (FP4) {
-            const uint32_t t = tid % (n_threads / 2), tile = t / 64, at = t % 64;
-            if (tid < n_threads / 2) {
-                const uint32_t key = tile * fp4_tile + at / 4;
-                const bool there = whole || key0 + key <= w.pos_last;
-                if constexpr (D == 64) {
-                    const float scale = there ? fp4_scale(next.scale[0]) : 1.0f;
+            const uint32_t token0 = (wave & 1) * fp4_tile;
+            if (!v_wave) {
+                const uint32_t key = token0 + lane / 4;
+                const bool there = ALL || key0 + key <= w.pos_last;
 #pragma unroll
-                    for (uint32_t i = 0; i < 2; ++i)
-                        put_k(st, key, at % 4 * 2 + i, fp4_eight<F16>(there ? next.code[i] : 0, scale));
-                } else {
-#pragma unroll
-                    for (uint32_t i = 0; i < held::words; ++i) {
-                        const float scale = there ? fp4_scale(next.scale[i / 4]) : 1.0f;
-                        put_k(st, key, i / 4 * 16 + at % 4 * 4 + i % 4, fp4_eight<F16>(there ? next.code[i] : 0, scale));
-                    }
+                for (uint32_t i = 0; i < held::words; ++i) {
+                    const float scale = there ? fp4_scale(next.scale[i / 4] >> k_shift & 255) : 1.0f;
+                    const uint32_t chunk = D == 64 ? lane % 4 * 2 + i : i / 4 * 16 + lane % 4 * 4 + i % 4;
+                    put_k(st, key, chunk, fp4_eight<F16>(there ? next.code[i] : 0, scale));
                 }
             } else {
-                const uint32_t token0 = tile * fp4_tile + at / 16 * 4, cc = at % 16;
+                const uint32_t quad = token0 + lane / 16 * 4, cc = lane % 16;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
-                    const bool there = whole || key0 + token0 + i <= w.pos_last;
-                    uint8_t* to = v_at(st, token0 + i);
+                    const bool there = ALL || key0 + quad + i <= w.pos_last;
+                    uint8_t* to = v_at(st, quad + i);
 #pragma unroll
                     for (uint32_t part = 0; part < (D == 256 ? 2 : 1); ++part) {
                         const float scale = there ? fp4_scale(next.scale[part] >> (8 * i) & 255) : 1.0f;
@@ -442,12 +445,19 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
 #pragma unroll
             for (uint32_t i = 0; i < held::per; ++i) {
                 const uint32_t word = i * n_threads + tid, key = word / (D / 8), chunk = word % (D / 8);
-                const bool there = whole || key0 + key <= w.pos_last;
-                const uint4 zero = make_uint4(0, 0, 0, 0);
-                put_k(st, key, chunk, there ? next.k[i] : zero);
-                *reinterpret_cast<uint4*>(v_at(st, key) + chunk * 16) = there ? next.v[i] : zero;
+                uint4 k = next.k[i], v = next.v[i];
+                if (!ALL && key0 + key > w.pos_last)
+                    k = v = make_uint4(0, 0, 0, 0);
+                put_k(st, key, chunk, k);
+                *reinterpret_cast<uint4*>(v_at(st, key) + chunk * 16) = v;
             }
         }
+    };
+    auto store = [&](uint32_t kb, const held& next, uint8_t* st) {
+        if (kb * block_keys + block_keys - 1 <= w.pos_last)
+            store_keys(kb, next, st, std::true_type {});
+        else
+            store_keys(kb, next, st, std::false_type {});
     };
 
     f32x16_t o[MT];
@@ -457,12 +467,13 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
     float m = -__builtin_inff(), l = 0.0f, m_limit = -__builtin_inff(), mx = 0.0f;
     const float rescale_raw = rescale_log2 / c;
     f32x16_t sc, sp;
-    auto scores = [&](uint32_t kb) {
-        const uint8_t* kl = lds + kb % n_stages * stage_bytes + g * k_chunk + n * 16;
-        uint4 ka[KS];
+    auto read_k = [&](const uint8_t* st, uint4 (&ka)[KS]) {
+        const uint8_t* kl = st + g * k_chunk + n * 16;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
             ka[ks] = *reinterpret_cast<const uint4*>(kl + ks * 2 * k_chunk);
+    };
+    auto scores = [&](const uint4 (&ka)[KS]) {
         sc = f32x16_t {};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
@@ -485,8 +496,8 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
                                pack2<F16>(sp[8 * h + 4], sp[8 * h + 5]), pack2<F16>(sp[8 * h + 6], sp[8 * h + 7]));
     };
     const uint32_t vr_off = ((lane & 15) >> 2) * v_group + (lane >> 5) * 2 * v_row + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
-    auto values = [&](uint32_t kb, const uint4 (&pt)[2]) {
-        uint32_t vaddr = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) uint8_t*)(lds + kb % n_stages * stage_bytes + k_bytes)) + vr_off;
+    auto values = [&](const uint8_t* st, const uint4 (&pt)[2]) {
+        uint32_t vaddr = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) uint8_t*)(const_cast<uint8_t*>(st) + k_bytes)) + vr_off;
         asm volatile("" : "+v"(vaddr));
         auto* vb = (__attribute__((address_space(3))) uint8_t*)(uintptr_t)vaddr;
 #pragma unroll
@@ -523,37 +534,56 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
         }
     };
 
-    load(w.kb_begin);
-    store(w.kb_begin);
-    if (w.kb_begin + 1 < w.kb_end)
-        load(w.kb_begin + 1);
-    __syncthreads();
     // Iteration kb finishes block kb - 1 and scores block kb; it stages block kb + 1, whose
-    // stage was block kb - 2's, last read in iteration kb - 1.
-    uint32_t kb = w.kb_begin;
-    scores(kb);
-    if (kb + 1 < w.kb_end)
-        store(kb + 1);
-    if (kb + 2 < w.kb_end)
-        load(kb + 2);
-    stats(kb);
+    // stage was block kb - 2's, last read in iteration kb - 1. The loop goes round the stages,
+    // and the registers of the blocks in flight, in turn: iteration kb_begin + 3i + S.
+    static_assert(n_stages % ahead == 0);
+#pragma unroll
+    for (uint32_t i = 0; i < ahead; ++i)
+        if (w.kb_begin + i < w.kb_end)
+            load(w.kb_begin + i, flight[i]);
+    store(w.kb_begin, flight[0], lds);
+    if (w.kb_begin + ahead < w.kb_end)
+        load(w.kb_begin + ahead, flight[0]);
     __syncthreads();
-    for (++kb; kb < w.kb_end; ++kb) {
-        uint4 pt[2];
-        probabilities(pt);
-        scores(kb);
+    auto iteration = [&](uint32_t kb, auto turn, auto is_first) {
+        constexpr uint32_t S = decltype(turn)::value;
+        constexpr bool FIRST = decltype(is_first)::value;
+        uint4 ka[KS], pt[2];
+        read_k(lds + S * stage_bytes, ka);
+        held& next = flight[(S + 1) % ahead];
         if (kb + 1 < w.kb_end)
-            store(kb + 1);
-        if (kb + 2 < w.kb_end)
-            load(kb + 2);
-        values(kb - 1, pt);
+            store(kb + 1, next, lds + (S + 1) % n_stages * stage_bytes);
+        if (kb + 1 + ahead < w.kb_end)
+            load(kb + 1 + ahead, next);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!FIRST)
+            probabilities(pt);
+        scores(ka);
+        if constexpr (!FIRST)
+            values(lds + (S + 2) % n_stages * stage_bytes, pt);
         stats(kb);
         __syncthreads();
+    };
+    uint32_t kb = w.kb_begin;
+    uint32_t last = 0; // the stage of the last block
+    iteration(kb, std::integral_constant<uint32_t, 0> {}, std::true_type {});
+    while (++kb < w.kb_end) {
+        iteration(kb, std::integral_constant<uint32_t, 1> {}, std::false_type {});
+        last = 1;
+        if (++kb >= w.kb_end)
+            break;
+        iteration(kb, std::integral_constant<uint32_t, 2> {}, std::false_type {});
+        last = 2;
+        if (++kb >= w.kb_end)
+            break;
+        iteration(kb, std::integral_constant<uint32_t, 0> {}, std::false_type {});
+        last = 0;
     }
     {
         uint4 pt[2];
         probabilities(pt);
-        values(kb - 1, pt);
+        values(lds + last * stage_bytes, pt);
     }
 
     float lt = l + __shfl_xor(l, 32);
@@ -609,11 +639,12 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
 // contraction over features pairs 8i + e with 8i + 4 + e, so that a lane's operands are
 // 16-byte words; that over keys pairs the two keys of an accumulator element, so that a
 // probability is an operand where it was computed. Two LDS stages of whole rows.
-template <int D, int GH, bool FP4>
+template <int D, int GH, source SRC>
 __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel(
     pool_view p, meta_view md, uint32_t layer, prompt_rows x, float* __restrict__ out, uint32_t q_heads,
     float c, float q_sign, const float* __restrict__ gate, prefill_split split)
 {
+    constexpr bool FP4 = SRC == FROM_FP4;
     constexpr int MT = D / 32, K4 = D / 8;
     constexpr uint32_t pitch = D + 4, stage_floats = 2 * block_keys * pitch;
     __shared__ __attribute__((aligned(16))) float lds[2 * stage_floats];
@@ -633,8 +664,8 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel
     if constexpr (FP4) {
         const uint64_t layer_bytes = (uint64_t)p.blocks * p.block_size / fp4_tile * p.kv_heads * fp4_tile_bytes(D);
         s = { static_cast<const uint8_t*>(p.keys) + layer * layer_bytes,
-              static_cast<const uint8_t*>(p.values) + layer * layer_bytes, md.table + w.table, 0, p.block_size,
-              p.kv_heads, w.kvh };
+              static_cast<const uint8_t*>(p.values) + layer * layer_bytes, md.table + w.table, 0,
+              (uint32_t)__builtin_ctz(p.block_size / fp4_tile), p.kv_heads, w.kvh };
     } else {
         const uint64_t first = (uint64_t)(w.row0 - w.pos0) * x.kv_stride + w.kvh * D;
         s = { static_cast<const uint8_t*>(x.keys) + 4 * first, static_cast<const uint8_t*>(x.values) + 4 * first,
@@ -663,7 +694,7 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel
             const uint32_t word = i * n_threads + tid;
             if constexpr (FP4) {
                 const uint32_t key = min(key0 + word / (D / 8), w.pos_last), f8 = word % (D / 8), t = key % fp4_tile;
-                const uint64_t at = tile_offset<D>(s, key);
+                const uint64_t at = tile_offset<D>(s, key / fp4_tile);
                 code_k[i] = *reinterpret_cast<const uint32_t*>(s.keys + at + fp4_word_at(D, t, f8, false));
                 const uint8_t* v = s.values + at + fp4_word_at(D, t, f8, true);
                 if constexpr (D == 64)
@@ -676,7 +707,7 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel
                 const uint32_t key = min(key0 + word / (D / 4), w.pos_last), f = word % (D / 4) * 4;
                 const float* k = reinterpret_cast<const float*>(s.keys + key * s.stride) + f;
                 const float* v = reinterpret_cast<const float*>(s.values + key * s.stride) + f;
-                if (x.vectors) {
+                if constexpr (SRC == FROM_WORDS) {
                     next_k[i] = *reinterpret_cast<const float4*>(k);
                     next_v[i] = *reinterpret_cast<const float4*>(v);
                 } else {
@@ -689,7 +720,6 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel
     auto store = [&](uint32_t kb) {
         float* st = lds + kb % 2 * stage_floats;
         const uint32_t key0 = kb * block_keys;
-        const float4 zero = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (uint32_t i = 0; i < per; ++i) {
             const uint32_t word = i * n_threads + tid;
@@ -705,9 +735,11 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel
                 put(st + (block_keys + key) * pitch + f, code_v[i], scale_v[i]);
             } else {
                 const uint32_t key = word / (D / 4), f = word % (D / 4) * 4;
-                const bool there = key0 + key <= w.pos_last;
-                *reinterpret_cast<float4*>(st + key * pitch + f) = there ? next_k[i] : zero;
-                *reinterpret_cast<float4*>(st + (block_keys + key) * pitch + f) = there ? next_v[i] : zero;
+                float4 k = next_k[i], v = next_v[i];
+                if (key0 + key > w.pos_last)
+                    k = v = make_float4(0, 0, 0, 0);
+                *reinterpret_cast<float4*>(st + key * pitch + f) = k;
+                *reinterpret_cast<float4*>(st + (block_keys + key) * pitch + f) = v;
             }
         }
     };
@@ -824,7 +856,7 @@ bool aligned16(const void* ptr)
     return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0;
 }
 
-template <int D, int GH, bool FP4>
+template <int D, int GH, source SRC>
 hipError_t launch_gh(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer, const prompt_rows& x,
                      uint32_t q_heads, float scale, void* out, const void* gate, const prefill_split& split)
 {
@@ -836,31 +868,31 @@ hipError_t launch_gh(hipStream_t s, const pool_view& p, const meta_view& m, uint
     const float c = scale == 0.0f ? log2e : __builtin_fabsf(scale) * log2e;
     const dim3 blocks((uint32_t)grid), threads(n_threads);
     if (p.dtype == CKV_F32) {
-        prompt_f32_kernel<D, GH, FP4><<<blocks, threads, 0, s>>>(
+        prompt_f32_kernel<D, GH, SRC><<<blocks, threads, 0, s>>>(
             p, m, layer, x, static_cast<float*>(out), q_heads, c, scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f,
             static_cast<const float*>(gate), split);
         return hipGetLastError();
     }
-    auto* kernel = p.dtype == CKV_F16 ? prompt_kernel<D, GH, true, FP4> : prompt_kernel<D, GH, false, FP4>;
+    auto* kernel = p.dtype == CKV_F16 ? prompt_kernel<D, GH, true, SRC> : prompt_kernel<D, GH, false, SRC>;
     kernel<<<blocks, threads, 0, s>>>(p, m, layer, x, static_cast<uint16_t*>(out), q_heads, c,
                                       scale == 0.0f ? 0u : ~0u, scale < 0.0f ? 0x80008000u : 0u,
                                       static_cast<const uint16_t*>(gate), split);
     return hipGetLastError();
 }
 
-template <int D, bool FP4, class... Args>
+template <int D, source SRC, class... Args>
 hipError_t launch_group(uint32_t heads, const Args&... args)
 {
-    return heads == 4 ? launch_gh<D, 4, FP4>(args...) : heads == 2 ? launch_gh<D, 2, FP4>(args...)
-                                                                  : launch_gh<D, 1, FP4>(args...);
+    return heads == 4 ? launch_gh<D, 4, SRC>(args...) : heads == 2 ? launch_gh<D, 2, SRC>(args...)
+                                                                  : launch_gh<D, 1, SRC>(args...);
 }
 
-template <bool FP4, class... Args>
+template <source SRC, class... Args>
 hipError_t launch_dim(uint32_t head_dim, uint32_t heads, const Args&... args)
 {
-    return head_dim == 64 ? launch_group<64, FP4>(heads, args...)
-        : head_dim == 128 ? launch_group<128, FP4>(heads, args...)
-                          : launch_group<256, FP4>(heads, args...);
+    return head_dim == 64 ? launch_group<64, SRC>(heads, args...)
+        : head_dim == 128 ? launch_group<128, SRC>(heads, args...)
+                          : launch_group<256, SRC>(heads, args...);
 }
 
 // Heads of a GQA group that share a workgroup's key blocks.
@@ -931,8 +963,13 @@ hipError_t launch_prompt(hipStream_t s, const pool_view& p, const meta_view& m, 
         return launch_prefill_rows(s, p, m, rows, q_heads, scale, out, gate, form.heads, form.waves, split);
     prompt_rows x = rows;
     set_vectors(p, x, out, gate, fp4);
-    return fp4 ? launch_dim<true>(p.head_dim, form.heads, s, p, m, layer, x, q_heads, scale, out, gate, split)
-               : launch_dim<false>(p.head_dim, form.heads, s, p, m, layer, x, q_heads, scale, out, gate, split);
+    const auto launch = [&](auto src) {
+        return launch_dim<decltype(src)::value>(p.head_dim, form.heads, s, p, m, layer, x, q_heads, scale, out, gate,
+                                                split);
+    };
+    return fp4        ? launch(std::integral_constant<source, FROM_FP4> {})
+        : x.vectors ? launch(std::integral_constant<source, FROM_WORDS> {})
+                    : launch(std::integral_constant<source, FROM_ROWS> {});
 }
 
 } // namespace ckv

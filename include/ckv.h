@@ -179,8 +179,8 @@ int ckv_pool_wrap(ckv_context* ctx, size_t layers, size_t blocks, size_t block_s
  * Attention takes any number of query heads per kv head and any scale, with products of
  * bf16 terms that keep at least 16 bits of queries and probabilities in decode rows, and of
  * the rows' type in prefill tiles (f32 rows: 24 bits in both).
- * Checks: those of ckv_pool_create, in their order, where the block size must be a multiple
- * of 16 (invalid_block_size) and head_dim 64, 128 or 256 (invalid_head_dimension); wrapped
+ * Checks: those of ckv_pool_create, in their order, where the block size must be a power of
+ * two from 16 to 4096 (invalid_block_size) and head_dim 64, 128 or 256 (invalid_head_dimension); wrapped
  * buffers must be aligned to 16 bytes (invalid_argument) and hold the bytes_each of
  * ckv_pool_buffers: layers * blocks * block_size * kv_heads * head_dim * 17 / 32. */
 int ckv_pool_create_fp4(ckv_context* ctx, size_t layers, size_t blocks, size_t block_size,
