@@ -55,13 +55,18 @@ struct fp4_lane {
     uint32_t ks[parts], vs[parts];
 };
 
-constexpr uint32_t fp4_lane_waves = 8;
+// Waves of a workgroup, at most.
+constexpr uint32_t fp4_waves_of(int head_dim)
+{
+    return head_dim == 256 ? 4 : 8;
+}
 
 template <int D, int DT>
-__global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
+__global__ __launch_bounds__(64 * fp4_waves_of(D), D == 256 ? 3 : 4) void fp4_decode_kernel(
     pool_view p, meta_view m, uint32_t layer, const void* __restrict__ q, uint32_t q_heads, float scale_log2,
-    void* __restrict__ out, const void* __restrict__ gate, split_scratch split, uint32_t passes)
+    float q_sign, void* __restrict__ out, const void* __restrict__ gate, split_scratch split, uint32_t passes)
 {
+    constexpr bool SUMMED = DT != CKV_BF16; // bf16 queries stand whole in the columns of all terms
     constexpr int TERMS = DT == CKV_F32 ? 4 : 2, GQ = 16 / TERMS;
     constexpr uint32_t KS = D / 32, MT = D / 16, RF = D + 4;
     using tile_t = fp4_lane<D>;
@@ -72,11 +77,13 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
     const uint32_t H = p.kv_heads, group = q_heads / H;
     const uint32_t kv_head = blockIdx.x % H, pass = blockIdx.x / H % passes;
     const uint32_t qh0 = kv_head * group + pass * GQ, nq = min((uint32_t)GQ, group - pass * GQ);
-    const uint32_t tiles_per_page = p.block_size / fp4_tile;
+    const uint32_t page_log = __builtin_ctz(p.block_size / fp4_tile); // a page's tiles
     constexpr uint32_t tile_bytes = fp4_tile_bytes(D);
-    const uint64_t layer_bytes = (uint64_t)p.blocks * tiles_per_page * H * tile_bytes;
+    const uint64_t layer_bytes = ((uint64_t)p.blocks * H << page_log) * tile_bytes;
     const uint8_t* kl = static_cast<const uint8_t*>(p.keys) + layer * layer_bytes;
     const uint8_t* vl = static_cast<const uint8_t*>(p.values) + layer * layer_bytes;
+    const float slack = 8.0f / scale_log2;
+    const bool q_vectors = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
     // a term takes what the terms before it left: bits of each earlier rounding to subtract
     const uint32_t query = c % GQ, term = c / GQ;
     const uint32_t minus1 = term >= 1 ? ~0u : 0, minus2 = term >= 2 ? ~0u : 0, minus3 = term >= 3 ? ~0u : 0;
@@ -98,84 +105,113 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
 
     auto segment = [&](const uint4 e0, const uint4 e1) {
         const uint32_t row = e0.x, chunk = e0.y, position = e0.z, n_chunks = e1.z;
-        const uint32_t u_first = e1.x * tiles_per_page, u_last = position / fp4_tile;
-        const uint32_t u_end = min(e1.y * tiles_per_page, u_last + 1);
+        const uint32_t u_first = e1.x << page_log, u_last = position / fp4_tile;
+        const uint32_t u_end = min(e1.y << page_log, u_last + 1);
         const uint32_t* tbl = m.table + (e0.w - e1.x); // the row's table
 
         // step s of the contraction: features 128i + 32g + 8w of s = 4i + w (64-wide: 16g + 8s)
+        // (256-wide heads keep them in LDS behind the records: 32 registers fewer let three
+        // waves run on a SIMD in place of two)
+        constexpr bool Q_LDS = D == 256;
+        uint4* const q_lds = reinterpret_cast<uint4*>(lds + W * GQ * RF + 4);
         uint4 qv[KS];
-#pragma unroll
-        for (uint32_t s = 0; s < KS; ++s) {
+        auto load_query = [&](uint32_t s) {
             const uint32_t f = D == 64 ? 16 * g + 8 * s : s / 4 * 128 + 32 * g + s % 4 * 8;
             const uint64_t at = ((uint64_t)row * q_heads + qh0 + min(query, nq - 1)) * D + f;
-            uint32_t w[4] = {};
-            if (query < nq) {
-                if constexpr (DT == CKV_BF16) {
-                    if (term == 0)
-                        for (int i = 0; i < 4; ++i) {
-                            const uint16_t* e = static_cast<const uint16_t*>(q) + at + 2 * i;
-                            w[i] = e[0] | (uint32_t)e[1] << 16;
-                        }
-                } else {
+            float x[8];
+            if (q_vectors) {
+                float lo[4], hi[4];
+                load4<DT>(q, at, lo);
+                load4<DT>(q, at + 4, hi);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        w[i] = split_terms(load_elem<DT>(q, at + 2 * i), load_elem<DT>(q, at + 2 * i + 1));
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = lo[i];
+                    x[4 + i] = hi[i];
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[i] = load_elem<DT>(q, at + i);
             }
-            qv[s] = make_uint4(w[0], w[1], w[2], w[3]);
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // (a negative scale turns the sign, a scale of 0 leaves nothing)
+                const float u = q_sign == 0.0f ? 0.0f : x[2 * i] * q_sign;
+                const float v = q_sign == 0.0f ? 0.0f : x[2 * i + 1] * q_sign;
+                w[i] = SUMMED ? split_terms(u, v) : pack_bf16(u, v);
+            }
+            return query < nq ? make_uint4(w[0], w[1], w[2], w[3]) : make_uint4(0, 0, 0, 0);
+        };
+        if constexpr (Q_LDS) {
+            for (uint32_t s = wave; s < KS; s += W)
+                q_lds[s * 64 + lane] = load_query(s);
+        } else {
+#pragma unroll
+            for (uint32_t s = 0; s < KS; ++s)
+                qv[s] = load_query(s);
         }
 
+        // the running maximum of the scores (unscaled), and where it has to move: states start at
+        // the lowest finite one, so that a score of -inf weighs 0 also where no other came yet
         float mx = -FLT_MAX, limit = -FLT_MAX, den = 0.0f;
         f32x4_t o[MT];
 #pragma unroll
         for (uint32_t t = 0; t < MT; ++t)
             o[t] = f32x4_t {};
 
-        auto load_tile = [&](uint32_t u, tile_t& x) {
-            const uint64_t at = ((uint64_t)tbl[u / tiles_per_page] * H + kv_head) * tiles_per_page + u % tiles_per_page;
-            const uint8_t* kb = kl + at * tile_bytes;
-            const uint8_t* vb = vl + at * tile_bytes;
+        auto tile_base = [&](uint32_t u) {
+            using c32 = const __attribute__((address_space(4))) uint32_t;
+            const uint64_t page = (uint64_t)*((c32*)(uintptr_t)tbl + (u >> page_log)) * H + kv_head;
+            return ((page << page_log) + (u & ((1u << page_log) - 1))) * tile_bytes;
+        };
+        // Of a tile past the segment's last the last is loaded again.
+        auto load_keys = [&](uint64_t base, tile_t& x) {
+            const uint8_t* kb = kl + base;
             if constexpr (D == 64) {
                 const uint2 kk = *reinterpret_cast<const uint2*>(kb + c * 32 + g * 8);
-                const uint2 vv = *reinterpret_cast<const uint2*>(vb + lane * 8);
                 x.k[0] = kk.x;
                 x.k[1] = kk.y;
-                x.v[0] = vv.x;
-                x.v[1] = vv.y;
                 x.ks[0] = kb[8 * D + c * 2 + g / 2];
-                x.vs[0] = *reinterpret_cast<const uint32_t*>(vb + 8 * D + c / 8 * 16 + g * 4);
             } else {
 #pragma unroll
                 for (uint32_t i = 0; i < tile_t::parts; ++i) {
                     const uint4 kk = load_stream(kb + c * (D / 2) + i * 64 + g * 16);
-                    const uint4 vv = load_stream(vb + i * 1024 + lane * 16);
                     x.k[4 * i] = kk.x;
                     x.k[4 * i + 1] = kk.y;
                     x.k[4 * i + 2] = kk.z;
                     x.k[4 * i + 3] = kk.w;
+                    x.ks[i] = kb[8 * D + c * (D / 32) + 4 * i + g];
+                }
+            }
+        };
+        auto load_values = [&](uint64_t base, tile_t& x) {
+            const uint8_t* vb = vl + base;
+            if constexpr (D == 64) {
+                const uint2 vv = *reinterpret_cast<const uint2*>(vb + lane * 8);
+                x.v[0] = vv.x;
+                x.v[1] = vv.y;
+                x.vs[0] = *reinterpret_cast<const uint32_t*>(vb + 8 * D + c / 8 * 16 + g * 4);
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < tile_t::parts; ++i) {
+                    const uint4 vv = load_stream(vb + i * 1024 + lane * 16);
                     x.v[4 * i] = vv.x;
                     x.v[4 * i + 1] = vv.y;
                     x.v[4 * i + 2] = vv.z;
                     x.v[4 * i + 3] = vv.w;
-                    x.ks[i] = kb[8 * D + c * (D / 32) + 4 * i + g];
                     x.vs[i] = *reinterpret_cast<const uint32_t*>(vb + 8 * D + (4 * i + c / 4) * 16 + g * 4);
                 }
             }
         };
-        // A tile past the segment's last: its tokens weigh nothing, its values are zeros.
-        auto no_tile = [&](tile_t& x) {
-#pragma unroll
-            for (uint32_t i = 0; i < tile_t::words; ++i)
-                x.k[i] = x.v[i] = 0;
-#pragma unroll
-            for (uint32_t i = 0; i < tile_t::parts; ++i)
-                x.ks[i] = x.vs[i] = 0;
-        };
         auto scores = [&](const tile_t& x) {
             f32x4_t s {};
+            uint32_t at = lane;
+            if constexpr (Q_LDS)
+                asm volatile("" : "+v"(at)); // read in each step, not held
 #pragma unroll
             for (uint32_t i = 0; i < KS; ++i)
-                s = mfma16(fp4_eight<false>(x.k[i], fp4_scale(x.ks[i / 4])), qv[i], s);
+                s = mfma16(fp4_eight<false>(x.k[i], fp4_scale(x.ks[i / 4])), Q_LDS ? q_lds[i * 64 + at] : qv[i], s);
             return s;
         };
         // the two operand words of a feature's four tokens: features 8c + 2j and + 1 of part i
@@ -204,14 +240,39 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
                 odd[h] = __builtin_amdgcn_perm(cv[2 * h + 1], cv[2 * h], 0x07060302);
             }
         };
-        auto process = [&](tile_t& a, tile_t& b, uint32_t u) {
+        // A wave has one step's tiles in its registers: the next one's keys are on their way once
+        // the scores are taken, its values once these are (two sets of registers would leave
+        // a compute unit half its waves, which cover more of the latency).
+        tile_t a, b;
+        uint32_t u = u_first + 2 * wave;
+        uint64_t base_a = 0, base_b = 0;
+        auto find = [&](uint32_t at) {
+            base_a = tile_base(at);
+            base_b = tile_base(min(at + 1, u_end - 1));
+        };
+        if (u < u_end) {
+            find(u);
+            load_keys(base_a, a);
+            load_keys(base_b, b);
+            load_values(base_a, a);
+            load_values(base_b, b);
+        }
+        if constexpr (Q_LDS)
+            __syncthreads();
+        while (u < u_end) {
+            const uint32_t next = u + 2 * W;
             const bool two = u + 1 < u_end;
-            f32x4_t sa = scores(a), sb = scores(b);
+            const f32x4_t sa = scores(a), sb = scores(b);
+            if (next < u_end) {
+                find(next);
+                load_keys(base_a, a);
+                load_keys(base_b, b);
+            }
             float t[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                t[i] = terms_sum<TERMS>(sa[i]) * scale_log2;
-                t[4 + i] = terms_sum<TERMS>(sb[i]) * scale_log2;
+                t[i] = SUMMED ? terms_sum<TERMS>(sa[i]) : sa[i];
+                t[4 + i] = SUMMED ? terms_sum<TERMS>(sb[i]) : sb[i];
             }
             if (!two || u + 1 >= u_last) { // the row's end
                 const uint32_t first = u * fp4_tile + 4 * g; // the lane's first token
@@ -236,18 +297,19 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
             if (__builtin_amdgcn_ballot_w64(top > limit)) {
                 float nm = swap16(top, [](float x, float y) { return fmaxf(x, y); });
                 nm = fmaxf(mx, swap32(nm, [](float x, float y) { return fmaxf(x, y); }));
-                const float alpha = fast_exp2(mx - nm);
+                const float alpha = fast_exp2((mx - nm) * scale_log2);
                 den *= alpha;
 #pragma unroll
                 for (uint32_t i = 0; i < MT; ++i)
                     o[i] *= alpha;
                 mx = nm;
-                limit = nm + 8.0f; // probabilities up to 2^8 weigh as exactly
+                limit = nm + slack; // probabilities up to 2^8 weigh as exactly
             }
+            const float shift = -mx * scale_log2;
             float pr[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                pr[i] = fast_exp2(t[i] - mx);
+                pr[i] = fast_exp2(__builtin_fmaf(t[i], scale_log2, shift));
             den += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
             const uint4 pt = make_uint4(split_terms(pr[0], pr[1]), split_terms(pr[2], pr[3]),
                                         split_terms(pr[4], pr[5]), split_terms(pr[6], pr[7]));
@@ -263,30 +325,10 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
                     even = mfma16(make_uint4(ae[0], ae[1], be[0], be[1]), pt, even);
                     odd = mfma16(make_uint4(ao[0], ao[1], bo[0], bo[1]), pt, odd);
                 }
-        };
-        auto load_two = [&](uint32_t u, tile_t& a, tile_t& b) {
-            load_tile(u, a);
-            if (u + 1 < u_end)
-                load_tile(u + 1, b);
-            else
-                no_tile(b);
-        };
-        tile_t a0, b0, a1, b1;
-        uint32_t u = u_first + 2 * wave;
-        if (u < u_end)
-            load_two(u, a0, b0);
-        while (u < u_end) {
-            uint32_t next = u + 2 * W;
-            if (next < u_end)
-                load_two(next, a1, b1);
-            process(a0, b0, u);
-            u = next;
-            if (u >= u_end)
-                break;
-            next = u + 2 * W;
-            if (next < u_end)
-                load_two(next, a0, b0);
-            process(a1, b1, u);
+            if (next < u_end) {
+                load_values(base_a, a);
+                load_values(base_b, b);
+            }
             u = next;
         }
 
@@ -316,7 +358,8 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
             }
         }
         __syncthreads();
-        // n records of query j, features f .. f + 3, `stride` floats apart, folded online
+        // n records of a query, four features of theirs, folded online (what is at r >= n is
+        // read, in bounds, but not used)
         auto fold = [&](auto&& head_at, auto&& acc_at, uint32_t n, float& M, float& d, float (&x)[4]) {
             M = -FLT_MAX;
             d = 0.0f;
@@ -326,15 +369,15 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
                 float4 v[4];
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
-                    h[i] = head_at(min(r0 + i, n - 1));
-                    v[i] = acc_at(min(r0 + i, n - 1));
+                    h[i] = head_at(r0 + i);
+                    v[i] = acc_at(r0 + i);
                     if (r0 + i >= n) { // (weights of 0 would make NaN of an infinity)
                         h[i] = make_float2(-FLT_MAX, 0.0f);
                         v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     }
                 }
                 const float nm = fmaxf(fmaxf(M, fmaxf(h[0].x, h[1].x)), fmaxf(h[2].x, h[3].x));
-                const float keep = fast_exp2(M - nm);
+                const float keep = fast_exp2((M - nm) * scale_log2);
                 M = nm;
                 d *= keep;
 #pragma unroll
@@ -342,7 +385,7 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
                     x[e] *= keep;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
-                    const float weight = fast_exp2(h[i].x - nm);
+                    const float weight = fast_exp2((h[i].x - nm) * scale_log2);
                     d += h[i].y * weight;
                     x[0] += v[i].x * weight;
                     x[1] += v[i].y * weight;
@@ -351,9 +394,11 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
                 }
             }
         };
-        auto waves_state = [&](uint32_t j, uint32_t f, float& M, float& d, float (&x)[4]) {
-            fold([&](uint32_t r) { return *reinterpret_cast<const float2*>(lds + (r * GQ + j) * RF); },
-                 [&](uint32_t r) { return *reinterpret_cast<const float4*>(lds + (r * GQ + j) * RF + 4 + f); }, W, M, d, x);
+        // the first n records in LDS (the waves', or the slices' below)
+        auto states = [&](uint32_t n, uint32_t j, uint32_t f, float& M, float& d, float (&x)[4]) {
+            const auto record = [&](uint32_t r) { return lds + (min(r, n - 1) * GQ + j) * RF; };
+            fold([&](uint32_t r) { return *reinterpret_cast<const float2*>(record(r)); },
+                 [&](uint32_t r) { return *reinterpret_cast<const float4*>(record(r) + 4 + f); }, n, M, d, x);
         };
         const uint64_t out_row = ((uint64_t)row * q_heads + qh0) * D;
         auto emit = [&](uint32_t t, const float (&x)[4], float d) {
@@ -376,7 +421,7 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
         if (n_chunks == 1) {
             for (uint32_t t = tid; t < T4; t += blockDim.x) {
                 float M, d, x[4];
-                waves_state(t / (D / 4), 4 * t % D, M, d, x);
+                states(W, t / (D / 4), 4 * t % D, M, d, x);
                 emit(t, x, d);
             }
             return;
@@ -389,7 +434,7 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
             for (uint32_t t = tid; t < T4; t += blockDim.x) {
                 const uint32_t j = t / (D / 4), f = 4 * t % D;
                 float M, d, x[4];
-                waves_state(j, f, M, d, x);
+                states(W, j, f, M, d, x);
                 agent_store4(rec, (j * RF + 4 + f) * 4, x[0], x[1], x[2], x[3]);
                 if (f == 0)
                     agent_store4(rec, j * RF * 4, M, d, 0.0f, 0.0f);
@@ -398,7 +443,7 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
         wait_vector_memory();
         __syncthreads();
         uint32_t* const arrivals = split.arrivals + ((uint64_t)m.split_first[row] * H + kv_head) * passes + pass;
-        uint32_t* const last_flag = reinterpret_cast<uint32_t*>(lds);
+        uint32_t* const last_flag = reinterpret_cast<uint32_t*>(lds + W * GQ * RF);
         if (tid == 0) {
             const uint32_t before = __hip_atomic_fetch_add(arrivals, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             const uint32_t last = before == n_chunks - 1;
@@ -409,12 +454,20 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
         __syncthreads();
         if (!*last_flag)
             return;
-        for (uint32_t t = tid; t < T4; t += blockDim.x) {
-            const uint32_t j = t / (D / 4), f = 4 * t % D;
+        // Thread (slice, j, f) folds records slice, slice + S, ... of query j; the slices are
+        // folded through LDS. Slices enough for four records each, W of them fit.
+        const uint32_t S = max(1u, min(min(blockDim.x / T4, W), (n_chunks + 3) / 4));
+        for (uint32_t t = tid; t < S * T4; t += blockDim.x) {
+            const uint32_t slice = t / T4, j = t % T4 / (D / 4), f = 4 * t % D;
+            const uint32_t n = (n_chunks - slice + S - 1) / S;
             float M, d, x[4];
-            // (a descriptor for each record: a row's may span more than 4 GiB)
+            // records r S .. r S + S - 1, those past the row's last out of the descriptor's range: 0
             auto at = [&](uint32_t r, uint32_t off) {
-                return agent_load4(record_rsrc(records + (uint64_t)r * record_stride, nq * RF * 4), (j * RF + off) * 4);
+                const uint32_t first = r * S, left = first < n_chunks ? min(S, n_chunks - first) : 0;
+                const __amdgpu_buffer_rsrc_t rec =
+                    record_rsrc(records + (uint64_t)first * record_stride,
+                                left ? ((left - 1) * record_stride + nq * RF) * 4 : 0);
+                return agent_load4(rec, (slice * record_stride + j * RF + off) * 4);
             };
             fold(
                 [&](uint32_t r) {
@@ -425,7 +478,22 @@ __global__ __launch_bounds__(64 * fp4_lane_waves, 2) void fp4_decode_kernel(
                     const u32x4_t v = at(r, 4 + f);
                     return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
                 },
-                n_chunks, M, d, x);
+                n, M, d, x);
+            if (S == 1) {
+                emit(t, x, d);
+                continue;
+            }
+            float* dst = lds + (slice * GQ + j) * RF;
+            *reinterpret_cast<float4*>(dst + 4 + f) = make_float4(x[0], x[1], x[2], x[3]);
+            if (f == 0)
+                *reinterpret_cast<float2*>(dst) = make_float2(M, d);
+        }
+        if (S == 1)
+            return;
+        __syncthreads();
+        for (uint32_t t = tid; t < T4; t += blockDim.x) {
+            float M, d, x[4];
+            states(S, t / (D / 4), 4 * t % D, M, d, x);
             emit(t, x, d);
         }
     };
@@ -467,10 +535,13 @@ hipError_t launch_fp4_decode(hipStream_t s, const pool_view& p, const meta_view&
         return hipSuccess;
     if (grid > 0x7FFFFFFFull)
         return hipErrorInvalidValue;
-    const uint32_t waves = fp4_lane_waves, queries = p.dtype == CKV_F32 ? 4 : 8;
-    const size_t lds = (size_t)waves * queries * (p.head_dim + 4) * sizeof(float);
+    const uint32_t waves = fp4_waves_of(p.head_dim), queries = p.dtype == CKV_F32 ? 4 : 8;
+    const size_t lds = ((size_t)waves * queries * (p.head_dim + 4) + 4) * sizeof(float)
+        + (p.head_dim == 256 ? 8192 : 0);
+    const float scale_log2 = scale == 0.0f ? log2e : std::fabs(scale) * log2e;
+    const float sign = scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f;
     auto launch = [&](auto* kernel) {
-        kernel<<<(uint32_t)grid, 64 * waves, lds, s>>>(p, m, layer, q, q_heads, scale * log2e, out, gate, split, passes);
+        kernel<<<(uint32_t)grid, 64 * waves, lds, s>>>(p, m, layer, q, q_heads, scale_log2, sign, out, gate, split, passes);
         return hipGetLastError();
     };
     auto typed = [&](auto dim) {
