@@ -1195,12 +1195,12 @@ int setup_fp4_decode(ckv_pool* pool, size_t q_heads, split_scratch& split)
 }
 
 int launch_fp4_rows(ckv_pool* pool, size_t layer, const void* queries, size_t q_heads, float scale, void* output,
-                    const void* gate, const split_scratch& split)
+                    const void* gate, const split_scratch& split, bool float_queries = false)
 {
     ckv_context* ctx = pool->ctx;
     return run_kernel(ctx, "fp4_attention_decode", [&] {
         return launch_fp4_decode(ctx->stream, view_of(pool), pool->meta, (uint32_t)layer, queries,
-                                 (uint32_t)q_heads, scale, output, gate, split);
+                                 float_queries, (uint32_t)q_heads, scale, output, gate, split);
     });
 }
 
@@ -1220,9 +1220,10 @@ int run_rotate_append_decode(ckv_pool* pool, size_t layer, const ckv::rotation_t
                              const void* values, const void* queries, size_t q_heads, float scale,
                              const void* gate, void* held_keys, void* held_values, void* output, size_t rows)
 {
-    const bool turned = by.rotary != 0;
+    // (a 4-bit pool's kernel takes float queries: they are not rounded on the way)
+    const bool turned = by.rotary != 0, floats = turned && pool->fp4;
     if (turned) {
-        const size_t bytes = rows * q_heads * pool->head_dim * pool->elem_size;
+        const size_t bytes = rows * q_heads * pool->head_dim * (floats ? sizeof(float) : pool->elem_size);
         if (const int status = ensure_device(pool, &pool->d_rope_q, &pool->d_rope_q_bytes, bytes, "rotated queries"))
             return status;
     }
@@ -1233,11 +1234,11 @@ int run_rotate_append_decode(ckv_pool* pool, size_t layer, const ckv::rotation_t
                            : setup_decode(pool, rotated, q_heads, output, all_keys, setup);
     if (!status)
         status = run_rotate_append(pool, layer,
-                                   { queries, turned ? pool->d_rope_q : nullptr, keys, values, held_keys, held_values },
+                                   { queries, turned ? pool->d_rope_q : nullptr, keys, values, held_keys, held_values, floats },
                                    turned ? q_heads : 0, rows, by);
     if (status)
         return status;
-    return pool->fp4 ? launch_fp4_rows(pool, layer, rotated, q_heads, scale, output, gate, split)
+    return pool->fp4 ? launch_fp4_rows(pool, layer, rotated, q_heads, scale, output, gate, split, floats)
                      : run_decode(pool, layer, rotated, q_heads, scale, output, gate);
 }
 
@@ -2212,7 +2213,7 @@ int ckv_append(ckv_pool* pool, size_t layer, const void* keys, const void* value
     if (layer >= pool->layers)
         return set_error(ctx, CKV_E_CACHE_LAYER_OUT_OF_RANGE, "layer >= layers");
     if (pool->fp4)
-        return run_rotate_append(pool, layer, { nullptr, nullptr, keys, values, nullptr, nullptr }, 0, rows,
+        return run_rotate_append(pool, layer, { nullptr, nullptr, keys, values, nullptr, nullptr, false }, 0, rows,
                                  no_rotation);
     const pool_view view = view_of(pool);
     return run_kernel(ctx, "store_kv", [&] {
@@ -2298,7 +2299,7 @@ int ckv_rope_append(ckv_pool* pool, size_t layer, const void* keys, const void* 
         const ckv::rotation_table* by = nullptr;
         const int status = check_rotation(pool, pool->kv_heads, &rotation, by);
         return status ? status
-                      : run_rotate_append(pool, layer, { nullptr, nullptr, keys, values, nullptr, nullptr }, 0, rows, *by);
+                      : run_rotate_append(pool, layer, { nullptr, nullptr, keys, values, nullptr, nullptr, false }, 0, rows, *by);
     }
     const pool_view view = view_of(pool);
     return run_kernel(ctx, "rope_append", [&] {
@@ -2942,7 +2943,7 @@ int ckv_rotate(ckv_pool* pool, const ckv_rotation* rotation, const void* input, 
             return status;
         return run_kernel(ctx, "rotate", [&] {
             return launch_rotate(ctx->stream, view_of(pool), pool->meta, 0,
-                                 { input, output, nullptr, nullptr, nullptr, nullptr }, (uint32_t)rows,
+                                 { input, output, nullptr, nullptr, nullptr, nullptr, false }, (uint32_t)rows,
                                  (uint32_t)heads, *by);
         });
     });
@@ -2988,7 +2989,7 @@ int ckv_rotate_append(ckv_pool* pool, size_t layer, const ckv_rotation* rotation
             status = check_rotation(pool, heads, rotation, by);
         if (status || !rows)
             return status;
-        return run_rotate_append(pool, layer, { queries, rotated, keys, values, held_keys, held_values }, q_heads,
+        return run_rotate_append(pool, layer, { queries, rotated, keys, values, held_keys, held_values, false }, q_heads,
                                  rows, *by);
     });
 }

@@ -644,6 +644,7 @@ struct rotate_rows {
     const void* values;
     void* held_keys;
     void* held_values;
+    bool float_queries; // `rotated` holds floats, whatever the rows' type
 };
 hipError_t launch_rotate(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
                          const rotate_rows& x, uint32_t rows, uint32_t q_heads,
@@ -659,12 +660,13 @@ void rotation_steps(const long double* turns, uint32_t rotary, rotation_table& o
 
 // ---- launchers (kernels_fp4_decode.hip) -------------------------------------------------
 decode_form fp4_decode_form();
+// (float_queries: the queries are floats, whatever the rows' type.)
 // Workgroups that share a (plan workgroup, kv head): each takes at most eight query heads
 // (f32 rows: four).
 uint32_t fp4_decode_passes(const pool_view& p, uint32_t q_heads);
 hipError_t launch_fp4_decode(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
-                             const void* q, uint32_t q_heads, float scale, void* out,
-                             const void* gate, split_scratch split);
+                             const void* q, bool float_queries, uint32_t q_heads, float scale,
+                             void* out, const void* gate, split_scratch split);
 
 // ---- launchers (kernels_prompt.hip) ------------------------------------------------------
 // Rows of an attention of tiles; keys and values only where they are not a 4-bit pool's.

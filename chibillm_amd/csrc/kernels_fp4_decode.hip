@@ -61,12 +61,13 @@ constexpr uint32_t fp4_waves_of(int head_dim)
     return head_dim == 256 ? 4 : 8;
 }
 
-template <int D, int DT>
+// QT: the queries' type, the rows' or float (rotated and not rounded since).
+template <int D, int DT, int QT>
 __global__ __launch_bounds__(64 * fp4_waves_of(D), D == 256 ? 3 : 4) void fp4_decode_kernel(
     pool_view p, meta_view m, uint32_t layer, const void* __restrict__ q, uint32_t q_heads, float scale_log2,
     float q_sign, void* __restrict__ out, const void* __restrict__ gate, split_scratch split, uint32_t passes)
 {
-    constexpr bool SUMMED = DT != CKV_BF16; // bf16 queries stand whole in the columns of all terms
+    constexpr bool SUMMED = QT != CKV_BF16; // bf16 queries stand whole in the columns of all terms
     constexpr int TERMS = DT == CKV_F32 ? 4 : 2, GQ = 16 / TERMS;
     constexpr uint32_t KS = D / 32, MT = D / 16, RF = D + 4;
     using tile_t = fp4_lane<D>;
@@ -121,8 +122,8 @@ __global__ __launch_bounds__(64 * fp4_waves_of(D), D == 256 ? 3 : 4) void fp4_de
             float x[8];
             if (q_vectors) {
                 float lo[4], hi[4];
-                load4<DT>(q, at, lo);
-                load4<DT>(q, at + 4, hi);
+                load4<QT>(q, at, lo);
+                load4<QT>(q, at + 4, hi);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     x[i] = lo[i];
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(64 * fp4_waves_of(D), D == 256 ? 3 : 4) void fp4_de
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    x[i] = load_elem<DT>(q, at + i);
+                    x[i] = load_elem<QT>(q, at + i);
             }
             uint32_t w[4];
 #pragma unroll
@@ -525,7 +526,8 @@ uint32_t fp4_decode_passes(const pool_view& p, uint32_t q_heads)
 }
 
 hipError_t launch_fp4_decode(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer, const void* q,
-                             uint32_t q_heads, float scale, void* out, const void* gate, split_scratch split)
+                             bool float_queries, uint32_t q_heads, float scale, void* out, const void* gate,
+                             split_scratch split)
 {
     if (!m.plan || (m.n_cut && (!split.records || !split.arrivals)))
         return hipErrorInvalidValue;
@@ -546,9 +548,13 @@ hipError_t launch_fp4_decode(hipStream_t s, const pool_view& p, const meta_view&
     };
     auto typed = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
-        return p.dtype == CKV_F32 ? launch(fp4_decode_kernel<D, CKV_F32>)
-            : p.dtype == CKV_BF16 ? launch(fp4_decode_kernel<D, CKV_BF16>)
-                                  : launch(fp4_decode_kernel<D, CKV_F16>);
+        if (p.dtype == CKV_F32)
+            return launch(fp4_decode_kernel<D, CKV_F32, CKV_F32>);
+        if (p.dtype == CKV_BF16)
+            return float_queries ? launch(fp4_decode_kernel<D, CKV_BF16, CKV_F32>)
+                                 : launch(fp4_decode_kernel<D, CKV_BF16, CKV_BF16>);
+        return float_queries ? launch(fp4_decode_kernel<D, CKV_F16, CKV_F32>)
+                             : launch(fp4_decode_kernel<D, CKV_F16, CKV_F16>);
     };
     return p.head_dim == 64 ? typed(std::integral_constant<int, 64> {})
         : p.head_dim == 128 ? typed(std::integral_constant<int, 128> {})

@@ -107,15 +107,34 @@ __device__ __forceinline__ void rotate_words(uint64_t item, const pool_view& p,
         const uint32_t h = head0 + i;
         if (h >= heads)
             break;
+        float fa[each], fb[each];
+#pragma unroll
+        for (uint32_t e = 0; e < each; ++e) {
+            fa[e] = E::load(a[i].e[e]);
+            fb[e] = E::load(b[i].e[e]);
+        }
         if (turned) {
 #pragma unroll
             for (uint32_t e = 0; e < each; ++e) {
-                T& first = PAIRS ? (2 * e < each ? a[i] : b[i]).e[2 * e % each] : a[i].e[e];
-                T& second = PAIRS ? (2 * e < each ? a[i] : b[i]).e[2 * e % each + 1] : b[i].e[e];
-                float r1, r2;
-                rope_pair(E::load(first), E::load(second), c[e], s[e], r1, r2);
-                first = E::store(r1);
-                second = E::store(r2);
+                float& first = PAIRS ? (2 * e < each ? fa : fb)[2 * e % each] : fa[e];
+                float& second = PAIRS ? (2 * e < each ? fa : fb)[2 * e % each + 1] : fb[e];
+                rope_pair(first, second, c[e], s[e], first, second);
+            }
+        }
+        if (x.float_queries && h < q_heads) {
+            float* to = static_cast<float*>(x.rotated) + q_row + h * d + at;
+#pragma unroll
+            for (uint32_t e = 0; e < each; e += 4) {
+                *reinterpret_cast<float4*>(to + e) = make_float4(fa[e], fa[e + 1], fa[e + 2], fa[e + 3]);
+                *reinterpret_cast<float4*>(to + apart + e) = make_float4(fb[e], fb[e + 1], fb[e + 2], fb[e + 3]);
+            }
+            continue;
+        }
+        if (turned) {
+#pragma unroll
+            for (uint32_t e = 0; e < each; ++e) {
+                a[i].e[e] = E::store(fa[e]);
+                b[i].e[e] = E::store(fb[e]);
             }
         }
         T* dst;
@@ -177,12 +196,19 @@ __global__ __launch_bounds__(block_threads) void rotate_pairs_kernel(
         const uint64_t width = query ? (uint64_t)q_heads * d : p.features;
         const T* src = static_cast<const T*>(query ? x.queries : x.keys) + row * width + at;
         T o1 = src[a], o2 = src[b];
+        float r1 = E::load(o1), r2 = E::load(o2);
         if (turned) {
-            float s, c, r1, r2;
+            float s, c;
             sincos_turn(by.turns.step[pair], positions[row], s, c);
-            rope_pair(E::load(o1), E::load(o2), c * by.magnitude, s * by.magnitude, r1, r2);
+            rope_pair(r1, r2, c * by.magnitude, s * by.magnitude, r1, r2);
             o1 = E::store(r1);
             o2 = E::store(r2);
+        }
+        if (query && x.float_queries) {
+            float* dst = static_cast<float*>(x.rotated) + row * width + at;
+            dst[a] = r1;
+            dst[b] = r2;
+            continue;
         }
         const auto put = [&](void* to, uint64_t first, T v1, T v2) {
             T* dst = static_cast<T*>(to) + first;
@@ -514,6 +540,7 @@ hipError_t launch_fp4_append(hipStream_t s, const pool_view& p, const meta_view&
     rotate_rows alone {};
     alone.queries = x.queries;
     alone.rotated = x.rotated;
+    alone.float_queries = x.float_queries;
     return launch_rotate(s, p, m, 0, alone, rows, q_heads, by);
 }
 
