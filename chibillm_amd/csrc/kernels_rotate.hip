@@ -232,17 +232,21 @@ __global__ __launch_bounds__(block_threads) void rotate_pairs_kernel(
     }
 }
 
-// Eight elements from `src` as floats; VECTOR: 16-byte words.
+// Eight elements of a row; VECTOR: read in 16-byte words.
+template <int DT>
+union eight {
+    using T = typename turn_element<DT>::type;
+    uint4 v[sizeof(T) / 2];
+    T e[8];
+    __device__ __forceinline__ float at(uint32_t i) const { return turn_element<DT>::load(e[i]); }
+};
+
 template <int DT, bool VECTOR>
-__device__ __forceinline__ void load_eight(const void* base, uint64_t at, float (&f)[8])
+__device__ __forceinline__ eight<DT> load_eight(const void* base, uint64_t at)
 {
-    using E = turn_element<DT>;
-    using T = typename E::type;
+    using T = typename eight<DT>::T;
     const T* src = static_cast<const T*>(base) + at;
-    union {
-        uint4 v[sizeof(T) / 2];
-        T e[8];
-    } x;
+    eight<DT> x;
     if constexpr (VECTOR) {
 #pragma unroll
         for (uint32_t i = 0; i < sizeof(T) / 2; ++i)
@@ -252,9 +256,7 @@ __device__ __forceinline__ void load_eight(const void* base, uint64_t at, float 
         for (uint32_t i = 0; i < 8; ++i)
             x.e[i] = src[i];
     }
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-        f[i] = E::load(x.e[i]);
+    return x;
 }
 
 // Eight numbers of a code word as the rows' type.
@@ -306,101 +308,121 @@ __device__ __forceinline__ void store_fp4(uint8_t* tile, uint32_t d, uint32_t to
         tile[fp4_scale_at(d, token, w / 4, v)] = (uint8_t)byte;
 }
 
-// One thread per (row, kv head, word of 8 features), the four words of a block in
-// neighbouring lanes. VECTOR: rows in 16-byte words, rotary a multiple of 16.
-template <int DT, bool PAIRS, bool VECTOR>
+// One thread per (row, PER kv heads, word of 8 features), the four words of a block in
+// neighbouring lanes; the word's angles serve its heads. VECTOR: rows in 16-byte words,
+// rotary a multiple of 16.
+template <int DT, bool PAIRS, bool VECTOR, int PER>
 __device__ __forceinline__ void fp4_append(uint64_t item, const pool_view& p,
                                            const uint32_t* __restrict__ slots, uint32_t layer,
                                            const rotate_rows& x, uint32_t rows,
                                            const rotation_table& by,
                                            const uint32_t* __restrict__ positions)
 {
+    constexpr uint32_t angles = PAIRS ? 4 : 8; // of a word's features
     const uint32_t d = p.head_dim, half = by.rotary / 2, words = d / 8;
-    const uint32_t row = (uint32_t)(item / (words * p.kv_heads));
+    const uint32_t parts = (p.kv_heads + PER - 1) / PER;
+    const uint32_t row = (uint32_t)(item / (words * parts));
     if (row >= rows) // whole blocks of lanes
         return;
-    const uint32_t rest = (uint32_t)(item % (words * p.kv_heads));
-    const uint32_t w = rest % words, head = rest / words, f0 = 8 * w;
-    const uint64_t at_head = (uint64_t)row * p.features + head * d;
-    float k[8], v[8];
-    load_eight<DT, VECTOR>(x.keys, at_head + f0, k);
-    load_eight<DT, VECTOR>(x.values, at_head + f0, v);
-    const uint32_t slot = slots[row], position = positions[row];
-    double y[8];
+    const uint32_t rest = (uint32_t)(item % (words * parts));
+    const uint32_t w = rest % words, head0 = rest / words * PER, f0 = 8 * w;
+    const uint64_t at_row = (uint64_t)row * p.features + f0;
+    const bool turned = f0 < by.rotary;
+    eight<DT> k[PER], other[PAIRS ? 1 : PER], v[PER];
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-        y[i] = k[i];
-    if (f0 < by.rotary) {
-        if constexpr (PAIRS) {
+    for (uint32_t i = 0; i < PER; ++i) {
+        const uint64_t at = at_row + min(head0 + i, p.kv_heads - 1) * d; // past the last head: it again
+        k[i] = load_eight<DT, VECTOR>(x.keys, at);
+        v[i] = load_eight<DT, VECTOR>(x.values, at);
+        if constexpr (!PAIRS) {
+            if (turned) {
+                if constexpr (VECTOR) {
+                    other[i] = load_eight<DT, true>(x.keys, f0 < half ? at + half : at - half);
+                } else {
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i += 2)
-                if (VECTOR || f0 + i < by.rotary) {
-                    double s, c;
-                    sincos_turn64(by.turns.step[(f0 + i) / 2], position, s, c);
-                    const double a = y[i], b = y[i + 1];
-                    y[i] = (a * c - b * s) * by.magnitude64;
-                    y[i + 1] = (b * c + a * s) * by.magnitude64;
-                }
-        } else {
-            float other[8];
-            if constexpr (VECTOR) {
-                load_eight<DT, true>(x.keys, at_head + (f0 < half ? f0 + half : f0 - half), other);
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {
-                    using E = turn_element<DT>;
-                    const uint32_t f = f0 + i, o = f < half ? f + half : f < by.rotary ? f - half : f;
-                    other[i] = E::load(static_cast<const typename E::type*>(x.keys)[at_head + o]);
-                }
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const uint32_t f = f0 + i;
-                if (VECTOR || f < by.rotary) {
-                    double s, c;
-                    sincos_turn64(by.turns.step[f < half ? f : f - half], position, s, c);
-                    y[i] = (f < half ? y[i] * c - other[i] * s : y[i] * c + other[i] * s) * by.magnitude64;
+                    for (uint32_t e = 0; e < 8; ++e) {
+                        const uint32_t f = f0 + e, o = f < half ? f + half : f < by.rotary ? f - half : f;
+                        other[i].e[e] = static_cast<const typename eight<DT>::T*>(x.keys)[at - f0 + o];
+                    }
                 }
             }
         }
     }
-    // the largest magnitudes' exponents, biased as a float's
-    uint32_t largest_k = 0, largest_v = 0;
+    const uint32_t slot = slots[row], position = positions[row];
+    double s[angles], c[angles];
+    if (turned) {
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        largest_k = max(largest_k, (uint32_t)(__builtin_bit_cast(uint64_t, y[i]) >> 32) & 0x7FFFFFFFu);
-        largest_v = max(largest_v, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
+        for (uint32_t e = 0; e < angles; ++e) {
+            const uint32_t f = PAIRS ? f0 + 2 * e : f0 + e;
+            if (!VECTOR && f >= by.rotary)
+                break;
+            sincos_turn64(by.turns.step[PAIRS ? f / 2 : f < half ? f : f - half], position, s[e], c[e]);
+            s[e] *= by.magnitude64;
+            c[e] *= by.magnitude64;
+        }
     }
-    const uint32_t byte_k = fp4_scale_byte<DT>((uint32_t)max((int)(block_max(largest_k) >> 20) - 896, 0));
-    const uint32_t byte_v = fp4_scale_byte<DT>(block_max(largest_v) >> 23);
-    const double to_unit = __builtin_bit_cast(double, (uint64_t)(1023 + 127 - byte_k) << 52);
-    float z[8];
+    const uint64_t layer_at = layer * ((uint64_t)p.blocks * p.block_size / fp4_tile * p.kv_heads * fp4_tile_bytes(d));
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-        z[i] = fp4_side(y[i] * to_unit);
-    uint32_t codes_k = fp4_codes(z, 1.0f), codes_v = fp4_codes(v, fp4_scale(byte_v));
-    if (byte_k == 255)
-        codes_k = 0;
-    if (byte_v == 255)
-        codes_v = 0;
-    const uint64_t tile = layer * ((uint64_t)p.blocks * p.block_size / fp4_tile * p.kv_heads * fp4_tile_bytes(d))
-        + fp4_tile_at(slot, head, p.block_size, p.kv_heads, d);
-    store_fp4(static_cast<uint8_t*>(p.keys) + tile, d, slot % fp4_tile, w, false, codes_k, byte_k);
-    store_fp4(static_cast<uint8_t*>(p.values) + tile, d, slot % fp4_tile, w, true, codes_v, byte_v);
-    if (x.held_keys)
-        store_codes<DT, VECTOR>(x.held_keys, at_head + f0, codes_k, fp4_scale(byte_k));
-    if (x.held_values)
-        store_codes<DT, VECTOR>(x.held_values, at_head + f0, codes_v, fp4_scale(byte_v));
+    for (uint32_t i = 0; i < PER; ++i) {
+        const uint32_t head = head0 + i;
+        if (head >= p.kv_heads)
+            break;
+        double y[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e)
+            y[e] = k[i].at(e);
+        if (turned) {
+#pragma unroll
+            for (uint32_t e = 0; e < angles; ++e) {
+                const uint32_t f = PAIRS ? f0 + 2 * e : f0 + e;
+                if (!VECTOR && f >= by.rotary)
+                    break;
+                if constexpr (PAIRS) {
+                    const double a = y[2 * e], b = y[2 * e + 1];
+                    y[2 * e] = a * c[e] - b * s[e];
+                    y[2 * e + 1] = b * c[e] + a * s[e];
+                } else {
+                    const double o = other[i].at(e);
+                    y[e] = f < half ? y[e] * c[e] - o * s[e] : y[e] * c[e] + o * s[e];
+                }
+            }
+        }
+        // the largest magnitudes' exponents, biased as a float's
+        uint32_t largest_k = 0, largest_v = 0;
+        float u[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            u[e] = v[i].at(e);
+            largest_k = max(largest_k, (uint32_t)(__builtin_bit_cast(uint64_t, y[e]) >> 32) & 0x7FFFFFFFu);
+            largest_v = max(largest_v, __builtin_bit_cast(uint32_t, u[e]) & 0x7FFFFFFFu);
+        }
+        const uint32_t byte_k = fp4_scale_byte<DT>((uint32_t)max((int)(block_max(largest_k) >> 20) - 896, 0));
+        const uint32_t byte_v = fp4_scale_byte<DT>(block_max(largest_v) >> 23);
+        const double to_unit = __builtin_bit_cast(double, (uint64_t)(1023 + 127 - byte_k) << 52);
+        float z[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e)
+            z[e] = fp4_side(y[e] * to_unit);
+        const uint32_t codes_k = byte_k == 255 ? 0 : fp4_codes(z, 1.0f);
+        const uint32_t codes_v = byte_v == 255 ? 0 : fp4_codes(u, fp4_scale(byte_v));
+        const uint64_t tile = layer_at + fp4_tile_at(slot, head, p.block_size, p.kv_heads, d);
+        store_fp4(static_cast<uint8_t*>(p.keys) + tile, d, slot % fp4_tile, w, false, codes_k, byte_k);
+        store_fp4(static_cast<uint8_t*>(p.values) + tile, d, slot % fp4_tile, w, true, codes_v, byte_v);
+        if (x.held_keys)
+            store_codes<DT, VECTOR>(x.held_keys, at_row + head * d, codes_k, fp4_scale(byte_k));
+        if (x.held_values)
+            store_codes<DT, VECTOR>(x.held_values, at_row + head * d, codes_v, fp4_scale(byte_v));
+    }
 }
 
 // The first `append_blocks` workgroups append, the others rotate queries.
-template <int DT, bool PAIRS>
+template <int DT, bool PAIRS, int PER>
 __global__ __launch_bounds__(block_threads) void fp4_rotate_append_kernel(
     pool_view p, const uint32_t* __restrict__ slots, uint32_t layer, rotate_rows x, uint32_t rows,
     uint32_t q_heads, rotation_table by, const uint32_t* __restrict__ positions, uint32_t append_blocks)
 {
     if (blockIdx.x < append_blocks)
-        fp4_append<DT, PAIRS, true>((uint64_t)blockIdx.x * block_threads + threadIdx.x, p, slots, layer,
+        fp4_append<DT, PAIRS, true, PER>((uint64_t)blockIdx.x * block_threads + threadIdx.x, p, slots, layer,
                                     x, rows, by, positions);
     else
         rotate_words<DT, PAIRS, 4>((uint64_t)(blockIdx.x - append_blocks) * block_threads + threadIdx.x,
@@ -412,7 +434,7 @@ __global__ __launch_bounds__(block_threads) void fp4_append_any_kernel(
     pool_view p, const uint32_t* __restrict__ slots, uint32_t layer, rotate_rows x, uint32_t rows,
     rotation_table by, const uint32_t* __restrict__ positions)
 {
-    fp4_append<DT, PAIRS, false>((uint64_t)blockIdx.x * block_threads + threadIdx.x, p, slots, layer, x,
+    fp4_append<DT, PAIRS, false, 1>((uint64_t)blockIdx.x * block_threads + threadIdx.x, p, slots, layer, x,
                                  rows, by, positions);
 }
 
@@ -515,21 +537,28 @@ hipError_t launch_fp4_append(hipStream_t s, const pool_view& p, const meta_view&
     if (!rows)
         return hipSuccess;
     uint32_t append = 0, queries = 0;
-    if (const hipError_t e = grid_of((uint64_t)rows * p.kv_heads * (p.head_dim / 8), append))
-        return e;
+    const uint64_t words = (uint64_t)rows * (p.head_dim / 8);
     if (by.rotary % 16 == 0 && in_words(p, x, by.rotary, false)) {
+        // four heads share their angles, unless that leaves under two workgroups a compute unit
+        const bool four = words * ((p.kv_heads + 3) / 4) >= 512 * block_threads;
+        if (const hipError_t e = grid_of(words * (four ? (p.kv_heads + 3) / 4 : p.kv_heads), append))
+            return e;
         if (const hipError_t e = grid_of((uint64_t)rows * (p.head_dim / (32 / p.elem_size)) * ((q_heads + 3) / 4), queries))
             return e;
         if ((uint64_t)append + queries > 0x7FFFFFFFull)
             return hipErrorInvalidValue;
         of_type(p.dtype, [&](auto dt) {
             constexpr int DT = decltype(dt)::value;
-            auto* kernel = by.neighbours ? fp4_rotate_append_kernel<DT, true> : fp4_rotate_append_kernel<DT, false>;
+            auto* kernel = by.neighbours
+                ? (four ? fp4_rotate_append_kernel<DT, true, 4> : fp4_rotate_append_kernel<DT, true, 1>)
+                : (four ? fp4_rotate_append_kernel<DT, false, 4> : fp4_rotate_append_kernel<DT, false, 1>);
             kernel<<<append + queries, block_threads, 0, s>>>(p, m.slots, layer, x, rows, q_heads, by,
                                                               m.positions, append);
         });
         return hipGetLastError();
     }
+    if (const hipError_t e = grid_of(words * p.kv_heads, append))
+        return e;
     of_type(p.dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         auto* kernel = by.neighbours ? fp4_append_any_kernel<DT, true> : fp4_append_any_kernel<DT, false>;
