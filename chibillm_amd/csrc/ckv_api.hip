@@ -1242,6 +1242,51 @@ int run_rotate_append_decode(ckv_pool* pool, size_t layer, const ckv::rotation_t
                      : run_decode(pool, layer, rotated, q_heads, scale, output, gate);
 }
 
+// The batch's work list for a form of launch, made and uploaded at its first.
+int ensure_prompt_list(ckv_pool* pool, const pool_view& view, const prompt_form& form, uint32_t q_heads,
+                       prompt_batch*& list)
+{
+    ckv_context* ctx = pool->ctx;
+    auto& all = pool->prompts;
+    size_t at = 0;
+    while (at < pool->n_prompts
+           && !(all[at]->q_heads == q_heads && all[at]->waves == form.waves && all[at]->heads == form.heads
+                && all[at]->paged_kernel == form.paged_kernel && all[at]->fp4 == form.fp4))
+        ++at;
+    if (at == pool->n_prompts) {
+        if (at == all.size())
+            all.push_back(std::make_unique<prompt_batch>());
+        prompt_batch& made = *all[pool->n_prompts++];
+        made.ready = false;
+        made.q_heads = q_heads;
+        made.waves = form.waves;
+        made.heads = form.heads;
+        made.paged_kernel = form.paged_kernel;
+        made.fp4 = form.fp4;
+    }
+    list = all[at].get();
+    if (list->ready)
+        return CKV_OK;
+    prompt_list made;
+    write_prompt_list(view, pool->tiles, form, q_heads, ctx->cu_count, made);
+    const size_t words = std::max<size_t>(made.words.size(), 4);
+    void* host = nullptr;
+    int status = stage(ctx, words * sizeof(uint32_t), &host);
+    if (!status)
+        status = ensure_device(pool, &list->d_list, &list->d_list_words, words, "prompt work list");
+    if (status)
+        return status;
+    std::copy(made.words.begin(), made.words.end(), static_cast<uint32_t*>(host));
+    status = upload_staged(ctx, list->d_list, words * sizeof(uint32_t));
+    list->meta = pool->meta;
+    list->meta.tiles = list->d_list;
+    list->meta.n_tiles = (uint32_t)(made.words.size() / prompt_entry_words);
+    list->n_records = made.n_records;
+    list->n_cut = made.n_cut;
+    list->ready = status == CKV_OK;
+    return status;
+}
+
 // The attention of the batch's tiles by kernels_prompt.hip: over a 4-bit pool's cache, or
 // over rows (whole prompts).
 int run_prompt(ckv_pool* pool, size_t layer, const prompt_rows& x, size_t q_heads, float scale, void* output,
@@ -1251,16 +1296,18 @@ int run_prompt(ckv_pool* pool, size_t layer, const prompt_rows& x, size_t q_head
     const pool_view view = view_of(pool);
     const prompt_form form = prompt_form_of(view, pool->meta, x, (uint32_t)q_heads, scale, output, gate, !rows,
                                             ctx->cu_count);
-    window_batch& through = select_window(pool, { UINT32_MAX - 1, 0 }, form.tile_rows());
-    int status = ensure_window_tiles(pool, through);
-    if (status)
+    prompt_batch* list = nullptr;
+    if (const int status = ensure_prompt_list(pool, view, form, (uint32_t)q_heads, list))
         return status;
-    const prefill_shape_info plan = prompt_plan(view, through.meta, form, (uint32_t)q_heads, ctx->cu_count);
+    const uint64_t units = q_heads / form.heads;
+    const prefill_shape_info plan { form.waves, list->n_cut ? 2u : 1u, 1,
+                                    units * list->n_records * 32 * form.waves * (pool->head_dim + 4),
+                                    units * list->n_cut };
     prefill_split split { nullptr, nullptr, plan.n_split, plan.min_blocks };
-    if ((status = ensure_prefill_split(pool, plan, split)))
+    if (const int status = ensure_prefill_split(pool, plan, split))
         return status;
     return run_kernel(ctx, rows ? "prompt_attention" : "fp4_attention_prefill", [&] {
-        return launch_prompt(ctx->stream, view, through.meta, (uint32_t)layer, x, form, (uint32_t)q_heads, scale,
+        return launch_prompt(ctx->stream, view, list->meta, (uint32_t)layer, x, form, (uint32_t)q_heads, scale,
                              output, gate, !rows, split);
     });
 }
@@ -1667,6 +1714,9 @@ int ckv_pool_destroy(ckv_pool* pool)
         for (uint32_t* buffer : { w->d_plan, w->d_work, w->d_tiles })
             if (buffer)
                 (void)dev_free(ctx, buffer);
+    for (const auto& list : pool->prompts)
+        if (list->d_list)
+            (void)dev_free(ctx, list->d_list);
     if (pool->d_axes)
         (void)dev_free(ctx, pool->d_axes);
     if (pool->d_spare)
@@ -1747,6 +1797,7 @@ void adopt_batch(ckv_pool* pool, size_t rows, size_t n_entries, bool with_slots,
     pool->plan_ready = plan_uploaded;
     pool->work_ready = false;
     pool->n_windows = 0;
+    pool->n_prompts = 0;
     pool->axes = 0;
     pool->whole_prompts = -1;
     pool->uploaded = true;

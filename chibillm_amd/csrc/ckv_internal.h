@@ -223,6 +223,18 @@ struct window_batch {
     size_t d_plan_words = 0, d_work_words = 0, d_tiles_words = 0;
 };
 
+// A batch's work list of kernels_prompt.hip for one form of launch, made and kept as a
+// window_batch's.
+struct prompt_batch {
+    bool ready = false;
+    uint32_t q_heads = 0, waves = 0, heads = 0;
+    bool paged_kernel = false, fp4 = false;
+    meta_view meta {};
+    uint32_t n_records = 0, n_cut = 0;
+    uint32_t* d_list = nullptr;
+    size_t d_list_words = 0;
+};
+
 struct pending_timing {
     const char* name;
     hipEvent_t start;
@@ -356,6 +368,8 @@ struct ckv_pool {
     // the current batch through each window it was attended through, then spare ones
     std::vector<std::unique_ptr<ckv::window_batch>> windows;
     size_t n_windows = 0;
+    std::vector<std::unique_ptr<ckv::prompt_batch>> prompts; // the same of work lists
+    size_t n_prompts = 0;
     std::vector<uint32_t> window_positions; // positions less the tokens of the skipped units
 
     // the batch rows' positions on several axes ([axes][rows], ckv_rope_axes_upload)
@@ -682,13 +696,22 @@ struct prompt_rows {
 // rows), and whether it is kernels_prefill.hip's at all.
 struct prompt_form {
     uint32_t waves, heads; // of a workgroup
-    bool paged_kernel;
-    uint32_t tile_rows() const { return 32 * waves / heads; } // which the tiles' are at most
+    bool paged_kernel, fp4;
+    uint32_t tile_rows() const { return 32 * waves / heads; }
 };
 prompt_form prompt_form_of(const pool_view& p, const meta_view& m, const prompt_rows& x, uint32_t q_heads,
                            float scale, const void* out, const void* gate, bool fp4, int cu_count);
-prefill_shape_info prompt_plan(const pool_view& p, const meta_view& m, const prompt_form& form,
-                               uint32_t q_heads, int cu_count);
+// A launch's work list: the batch's tiles cut into a workgroup's rows and, where that leaves
+// compute units idle, each into ranges of its keys. An entry of prompt_entry_words for each
+// range: first row, rows, first position, table offset, range, ranges, the tile's first
+// record and its place among the tiles that are cut; most key blocks first.
+constexpr size_t prompt_entry_words = 8;
+struct prompt_list {
+    std::vector<uint32_t> words;
+    uint32_t n_records = 0, n_cut = 0; // for each (pass, kv head)
+};
+void write_prompt_list(const pool_view& p, const std::vector<uint32_t>& tiles, const prompt_form& form,
+                       uint32_t q_heads, int cu_count, prompt_list& list);
 hipError_t launch_prompt(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
                          const prompt_rows& rows, const prompt_form& form, uint32_t q_heads,
                          float scale, void* out, const void* gate, bool fp4,

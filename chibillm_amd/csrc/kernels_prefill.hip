@@ -179,14 +179,16 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     // key ranges vary slowest: every tile's first range is dispatched before
     // any second one (ranges interleaved with the rows placed the ranges that
     // find no keys, and the long ones, unevenly: +5 to +29 % launch time)
-    const uint32_t n_split = SPLIT ? split_scratch.n_split : 1;
+    const uint32_t n_split = SPLIT && !ROWS ? split_scratch.n_split : 1;
     const uint32_t n_rest = md.n_tiles * subs;
     const uint32_t rest = of_pass % n_rest;
-    const uint32_t part = of_pass / n_rest; // this workgroup's range of the keys
+    // (ROWS: the work list tells it)
+    const uint4 range = ROWS ? *reinterpret_cast<const uint4*>(md.tiles + prompt_entry_words * rest + 4) : uint4 {};
+    const uint32_t part = ROWS ? range.x : of_pass / n_rest; // this workgroup's range of the keys
     const uint32_t sub = rest % subs;
     const uint32_t tile = rest / subs;
     // one scalar load gives the tile: first row, rows, first position, table offset
-    const uint4 te = *reinterpret_cast<const uint4*>(md.tiles + tile_entry_words * tile);
+    const uint4 te = *reinterpret_cast<const uint4*>(md.tiles + (ROWS ? prompt_entry_words : tile_entry_words) * tile);
     const uint32_t count = te.y;
     const uint32_t r0 = sub * tile_rows;
     if (r0 >= count)
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
     // workgroups), range `part`.
     uint32_t n_parts = 1, kb_begin = 0, kb_end = n_blocks;
     if constexpr (SPLIT && RANGES) {
-        n_parts = prefill_range_count(n_blocks, n_split, split_scratch.min_blocks);
+        n_parts = ROWS ? range.y : prefill_range_count(n_blocks, n_split, split_scratch.min_blocks);
         if (part >= n_parts)
             return;
         prefill_range_bounds(n_blocks, n_parts, part, kb_begin, kb_end);
@@ -673,12 +675,14 @@ __global__ __launch_bounds__(64 * W, 2) void prefill_kernel(
         // bytes per access. The share that arrives last folds every share's
         // record, its own included, in share order (the result does not
         // depend on the order of arrival), with weights 2^(m_s - M).
-        const uint32_t pair = ((tile * subs + sub) * passes + pass) * kv_heads + kvh;
+        const uint32_t units = passes * kv_heads, in_units = pass * kv_heads + kvh;
+        const uint32_t pair = (ROWS ? range.w : tile * subs + sub) * units + in_units;
+        const uint64_t first_record = ROWS ? (uint64_t)range.z * units + in_units * n_parts : (uint64_t)pair * n_split;
         const uint32_t qv = wave * 32 + n; // this lane's query vector in the workgroup
         constexpr uint32_t QV = 32 * W, chunks = prefill_record_floats / 4;
         const __amdgpu_buffer_rsrc_t rs = record_rsrc(
-            split_scratch.records + (uint64_t)pair * n_split * (chunks * QV * 4),
-            n_split * chunks * QV * 16);
+            split_scratch.records + first_record * (chunks * QV * 4),
+            (ROWS ? n_parts : n_split) * chunks * QV * 16);
         auto off = [&](uint32_t share, uint32_t chunk) {
             return ((share * chunks + chunk) * QV + qv) * 16u;
         };
@@ -864,7 +868,7 @@ template <int G, int W>
 hipError_t launch_rows(hipStream_t s, const pool_view& p, const meta_view& m, const prompt_rows& x,
                        uint32_t q_heads, float c, void* out, const void* gate, const prefill_split& split)
 {
-    const uint64_t grid = (uint64_t)m.n_tiles * (q_heads / G) * split.n_split;
+    const uint64_t grid = (uint64_t)m.n_tiles * (q_heads / G);
     if (!grid)
         return hipSuccess;
     if (grid > 0x7FFFFFFFull)

@@ -29,6 +29,7 @@
 #include "store_rows.h"
 
 #include <algorithm>
+#include <array>
 #include <cfloat>
 #include <cstdlib>
 #include <type_traits>
@@ -40,6 +41,7 @@ namespace {
 enum source { FROM_FP4, FROM_WORDS, FROM_ROWS };
 
 constexpr uint32_t block_keys = 32;
+constexpr uint32_t prompt_most_ranges = 16; // of a tile's keys
 constexpr uint32_t n_waves = 4, n_threads = 64 * n_waves;
 
 // Where a tile's keys are. Sequence positions are rows of `keys` and `values` (ROWS), or go
@@ -169,35 +171,35 @@ __device__ __forceinline__ void attend_row(const key_source& s, uint32_t positio
 
 // A workgroup's part of a launch.
 struct tile_part {
-    uint32_t pair;  // the (tile, pass, kv head)
-    uint32_t kvh, pass, part;
+    uint32_t kvh, pass, part, n_parts;
+    uint32_t records, arrival; // of this (tile, pass, kv head)
     uint32_t row0, nrows, pos0, pos_last;
     uint32_t table; // the sequence's first table entry
-    uint32_t n_blocks, n_parts, kb_begin, kb_end;
+    uint32_t n_blocks, kb_begin, kb_end;
 };
 
-// Blocks run over kv heads, then passes, then tiles, then key ranges. False: no keys.
-__device__ __forceinline__ bool part_of(const meta_view& md, uint32_t kv_heads, uint32_t passes,
-                                        const prefill_split& split, tile_part& w)
+// Workgroups run over kv heads, then passes, then the list's entries.
+__device__ __forceinline__ tile_part part_of(const meta_view& md, uint32_t kv_heads, uint32_t passes)
 {
+    tile_part w;
     w.kvh = blockIdx.x % kv_heads;
-    const uint32_t unit = blockIdx.x / kv_heads;
-    w.pass = unit % passes;
-    const uint32_t tile = unit / passes % md.n_tiles;
-    w.part = unit / passes / md.n_tiles;
-    w.pair = (tile * passes + w.pass) * kv_heads + w.kvh;
-    const uint4 te = *reinterpret_cast<const uint4*>(md.tiles + tile_entry_words * tile);
-    w.row0 = te.x;
-    w.nrows = te.y;
-    w.pos0 = te.z;
-    w.table = te.w;
+    const uint32_t rest = blockIdx.x / kv_heads;
+    w.pass = rest % passes;
+    const uint4* e = reinterpret_cast<const uint4*>(md.tiles + prompt_entry_words * (rest / passes));
+    const uint4 tile = e[0], range = e[1];
+    w.row0 = tile.x;
+    w.nrows = tile.y;
+    w.pos0 = tile.z;
+    w.table = tile.w;
+    w.part = range.x;
+    w.n_parts = range.y;
+    const uint32_t units = passes * kv_heads, unit = w.pass * kv_heads + w.kvh;
+    w.records = range.z * units + unit * w.n_parts;
+    w.arrival = range.w * units + unit;
     w.pos_last = w.pos0 + w.nrows - 1;
     w.n_blocks = w.pos_last / block_keys + 1;
-    w.n_parts = prefill_range_count(w.n_blocks, split.n_split, split.min_blocks);
-    if (w.part >= w.n_parts)
-        return false;
     prefill_range_bounds(w.n_blocks, w.n_parts, w.part, w.kb_begin, w.kb_end);
-    return true;
+    return w;
 }
 
 // The state of a query vector's range of keys, as records in chunks of four floats, chunk 0
@@ -211,7 +213,7 @@ __device__ __forceinline__ bool fold_ranges(const prefill_split& split, const ti
 {
     constexpr uint32_t QV = 32 * n_waves, chunks = (D + 4) / 4;
     const __amdgpu_buffer_rsrc_t rs = record_rsrc(
-        split.records + (uint64_t)w.pair * split.n_split * (chunks * QV * 4), split.n_split * chunks * QV * 16);
+        split.records + (uint64_t)w.records * (chunks * QV * 4), w.n_parts * chunks * QV * 16);
     auto off = [&](uint32_t share, uint32_t chunk) { return ((share * chunks + chunk) * QV + qv) * 16u; };
 #pragma unroll
     for (int mt = 0; mt < D / 32; ++mt)
@@ -226,11 +228,11 @@ __device__ __forceinline__ bool fold_ranges(const prefill_split& split, const ti
     wait_vector_memory();
     __syncthreads(); // also: every wave is past its LDS reads
     if (tid == 0) {
-        const uint32_t before = __hip_atomic_fetch_add(split.arrivals + w.pair, 1u, __ATOMIC_RELAXED,
+        const uint32_t before = __hip_atomic_fetch_add(split.arrivals + w.arrival, 1u, __ATOMIC_RELAXED,
                                                        __HIP_MEMORY_SCOPE_AGENT);
         const uint32_t last = before == w.n_parts - 1;
         if (last)
-            __hip_atomic_store(split.arrivals + w.pair, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(split.arrivals + w.arrival, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *last_flag = last;
     }
     __syncthreads();
@@ -301,9 +303,7 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
     constexpr uint32_t lds_bytes = n_stages * stage_bytes > out_bytes ? n_stages * stage_bytes : out_bytes;
     __shared__ __attribute__((aligned(16))) uint8_t lds[lds_bytes];
     const uint32_t group = q_heads / p.kv_heads;
-    tile_part w;
-    if (!part_of(md, p.kv_heads, group / GH, split, w))
-        return;
+    const tile_part w = part_of(md, p.kv_heads, group / GH);
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t n = lane & 31, g = lane >> 5;
     const uint32_t head = w.kvh * group + w.pass * GH + wave % GH, rb = wave / GH;
@@ -650,9 +650,7 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel
     __shared__ __attribute__((aligned(16))) float lds[2 * stage_floats];
     static_assert(n_waves * 32 * row_floats<D> <= 2 * stage_floats);
     const uint32_t group = q_heads / p.kv_heads;
-    tile_part w;
-    if (!part_of(md, p.kv_heads, group / GH, split, w))
-        return;
+    const tile_part w = part_of(md, p.kv_heads, group / GH);
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t n = lane & 31, g = lane >> 5;
     const uint32_t head = w.kvh * group + w.pass * GH + wave % GH, rb = wave / GH;
@@ -860,7 +858,7 @@ template <int D, int GH, source SRC>
 hipError_t launch_gh(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer, const prompt_rows& x,
                      uint32_t q_heads, float scale, void* out, const void* gate, const prefill_split& split)
 {
-    const uint64_t grid = (uint64_t)m.n_tiles * (q_heads / GH) * split.n_split;
+    const uint64_t grid = (uint64_t)m.n_tiles * (q_heads / GH);
     if (!grid)
         return hipSuccess;
     if (grid > 0x7FFFFFFFull)
@@ -922,7 +920,7 @@ prompt_form prompt_form_of(const pool_view& p, const meta_view& m, const prompt_
 {
     prompt_rows x = rows;
     set_vectors(p, x, out, gate, fp4);
-    prompt_form form { n_waves, heads_of(p, q_heads), false };
+    prompt_form form { n_waves, heads_of(p, q_heads), false, fp4 };
     form.paged_kernel = !fp4 && p.head_dim == 128 && p.dtype != CKV_F32 && x.vectors && x.out_vectors
         && scale > 0.0f && x.kv_stride <= UINT32_MAX;
     if (!form.paged_kernel)
@@ -935,24 +933,104 @@ prompt_form prompt_form_of(const pool_view& p, const meta_view& m, const prompt_
     return form;
 }
 
-prefill_shape_info prompt_plan(const pool_view& p, const meta_view& m, const prompt_form& form,
-                               uint32_t q_heads, int cu_count)
+namespace {
+
+// What a launch's time is estimated from, us: a key block of a workgroup alone on its compute
+// unit (two there: `shared` of that more for each), what comes before and after the blocks,
+// in blocks, and of a tile that is cut the handoff and each record. Fitted to times of 14
+// batches in 1 to 16 ranges; the ranges it chooses are the fastest measured or within 8 % of
+// that. Uncut and as chosen, us: 512 rows behind 6000 tokens of 4 bits 164 and 46, 4 x 256
+// behind 2000 60 and 34, 900 rows of one prompt 21 and 17, five short float prompts 58 and
+// 21; 8 x 1024 behind 3000 stays uncut (242, in two ranges 271).
+struct prompt_cost {
+    double block, shared, ends, handoff, record;
+    uint32_t per_cu;
+};
+
+prompt_cost cost_of(const pool_view& p, const prompt_form& form)
 {
-    prefill_shape_info plan { form.waves, 1, 4, 0, 0 };
-    const uint64_t grid = (uint64_t)m.n_tiles * (q_heads / form.heads);
-    const uint64_t cus = (uint64_t)std::max(cu_count, 1);
-    if (form.waves == n_waves && grid && grid < cus)
-        plan.n_split = (uint32_t)std::min<uint64_t>(split_max, 2 * cus / grid);
-    if (const char* forced = std::getenv("CKV_PREFILL_SPLIT"))
-        plan.n_split = (uint32_t)std::clamp(std::strtol(forced, nullptr, 10), 1L, (long)split_max);
-    if (form.waves != n_waves
-        || (plan.n_split > 1 && prefill_range_count(m.longest_blocks, plan.n_split, plan.min_blocks) == 1))
-        plan.n_split = 1;
-    if (plan.n_split > 1) {
-        plan.records_floats = grid * plan.n_split * 32 * n_waves * (p.head_dim + 4);
-        plan.counters = grid;
+    const double wide = p.head_dim / 128.0;
+    if (p.dtype == CKV_F32)
+        return { 4.1 * wide, 0.71, 2.6, 5.9, 0.07 * wide, p.head_dim == 256 ? 1u : 2u };
+    if (p.head_dim == 256)
+        return { 1.2, 0.62, 7.8, 6.6, 1.8, 1 };
+    if (p.head_dim == 64)
+        return { 0.42, 0.27, 0.25, 2.8, 1.8, 2 };
+    if (form.paged_kernel)
+        return { 0.67, 0.0, 5.2, 6.3, 0.2, 2 };
+    return { 0.82, 0.24, 1.4, 0.1, 1.5, 2 };
+}
+
+} // namespace
+
+void write_prompt_list(const pool_view& p, const std::vector<uint32_t>& tiles, const prompt_form& form,
+                       uint32_t q_heads, int cu_count, prompt_list& list)
+{
+    struct tile_rows {
+        uint32_t blocks, row, rows, first, table;
+    };
+    const uint32_t rows = form.tile_rows(), units = q_heads / form.heads;
+    std::vector<tile_rows> parts;
+    uint32_t longest = 0;
+    for (size_t t = 0; t < tiles.size(); t += tile_entry_words)
+        for (uint32_t r = 0; r < tiles[t + 1]; r += rows) {
+            const uint32_t n = std::min(rows, tiles[t + 1] - r), first = tiles[t + 2] + r;
+            parts.push_back({ (first + n - 1) / block_keys + 1, tiles[t] + r, n, first, tiles[t + 3] });
+            longest = std::max(longest, parts.back().blocks);
+        }
+    const prompt_cost cost = cost_of(p, form);
+    const double cus = std::max(cu_count, 1);
+    // the longest range of least time
+    const auto ranges_of = [](uint32_t blocks, uint32_t most) { return (blocks + most - 1) / most; };
+    const auto time_of = [&](uint32_t most) {
+        double work = 0, workgroups = 0, records = 0;
+        uint32_t longest_range = 0, most_ranges = 1;
+        for (const tile_rows& t : parts) {
+            const uint32_t n = ranges_of(t.blocks, most);
+            work += units * (t.blocks + n * cost.ends);
+            workgroups += (double)units * n;
+            records += n > 1 ? (double)units * n : 0;
+            longest_range = std::max(longest_range, (t.blocks + n - 1) / n);
+            most_ranges = std::max(most_ranges, n);
+        }
+        const bool shared = cost.per_cu == 2 && workgroups > cus;
+        const double block = cost.block * (shared ? 1 + cost.shared : 1);
+        const double us = std::max((longest_range + cost.ends) * block, work * block / (cus * (shared ? 2 : 1)));
+        // records are written and read, out of the caches, at about 8 bytes a picosecond
+        return us + (most_ranges > 1 ? cost.handoff + most_ranges * cost.record
+                             + records * 128 * (p.head_dim + 4) * 8 / 8e6 : 0.0);
+    };
+    uint32_t most = std::max(longest, 1u);
+    if (form.waves == n_waves) {
+        const auto length_of = [&](uint32_t n) { return std::max(ranges_of(longest, n), 1u); };
+        double best = time_of(most);
+        for (uint32_t n = 2; n <= prompt_most_ranges; ++n)
+            if (const double us = time_of(length_of(n)); us < best) {
+                best = us;
+                most = length_of(n);
+            }
+        if (const char* forced = std::getenv("CKV_PREFILL_SPLIT"))
+            most = length_of((uint32_t)std::clamp(std::strtol(forced, nullptr, 10), 1L, (long)prompt_most_ranges));
     }
-    return plan;
+    struct entry {
+        uint32_t blocks;
+        std::array<uint32_t, prompt_entry_words> words;
+    };
+    std::vector<entry> entries;
+    list.n_records = list.n_cut = 0;
+    for (const tile_rows& t : parts) {
+        const uint32_t n = ranges_of(t.blocks, most);
+        for (uint32_t i = 0; i < n; ++i)
+            entries.push_back({ (t.blocks + n - 1) / n, { t.row, t.rows, t.first, t.table, i, n, list.n_records, list.n_cut } });
+        if (n > 1) {
+            list.n_records += n;
+            ++list.n_cut;
+        }
+    }
+    std::stable_sort(entries.begin(), entries.end(), [](const entry& a, const entry& b) { return a.blocks > b.blocks; });
+    list.words.clear();
+    for (const entry& e : entries)
+        list.words.insert(list.words.end(), e.words.begin(), e.words.end());
 }
 
 hipError_t launch_prompt(hipStream_t s, const pool_view& p, const meta_view& m, uint32_t layer,
