@@ -1019,7 +1019,7 @@ uint32_t fast_waves(uint32_t group, int dtype, uint32_t units, int cu_count,
 // 22.2, 64 behind 1,024 54.4 and 50.3; 8: 64 behind 1,024 75.2 and 68.2, 80 109 and 115.
 // Pieces of 4 pages, at 8 and 4 waves: 4 rows behind 512 6.8 and 6.4, 1 behind 256 6.2
 // and 6.0.
-uint32_t window_waves(uint32_t head_dim, uint32_t group, int dtype, uint32_t units, int cu_count,
+[[maybe_unused]] uint32_t window_waves(uint32_t head_dim, uint32_t group, int dtype, uint32_t units, int cu_count,
                       uint32_t mean_pages, uint32_t split_pages)
 {
     const uint32_t waves = fast_waves(group, dtype, units, cu_count, mean_pages, split_pages);
