@@ -1,15 +1,15 @@
 // Keys and values held in 4 bits: the numbers, the pages' layout and the conversions.
 //
-// A number is a 4-bit float (sign, two exponent bits, one mantissa bit: 0, 1/2, 1, 3/2, 2,
-// 3, 4, 6 and their negatives) times its block's scale, a power of two. A block is 32
-// consecutive features of a head; its scale is 2^(floor(log2 m) - 2) for the block's largest
-// magnitude m, kept as the biased exponent in a byte, so that m / scale is in [4, 8).
-// Numbers round to the nearest, ties to the even code, and those past 6 (m / scale above 7
-// loses at most a quarter) become 6. A scale is no smaller than 2^-23 for f16 rows, whose
-// smallest number is then half of it, and 2^-100 for others: every cached number is one of
-// the rows' type, and of bf16, so that the matrix cores take it exactly. A block with an
-// infinity or NaN has scale byte 255: all of it reads as NaN. 17 bytes a block, 4.25 bits
-// a number: against bf16 a decode step reads 3.76 times as many tokens in its time.
+// A number is a 4-bit float (sign, two exponent bits, one mantissa bit: 0, 1/2, 1, 3/2, 2, 3,
+// 4, 6 and their negatives) times its block's scale, a power of two. A block is 32 consecutive
+// features of a head; its scale is 2^(floor(log2 m) - 2) for the block's largest magnitude m,
+// kept as the biased exponent in a byte, so that m / scale is in [4, 8). Numbers round to the
+// nearest, ties to the even code, and those past 6 (m / scale above 7 loses at most a quarter)
+// become 6. A scale is no smaller than 2^-23 for f16 rows, whose smallest number is then half
+// of it, and 2^-100 for others: every cached number is one of the rows' type, and of bf16, so
+// that the matrix cores take it exactly. A block with an infinity or NaN, or rotated past the
+// type's range, has scale byte 255: all of it reads as NaN. 17 bytes a block, 4.25 bits a
+// number: against bf16 a decode step reads 3.76 times as many tokens in its time.
 //
 // gfx950 converts a pair of codes with its scale in one full-rate instruction (measured:
 // 4.7 cycles a wave against 4.4 of an addition), so a K or V operand of a matrix
@@ -79,12 +79,12 @@ typedef __bf16 fp4_bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 fp4_f16x2_t __attribute__((ext_vector_type(2)));
 
 // The scale byte of a block from the biased exponent (of 127) of its largest magnitude, 255
-// for an infinity or NaN.
+// for an infinity or NaN, and for what f16 has no number for: rotated rows reach 2^16.
 template <int DT>
 __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t biased)
 {
     constexpr int least = 127 + fp4_least_exponent(DT);
-    return biased >= 255 ? 255 : (uint32_t)max((int)biased - 2, least);
+    return biased >= (DT == CKV_F16 ? 127u + 16 : 255u) ? 255 : (uint32_t)max((int)biased - 2, least);
 }
 
 __device__ __forceinline__ float fp4_scale(uint32_t byte)

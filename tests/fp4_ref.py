@@ -18,7 +18,7 @@ def held(x, dtype):
     """x [..., 32 n] in 64 bits as a 4-bit pool of rows of `dtype` holds it."""
     y = x.double().unflatten(-1, (-1, 32))
     largest = y.abs().amax(-1, keepdim=True)
-    lost = ~(largest < 2.0 ** 128)
+    lost = ~(largest < 2.0 ** (16 if dtype == "f16" else 128))
     exponent = torch.frexp(torch.where(lost, 1.0, largest)).exponent - 3
     exponent = torch.where(largest == 0, LEAST[dtype], exponent).clamp(min=LEAST[dtype])
     scale = torch.ldexp(torch.ones_like(largest), exponent)
@@ -56,10 +56,10 @@ def magnitude(rotation):
     return 0.1 * math.log(factor) + 1 if rotation.scaling == 3 and factor > 1 else 1.0
 
 
-def rotated(x, positions, rotation):
+def rotated(x, positions, rotation, angle_error=0.0):
     """x [rows, heads, d] in 64 bits at `positions`, and the error of a 32-bit rotation before its
     rounding: sine and cosine within two steps, products and their sum half a step each, the
-    magnitude another."""
+    magnitude another; and of angles off by `angle_error` of themselves."""
     d = x.shape[-1]
     r = rotation.rotary_dim or d
     turn = np.asarray(positions, np.longdouble)[:, None] * frequencies(rotation, d)
@@ -70,7 +70,8 @@ def rotated(x, positions, rotation):
     first, second = (slice(0, r // 2), slice(r // 2, r)) if rotation.layout == 0 else (slice(0, r, 2), slice(1, r, 2))
     a, b = y[..., first].clone(), y[..., second].clone()
     room = torch.zeros_like(y)
-    room[..., first] = room[..., second] = (a.abs() + b.abs()) * m * 6 * STEP32
+    off = torch.from_numpy((turn * 2 * np.pi).astype(np.float64))[:, None] * angle_error
+    room[..., first] = room[..., second] = (a.abs() + b.abs()) * m * (6 * STEP32 + off)
     y[..., first], y[..., second] = a * c - b * s, b * c + a * s
     return y, room
 
@@ -156,7 +157,7 @@ class Cache:
         return torch.randn(*shape, generator=self.g).to(self.dtype)
 
     def slots(self, i, positions):
-        p = np.asarray(positions)
+        p = np.asarray(positions, int)
         return self.tables[i][p // self.page].astype(np.int64) * self.page + p % self.page
 
     def upload(self, first, counts, with_slots=True):
