@@ -442,6 +442,15 @@ int refuse_fp4(const ckv_pool* pool)
     return pool->fp4 ? set_error(pool->ctx, CKV_E_UNSUPPORTED_DTYPE, "the pool is held in 4 bits") : CKV_OK;
 }
 
+// A run of captured launches over a 4-bit pool of 256-wide heads ended in a GPU fault whose
+// cause was not found: none is captured.
+int refuse_wide_capture(ckv_pool* pool)
+{
+    if (pool->fp4 && pool->head_dim == 256 && capturing(pool->ctx))
+        return set_error(pool->ctx, CKV_E_INVALID_ARGUMENT, "4-bit pools of 256-wide heads: no launch is captured");
+    return CKV_OK;
+}
+
 // The fast decode plan of a batch uploaded without it (one served by the
 // prefill kernel), at its first decode launch.
 int ensure_plan(ckv_pool* pool)
@@ -1175,6 +1184,8 @@ ckv_rotation plain_rotation(float theta, size_t rotary_dim)
 int run_rotate_append(ckv_pool* pool, size_t layer, const rotate_rows& x, size_t q_heads, size_t rows,
                       const ckv::rotation_table& by)
 {
+    if (const int refused = refuse_wide_capture(pool))
+        return refused;
     ckv_context* ctx = pool->ctx;
     const pool_view view = view_of(pool);
     return run_kernel(ctx, pool->fp4 ? "fp4_append" : "rotate_append", [&] {
@@ -1188,6 +1199,10 @@ int run_rotate_append(ckv_pool* pool, size_t layer, const rotate_rows& x, size_t
 // The plan and scratch of a decode launch of a 4-bit pool.
 int setup_fp4_decode(ckv_pool* pool, size_t q_heads, split_scratch& split)
 {
+    if (q_heads > ((size_t)1 << 26) / (pool->head_dim + 4)) // (the kernel's offsets in records are 32 bits)
+        return set_error(pool->ctx, CKV_E_INVALID_ARGUMENT, "row too wide");
+    if (const int refused = refuse_wide_capture(pool))
+        return refused;
     const int status = ensure_plan(pool);
     return status ? status
                   : ensure_split(pool, pool->meta, q_heads, split,
@@ -1316,6 +1331,8 @@ int run_fp4_prefill(ckv_pool* pool, size_t layer, const void* queries, size_t q_
                     const void* gate)
 {
     return guarded(pool, [&]() -> int {
+        if (const int refused = refuse_wide_capture(pool))
+            return refused;
         prompt_rows x {};
         x.queries = queries;
         x.q_stride = (uint64_t)q_heads * pool->head_dim;

@@ -166,7 +166,8 @@ int ckv_pool_wrap(ckv_context* ctx, size_t layers, size_t blocks, size_t block_s
  *   scale = 2^(floor(log2 m) - 2) for the largest magnitude m of the 32, at least 2^-23
  *           (f16 rows) or 2^-100;
  *   x is kept as the nearest of the 16 numbers to x / scale, ties to the even code, at
- *   most 6; a block that holds an infinity or a NaN (or, rotated, 2^128) reads as NaN.
+ *   most 6; a block that holds an infinity or a NaN reads as NaN, and one that its
+ *           rotation takes to 2^128 (f16 rows: 2^16).
  * Every cached number is one of the rows' type. Rows rotated on their way in
  * (ckv_rope_append, ckv_rotate_append and their decode forms) are turned in 64 bits and
  * rounded once.
@@ -176,9 +177,11 @@ int ckv_pool_wrap(ckv_context* ctx, size_t layers, size_t blocks, size_t block_s
  * ckv_rotate calls, ckv_prompt_attention, ckv_copy_blocks, ckv_decode_plan. The others that
  * touch keys and values (windows, ckv_rope_axes_append, ckv_compact,
  * ckv_append_decode_noalloc, checkpoints, ckv_element_offset) return unsupported_dtype.
- * Attention takes any number of query heads per kv head and any scale, with products of
+ * Attention takes any number of query heads per kv head (decode rows of up to 2^26 numbers,
+ * counting four more for each head: invalid_argument) and any scale, with products of
  * bf16 terms that keep at least 16 bits of queries and probabilities in decode rows, and of
  * the rows' type in prefill tiles (f32 rows: 24 bits in both).
+ * Launches on a pool of 256-wide heads are not captured into graphs (invalid_argument).
  * Checks: those of ckv_pool_create, in their order, where the block size must be a power of
  * two from 16 to 4096 (invalid_block_size) and head_dim 64, 128 or 256 (invalid_head_dimension); wrapped
  * buffers must be aligned to 16 bytes (invalid_argument) and hold the bytes_each of

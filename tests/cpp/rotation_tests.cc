@@ -237,6 +237,7 @@ TEST("4-bit pools: geometries and calls that are refused")
     two_rows t;
     t.upload();
     ckv_pool* p = &t.pool;
+    p->positions = { 5, 9 }; // two decode rows
     p->fp4 = true;
     void *q = t.x, *k = t.x + 1, *v = t.x + 2, *o = t.x + 3;
     size_t offset = 0;
@@ -252,6 +253,7 @@ TEST("4-bit pools: geometries and calls that are refused")
     CHECK(ckv_element_offset(p, 0, 0, 0, 0, 0, &offset) == CKV_E_UNSUPPORTED_DTYPE);
     CHECK(ckv_checkpoint_pack(p, words, 1, 16, k, v) == CKV_E_UNSUPPORTED_DTYPE);
     CHECK(ckv_checkpoint_unpack(p, words, 1, 16, k, v) == CKV_E_UNSUPPORTED_DTYPE);
+    CHECK(ckv_decode_attention(p, 0, q, 2 << 19, 1.0f, o, 2) == CKV_E_INVALID_ARGUMENT); // decode rows too wide
     // what they refuse of every pool they refuse of these
     CHECK(ckv_append(p, 0, nullptr, v, 2) == CKV_E_INVALID_ARGUMENT);
     CHECK(ckv_append(p, 0, k, v, 3) == CKV_E_CACHE_SLOT_COUNT_MISMATCH);
