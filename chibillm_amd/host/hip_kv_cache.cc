@@ -144,17 +144,18 @@ host_buffer::~host_buffer()
 // ---- hip_kv_cache ------------------------------------------------------------------
 
 result<hip_kv_cache, kv_cache_error>
-hip_kv_cache::make(const hip_context& ctx, kv_cache_config c, kv_dtype type)
+hip_kv_cache::make(const hip_context& ctx, kv_cache_config c, kv_dtype type, kv_storage storage)
 {
     ckv_pool* pool = nullptr;
-    const int rc = ckv_pool_create(ctx.get(), c.layer_count, c.block_count, c.block_size,
-                                   c.kv_head_count, c.head_dimension, static_cast<int>(type), &pool);
+    const auto create = storage == kv_storage::fp4 ? ckv_pool_create_fp4 : ckv_pool_create;
+    const int rc = create(ctx.get(), c.layer_count, c.block_count, c.block_size, c.kv_head_count,
+                          c.head_dimension, static_cast<int>(type), &pool);
     if (rc >= 200 && rc < 212)
         return fail(kv_cache_error { static_cast<kv_cache_errc>(rc - 200), ckv_last_error(ctx.get()) });
     if (rc)
         return fail(kv_cache_error { kv_cache_errc::allocation_failed,
                                      describe_error(ctx.last(rc)) });
-    return hip_kv_cache(&ctx, pool, c, type);
+    return hip_kv_cache(&ctx, pool, c, type, storage);
 }
 
 hip_kv_cache::hip_kv_cache(hip_kv_cache&& other) noexcept
@@ -162,6 +163,7 @@ hip_kv_cache::hip_kv_cache(hip_kv_cache&& other) noexcept
     , pool_(std::exchange(other.pool_, nullptr))
     , config_(other.config_)
     , type_(other.type_)
+    , storage_(other.storage_)
 {}
 
 hip_kv_cache&
@@ -174,6 +176,7 @@ hip_kv_cache::operator=(hip_kv_cache&& other) noexcept
         pool_ = std::exchange(other.pool_, nullptr);
         config_ = other.config_;
         type_ = other.type_;
+        storage_ = other.storage_;
     }
     return *this;
 }
@@ -207,7 +210,7 @@ hip_kv_cache::element_offset(std::size_t layer, std::size_t block, std::size_t t
     std::size_t offset = 0;
     const int rc = ckv_element_offset(pool_, layer, block, token_offset, kv_head, feature, &offset);
     if (rc)
-        return fail(static_cast<kv_cache_errc>(rc - 200));
+        return fail(rc < 200 ? kv_cache_errc::head_feature_out_of_range : static_cast<kv_cache_errc>(rc - 200));
     return offset;
 }
 

@@ -25,6 +25,13 @@ element_bytes(kv_dtype t) noexcept
     return t == kv_dtype::f32 ? 4 : 2;
 }
 
+// How a cache holds its numbers: as the rows' type, or in 4 bits with a power of two for
+// each 32 (ckv_pool_create_fp4; the type is then the rows'). New.
+enum class kv_storage : std::uint8_t {
+    rows,
+    fp4,
+};
+
 // Status of a libckv call with its name and the context's detail text.
 struct ckv_failure {
     int code;
@@ -177,7 +184,8 @@ struct host_kv_checkpoint : model_checkpoint {
 class hip_kv_cache {
 public:
     [[nodiscard]] static result<hip_kv_cache, kv_cache_error>
-    make(const hip_context& ctx, kv_cache_config config, kv_dtype type = kv_dtype::bf16);
+    make(const hip_context& ctx, kv_cache_config config, kv_dtype type = kv_dtype::bf16,
+         kv_storage storage = kv_storage::rows);
 
     hip_kv_cache(hip_kv_cache&& other) noexcept;
     hip_kv_cache& operator=(hip_kv_cache&& other) noexcept;
@@ -187,6 +195,7 @@ public:
 
     const kv_cache_config& config() const noexcept { return config_; }
     kv_dtype type() const noexcept { return type_; }
+    kv_storage storage() const noexcept { return storage_; }
     std::size_t layer_count() const noexcept { return config_.layer_count; }
     std::size_t block_count() const noexcept { return config_.block_count; }
     std::size_t block_size() const noexcept { return config_.block_size; }
@@ -208,9 +217,11 @@ public:
     // Bytes of one page across all layers, keys and values.
     std::size_t page_bytes_all_layers() const noexcept
     {
-        return 2 * config_.layer_count * elements_per_block() * element_bytes(type_);
+        const std::size_t elements = 2 * config_.layer_count * elements_per_block();
+        return storage_ == kv_storage::fp4 ? elements / 32 * 17 : elements * element_bytes(type_);
     }
 
+    // (of a cache held in 4 bits no element has one: head_feature_out_of_range)
     [[nodiscard]] result<std::size_t, kv_cache_error> element_offset(std::size_t layer,
                                                                      std::size_t block,
                                                                      std::size_t token_offset,
@@ -224,7 +235,8 @@ public:
     void* values() const noexcept;
 
     // Packed checkpoints with the reference's semantics (metal_kv_cache.cc:205-253):
-    // only the first `tokens` tokens are copied, the tail page partially.
+    // only the first `tokens` tokens are copied, the tail page partially. Caches held in 4
+    // bits have none (backend_failure), and no compaction (invalid_reservation).
     std::size_t checkpoint_bytes(std::size_t tokens) const noexcept;
     result<std::unique_ptr<kv_cache_checkpoint>, state_error>
     checkpoint(std::span<const block_id> blocks, std::size_t tokens) const;
@@ -250,16 +262,19 @@ public:
                                          std::span<const block_id> to);
 
 private:
-    hip_kv_cache(const hip_context* ctx, ckv_pool* pool, kv_cache_config config, kv_dtype type)
+    hip_kv_cache(const hip_context* ctx, ckv_pool* pool, kv_cache_config config, kv_dtype type,
+                 kv_storage storage)
         : ctx_(ctx)
         , pool_(pool)
         , config_(config)
         , type_(type)
+        , storage_(storage)
     {}
     const hip_context* ctx_ = nullptr;
     ckv_pool* pool_ = nullptr;
     kv_cache_config config_ {};
     kv_dtype type_ = kv_dtype::bf16;
+    kv_storage storage_ = kv_storage::rows;
 };
 
 } // namespace chibillm

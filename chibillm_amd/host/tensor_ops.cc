@@ -493,4 +493,110 @@ store_kv_rotated_axes(hip_kv_cache& cache, const device_tensor& queries, device_
     return {};
 }
 
+result<void, tensor_op_error>
+rotate(hip_kv_cache& cache, const ckv_rotation& rotation, const device_tensor& input,
+       std::size_t head_count, device_tensor& output)
+{
+    const dtype t = cache_dtype(cache);
+    CL_TRY(validate_layouts({ { input, 2, t }, { output, 2, t } }));
+    if (output.dims != input.dims)
+        return fail(tensor_op_errc::output_shape_mismatch);
+    if (head_count && input.dims[1] != head_count * cache.head_dimension())
+        return fail(tensor_op_errc::invalid_head_dimension);
+    const int rc = ckv_rotate(cache.pool(), &rotation, input.data, output.data, head_count, input.dims[0]);
+    if (rc)
+        return from_ckv(cache, rc);
+    return {};
+}
+
+namespace {
+
+// Held rows, where asked for, are of the appended rows' shape.
+result<void, tensor_op_error>
+validate_held(const hip_kv_cache& cache, const device_tensor& keys, const device_tensor* held_keys,
+              const device_tensor* held_values)
+{
+    for (const device_tensor* held : { held_keys, held_values })
+        if (held) {
+            CL_TRY(validate_layouts({ { *held, 2, cache_dtype(cache) } }));
+            if (held->dims != keys.dims)
+                return fail(tensor_op_errc::output_shape_mismatch);
+        }
+    return {};
+}
+
+} // namespace
+
+result<void, tensor_op_error>
+store_kv_rotated_by(hip_kv_cache& cache, const ckv_rotation* rotation, const device_tensor& queries,
+                    device_tensor& rotated, std::size_t q_heads, const device_tensor& keys,
+                    const device_tensor& values, std::size_t layer, device_tensor* held_keys,
+                    device_tensor* held_values)
+{
+    std::size_t rows = 0;
+    CL_TRY_ASSIGN(rows, validate_store(cache, keys, values, layer));
+    const dtype t = cache_dtype(cache);
+    CL_TRY(validate_layouts({ { queries, 2, t }, { rotated, 2, t } }));
+    if (rotated.dims != queries.dims)
+        return fail(tensor_op_errc::output_shape_mismatch);
+    if (queries.dims[0] != rows)
+        return fail(tensor_op_errc::position_count_mismatch);
+    if (queries.dims[1] != q_heads * cache.head_dimension())
+        return fail(tensor_op_errc::invalid_head_dimension);
+    CL_TRY(validate_held(cache, keys, held_keys, held_values));
+    const int rc = ckv_rotate_append(cache.pool(), layer, rotation, queries.data, rotated.data, q_heads,
+                                     keys.data, values.data, held_keys ? held_keys->data : nullptr,
+                                     held_values ? held_values->data : nullptr, rows);
+    if (rc)
+        return from_ckv(cache, rc);
+    return {};
+}
+
+result<void, tensor_op_error>
+store_kv_rotated_by_and_attend(hip_kv_cache& cache, const ckv_rotation* rotation,
+                               const device_tensor& keys, const device_tensor& values,
+                               const device_tensor& queries, std::size_t layer, std::size_t q_heads,
+                               device_tensor& output, const device_tensor* gate,
+                               device_tensor* held_keys, device_tensor* held_values)
+{
+    std::size_t rows = 0;
+    CL_TRY_ASSIGN(rows, validate_store(cache, keys, values, layer));
+    std::size_t q_rows = 0;
+    CL_TRY_ASSIGN(q_rows, validate_attention(cache, queries, layer, q_heads, output));
+    if (q_rows != rows)
+        return fail(tensor_op_errc::position_count_mismatch);
+    if (gate)
+        CL_TRY(validate_gate(cache, *gate, output));
+    CL_TRY(validate_held(cache, keys, held_keys, held_values));
+    const int rc = ckv_rotate_append_decode(cache.pool(), layer, rotation, keys.data, values.data,
+                                            queries.data, q_heads, attention_scale(cache),
+                                            gate ? gate->data : nullptr,
+                                            held_keys ? held_keys->data : nullptr,
+                                            held_values ? held_values->data : nullptr, output.data, rows);
+    if (rc)
+        return from_ckv(cache, rc);
+    return {};
+}
+
+result<void, tensor_op_error>
+prompt_attention(hip_kv_cache& cache, const device_tensor& queries, const device_tensor& keys,
+                 const device_tensor& values, std::size_t q_heads, device_tensor& output,
+                 const device_tensor* gate)
+{
+    std::size_t rows = 0;
+    CL_TRY_ASSIGN(rows, validate_store(cache, keys, values, 0));
+    std::size_t q_rows = 0;
+    CL_TRY_ASSIGN(q_rows, validate_attention(cache, queries, 0, q_heads, output));
+    if (q_rows != rows)
+        return fail(tensor_op_errc::position_count_mismatch);
+    if (gate)
+        CL_TRY(validate_gate(cache, *gate, output));
+    const int rc = ckv_prompt_attention(cache.pool(), queries.data, 0, keys.data, values.data, 0, q_heads,
+                                        attention_scale(cache), gate ? gate->data : nullptr, output.data,
+                                        rows);
+    if (rc)
+        return from_ckv(cache, rc);
+    return {};
+}
+
 } // namespace chibillm

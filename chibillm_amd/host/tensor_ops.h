@@ -236,4 +236,33 @@ result<void, tensor_op_error> store_kv_rotated(hip_kv_cache& cache, const device
                                                const device_tensor& values, std::size_t layer,
                                                float theta, std::size_t rotary_dimension = 0);
 
+// Rotations in their forms (ckv_rotation): rows rotated (ckv_rotate), a layer's queries and
+// keys with store_kv in one launch (ckv_rotate_append; held_keys and held_values, which may be
+// null, take the rows as the cache holds them), and a decode step from unrotated rows
+// (ckv_rotate_append_decode; gate may be null). rotation null: rows as they are. New.
+result<void, tensor_op_error> rotate(hip_kv_cache& cache, const ckv_rotation& rotation,
+                                     const device_tensor& input, std::size_t head_count,
+                                     device_tensor& output);
+result<void, tensor_op_error> store_kv_rotated_by(hip_kv_cache& cache, const ckv_rotation* rotation,
+                                                  const device_tensor& queries,
+                                                  device_tensor& rotated,
+                                                  std::size_t query_head_count,
+                                                  const device_tensor& keys,
+                                                  const device_tensor& values, std::size_t layer,
+                                                  device_tensor* held_keys = nullptr,
+                                                  device_tensor* held_values = nullptr);
+result<void, tensor_op_error> store_kv_rotated_by_and_attend(
+    hip_kv_cache& cache, const ckv_rotation* rotation, const device_tensor& keys,
+    const device_tensor& values, const device_tensor& queries, std::size_t layer,
+    std::size_t query_head_count, device_tensor& output, const device_tensor* gate = nullptr,
+    device_tensor* held_keys = nullptr, device_tensor* held_values = nullptr);
+
+// Attention of whole prompts, packed one after another in the uploaded batch, from their own
+// key and value rows (ckv_prompt_attention); gate may be null. New.
+result<void, tensor_op_error> prompt_attention(hip_kv_cache& cache, const device_tensor& queries,
+                                               const device_tensor& keys,
+                                               const device_tensor& values,
+                                               std::size_t query_head_count, device_tensor& output,
+                                               const device_tensor* gate = nullptr);
+
 } // namespace chibillm
