@@ -922,7 +922,7 @@ prompt_form prompt_form_of(const pool_view& p, const meta_view& m, const prompt_
     set_vectors(p, x, out, gate, fp4);
     prompt_form form { n_waves, heads_of(p, q_heads), false, fp4 };
     form.paged_kernel = !fp4 && p.head_dim == 128 && p.dtype != CKV_F32 && x.vectors && x.out_vectors
-        && scale > 0.0f && x.kv_stride <= UINT32_MAX;
+        && scale > 0.0f && x.kv_stride <= 1u << 26; // (its offsets within 16 rows are 32 bits)
     if (!form.paged_kernel)
         return form;
     const uint32_t eight = form.heads == 4 ? m.row_blocks[1] : form.heads == 2 ? m.row_blocks[2] : m.n_tiles;
