@@ -15,8 +15,15 @@
 //
 // Staging goes through registers, a block ahead: 4-bit codes become the rows' type on the
 // way, exactly, once for the four waves; rows of any stride and alignment are taken as they
-// are. Three LDS stages, one barrier a block. Float rows have a kernel of their own below,
-// on v_mfma_f32_32x32x2 (exact products, as the paged f32 prefill).
+// are. Three LDS stages, one barrier a block.
+//
+// Float rows enter as three bf16 terms, each the rounding of what those before it left: 24
+// bits. Of queries and probabilities always, of keys and values where they are rows (4-bit
+// numbers are bf16's): 6 or 3 products of terms in place of one of floats, which takes 16
+// times as long as one of these. On v_mfma_f32_32x32x2 (exact products) 200 rows behind
+// 1,500 tokens of 4 bits took 52 us and take 26, 4 x 512 behind 3,000 457 and 150, two
+// prompts of 3,000 rows 642 and 432, five of up to 700 of 64-wide heads 21.6 and 15.7; errors
+// against 64 bits are the same. Rows of 256-wide heads have a kernel of their own below.
 //
 // Keys past the tile's last position are staged as zeros. A masked key's probability is 0,
 // which meets its value in P.V all the same: where that is infinite or NaN, the rows that
@@ -267,30 +274,61 @@ __device__ __forceinline__ bool fold_ranges(const prefill_split& split, const ti
     return true;
 }
 
-// What a thread holds of a block on its way to LDS: 16-bit rows, or 4-bit codes.
-template <int D, bool FP4>
-struct staged;
-template <int D>
-struct staged<D, false> {
-    static constexpr uint32_t per = D / 64; // 16-byte words of K, and of V: 32 rows of D/8
-    uint4 k[per], v[per];
+// Eight floats as `N` words of packed bf16 terms each: the rounding of what those before it left.
+template <int N>
+__device__ __forceinline__ void terms_of(float a, float b, uint32_t (&w)[N])
+{
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+        w[t] = pack2<false>(a, b);
+        a -= __builtin_bit_cast(float, w[t] << 16);
+        b -= __builtin_bit_cast(float, w[t] & 0xFFFF0000u);
+    }
+}
+template <int N>
+__device__ __forceinline__ void terms_of(const float (&x)[8], uint4 (&out)[N])
+{
+    uint32_t w[4][N];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        terms_of<N>(x[2 * i], x[2 * i + 1], w[i]);
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+        out[t] = make_uint4(w[0][t], w[1][t], w[2][t], w[3][t]);
+}
+
+// What a thread holds of a block on its way to LDS: rows, eight elements at a time, or 4-bit
+// codes.
+template <bool F32>
+struct eight_of { // (native vectors: arrays of uint4 are not kept in registers)
+    u32x4_t w[F32 ? 2 : 1];
 };
-template <int D>
-struct staged<D, true> {
+template <int D, bool FP4, bool F32>
+struct staged {
+    static constexpr uint32_t per = D / 64; // of K, and of V: 32 rows of D/8
+    eight_of<F32> k[per], v[per];
+};
+template <int D, bool F32>
+struct staged<D, true, F32> {
     // 4-byte words of K or of V: threads below half take K, the others V
     static constexpr uint32_t words = D / 32;
     uint32_t code[words];
     uint32_t scale[D == 256 ? 2 : 1];
 };
 
-// 16-bit rows. GH heads of a GQA group share a workgroup: 128 / GH rows.
-template <int D, int GH, bool F16, source SRC>
-__global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
-    pool_view p, meta_view md, uint32_t layer, prompt_rows x, uint16_t* __restrict__ out, uint32_t q_heads,
-    float c, uint32_t q_and, uint32_t q_xor, const uint16_t* __restrict__ gate, prefill_split split)
+// GH heads of a GQA group share a workgroup: 128 / GH rows.
+template <int D, int GH, int DT, source SRC>
+__global__ __launch_bounds__(n_threads, D == 256 || (D == 128 && DT == CKV_F32) ? 1 : 2) void prompt_kernel(
+    pool_view p, meta_view md, uint32_t layer, prompt_rows x, void* __restrict__ out_rows, uint32_t q_heads,
+    float c, uint32_t q_and, uint32_t q_xor, const void* __restrict__ gate_rows, prefill_split split)
 {
-    constexpr bool FP4 = SRC == FROM_FP4;
-    constexpr int KS = D / 16, MT = D / 32, DT = F16 ? CKV_F16 : CKV_BF16;
+    constexpr bool FP4 = SRC == FROM_FP4, F32 = DT == CKV_F32, F16 = DT == CKV_F16;
+    using T = std::conditional_t<F32, float, uint16_t>;
+    T* const out = static_cast<T*>(out_rows);
+    const T* const gate = static_cast<const T*>(gate_rows);
+    constexpr int KS = D / 16, MT = D / 32;
+    // terms of queries and probabilities, and of keys and values (4-bit numbers are bf16's)
+    constexpr int TQ = F32 ? 3 : 1, TK = F32 && !FP4 ? 3 : 1;
     constexpr uint32_t n_stages = 3;
     // K stage: chunk i (features 8i .. 8i + 7) holds the block's keys in the LDS rows of the
     // A operand, 16 bytes each; 16 more bytes a chunk spread a key's chunks over the banks.
@@ -298,7 +336,7 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
     // V stage: rows as they are, read transposed; key k is row (k / 4) % 4 of group
     // k % 4 + 4 * (k / 16), 64 bytes between groups (kernels_prefill.hip).
     constexpr uint32_t v_row = 2 * D, v_group = 4 * v_row + 64, v_bytes = 8 * v_group;
-    constexpr uint32_t stage_bytes = k_bytes + v_bytes;
+    constexpr uint32_t plane = k_bytes + v_bytes, stage_bytes = TK * plane; // a plane for each term
     constexpr uint32_t out_bytes = n_waves * 32 * row_floats<D> * 4;
     constexpr uint32_t lds_bytes = n_stages * stage_bytes > out_bytes ? n_stages * stage_bytes : out_bytes;
     __shared__ __attribute__((aligned(16))) uint8_t lds[lds_bytes];
@@ -320,28 +358,61 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
               (uint32_t)__builtin_ctz(p.block_size / fp4_tile), p.kv_heads, w.kvh };
     } else {
         const uint64_t first = (uint64_t)(w.row0 - w.pos0) * x.kv_stride + w.kvh * D;
-        s = { static_cast<const uint8_t*>(x.keys) + 2 * first, static_cast<const uint8_t*>(x.values) + 2 * first,
-              nullptr, 2 * x.kv_stride, 0, 0, 0 };
+        s = { static_cast<const uint8_t*>(x.keys) + sizeof(T) * first, static_cast<const uint8_t*>(x.values) + sizeof(T) * first,
+              nullptr, sizeof(T) * x.kv_stride, 0, 0, 0 };
     }
-    const uint16_t* q_row = static_cast<const uint16_t*>(x.queries)
+    // eight elements, from any alignment of them
+    using eight = eight_of<F32>;
+    auto gather = [](const void* from) {
+        const T* e = static_cast<const T*>(from);
+        eight x;
+        if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x.w[i / 4][i % 4] = __float_as_uint(e[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x.w[0][i] = e[2 * i] | (uint32_t)e[2 * i + 1] << 16;
+        }
+        return x;
+    };
+    auto read = [](const void* from) {
+        eight x;
+        x.w[0] = static_cast<const u32x4_t*>(from)[0];
+        if constexpr (F32)
+            x.w[1] = static_cast<const u32x4_t*>(from)[1];
+        return x;
+    };
+    // and as an operand's words, a term each
+    auto operands = [](const eight& x, auto& to) {
+        if constexpr (F32) {
+            const u32x4_t a = x.w[0], b = x.w[1];
+            const float f[8] = { __uint_as_float(a[0]), __uint_as_float(a[1]), __uint_as_float(a[2]), __uint_as_float(a[3]),
+                                 __uint_as_float(b[0]), __uint_as_float(b[1]), __uint_as_float(b[2]), __uint_as_float(b[3]) };
+            terms_of<3>(f, to);
+        } else {
+            to[0] = __builtin_bit_cast(uint4, x.w[0]);
+        }
+    };
+    const T* q_row = static_cast<const T*>(x.queries)
         + (uint64_t)(w.row0 + min(row, w.nrows - 1)) * x.q_stride + (uint64_t)head * D;
-    uint4 qr[KS];
+    uint4 qr[KS][TQ];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        uint4 v = make_uint4(0, 0, 0, 0);
+        eight v {};
         if (valid) {
-            const uint16_t* at = q_row + ks * 16 + g * 8;
-            if (x.vectors)
-                v = *reinterpret_cast<const uint4*>(at);
-            else
-                v = make_uint4(at[0] | (uint32_t)at[1] << 16, at[2] | (uint32_t)at[3] << 16,
-                               at[4] | (uint32_t)at[5] << 16, at[6] | (uint32_t)at[7] << 16);
+            const T* at = q_row + ks * 16 + g * 8;
+            v = x.vectors ? read(at) : gather(at);
         }
         // a negative scale turns the queries' sign, a scale of 0 leaves nothing of them
-        qr[ks] = make_uint4((v.x & q_and) ^ q_xor, (v.y & q_and) ^ q_xor, (v.z & q_and) ^ q_xor, (v.w & q_and) ^ q_xor);
+#pragma unroll
+        for (int i = 0; i < (F32 ? 2 : 1); ++i)
+            v.w[i] = (v.w[i] & q_and) ^ q_xor;
+        operands(v, qr[ks]);
     }
 
-    using held = staged<D, FP4>;
+    using held = staged<D, FP4, F32>;
     // Blocks on their way: 4-bit ones three ahead of the one that is stored (a block takes less
     // than a load from HBM), rows one.
     constexpr uint32_t ahead = FP4 ? 3 : 1;
@@ -355,7 +426,7 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
                   : lane / 4 * (D / 32) + (D == 64 ? lane % 4 / 2 : lane % 4));
     const uint32_t scale_part = v_wave ? 64 : 4, k_shift = scale_at % 4 * 8;
     // block kb's words of this thread into registers
-    auto load = [&](uint32_t kb, held& next) {
+    auto load = [&](uint32_t kb, held& next) __attribute__((always_inline)) {
         const uint32_t key0 = kb * block_keys;
         if constexpr (FP4) {
             // waves 0 and 1 take K of the block's two tiles, 2 and 3 V. Of K, lane 4t + i takes
@@ -384,16 +455,11 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
 #pragma unroll
             for (uint32_t i = 0; i < held::per; ++i) {
                 const uint32_t word = i * n_threads + tid, key = key0 + word / (D / 8), f = word % (D / 8) * 8;
-                const uint64_t at = min(key, w.pos_last) * s.stride + 2 * f;
+                const uint64_t at = min(key, w.pos_last) * s.stride + sizeof(T) * f;
                 if constexpr (SRC == FROM_WORDS) {
-                    next.k[i] = *reinterpret_cast<const uint4*>(s.keys + at);
-                    next.v[i] = *reinterpret_cast<const uint4*>(s.values + at);
+                    next.k[i] = read(s.keys + at);
+                    next.v[i] = read(s.values + at);
                 } else {
-                    const auto gather = [](const uint8_t* from) {
-                        const auto* e = reinterpret_cast<const uint16_t*>(from);
-                        return make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
-                                          e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
-                    };
                     next.k[i] = gather(s.keys + at);
                     next.v[i] = gather(s.values + at);
                 }
@@ -407,7 +473,7 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
         return st + k_bytes + (key % 4 + 4 * (key / 16)) * v_group + key / 4 % 4 * v_row;
     };
     // and from there into its stage, zeros past the tile's last position
-    auto store_keys = [&](uint32_t kb, const held& next, uint8_t* st, auto all) {
+    auto store_keys = [&](uint32_t kb, const held& next, uint8_t* st, auto all) __attribute__((always_inline)) {
         constexpr bool ALL = decltype(all)::value;
         const uint32_t key0 = kb * block_keys;
         if constexpr (FP4) {
@@ -445,15 +511,21 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
 #pragma unroll
             for (uint32_t i = 0; i < held::per; ++i) {
                 const uint32_t word = i * n_threads + tid, key = word / (D / 8), chunk = word % (D / 8);
-                uint4 k = next.k[i], v = next.v[i];
-                if (!ALL && key0 + key > w.pos_last)
-                    k = v = make_uint4(0, 0, 0, 0);
-                put_k(st, key, chunk, k);
-                *reinterpret_cast<uint4*>(v_at(st, key) + chunk * 16) = v;
+                uint4 k[TK], v[TK];
+                operands(next.k[i], k);
+                operands(next.v[i], v);
+                const bool there = ALL || key0 + key <= w.pos_last;
+#pragma unroll
+                for (int t = 0; t < TK; ++t) {
+                    if (!there)
+                        k[t] = v[t] = make_uint4(0, 0, 0, 0);
+                    put_k(st + t * plane, key, chunk, k[t]);
+                    *reinterpret_cast<uint4*>(v_at(st + t * plane, key) + chunk * 16) = v[t];
+                }
             }
         }
     };
-    auto store = [&](uint32_t kb, const held& next, uint8_t* st) {
+    auto store = [&](uint32_t kb, const held& next, uint8_t* st) __attribute__((always_inline)) {
         if (kb * block_keys + block_keys - 1 <= w.pos_last)
             store_keys(kb, next, st, std::true_type {});
         else
@@ -467,19 +539,35 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
     float m = -__builtin_inff(), l = 0.0f, m_limit = -__builtin_inff(), mx = 0.0f;
     const float rescale_raw = rescale_log2 / c;
     f32x16_t sc, sp;
-    auto read_k = [&](const uint8_t* st, uint4 (&ka)[KS]) {
+    auto read_k = [&](const uint8_t* st, uint4 (&ka)[KS]) __attribute__((always_inline)) {
         const uint8_t* kl = st + g * k_chunk + n * 16;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
             ka[ks] = *reinterpret_cast<const uint4*>(kl + ks * 2 * k_chunk);
     };
-    auto scores = [&](const uint4 (&ka)[KS]) {
+    // products of terms i and j of their operands with i + j < TQ: what is left out is under
+    // 2^-24 of the whole
+    auto scores = [&](const uint8_t* st, const uint4 (&first)[KS]) __attribute__((always_inline)) {
         sc = f32x16_t {};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-            sc = mfma<F16>(ka[ks], qr[ks], sc);
+        for (int t = 0; t < TK; ++t) {
+            uint4 ka[KS];
+            if (t) {
+                __builtin_amdgcn_sched_barrier(0); // one plane's registers at a time
+                read_k(st + t * plane, ka);
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+                    ka[ks] = first[ks];
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int j = 0; j < TQ - t; ++j)
+                    sc = mfma<F16>(ka[ks], qr[ks][j], sc);
+        }
     };
-    auto probabilities = [&](uint4 (&pt)[2]) {
+    auto probabilities = [&](uint4 (&pt)[2][TQ]) __attribute__((always_inline)) {
         // a range of the keys may hold none that a row attends: its maximum stays -inf
         const float mc = m == -__builtin_inff() ? 0.0f : m * c;
         float sum[4];
@@ -491,28 +579,42 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
             sum[i] = (sp[4 * i] + sp[4 * i + 1]) + (sp[4 * i + 2] + sp[4 * i + 3]);
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            pt[h] = make_uint4(pack2<F16>(sp[8 * h], sp[8 * h + 1]), pack2<F16>(sp[8 * h + 2], sp[8 * h + 3]),
-                               pack2<F16>(sp[8 * h + 4], sp[8 * h + 5]), pack2<F16>(sp[8 * h + 6], sp[8 * h + 7]));
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (F32) {
+                const float f[8] = { sp[8 * h], sp[8 * h + 1], sp[8 * h + 2], sp[8 * h + 3],
+                                     sp[8 * h + 4], sp[8 * h + 5], sp[8 * h + 6], sp[8 * h + 7] };
+                terms_of<TQ>(f, pt[h]);
+            } else {
+                pt[h][0] = make_uint4(pack2<F16>(sp[8 * h], sp[8 * h + 1]), pack2<F16>(sp[8 * h + 2], sp[8 * h + 3]),
+                                      pack2<F16>(sp[8 * h + 4], sp[8 * h + 5]), pack2<F16>(sp[8 * h + 6], sp[8 * h + 7]));
+            }
+        }
     };
     const uint32_t vr_off = ((lane & 15) >> 2) * v_group + (lane >> 5) * 2 * v_row + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
-    auto values = [&](const uint8_t* st, const uint4 (&pt)[2]) {
+    auto values = [&](const uint8_t* st, const uint4 (&pt)[2][TQ]) __attribute__((always_inline)) {
         uint32_t vaddr = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) uint8_t*)(const_cast<uint8_t*>(st) + k_bytes)) + vr_off;
         asm volatile("" : "+v"(vaddr));
         auto* vb = (__attribute__((address_space(3))) uint8_t*)(uintptr_t)vaddr;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int t = 0; t < TK; ++t) {
+            if (t)
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) i16x4_t*)(vb + 4 * h * v_group + 64 * mt));
-                const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) i16x4_t*)(vb + 4 * h * v_group + v_row + 64 * mt));
-                const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-                o[mt] = mfma<F16>(make_uint4(l2.x, l2.y, h2.x, h2.y), pt[h], o[mt]);
-            }
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    auto* at = vb + t * plane + 4 * h * v_group + 64 * mt;
+                    const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)at);
+                    const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) i16x4_t*)(at + v_row));
+                    const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+#pragma unroll
+                    for (int j = 0; j < TQ - t; ++j)
+                        o[mt] = mfma<F16>(make_uint4(l2.x, l2.y, h2.x, h2.y), pt[h][j], o[mt]);
+                }
+        }
     };
-    auto stats = [&](uint32_t kb) {
+    auto stats = [&](uint32_t kb) __attribute__((always_inline)) {
         const uint32_t key0 = kb * block_keys;
         if (key0 + block_keys - 1 > pos_lo) { // the diagonal crosses this block
 #pragma unroll
@@ -546,10 +648,10 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
     if (w.kb_begin + ahead < w.kb_end)
         load(w.kb_begin + ahead, flight[0]);
     __syncthreads();
-    auto iteration = [&](uint32_t kb, auto turn, auto is_first) {
+    auto iteration = [&](uint32_t kb, auto turn, auto is_first) __attribute__((always_inline)) {
         constexpr uint32_t S = decltype(turn)::value;
         constexpr bool FIRST = decltype(is_first)::value;
-        uint4 ka[KS], pt[2];
+        uint4 ka[KS], pt[2][TQ];
         read_k(lds + S * stage_bytes, ka);
         held& next = flight[(S + 1) % ahead];
         if (kb + 1 < w.kb_end)
@@ -559,7 +661,7 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (!FIRST)
             probabilities(pt);
-        scores(ka);
+        scores(lds + S * stage_bytes, ka);
         if constexpr (!FIRST)
             values(lds + (S + 2) % n_stages * stage_bytes, pt);
         stats(kb);
@@ -581,7 +683,7 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
         last = 0;
     }
     {
-        uint4 pt[2];
+        uint4 pt[2][TQ];
         probabilities(pt);
         values(lds + last * stage_bytes, pt);
     }
@@ -620,9 +722,14 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
             for (uint32_t f = lane; f < D; f += 64)
                 if (!(alone >> r & 1)) {
                     float y = tile_out[r * row_floats<D> + f];
-                    if (gate)
-                        y *= sigmoid(half_value<F16>(gate[first + r * o_stride + f]));
-                    out[first + r * o_stride + f] = (uint16_t)pack2<F16>(y, 0.0f);
+                    const size_t at = first + r * o_stride + f;
+                    if constexpr (F32) {
+                        out[at] = gate ? y * sigmoid(gate[at]) : y;
+                    } else {
+                        if (gate)
+                            y *= sigmoid(half_value<F16>(gate[at]));
+                        out[at] = (uint16_t)pack2<F16>(y, 0.0f);
+                    }
                 }
     }
     const float cs = q_and ? (q_xor ? -c : c) : 0.0f; // the scale in log2 units
@@ -630,22 +737,22 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_kernel(
         const uint32_t r = __builtin_ctz(alone);
         alone &= alone - 1;
         const size_t at = first + r * o_stride;
-        attend_row<D, DT, FP4>(s, pos_lo + r, static_cast<const uint16_t*>(x.queries) + (uint64_t)(w.row0 + rb * 32 + r) * x.q_stride + (uint64_t)head * D,
+        attend_row<D, DT, FP4>(s, pos_lo + r, static_cast<const T*>(x.queries) + (uint64_t)(w.row0 + rb * 32 + r) * x.q_stride + (uint64_t)head * D,
                                cs, gate ? gate + at : nullptr, out + at, lane);
     }
 }
 
-// Float rows: S^T and O^T on v_mfma_f32_32x32x2, D/2 and D/2 products a block. The
+// Float rows of 256-wide heads, whose terms' planes LDS has no room for: S^T and O^T on
+// v_mfma_f32_32x32x2, 128 and 128 products a block, which are 85 % of its time (8.2 us). The
 // contraction over features pairs 8i + e with 8i + 4 + e, so that a lane's operands are
 // 16-byte words; that over keys pairs the two keys of an accumulator element, so that a
 // probability is an operand where it was computed. Two LDS stages of whole rows.
-template <int D, int GH, source SRC>
-__global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel(
+template <int GH, source SRC>
+__global__ __launch_bounds__(n_threads, 1) void prompt_f32_kernel(
     pool_view p, meta_view md, uint32_t layer, prompt_rows x, float* __restrict__ out, uint32_t q_heads,
     float c, float q_sign, const float* __restrict__ gate, prefill_split split)
 {
-    constexpr bool FP4 = SRC == FROM_FP4;
-    constexpr int MT = D / 32, K4 = D / 8;
+    constexpr int D = 256, MT = D / 32, K4 = D / 8;
     constexpr uint32_t pitch = D + 4, stage_floats = 2 * block_keys * pitch;
     __shared__ __attribute__((aligned(16))) float lds[2 * stage_floats];
     static_assert(n_waves * 32 * row_floats<D> <= 2 * stage_floats);
@@ -658,17 +765,9 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel
     const bool valid = row < w.nrows;
     const uint32_t qpos = w.pos0 + min(row, w.nrows - 1);
     const uint32_t pos_lo = w.pos0 + rb * 32;
-    key_source s;
-    if constexpr (FP4) {
-        const uint64_t layer_bytes = (uint64_t)p.blocks * p.block_size / fp4_tile * p.kv_heads * fp4_tile_bytes(D);
-        s = { static_cast<const uint8_t*>(p.keys) + layer * layer_bytes,
-              static_cast<const uint8_t*>(p.values) + layer * layer_bytes, md.table + w.table, 0,
-              (uint32_t)__builtin_ctz(p.block_size / fp4_tile), p.kv_heads, w.kvh };
-    } else {
-        const uint64_t first = (uint64_t)(w.row0 - w.pos0) * x.kv_stride + w.kvh * D;
-        s = { static_cast<const uint8_t*>(x.keys) + 4 * first, static_cast<const uint8_t*>(x.values) + 4 * first,
-              nullptr, 4 * x.kv_stride, 0, 0, 0 };
-    }
+    const uint64_t row_first = (uint64_t)(w.row0 - w.pos0) * x.kv_stride + w.kvh * D;
+    const key_source s { static_cast<const uint8_t*>(x.keys) + 4 * row_first,
+                         static_cast<const uint8_t*>(x.values) + 4 * row_first, nullptr, 4 * x.kv_stride, 0, 0, 0 };
     const float* q_row = static_cast<const float*>(x.queries)
         + (uint64_t)(w.row0 + min(row, w.nrows - 1)) * x.q_stride + (uint64_t)head * D;
     float4 qr[K4];
@@ -682,63 +781,34 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel
         qr[i] = q_sign == 0.0f ? make_float4(0, 0, 0, 0)
                                : make_float4(v.x * q_sign, v.y * q_sign, v.z * q_sign, v.w * q_sign);
     }
-    constexpr uint32_t per = FP4 ? D / 64 : D / 32; // 8-feature words, or 16-byte words
-    uint32_t code_k[FP4 ? per : 1], code_v[FP4 ? per : 1], scale_k[FP4 ? per : 1], scale_v[FP4 ? per : 1];
-    float4 next_k[FP4 ? 1 : per], next_v[FP4 ? 1 : per];
+    constexpr uint32_t per = D / 32; // 16-byte words
+    float4 next_k[per], next_v[per];
     auto load = [&](uint32_t kb) {
-        const uint32_t key0 = kb * block_keys;
 #pragma unroll
         for (uint32_t i = 0; i < per; ++i) {
             const uint32_t word = i * n_threads + tid;
-            if constexpr (FP4) {
-                const uint32_t key = min(key0 + word / (D / 8), w.pos_last), f8 = word % (D / 8), t = key % fp4_tile;
-                const uint64_t at = tile_offset<D>(s, key / fp4_tile);
-                code_k[i] = *reinterpret_cast<const uint32_t*>(s.keys + at + fp4_word_at(D, t, f8, false));
-                const uint8_t* v = s.values + at + fp4_word_at(D, t, f8, true);
-                if constexpr (D == 64)
-                    code_v[i] = *reinterpret_cast<const uint16_t*>(v) | (uint32_t)*reinterpret_cast<const uint16_t*>(v + 8) << 16;
-                else
-                    code_v[i] = *reinterpret_cast<const uint32_t*>(v);
-                scale_k[i] = s.keys[at + fp4_scale_at(D, t, f8 / 4, false)];
-                scale_v[i] = s.values[at + fp4_scale_at(D, t, f8 / 4, true)];
+            const uint32_t key = min(kb * block_keys + word / (D / 4), w.pos_last), f = word % (D / 4) * 4;
+            const float* k = reinterpret_cast<const float*>(s.keys + key * s.stride) + f;
+            const float* v = reinterpret_cast<const float*>(s.values + key * s.stride) + f;
+            if constexpr (SRC == FROM_WORDS) {
+                next_k[i] = *reinterpret_cast<const float4*>(k);
+                next_v[i] = *reinterpret_cast<const float4*>(v);
             } else {
-                const uint32_t key = min(key0 + word / (D / 4), w.pos_last), f = word % (D / 4) * 4;
-                const float* k = reinterpret_cast<const float*>(s.keys + key * s.stride) + f;
-                const float* v = reinterpret_cast<const float*>(s.values + key * s.stride) + f;
-                if constexpr (SRC == FROM_WORDS) {
-                    next_k[i] = *reinterpret_cast<const float4*>(k);
-                    next_v[i] = *reinterpret_cast<const float4*>(v);
-                } else {
-                    next_k[i] = make_float4(k[0], k[1], k[2], k[3]);
-                    next_v[i] = make_float4(v[0], v[1], v[2], v[3]);
-                }
+                next_k[i] = make_float4(k[0], k[1], k[2], k[3]);
+                next_v[i] = make_float4(v[0], v[1], v[2], v[3]);
             }
         }
     };
     auto store = [&](uint32_t kb) {
         float* st = lds + kb % 2 * stage_floats;
-        const uint32_t key0 = kb * block_keys;
 #pragma unroll
         for (uint32_t i = 0; i < per; ++i) {
-            const uint32_t word = i * n_threads + tid;
-            if constexpr (FP4) {
-                const uint32_t key = word / (D / 8), f = word % (D / 8) * 8;
-                const bool there = key0 + key <= w.pos_last;
-                auto put = [&](float* to, uint32_t code, uint32_t byte) {
-                    const uint4 v = fp4_eight<false>(there ? code : 0, there ? fp4_scale(byte) : 1.0f);
-                    reinterpret_cast<float4*>(to)[0] = make_float4(word_half(v.x, 0, false), word_half(v.x, 1, false), word_half(v.y, 0, false), word_half(v.y, 1, false));
-                    reinterpret_cast<float4*>(to)[1] = make_float4(word_half(v.z, 0, false), word_half(v.z, 1, false), word_half(v.w, 0, false), word_half(v.w, 1, false));
-                };
-                put(st + key * pitch + f, code_k[i], scale_k[i]);
-                put(st + (block_keys + key) * pitch + f, code_v[i], scale_v[i]);
-            } else {
-                const uint32_t key = word / (D / 4), f = word % (D / 4) * 4;
-                float4 k = next_k[i], v = next_v[i];
-                if (key0 + key > w.pos_last)
-                    k = v = make_float4(0, 0, 0, 0);
-                *reinterpret_cast<float4*>(st + key * pitch + f) = k;
-                *reinterpret_cast<float4*>(st + (block_keys + key) * pitch + f) = v;
-            }
+            const uint32_t word = i * n_threads + tid, key = word / (D / 4), f = word % (D / 4) * 4;
+            float4 k = next_k[i], v = next_v[i];
+            if (kb * block_keys + key > w.pos_last)
+                k = v = make_float4(0, 0, 0, 0);
+            *reinterpret_cast<float4*>(st + key * pitch + f) = k;
+            *reinterpret_cast<float4*>(st + (block_keys + key) * pitch + f) = v;
         }
     };
 
@@ -844,7 +914,7 @@ __global__ __launch_bounds__(n_threads, D == 256 ? 1 : 2) void prompt_f32_kernel
         const uint32_t r = __builtin_ctz(alone);
         alone &= alone - 1;
         const size_t at = first + r * o_stride;
-        attend_row<D, CKV_F32, FP4>(s, pos_lo + r, static_cast<const float*>(x.queries) + (uint64_t)(w.row0 + rb * 32 + r) * x.q_stride + (uint64_t)head * D,
+        attend_row<D, CKV_F32, false>(s, pos_lo + r, static_cast<const float*>(x.queries) + (uint64_t)(w.row0 + rb * 32 + r) * x.q_stride + (uint64_t)head * D,
                                     c * q_sign, gate ? gate + at : nullptr, out + at, lane);
     }
 }
@@ -865,16 +935,20 @@ hipError_t launch_gh(hipStream_t s, const pool_view& p, const meta_view& m, uint
         return hipErrorInvalidValue;
     const float c = scale == 0.0f ? log2e : __builtin_fabsf(scale) * log2e;
     const dim3 blocks((uint32_t)grid), threads(n_threads);
-    if (p.dtype == CKV_F32) {
-        prompt_f32_kernel<D, GH, SRC><<<blocks, threads, 0, s>>>(
-            p, m, layer, x, static_cast<float*>(out), q_heads, c, scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f,
-            static_cast<const float*>(gate), split);
-        return hipGetLastError();
-    }
-    auto* kernel = p.dtype == CKV_F16 ? prompt_kernel<D, GH, true, SRC> : prompt_kernel<D, GH, false, SRC>;
-    kernel<<<blocks, threads, 0, s>>>(p, m, layer, x, static_cast<uint16_t*>(out), q_heads, c,
-                                      scale == 0.0f ? 0u : ~0u, scale < 0.0f ? 0x80008000u : 0u,
-                                      static_cast<const uint16_t*>(gate), split);
+    if constexpr (D == 256 && SRC != FROM_FP4)
+        if (p.dtype == CKV_F32) {
+            prompt_f32_kernel<GH, SRC><<<blocks, threads, 0, s>>>(
+                p, m, layer, x, static_cast<float*>(out), q_heads, c, scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f,
+                static_cast<const float*>(gate), split);
+            return hipGetLastError();
+        }
+    auto* kernel = p.dtype == CKV_F16 ? prompt_kernel<D, GH, CKV_F16, SRC> : prompt_kernel<D, GH, CKV_BF16, SRC>;
+    if constexpr (D != 256 || SRC == FROM_FP4)
+        if (p.dtype == CKV_F32)
+            kernel = prompt_kernel<D, GH, CKV_F32, SRC>;
+    const uint32_t turned = p.dtype == CKV_F32 ? 0x80000000u : 0x80008000u;
+    kernel<<<blocks, threads, 0, s>>>(p, m, layer, x, out, q_heads, c, scale == 0.0f ? 0u : ~0u,
+                                      scale < 0.0f ? turned : 0u, gate, split);
     return hipGetLastError();
 }
 
@@ -937,11 +1011,11 @@ namespace {
 
 // What a launch's time is estimated from, us: a key block of a workgroup alone on its compute
 // unit (two there: `shared` of that more for each), what comes before and after the blocks,
-// in blocks, and of a tile that is cut the handoff and each record. Fitted to times of 14
+// in blocks, and of a tile that is cut the handoff and each record. Fitted to times of 20
 // batches in 1 to 16 ranges; the ranges it chooses are the fastest measured or within 8 % of
 // that. Uncut and as chosen, us: 512 rows behind 6000 tokens of 4 bits 164 and 46, 4 x 256
-// behind 2000 60 and 34, 900 rows of one prompt 21 and 17, five short float prompts 58 and
-// 21; 8 x 1024 behind 3000 stays uncut (242, in two ranges 271).
+// behind 2000 60 and 34, 900 rows of one prompt 21 and 17, five short float prompts 35 and
+// 16; 8 x 1024 behind 3000 stays uncut (242, in two ranges 271).
 struct prompt_cost {
     double block, shared, ends, handoff, record;
     uint32_t per_cu;
@@ -949,9 +1023,14 @@ struct prompt_cost {
 
 prompt_cost cost_of(const pool_view& p, const prompt_form& form)
 {
-    const double wide = p.head_dim / 128.0;
+    if (p.dtype == CKV_F32 && form.fp4)
+        return p.head_dim == 64 ? prompt_cost { 0.62, 0.07, 4.8, 3.8, 2.3, 2 }
+            : p.head_dim == 128 ? prompt_cost { 1.3, 0.0, 2.2, 3.1, 0.8, 1 }
+                                : prompt_cost { 2.9, 0.0, 5.5, 7.6, 2.3, 1 };
     if (p.dtype == CKV_F32)
-        return { 4.1 * wide, 0.71, 2.6, 5.9, 0.07 * wide, p.head_dim == 256 ? 1u : 2u };
+        return p.head_dim == 64 ? prompt_cost { 1.6, 0.72, 0.1, 4.5, 0.4, 2 }
+            : p.head_dim == 128 ? prompt_cost { 1.9, 0.0, 5.8, 0.3, 2.4, 1 }
+                                : prompt_cost { 8.2, 0.0, 2.6, 5.9, 0.14, 1 };
     if (p.head_dim == 256)
         return { 1.2, 0.62, 7.8, 6.6, 1.8, 1 };
     if (p.head_dim == 64)

@@ -582,7 +582,7 @@ int ckv_rotate_append_decode(ckv_pool* pool, size_t layer, const ckv_rotation* r
  * keys and values are in hand as rows and need not be read back from the cache (which may
  * hold them in 4 bits). Row r attends the rows of its sequence from position 0 to its own:
  * output = softmax(q . k * scale) . v with fp32 accumulation; probabilities enter the
- * matrix cores in the rows' type. The batch's tables tell the sequences: every row's
+ * matrix cores in the rows' type (f32 rows: everything does with 24 bits, as bf16 terms). The batch's tables tell the sequences: every row's
  * position is 0 or follows the row before it, in the same table range (invalid_argument
  * otherwise). The pool gives the geometry (head_dim 64, 128 or 256: otherwise
  * invalid_head_dimension) and type; its cache is neither read nor written, and any number

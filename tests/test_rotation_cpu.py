@@ -50,6 +50,9 @@ def test_the_reference_holds_what_the_levels_say(dtype):
     got = ref.held(torch.from_numpy(rows), dtype).numpy()
     for x, h in zip(rows, got):
         m = np.abs(x).max()
+        if dtype == "f16" and m >= 2.0 ** 16:  # past the type: the block is lost
+            assert np.isnan(h).all()
+            continue
         scale = 2.0 ** max(np.floor(np.log2(m)) - 2 if m else -1000, ref.LEAST[dtype])
         for a, b in zip(np.abs(x) / scale, np.abs(h) / scale):
             assert b in levels
