@@ -514,6 +514,13 @@ __global__ __launch_bounds__(64 * fp4_waves_of(D), D == 256 ? 3 : 4) void fp4_de
 
 } // namespace
 
+// Two workgroups a compute unit, chunks of 16 pages (one step of eight waves) at least, at
+// most 32 of a row; a row up to 47 pages past its share stays whole: a segment costs a
+// workgroup 3.5 us beside its pages, as much as 60 of them. As planned, in chunks of 16, 32
+// and 64 pages, and whole, us: 48 rows of 900 to 12,000 tokens 69.5, 148, 102, 81 and 84; 128
+// of 3,000 to 8,000 138, 327, 226, 179 and 137; 24 of 200 to 9,000 of 256-wide heads 23.2,
+// 26.0, 21.9, 22.2 and 113; 4 of 60 to 1,900 8.7, 8.6, 9.0, 11.3 and 12.8; one of 16,000 12.8,
+// 15.7, 12.5, 12.7 and 73; 8 of 4,000 13.1, 19.8, 14.0, 12.4 and 23.8.
 decode_form fp4_decode_form()
 {
     return { 2, 16, 32, 47, false };
