@@ -111,6 +111,9 @@ template <int D, int DT, bool FP4, class T>
 __device__ __forceinline__ void attend_row(const key_source& s, uint32_t position, const T* q, float c,
                                            const T* gate, T* out, uint32_t lane)
 {
+// (a score's product joined with the subtraction of its own rounding weighs more than 1, and
+// takes the largest floats to infinity)
+#pragma clang fp contract(off)
     constexpr uint32_t each = D / 16;
     const uint32_t f = (lane & 15) * each, sub = lane >> 4;
     float qf[each], acc[each], m = -FLT_MAX, l = 0.0f;

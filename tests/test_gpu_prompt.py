@@ -300,3 +300,36 @@ def test_a_run_of_them(ctx, dtype, heads, group, d):
     for layer in range(2):
         cache.check(layer, "at the end")
     pool.close()
+
+
+@pytest.mark.parametrize("heads,group,d", [(2, 2, 128), (1, 4, 64), (1, 1, 256)])
+def test_floats_past_the_largest_bf16(ctx, heads, group, d):
+    """Numbers between bf16's largest and float's own round to an infinity as bf16 terms: the rows that
+    attend them are right all the same, as are numbers that leave nothing in the lower terms."""
+    print(f"large floats {heads} {group} {d}", flush=True)
+    x = Prompts(ctx, "f32", [70, 150], heads, d, 36)
+    q, k, v = x.randn(x.n, heads * group, d), x.randn(x.n, heads, d), x.randn(x.n, heads, d)
+    v[90, 0, 3] = torch.finfo(torch.float32).max
+    v[20, 0, 5] = -torch.finfo(torch.float32).max * 0.9999
+    v[30:40] = torch.round(v[30:40])
+    v[100, 0, 9] = 2.0 ** -140
+    out = torch.empty_like(q.cuda().flatten(1))
+    x.pool.prompt_attention(*(t.cuda().flatten(1) for t in (q, k, v)), heads * group, 0.1, out)
+    ref.assert_within(out, *x.attended(q, k, v, 0.1), "large floats")
+    x.pool.close()
+
+
+def test_terms_keep_their_bits(ctx):
+    """Values that cancel: float rows' results are those of 24 bits, not of one bf16 term or two."""
+    x = Prompts(ctx, "f32", [64], 1, 128, 37)
+    q, k = torch.zeros(64, 1, 128), torch.zeros(64, 1, 128)
+    v = x.randn(64, 1, 128)
+    v[1::2] = -v[::2] * (1 - 2.0 ** -14)  # pairs leave 2^-14 of themselves
+    out = torch.empty(64, 128, device="cuda")
+    x.pool.prompt_attention(q.cuda().flatten(1), k.cuda().flatten(1), v.cuda().flatten(1), 1, 1.0, out)
+    # equal weights of 2^-1 .. 2^-6 at these rows: means of what floats hold, summed in 32 bits
+    for r in (1, 3, 7, 15, 31, 63):
+        want = v[:r + 1, 0].double().mean(0)
+        room = (r + 4) * 2.0 ** -23 * v[:r + 1, 0].double().abs().mean(0)
+        assert ((out[r].cpu().double() - want).abs() <= room).all(), r
+    x.pool.close()
