@@ -1307,6 +1307,8 @@ int ensure_prompt_list(ckv_pool* pool, const pool_view& view, const prompt_form&
 int run_prompt(ckv_pool* pool, size_t layer, const prompt_rows& x, size_t q_heads, float scale, void* output,
                const void* gate, bool rows)
 {
+    if (const int refused = refuse_wide_capture(pool))
+        return refused;
     ckv_context* ctx = pool->ctx;
     const pool_view view = view_of(pool);
     const prompt_form form = prompt_form_of(view, pool->meta, x, (uint32_t)q_heads, scale, output, gate, !rows,
@@ -1331,8 +1333,6 @@ int run_fp4_prefill(ckv_pool* pool, size_t layer, const void* queries, size_t q_
                     const void* gate)
 {
     return guarded(pool, [&]() -> int {
-        if (const int refused = refuse_wide_capture(pool))
-            return refused;
         prompt_rows x {};
         x.queries = queries;
         x.q_stride = (uint64_t)q_heads * pool->head_dim;
