@@ -182,8 +182,9 @@ int ckv_pool_wrap(ckv_context* ctx, size_t layers, size_t blocks, size_t block_s
  * bf16 terms that keep at least 16 bits of queries and probabilities in decode rows, and of
  * the rows' type in prefill tiles (f32 rows: 24 bits in both).
  * Sums are floats before they are divided: values past 2^100 may become infinite on the way.
- * Appends and attention of a 4-bit pool of 256-wide heads are not captured into graphs
- * (invalid_argument).
+ * Appends and attention of a 4-bit pool of 256-wide heads (ckv_prompt_attention with it)
+ * are refused under stream capture, and outside it too once a call on the pool has met one
+ * (invalid_argument): a run of that kind ended in a GPU fault whose cause is not known.
  * Checks: those of ckv_pool_create, in their order, where the block size must be a power of
  * two from 16 to 4096 (invalid_block_size) and head_dim 64, 128 or 256 (invalid_head_dimension); wrapped
  * buffers must be aligned to 16 bytes (invalid_argument) and hold the bytes_each of

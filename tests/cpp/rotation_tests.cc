@@ -319,3 +319,35 @@ TEST("work lists: every tile's key blocks once")
                             CHECK(list.n_cut == 0);
                     }
 }
+
+// 256-wide heads: once a call of a 4-bit pool has met a stream capture, what appends or attends
+// is refused, and what only reads the pool's metadata is not.
+TEST("4-bit pools of 256-wide heads after a capture")
+{
+    two_rows t;
+    t.pool.head_dim = 256;
+    t.pool.fp4 = t.pool.captured = true;
+    t.upload();
+    ckv_pool* p = &t.pool;
+    void *q = t.x, *o = t.x + 1, *k = t.x + 2, *v = t.x + 3, *a = t.x + 4, *b = t.x + 5;
+    const ckv_rotation r = plain();
+    const auto refused = [&](int status) {
+        const bool told = t.ctx.last_error.find("nor after a call under one") != std::string::npos;
+        t.ctx.last_error.clear();
+        return status == CKV_E_INVALID_ARGUMENT && told;
+    };
+    CHECK(refused(ckv_append(p, 0, k, v, 2)));
+    CHECK(refused(ckv_rope_append(p, 0, k, v, 1e4f, 0, 2)));
+    CHECK(refused(ckv_rotate_append(p, 0, &r, q, o, 4, k, v, a, b, 2)));
+    CHECK(refused(ckv_rotate_append(p, 0, nullptr, nullptr, nullptr, 0, k, v, nullptr, nullptr, 2)));
+    CHECK(refused(ckv_prompt_attention(p, q, 0, k, v, 0, 4, 1.0f, nullptr, o, 2)));
+    t.pool.shared_tile = true; // a chunk
+    CHECK(refused(ckv_attention(p, 0, q, 4, 1.0f, o, 2)));
+    CHECK(refused(ckv_attention_gated(p, 0, q, 4, 1.0f, a, o, 2)));
+    CHECK(refused(ckv_prefill_attention(p, 0, q, 4, 1.0f, o, 2)));
+    t.pool.shared_tile = false;
+    CHECK(refused(ckv_attention(p, 0, q, 4, 1.0f, o, 2)));
+    CHECK(refused(ckv_decode_attention(p, 0, q, 4, 1.0f, o, 2)));
+    CHECK(refused(ckv_append_decode(p, 0, k, v, q, 4, 1.0f, o, 2)));
+    CHECK(refused(ckv_rotate_append_decode(p, 0, nullptr, k, v, q, 4, 1.0f, nullptr, a, b, o, 2)));
+}
