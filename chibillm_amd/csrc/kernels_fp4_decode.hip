@@ -306,7 +306,8 @@ __global__ __launch_bounds__(64 * fp4_waves_of(D), D == 256 ? 3 : 4) void fp4_de
                 mx = nm;
                 limit = nm + slack; // probabilities up to 2^8 weigh as exactly
             }
-            const float shift = -mx * scale_log2;
+            // (while every score was -inf: finite, or their weights would be NaN in place of 0)
+            const float shift = fminf(-mx * scale_log2, FLT_MAX);
             float pr[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
