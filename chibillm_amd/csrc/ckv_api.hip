@@ -3250,9 +3250,9 @@ int ckv_copy_blocks(ckv_pool* pool, const uint32_t* src, const uint32_t* dst, si
     if (status)
         return status;
     pool_view view = view_of(pool);
-    if (pool->fp4) { // pages as bytes
-        view.features = (uint32_t)(pool->bytes_each / pool->layers / pool->blocks);
-        view.block_size = view.elem_size = 1;
+    if (pool->fp4) { // pages as bytes, a token's features in 17/32 of one each (head_dim is whole 32s)
+        view.features = view.features / 32 * 17;
+        view.elem_size = 1;
     }
     return run_kernel(ctx, "copy_blocks", [&] {
         return launch_copy_blocks(ctx->stream, view, (uint32_t)pool->layers, pool->d_pairs,
