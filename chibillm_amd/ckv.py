@@ -219,12 +219,18 @@ def _rotation(rotation: Optional[Rotation]):
     return None if rotation is None else C.addressof(rotation)
 
 
-def _rows(x):
-    """(address, elements from one row to the next) of a 2-D device tensor of whole rows."""
+def _rows(x, pool, heads: int, rows: int):
+    """(address, elements from one row to the next) of a 2-D device tensor of at least `rows`
+    whole rows of `heads` heads of the pool's."""
     if not x.is_cuda:
         raise ValueError("device arrays must be GPU tensors")
     if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ValueError("rows are [rows, features] with features side by side")
+    features = heads * pool.geometry[4]
+    if x.shape[1] != features or x.shape[0] < rows:
+        raise ValueError(f"{rows} rows of {features} features are needed, not {list(x.shape)}")
+    if x.shape[0] > 1 and x.stride(0) < features:  # (a stride of 0 would be passed as none given)
+        raise ValueError("rows overlap")
     return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else 0
 
 
@@ -554,7 +560,8 @@ class Pool:
         """Whole prompts' attention from their rows (ckv_prompt_attention); queries, and keys
         and values, may be parts of wider rows."""
         rows = queries.shape[0] if rows is None else rows
-        (q, q_stride), (k, k_stride), (v, v_stride) = _rows(queries), _rows(keys), _rows(values)
+        q, q_stride = _rows(queries, self, q_heads, rows)
+        (k, k_stride), (v, v_stride) = (_rows(x, self, self.geometry[3], rows) for x in (keys, values))
         if k_stride != v_stride:
             raise ValueError("keys and values have rows of one stride")
         self.ctx.check(load().ckv_prompt_attention(

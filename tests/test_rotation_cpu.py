@@ -39,6 +39,42 @@ def test_binding_refuses_rotations_and_rows_it_cannot_pass():
     pool.handle = None
 
 
+class OnDevice:
+    """A tensor that says it is on a GPU; its memory is never read."""
+
+    def __init__(self, x):
+        self.x, self.is_cuda, self.shape = x, True, x.shape
+
+    def dim(self):
+        return self.x.dim()
+
+    def stride(self, i):
+        return self.x.stride(i)
+
+    def data_ptr(self):
+        return self.x.data_ptr()
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("make,said", [
+    (lambda n: torch.zeros(1, n).expand(4, -1), "overlap"),            # one row, four times
+    (lambda n: torch.zeros(4 * n).as_strided((4, n), (n - 1, 1)), "overlap"),
+    (lambda n: torch.zeros(4, 2 * n)[:, :n - 8], "are needed"),        # part of a row
+    (lambda n: torch.zeros(4, n + 8), "are needed"),
+    (lambda n: torch.zeros(3, n), "are needed"),                       # a row too few
+    (lambda n: torch.zeros(4, 1, n), "side by side"),
+])
+def test_prompt_rows_that_would_be_read_past_their_end(which, make, said):
+    """Of a pool of 2 KV heads of 64 and 4 query heads, four rows."""
+    pool = object.__new__(ckv.Pool)
+    pool.geometry = (1, 1, 16, 2, 64)
+    rows = [torch.zeros(4, 256), torch.zeros(4, 128), torch.zeros(4, 128)]
+    rows[which] = make(rows[which].shape[1])
+    with pytest.raises(ValueError, match=said):
+        pool.prompt_attention(*map(OnDevice, rows), 4, 1.0, None, rows=4)
+    pool.handle = None
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
 def test_the_reference_holds_what_the_levels_say(dtype):
     """The oracle of the device tests against a search through all 16 numbers."""
