@@ -381,9 +381,13 @@ struct ckv_pool {
     float turns_theta = 0.0f;
     uint32_t turns_rotary = 0;
 
-    ckv::rotation_table rotation {}; // of the last ckv_rotation
-    ckv_rotation rotation_of {};
-    bool rotation_ready = false;
+    // the tables of the last few ckv_rotations: layers that alternate between some find theirs
+    struct kept_rotation {
+        ckv_rotation of;
+        ckv::rotation_table table;
+    };
+    kept_rotation rotations[8] = {};
+    uint32_t n_rotations = 0, next_rotation = 0;
     int whole_prompts = -1; // whether the batch's rows are whole prompts; -1: not yet looked at
 
     ckv::move_marks marks; // of ckv_compact's slots

@@ -351,3 +351,70 @@ TEST("4-bit pools of 256-wide heads after a capture")
     CHECK(refused(ckv_append_decode(p, 0, k, v, q, 4, 1.0f, o, 2)));
     CHECK(refused(ckv_rotate_append_decode(p, 0, nullptr, k, v, q, 4, 1.0f, nullptr, a, b, o, 2)));
 }
+
+// Layers that alternate between rotations find their tables; more than are kept are made anew,
+// and every table is its own rotation's.
+TEST("rotations kept by a pool")
+{
+    two_rows t;
+    t.upload();
+    t.pool.positions.clear(); // no rows: nothing is launched
+    t.pool.slot_rows = 0;
+    ckv_pool* p = &t.pool;
+    std::vector<ckv_rotation> all(1, plain());
+    const auto with = [&](auto change) {
+        ckv_rotation r = plain();
+        r.scaling = CKV_SCALING_YARN;
+        r.factor = 4.0f;
+        r.low = 1.0f;
+        r.high = 32.0f;
+        r.original = 4096;
+        change(r);
+        all.push_back(r);
+    };
+    with([](ckv_rotation&) {});
+    with([](ckv_rotation& r) { r.theta = 5e5f; });
+    with([](ckv_rotation& r) { r.layout = CKV_ROTARY_NEIGHBOURS; });
+    with([](ckv_rotation& r) { r.rotary_dim = 64; });
+    with([](ckv_rotation& r) { r.factor = 8.0f; });
+    with([](ckv_rotation& r) { r.original = 8192; });
+    with([](ckv_rotation& r) { r.magnitude = 2.0f; });
+    with([](ckv_rotation& r) { r.low = 2.0f; });
+    with([](ckv_rotation& r) { r.high = 40.0f; });
+    with([](ckv_rotation& r) { r.scaling = CKV_SCALING_LINEAR; });
+    const size_t most = sizeof(p->rotations) / sizeof(p->rotations[0]);
+    REQUIRE(all.size() > most);
+    const auto call = [&](ckv_pool* pool, const ckv_rotation& r) { return ckv_rotate(pool, &r, t.x, t.x + 1, 2, 0); };
+    for (int round = 0; round < 4; ++round)
+        for (size_t i = 0; i < most; ++i)
+            CHECK(call(p, all[i]) == CKV_OK);
+    CHECK(p->n_rotations == most && p->next_rotation == 0); // each made once
+    for (int round = 0; round < 3; ++round)
+        for (const ckv_rotation& r : all) {
+            CHECK(call(p, r) == CKV_OK);
+            two_rows fresh; // a pool that has met no other
+            fresh.upload();
+            fresh.pool.positions.clear();
+            CHECK(call(&fresh.pool, r) == CKV_OK);
+            REQUIRE(fresh.pool.n_rotations == 1);
+            const auto& want = fresh.pool.rotations[0];
+            size_t found = 0;
+            for (uint32_t i = 0; i < p->n_rotations; ++i) {
+                const auto& kept = p->rotations[i];
+                if (std::memcmp(&kept.of, &want.of, sizeof(ckv_rotation)))
+                    continue;
+                ++found;
+                const rotation_table &a = kept.table, &b = want.table;
+                CHECK(std::equal(a.turns.step, a.turns.step + b.rotary / 2, b.turns.step));
+                CHECK(a.magnitude == b.magnitude && a.magnitude64 == b.magnitude64 && a.rotary == b.rotary
+                      && a.neighbours == b.neighbours);
+            }
+            CHECK(found == 1);
+        }
+    // one that is refused leaves them as they are
+    const uint32_t next = p->next_rotation;
+    ckv_rotation bad = plain();
+    bad.theta = 0.0f;
+    CHECK(call(p, bad) == CKV_E_INVALID_ROPE_THETA);
+    CHECK(p->next_rotation == next);
+}
