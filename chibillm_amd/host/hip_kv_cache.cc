@@ -210,7 +210,8 @@ hip_kv_cache::element_offset(std::size_t layer, std::size_t block, std::size_t t
     std::size_t offset = 0;
     const int rc = ckv_element_offset(pool_, layer, block, token_offset, kv_head, feature, &offset);
     if (rc)
-        return fail(rc < 200 ? kv_cache_errc::head_feature_out_of_range : static_cast<kv_cache_errc>(rc - 200));
+        return rc < 200 ? fail(kv_cache_error { kv_cache_errc::head_feature_out_of_range, "held in 4 bits" })
+                        : fail(kv_cache_error { static_cast<kv_cache_errc>(rc - 200) });
     return offset;
 }
 

@@ -221,7 +221,8 @@ public:
         return storage_ == kv_storage::fp4 ? elements / 32 * 17 : elements * element_bytes(type_);
     }
 
-    // (of a cache held in 4 bits no element has one: head_feature_out_of_range)
+    // (of a cache held in 4 bits no element has one: head_feature_out_of_range, whose detail
+    // says so)
     [[nodiscard]] result<std::size_t, kv_cache_error> element_offset(std::size_t layer,
                                                                      std::size_t block,
                                                                      std::size_t token_offset,

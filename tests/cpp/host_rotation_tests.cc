@@ -174,3 +174,14 @@ TEST("rotations and prompts: shapes that are refused")
     CHECK(error_is(prompt_attention(*c, q.tensor, k.tensor, v.tensor, 1, q.tensor),
                    tensor_op_errc::unsupported_aliasing));
 }
+
+TEST("element offsets: a cache in 4 bits says why it has none")
+{
+    auto c = hip_kv_cache::make(gpu(), { 1, 2, 16, 1, dim }, kv_dtype::f32, kv_storage::fp4);
+    auto floats = hip_kv_cache::make(gpu(), { 1, 2, 16, 1, dim }, kv_dtype::f32);
+    REQUIRE(c && floats);
+    const auto none = c->element_offset(0, 0, 0, 0, 0), outside = floats->element_offset(0, 0, 0, 0, dim);
+    REQUIRE(!none && !outside);
+    CHECK(none.error().detail == "held in 4 bits");
+    CHECK(outside.error() == kv_cache_errc::head_feature_out_of_range && outside.error().detail.empty());
+}
