@@ -141,7 +141,7 @@ __host__ __device__ inline uint32_t prefill_range_count(uint32_t n_blocks, uint3
 // The key blocks [begin, end) of range `part` of n ranges. Range 0 starts at
 // block 0, of which every query attends some key where there is no window; through
 // one it may attend none there, but itself in some range. 32-bit:
-// n_blocks < 2^27 (positions are 32-bit) and part < split_max.
+// n_blocks < 2^27 (positions are 32-bit) and part < 16 (prompts' ranges; others' split_max).
 __host__ __device__ inline void prefill_range_bounds(uint32_t n_blocks, uint32_t n, uint32_t part,
                                                      uint32_t& begin, uint32_t& end)
 {

@@ -15,6 +15,8 @@
 //
 // Bound by the vector ALU's conversions beside HBM: 17 bytes of a block become 32 operands
 // by 16 conversions (V: and 16 permutes that pair a feature's tokens).
+// Registers are at the bound of the waves that share a SIMD: bf16 forms of 128- and 256-wide heads
+// spill 12 bytes a lane, float ones 20 and 16, outside the loop over tokens.
 #include "decode_wg.h"
 #include "fp4.h"
 
@@ -527,6 +529,9 @@ decode_form fp4_decode_form()
     return { 2, 16, 32, 47, false };
 }
 
+// A pass reads the cache again. 48 rows of 900 to 12,000 tokens, 8 KV heads, us: groups of 1, 2, 4
+// and 8 query heads 72, 74, 75 and 77, of 9 and 16 (two passes) 124 and 127, of 32 (four) 205;
+// float rows, groups of 1, 2 and 4 81, 82 and 85, of 8 (two) 133, of 16 (four) 238.
 uint32_t fp4_decode_passes(const pool_view& p, uint32_t q_heads)
 {
     const uint32_t each = p.dtype == CKV_F32 ? 4 : 8, group = q_heads / p.kv_heads;

@@ -9,9 +9,10 @@
 //   S^T[key][query] = K . Q^T      D/16 x v_mfma_f32_32x32x16
 //   O^T[feature][query] += V^T . P^T  D/16 of them, P^T straight from registers
 // with S(kb) on the matrix cores while the vector ALU turns S(kb - 1) into probabilities.
-// Probabilities enter P.V in the rows' type; that rounding and the result's own come to 1.27
-// times the result's own (a second term for what the first left would cost half as many
-// products again).
+// Probabilities enter P.V in the rows' type. Against 64 bits that rounding and the result's own
+// come to 1.27 times the result's own in nine fp16 prompts of 17 to 900 rows, 1.33 in bf16 ones of
+// 6,000 and 8,192 and 1.41 in 512 bf16 rows behind 6,000 tokens of 4 bits (a second term for
+// what the first left would cost half as many products again).
 //
 // Staging goes through registers, a block ahead: 4-bit codes become the rows' type on the
 // way, exactly, once for the four waves; rows of any stride and alignment are taken as they
@@ -21,9 +22,12 @@
 // bits. Of queries and probabilities always, of keys and values where they are rows (4-bit
 // numbers are bf16's): 6 or 3 products of terms in place of one of floats, which takes 16
 // times as long as one of these. On v_mfma_f32_32x32x2 (exact products) 200 rows behind
-// 1,500 tokens of 4 bits took 52 us and take 26, 4 x 512 behind 3,000 457 and 150, two
-// prompts of 3,000 rows 642 and 432, five of up to 700 of 64-wide heads 21.6 and 15.7; errors
-// against 64 bits are the same. Rows of 256-wide heads have a kernel of their own below.
+// 1,500 tokens of 4 bits took 53 us and take 27, 4 x 512 behind 3,000 456 and 148, two
+// prompts of 3,000 rows 641 and 425, five of up to 700 of 64-wide heads 22 and 15.5; errors
+// against 64 bits are the same. Over 4-bit pages of 256-wide heads the terms of a query are
+// more than a lane's registers: 240 bytes of them spill, and 2 x 300 rows behind 2,000 tokens
+// take 80 us where they took 254, 8 x 512 264 where 771. Rows of 256-wide heads have a kernel of
+// their own below.
 //
 // Keys past the tile's last position are staged as zeros. A masked key's probability is 0,
 // which meets its value in P.V all the same: where that is infinite or NaN, the rows that
@@ -746,7 +750,8 @@ __global__ __launch_bounds__(n_threads, D == 256 || (D == 128 && DT == CKV_F32) 
 }
 
 // Float rows of 256-wide heads, whose terms' planes LDS has no room for: S^T and O^T on
-// v_mfma_f32_32x32x2, 128 and 128 products a block, which are 85 % of its time (8.2 us). The
+// v_mfma_f32_32x32x2, 128 and 128 products a block, which are 85 % of its time (8.2 us; 56 to
+// 60 bytes a lane spill beside them). The
 // contraction over features pairs 8i + e with 8i + 4 + e, so that a lane's operands are
 // 16-byte words; that over keys pairs the two keys of an accumulator element, so that a
 // probability is an operand where it was computed. Two LDS stages of whole rows.
@@ -1016,9 +1021,11 @@ namespace {
 // unit (two there: `shared` of that more for each), what comes before and after the blocks,
 // in blocks, and of a tile that is cut the handoff and each record. Fitted to times of 20
 // batches in 1 to 16 ranges; the ranges it chooses are the fastest measured or within 8 % of
-// that. Uncut and as chosen, us: 512 rows behind 6000 tokens of 4 bits 164 and 46, 4 x 256
-// behind 2000 60 and 34, 900 rows of one prompt 21 and 17, five short float prompts 35 and
-// 16; 8 x 1024 behind 3000 stays uncut (242, in two ranges 271).
+// that. Uncut and as chosen, us back to back: 512 rows behind 6000 tokens of 4 bits 164 and 49,
+// 4 x 256 behind 2000 61 and 35, 900 rows of one prompt 21 and 17, five short float prompts 35
+// and 15.5; 8 x 1024 behind 3000 stays uncut (242, in two ranges 277). The list is made at a
+// batch's first call, which all layers share: 5 to 13 us more of the host's time than a later
+// call, 7 to 17 us to the end of the launch (one chunk of 512 rows, nine prompts, 100 prompts).
 struct prompt_cost {
     double block, shared, ends, handoff, record;
     uint32_t per_cu;
