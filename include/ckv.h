@@ -180,7 +180,8 @@ int ckv_pool_wrap(ckv_context* ctx, size_t layers, size_t blocks, size_t block_s
  * Attention takes any number of query heads per kv head (decode rows of up to 2^26 numbers,
  * counting four more for each head: invalid_argument) and any scale, with products of
  * bf16 terms that keep at least 16 bits of queries and probabilities in decode rows, and of
- * the rows' type in prefill tiles (f32 rows: 24 bits in both).
+ * the rows' type in prefill tiles (f32 rows: 24 bits in both, of queries under 2^-110 what
+ * is left above 2^-134).
  * Sums are floats before they are divided: values past 2^100 may become infinite on the way.
  * Appends and attention of a 4-bit pool of 256-wide heads (ckv_prompt_attention with it)
  * are refused under stream capture, and outside it too once a call on the pool has met one
@@ -585,9 +586,11 @@ int ckv_rotate_append_decode(ckv_pool* pool, size_t layer, const ckv_rotation* r
  * keys and values are in hand as rows and need not be read back from the cache (which may
  * hold them in 4 bits). Row r attends the rows of its sequence from position 0 to its own:
  * output = softmax(q . k * scale) . v with fp32 accumulation; probabilities enter the
- * matrix cores in the rows' type (f32 rows: everything does with 24 bits, as bf16 terms). The batch's tables tell the sequences: every row's
- * position is 0 or follows the row before it, in the same table range (invalid_argument
- * otherwise). The pool gives the geometry (head_dim 64, 128 or 256: otherwise
+ * matrix cores in the rows' type (f32 rows: everything does with 24 bits, as bf16 terms,
+ * which end at 2^-134: numbers under 2^-110 keep as many as are left above it, but for
+ * 256-wide heads, whose products are floats'). The batch's tables tell the sequences:
+ * every row's position is 0 or follows the row before it, in the same table range
+ * (invalid_argument otherwise). The pool gives the geometry (head_dim 64, 128 or 256: otherwise
  * invalid_head_dimension) and type; its cache is neither read nor written, and any number
  * of query heads per kv head, and any scale, is taken. Rows begin q_stride (queries) and kv_stride (keys, values)
  * elements apart, at least as many as they hold (input_shape_mismatch); 0: no gap. The
